@@ -148,6 +148,25 @@ def lib():
         "bsq_legacy_encode_device": (i32, [i32, P, u64, P, P]),
         "bsq_legacy_decode_device": (i32, [i32, P, u64, P, P]),
         "bsq_legacy_sweep": (i32, [i32, u64, u64, P, P]),
+        "bsq_mx4_codes_bytes": (u64, [u64, u64]),
+        "bsq_mx4_scales_bytes": (u64, [u64, u64]),
+        "bsq_mx4_encode": (i32, [P, i32, u64, u64, u64, u64, u64, P, P, P, P, P]),
+        "bsq_mx4_decode": (i32, [P, P, u64, u64, P, i32, u64, P]),
+        "bsq_mx4_product_workspace": (u64, [u64, u64, u64]),
+        "bsq_mx4_product": (i32, [P, P, u64, P, P, u64, u64, P, i32, u64, P, u64, P]),
+        "bsq_mx4_linear_workspace": (u64, [u64, u64, u64]),
+        "bsq_mx4_linear": (i32, [P, i32, u64, u64, u64, P, P, u64, P, i32, u64, P, P, P, u64, P]),
+        "bsq_mx4_linear_backward_workspace": (u64, [u64, u64, u64]),
+        "bsq_mx4_linear_backward": (i32, [P, i32, u64, u64, u64, P, P, P, P, u64, P, u64, P, u64, i32, P, u64, P]),
+        "bsq_moe_route": (i32, [P, i32, u64, u32, u64, P, i32, u32, u32, u32, i32, f32, P, P, P]),
+        "bsq_moe_route_backward": (i32, [P, i32, u64, u32, u64, i32, u32, i32, f32, P, P, P, u64, P]),
+        "bsq_moe_plan": (i32, [P, u64, u32, P, P, P]),
+        "bsq_moe_combine": (i32, [P, i32, u64, u32, u64, P, P, u32, P, i32, u64, P]),
+        "bsq_moe_linear_workspace": (u64, [u64, u32, u64, u64, u32]),
+        "bsq_moe_linear": (i32, [P, i32, u64, u64, u64, P, P, u32, P, P, u32, u64, P, P, P, i32, P, i32, u64, P, u64, P]),
+        "bsq_moe_linear_backward_workspace": (u64, [u64, u32, u64, u64, u32]),
+        "bsq_moe_linear_backward": (i32, [P, i32, u64, u64, u64, P, i32, u64, u64, P, P, u32, P, P, P, i32, P, P, u32, P,
+                                          u64, P, P, i32, P, u64, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -607,3 +626,185 @@ def legacy_sweep(kind: int, lo: int, hi: int) -> int:
     check(lib().bsq_legacy_sweep(kind, lo, hi, d.ptr, None), "legacy sweep")
     check(lib().bsq_stream_synchronize(None), "sync")
     return int(d.download(np.uint64, 1)[0])
+
+
+# ---------------------------------------------------------------------------
+# microscaled 4-bit matrices and the layers that compute with them
+# (include/bitsqz_llm_c.h, group 6)
+# ---------------------------------------------------------------------------
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+_TYPE_NUMPY = {TYPE_F32: np.dtype(np.float32), TYPE_BF16: np.dtype(np.uint16), TYPE_F16: np.dtype(np.float16)}
+
+
+def to_bf16(x: np.ndarray) -> np.ndarray:
+    """Bit patterns (uint16) of the nearest BF16 values, ties to even."""
+    x = np.ascontiguousarray(x, np.float32)
+    u = x.view(np.uint32)
+    r = ((u + (0x7FFF + ((u >> 16) & 1)).astype(np.uint32)) >> 16).astype(np.uint16)
+    return np.where(np.isnan(x), ((u >> 16) | 0x40).astype(np.uint16), r)
+
+
+def from_bf16(bits: np.ndarray) -> np.ndarray:
+    return (np.ascontiguousarray(bits, np.uint16).astype(np.uint32) << 16).view(np.float32)
+
+
+def _typed(x: np.ndarray, type: int) -> np.ndarray:
+    """Host values in a type's storage (BF16: bit patterns, or floats to round)."""
+    x = np.asarray(x)
+    if type == TYPE_BF16 and x.dtype != np.uint16:
+        return to_bf16(x)
+    return np.ascontiguousarray(x, _TYPE_NUMPY[type])
+
+
+class Mx4:
+    """A packed matrix of rows x cols (or several, one after another) on the GPU."""
+
+    def __init__(self, rows: int, cols: int, batch: int = 1):
+        self.rows, self.cols, self.batch = rows, cols, batch
+        self.codes = DeviceBuffer(batch * lib().bsq_mx4_codes_bytes(rows, cols))
+        self.scales = DeviceBuffer(batch * lib().bsq_mx4_scales_bytes(rows, cols))
+
+    def download(self):
+        """(codes, scales) as stored: batch * rows x padded cols / 2 and / 32."""
+        n = self.batch * self.rows
+        return (self.codes.download(np.uint8, self.codes.nbytes).reshape(n, -1),
+                self.scales.download(np.uint8, self.scales.nbytes).reshape(n, -1))
+
+    def decode(self, type: int = TYPE_F32) -> np.ndarray:
+        n = self.batch * self.rows
+        out = DeviceBuffer(n * self.cols * _TYPE_NUMPY[type].itemsize)
+        check(lib().bsq_mx4_decode(self.codes.ptr, self.scales.ptr, n, self.cols, out.ptr, type, self.cols, None),
+              "mx4_decode")
+        check(lib().bsq_stream_synchronize(None), "sync")
+        return out.download(_TYPE_NUMPY[type], n * self.cols).reshape(n, self.cols)
+
+
+def mx4_encode(x: np.ndarray, type: int = TYPE_F32, rows: bool = True, columns: bool = False):
+    """The packed rows and / or columns of x (rows x cols, or a batch of those)."""
+    x = _typed(x, type)
+    batch, r, c = (1, *x.shape) if x.ndim == 2 else x.shape
+    by_row = Mx4(r, c, batch) if rows else None
+    by_col = Mx4(c, r, batch) if columns else None
+    d = DeviceBuffer.from_array(x)
+    check(lib().bsq_mx4_encode(d.ptr, type, batch, r, c, c, r * c, by_row.codes.ptr if rows else None,
+                               by_row.scales.ptr if rows else None, by_col.codes.ptr if columns else None,
+                               by_col.scales.ptr if columns else None, None), "mx4_encode")
+    check(lib().bsq_stream_synchronize(None), "sync")
+    return (by_row, by_col) if rows and columns else by_row or by_col
+
+
+def mx4_product(a: Mx4, b: Mx4, type: int = TYPE_F32) -> np.ndarray:
+    out = DeviceBuffer(a.rows * b.rows * _TYPE_NUMPY[type].itemsize)
+    work = DeviceBuffer(lib().bsq_mx4_product_workspace(a.rows, b.rows, a.cols))
+    check(lib().bsq_mx4_product(a.codes.ptr, a.scales.ptr, a.rows, b.codes.ptr, b.scales.ptr, b.rows, a.cols, out.ptr,
+                                type, b.rows, work.ptr, work.nbytes, None), "mx4_product")
+    check(lib().bsq_stream_synchronize(None), "sync")
+    return out.download(_TYPE_NUMPY[type], a.rows * b.rows).reshape(a.rows, b.rows)
+
+
+def mx4_linear(x: np.ndarray, w: Mx4, type: int = TYPE_F32, out_type: int = TYPE_F32, keep: bool = False):
+    """out = q(x) W^T; with `keep` also the packed transpose of x."""
+    x = _typed(x, type)
+    m, k = x.shape
+    d, out = DeviceBuffer.from_array(x), DeviceBuffer(m * w.rows * _TYPE_NUMPY[out_type].itemsize)
+    work = DeviceBuffer(lib().bsq_mx4_linear_workspace(m, w.rows, k))
+    xt = Mx4(k, m) if keep else None
+    check(lib().bsq_mx4_linear(d.ptr, type, m, k, k, w.codes.ptr, w.scales.ptr, w.rows, out.ptr, out_type, w.rows,
+                               xt.codes.ptr if keep else None, xt.scales.ptr if keep else None, work.ptr, work.nbytes,
+                               None), "mx4_linear")
+    check(lib().bsq_stream_synchronize(None), "sync")
+    y = out.download(_TYPE_NUMPY[out_type], m * w.rows).reshape(m, w.rows)
+    return (y, xt) if keep else y
+
+
+def mx4_linear_backward(dy: np.ndarray, xt: Mx4, wt: Mx4, type: int = TYPE_F32, g_type: int = TYPE_F32):
+    """(dx, dw) of mx4_linear from the packed columns of x and of the weights."""
+    dy = _typed(dy, type)
+    (m, n), k = dy.shape, wt.rows
+    size = _TYPE_NUMPY[g_type].itemsize
+    d, dx, dw = DeviceBuffer.from_array(dy), DeviceBuffer(m * k * size), DeviceBuffer(n * k * size)
+    work = DeviceBuffer(lib().bsq_mx4_linear_backward_workspace(m, n, k))
+    check(lib().bsq_mx4_linear_backward(d.ptr, type, m, n, n, xt.codes.ptr, xt.scales.ptr, wt.codes.ptr, wt.scales.ptr,
+                                        k, dx.ptr, k, dw.ptr, k, g_type, work.ptr, work.nbytes, None),
+          "mx4_linear_backward")
+    check(lib().bsq_stream_synchronize(None), "sync")
+    return (dx.download(_TYPE_NUMPY[g_type], m * k).reshape(m, k), dw.download(_TYPE_NUMPY[g_type], n * k).reshape(n, k))
+
+
+def moe_route(logits: np.ndarray, k: int, type: int = TYPE_F32, bias: np.ndarray | None = None,
+              scoring: int = SCORE_SOFTMAX, groups: int = 1, kept: int = 1, renormalise: bool = True, scale: float = 1.0):
+    """(ids, weights), tokens x k."""
+    logits = _typed(logits, type)
+    tokens, experts = logits.shape
+    d = DeviceBuffer.from_array(logits)
+    db = DeviceBuffer.from_array(np.ascontiguousarray(bias, np.float32)) if bias is not None else None
+    ids, weights = DeviceBuffer(tokens * k * 4), DeviceBuffer(tokens * k * 4)
+    check(lib().bsq_moe_route(d.ptr, type, tokens, experts, experts, db.ptr if db else None, scoring, groups, kept, k,
+                              int(renormalise), scale, ids.ptr, weights.ptr, None), "moe_route")
+    check(lib().bsq_stream_synchronize(None), "sync")
+    return (ids.download(np.int32, tokens * k).reshape(tokens, k),
+            weights.download(np.float32, tokens * k).reshape(tokens, k))
+
+
+def moe_route_backward(logits: np.ndarray, ids: np.ndarray, d_weights: np.ndarray, type: int = TYPE_F32,
+                       scoring: int = SCORE_SOFTMAX, renormalise: bool = True, scale: float = 1.0) -> np.ndarray:
+    logits = _typed(logits, type)
+    (tokens, experts), k = logits.shape, ids.shape[1]
+    d, di = DeviceBuffer.from_array(logits), DeviceBuffer.from_array(np.ascontiguousarray(ids, np.int32))
+    dw, out = DeviceBuffer.from_array(np.ascontiguousarray(d_weights, np.float32)), DeviceBuffer(logits.nbytes)
+    check(lib().bsq_moe_route_backward(d.ptr, type, tokens, experts, experts, scoring, k, int(renormalise), scale, di.ptr,
+                                       dw.ptr, out.ptr, experts, None), "moe_route_backward")
+    check(lib().bsq_stream_synchronize(None), "sync")
+    return out.download(logits.dtype, tokens * experts).reshape(tokens, experts)
+
+
+def moe_plan(ids: np.ndarray, experts: int):
+    """(offsets, order) of the pairs in the experts' order."""
+    ids = np.ascontiguousarray(ids, np.int32)
+    d, off, order = DeviceBuffer.from_array(ids), DeviceBuffer(4 * (experts + 1)), DeviceBuffer(4 * ids.size)
+    check(lib().bsq_moe_plan(d.ptr, ids.size, experts, off.ptr, order.ptr, None), "moe_plan")
+    check(lib().bsq_stream_synchronize(None), "sync")
+    return off.download(np.int32, experts + 1), order.download(np.int32, ids.size)
+
+
+class MoeLinear:
+    """The experts' layer on packed weights: forward(), then backward() of it."""
+
+    def __init__(self, w: Mx4, wt: Mx4 | None = None):
+        """w: a batch of n x inputs; wt: the batch of its columns (inputs x n),
+        for the gradient of x."""
+        self.w, self.wt, self.experts, self.n, self.inputs = w, wt, w.batch, w.rows, w.cols
+
+    def forward(self, x, ids, weights, type: int = TYPE_F32, out_type: int = TYPE_F32, y_type: int = TYPE_F32):
+        x, ids = _typed(x, type), np.ascontiguousarray(ids, np.int32)
+        (m, _), k, e, n = x.shape, ids.shape[1], self.experts, self.n
+        self.type, self.m, self.k, self.y_type = type, m, k, y_type
+        self.x, self.ids = DeviceBuffer.from_array(x), DeviceBuffer.from_array(ids)
+        self.weights = DeviceBuffer.from_array(np.ascontiguousarray(weights, np.float32))
+        self.offsets, self.order = DeviceBuffer(4 * (e + 1)), DeviceBuffer(4 * m * k)
+        self.y = DeviceBuffer(m * k * n * _TYPE_NUMPY[y_type].itemsize)
+        out = DeviceBuffer(m * n * _TYPE_NUMPY[out_type].itemsize)
+        work = DeviceBuffer(lib().bsq_moe_linear_workspace(m, k, n, self.inputs, e))
+        check(lib().bsq_moe_linear(self.x.ptr, type, m, self.inputs, self.inputs, self.ids.ptr, self.weights.ptr, k,
+                                   self.w.codes.ptr, self.w.scales.ptr, e, n, self.offsets.ptr, self.order.ptr,
+                                   self.y.ptr, y_type, out.ptr, out_type, n, work.ptr, work.nbytes, None), "moe_linear")
+        check(lib().bsq_stream_synchronize(None), "sync")
+        return out.download(_TYPE_NUMPY[out_type], m * n).reshape(m, n)
+
+    def backward(self, d_out, type: int = TYPE_F32, g_type: int = TYPE_F32):
+        """(dx, d weights, dw)."""
+        d_out = _typed(d_out, type)
+        m, k, n, e, inputs = self.m, self.k, self.n, self.experts, self.inputs
+        t = _TYPE_NUMPY[g_type]
+        d, dx, dw = DeviceBuffer.from_array(d_out), DeviceBuffer(m * inputs * t.itemsize), DeviceBuffer(e * n * inputs * t.itemsize)
+        dweights = DeviceBuffer(4 * m * k)
+        work = DeviceBuffer(lib().bsq_moe_linear_backward_workspace(m, k, n, inputs, e))
+        check(lib().bsq_moe_linear_backward(d.ptr, type, m, n, n, self.x.ptr, self.type, inputs, inputs, self.ids.ptr,
+                                            self.weights.ptr, k, self.offsets.ptr, self.order.ptr, self.y.ptr,
+                                            self.y_type, self.wt.codes.ptr, self.wt.scales.ptr, e, dx.ptr, inputs,
+                                            dweights.ptr, dw.ptr, g_type, work.ptr, work.nbytes, None),
+              "moe_linear_backward")
+        check(lib().bsq_stream_synchronize(None), "sync")
+        return (dx.download(t, m * inputs).reshape(m, inputs), dweights.download(np.float32, m * k).reshape(m, k),
+                dw.download(t, e * n * inputs).reshape(e, n, inputs))

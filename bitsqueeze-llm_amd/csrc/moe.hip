@@ -1,0 +1,673 @@
+// Routing to experts and the experts' layer on MX4 weights: the choice of
+// experts with its gradient, the pairs (token, expert) in the experts' order,
+// the join of a token's experts, and the layer's forward and backward calls.
+// Compiled with -ffp-contract=off: the choice hangs on the last bit of a score
+// plus a bias, which is rounded as two operations.
+#include "mx4.hpp"
+
+#include <algorithm>
+#include <cfloat>
+#include <type_traits>
+
+#include <bitsqz_llm_c.h>
+
+namespace bsq {
+namespace {
+
+constexpr uint32_t kMaxExperts = 1024, kMaxChosen = 64, kMaxGroups = 64;
+
+// ---------------------------------------------------------------------------
+// one wave's reductions through DPP moves; the result in every lane
+// ---------------------------------------------------------------------------
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_or(float other, float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(other), __float_as_int(v), CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ float from_lane(float v, int lane) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, dpp_or<0xB1, 0xF>(v, v));
+    v = fmaxf(v, dpp_or<0x4E, 0xF>(v, v));
+    v = fmaxf(v, dpp_or<0x141, 0xF>(v, v));
+    v = fmaxf(v, dpp_or<0x140, 0xF>(v, v));
+    v = fmaxf(v, dpp_or<0x142, 0xA>(v, v));
+    v = fmaxf(v, dpp_or<0x143, 0xC>(v, v));
+    return from_lane(v, 63);
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    v += dpp_or<0xB1, 0xF>(0.0f, v);
+    v += dpp_or<0x4E, 0xF>(0.0f, v);
+    v += dpp_or<0x141, 0xF>(0.0f, v);
+    v += dpp_or<0x140, 0xF>(0.0f, v);
+    v += dpp_or<0x142, 0xA>(0.0f, v);
+    v += dpp_or<0x143, 0xC>(0.0f, v);
+    return from_lane(v, 63);
+}
+
+template <Mx4Type T>
+constexpr float kLowest = T == Mx4Type::F32 ? -FLT_MAX : T == Mx4Type::BF16 ? -0x1.FEp127f : -65504.0f;
+
+struct RouteArgs {
+    const void *logits;
+    const float *bias;
+    uint64_t tokens, ld;
+    uint32_t experts, k, groups, kept;
+    int sigmoid, renorm;
+    float scale;
+};
+
+// A token's logits: expert e = lane * NV + i.  Experts that are closed to the
+// token (at or below the type's lowest value, or NaN) and those past the end
+// read -infinity.
+template <Mx4Type T, int NV>
+__device__ __forceinline__ void load_logits(const RouteArgs &a, uint64_t t, uint32_t lane, float x[NV]) {
+    const uint32_t e0 = lane * NV;
+    const uint64_t at = t * a.ld + e0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        x[i] = -INFINITY;
+        if (e0 + i < a.experts) {
+            const float v = load_value<T>(a.logits, at + i);
+            x[i] = v > kLowest<T> ? fminf(v, FLT_MAX) : -INFINITY;
+        }
+    }
+}
+
+__device__ __forceinline__ float sigmoid_of(float x) { return 1.0f / (1.0f + expf(-x)); }
+
+// Softmax over the open experts: the largest logit and the sum of the
+// exponentials (1 where there is none).
+template <int NV>
+__device__ __forceinline__ void softmax_of(const float x[NV], float e[NV], float &top, float &sum) {
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < NV; ++i) m = fmaxf(m, x[i]);
+    top = wave_max(m);
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        e[i] = x[i] > -INFINITY ? expf(x[i] - top) : 0.0f;
+        s += e[i];
+    }
+    sum = fmaxf(wave_sum(s), 1.0f);
+}
+
+// One wave a token, its scores and keys in registers.  The largest key of the
+// wave is a DPP reduction; the lowest lane that holds it (and its lowest
+// index) is the expert, so that ties go to the lowest.
+template <Mx4Type T, int NV>
+__global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a, int32_t *__restrict__ ids,
+                                                        float *__restrict__ weights) {
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t t = static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (t >= a.tokens) return;  // whole waves
+    float x[NV], score[NV], key[NV];
+    load_logits<T, NV>(a, t, lane, x);
+    if (a.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) score[i] = sigmoid_of(x[i]);
+    } else {
+        float top, sum;
+        softmax_of<NV>(x, score, top, sum);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) score[i] /= sum;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        key[i] = x[i];
+        if (a.bias != nullptr && x[i] > -INFINITY) {
+            const float v = score[i] + a.bias[lane * NV + i];
+            key[i] = v > -INFINITY ? v : -INFINITY;
+        }
+    }
+    if (a.groups > 1) {
+        const uint32_t each = a.experts / a.groups;
+        uint32_t group[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) group[i] = (lane * NV + i) / each;
+        float of_group = -INFINITY;
+        for (uint32_t g = 0; g < a.groups; ++g) {
+            float m = -INFINITY;
+            uint32_t at = NV;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const bool more = group[i] == g && key[i] > m;
+                m = more ? key[i] : m;
+                at = more ? i : at;
+            }
+            const float best = wave_max(m);
+            float s = best;
+            if (a.bias != nullptr && best > -INFINITY) {  // and the second largest
+                const bool first = lane == static_cast<uint32_t>(__builtin_ctzll(__ballot(m == best)));
+                m = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (group[i] == g && !(first && at == static_cast<uint32_t>(i))) m = fmaxf(m, key[i]);
+                const float next = wave_max(m);
+                s = next > -INFINITY ? best + next : best;
+            }
+            of_group = lane == g ? s : of_group;
+        }
+        uint64_t chosen = 0;
+        bool taken = lane >= a.groups;
+        for (uint32_t j = 0; j < a.kept; ++j) {
+            const float best = wave_max(taken ? -INFINITY : of_group);
+            const uint64_t at = __ballot(!taken && of_group == best);
+            if (at == 0) break;
+            const int g = __builtin_ctzll(at);
+            chosen |= 1ull << g;
+            taken |= lane == static_cast<uint32_t>(g);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) key[i] = group[i] < 64 && ((chosen >> group[i]) & 1) ? key[i] : -INFINITY;
+    }
+    int32_t id = -1;
+    float mine = 0.0f, total = 0.0f;
+    for (uint32_t j = 0; j < a.k; ++j) {
+        float m = key[0], s = score[0];
+        uint32_t at = 0;
+#pragma unroll
+        for (int i = 1; i < NV; ++i) {
+            const bool more = key[i] > m;
+            m = more ? key[i] : m;
+            s = more ? score[i] : s;
+            at = more ? i : at;
+        }
+        const float best = wave_max(m);
+        if (!(best > -INFINITY)) break;  // uniform: no expert is left
+        const int from = __builtin_ctzll(__ballot(m == best));
+        const float w = from_lane(s, from);
+        const int32_t e = from * NV + __builtin_amdgcn_readlane(static_cast<int>(at), from);
+        total += w;
+        id = lane == j ? e : id;
+        mine = lane == j ? w : mine;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) key[i] = lane == static_cast<uint32_t>(from) && at == static_cast<uint32_t>(i) ? -INFINITY : key[i];
+    }
+    if (lane < a.k) {
+        ids[t * a.k + lane] = id;
+        weights[t * a.k + lane] = (a.renorm ? mine / fmaxf(total, FLT_MIN) : mine) * a.scale;
+    }
+}
+
+// d logits from d weights.  Lane j forms the score of the token's j-th expert
+// again from its own logit; with w_j = scale s_j / S the scores' gradient is
+// (g_j - sum g w / scale) / S, g = scale dw, and the scores' own rule follows.
+template <Mx4Type T, int NV>
+__global__ __launch_bounds__(256) void moe_route_backward_kernel(RouteArgs a, const int32_t *__restrict__ ids,
+                                                                 const float *__restrict__ d_weights,
+                                                                 void *__restrict__ d_logits, uint64_t ldd) {
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t t = static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (t >= a.tokens) return;
+    float x[NV], score[NV], top = 0.0f, sum = 1.0f;
+    load_logits<T, NV>(a, t, lane, x);
+    if (a.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) score[i] = sigmoid_of(x[i]);
+    } else {
+        softmax_of<NV>(x, score, top, sum);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) score[i] /= sum;
+    }
+    int32_t id = lane < a.k ? ids[t * a.k + lane] : -1;
+    float s = 0.0f, d = 0.0f;
+    if (static_cast<uint32_t>(id) < a.experts) {
+        const float v = load_value<T>(a.logits, t * a.ld + id);
+        if (v > kLowest<T>) {
+            const float c = fminf(v, FLT_MAX);
+            s = a.sigmoid ? sigmoid_of(c) : expf(c - top) / sum;
+            d = d_weights[t * a.k + lane] * a.scale;
+        } else {
+            id = -1;
+        }
+    }
+    if (a.renorm) {
+        const float total = fmaxf(wave_sum(s), FLT_MIN);
+        const float mean = wave_sum(d * (s / total));
+        d = static_cast<uint32_t>(id) < a.experts ? (d - mean) / total : 0.0f;
+    }
+    const float mean = a.sigmoid ? 0.0f : wave_sum(d * s);
+    float g[NV] = {};
+    for (uint32_t j = 0; j < a.k; ++j) {
+        const uint32_t e = static_cast<uint32_t>(__builtin_amdgcn_readlane(id, static_cast<int>(j)));
+        const float v = from_lane(d, static_cast<int>(j));
+#pragma unroll
+        for (int i = 0; i < NV; ++i) g[i] += lane * NV + i == e ? v : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const uint32_t e = lane * NV + i;
+        if (e >= a.experts) continue;
+        // 1 - sigmoid(x) = sigmoid(-x), without the difference
+        const float v = a.sigmoid ? g[i] * score[i] * sigmoid_of(-x[i]) : score[i] * (g[i] - mean);
+        store_value<T>(d_logits, t * ldd + e, x[i] > -INFINITY ? v : 0.0f);
+    }
+}
+
+// Pairs in the experts' order, the pairs of one expert by their number; those
+// of no expert last.  Workgroup e counts the pairs of lower experts and its own
+// (each wave a contiguous share), then writes its own in order: two reads of
+// the ids from cache a workgroup, no workspace and no atomics.
+__global__ void moe_plan_kernel(const int32_t *__restrict__ ids, uint32_t pairs, uint32_t experts,
+                                int32_t *__restrict__ offsets, int32_t *__restrict__ order) {
+    __shared__ uint32_t lower[16], own[16];
+    const uint32_t e = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const uint32_t share = ((pairs + waves - 1) / waves + 63) / 64 * 64;
+    const uint32_t from = min(wave * share, pairs), to = min(from + share, pairs);
+    auto expert = [&](uint32_t p) {
+        const uint32_t v = static_cast<uint32_t>(ids[p]);
+        return v < experts ? v : experts;
+    };
+    uint32_t lt = 0, eq = 0;
+    for (uint32_t p = from + lane; p < to; p += 64) {
+        const uint32_t v = expert(p);
+        lt += v < e;
+        eq += v == e;
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        lt += __shfl_xor(lt, d);
+        eq += __shfl_xor(eq, d);
+    }
+    if (lane == 0) {
+        lower[wave] = lt;
+        own[wave] = eq;
+    }
+    __syncthreads();
+    uint32_t begin = 0, at = 0;
+    for (uint32_t w = 0; w < waves; ++w) {
+        begin += lower[w];
+        at += w < wave ? own[w] : 0u;
+    }
+    if (threadIdx.x == 0) offsets[e] = static_cast<int32_t>(begin);
+    at += begin;
+    for (uint32_t p0 = from; p0 < to; p0 += 64) {
+        const uint32_t p = p0 + lane;
+        const bool mine = p < to && expert(p) == e;
+        const uint64_t who = __ballot(mine);
+        if (mine) order[at + __builtin_popcountll(who & ((1ull << lane) - 1))] = static_cast<int32_t>(p);
+        at += __builtin_popcountll(who);
+    }
+}
+
+// Eight consecutive values in FP32
+template <Mx4Type T>
+__device__ __forceinline__ void load8(const void *base, uint64_t at, uint32_t valid, float v[8]) {
+    if (valid >= 8) {
+        if constexpr (T == Mx4Type::F32) {
+            __builtin_memcpy(v, static_cast<const float *>(base) + at, 32);
+        } else {
+            uint32_t w[4];
+            __builtin_memcpy(w, static_cast<const uint16_t *>(base) + at, 16);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t b = (w[i / 2] >> (16 * (i & 1))) & 0xFFFFu;
+                v[i] = T == Mx4Type::BF16 ? bf16_value(b) : f16_value(b);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = static_cast<uint32_t>(i) < valid ? load_value<T>(base, at + i) : 0.0f;
+    }
+}
+template <Mx4Type T>
+__device__ __forceinline__ void store8(void *base, uint64_t at, uint32_t valid, const float v[8]) {
+    if (valid >= 8) {
+        if constexpr (T == Mx4Type::F32) {
+            __builtin_memcpy(static_cast<float *>(base) + at, v, 32);
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (T == Mx4Type::BF16) w[i] = bf16_bits(v[2 * i]) | (bf16_bits(v[2 * i + 1]) << 16);
+                else w[i] = f16_bits(v[2 * i]) | (f16_bits(v[2 * i + 1]) << 16);
+            }
+            __builtin_memcpy(static_cast<uint16_t *>(base) + at, w, 16);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (static_cast<uint32_t>(i) < valid) store_value<T>(base, at + i, v[i]);
+    }
+}
+
+// out[t] = sum over the token's experts of weight * y, in the pairs' order; a
+// lane takes eight columns.
+template <Mx4Type Y, Mx4Type O>
+__global__ __launch_bounds__(256) void moe_combine_kernel(const void *__restrict__ y, uint64_t tokens, uint32_t k,
+                                                          uint32_t cols, uint32_t chunks,
+                                                          const int32_t *__restrict__ ids,
+                                                          const float *__restrict__ weights, uint32_t experts,
+                                                          void *__restrict__ out, uint64_t ld) {
+    const uint64_t item = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const uint64_t t = item / chunks;
+    if (t >= tokens) return;
+    const uint32_t c = 8 * static_cast<uint32_t>(item - t * chunks), valid = cols - c;
+    float sum[8] = {};
+    for (uint32_t j = 0; j < k; ++j) {
+        const uint64_t p = t * k + j;
+        if (static_cast<uint32_t>(ids[p]) >= experts) continue;
+        const float w = weights[p];
+        float v[8];
+        load8<Y>(y, p * cols + c, valid, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] = __builtin_fmaf(w, v[i], sum[i]);
+    }
+    store8<O>(out, t * ld + c, valid, sum);
+}
+
+// d weights: a wave takes a pair's dot product with the token's d out.
+template <Mx4Type Y, Mx4Type D>
+__global__ __launch_bounds__(256) void moe_weights_backward_kernel(const void *__restrict__ y, uint64_t pairs, uint32_t k,
+                                                                   uint32_t cols, const int32_t *__restrict__ ids,
+                                                                   uint32_t experts, const void *__restrict__ d_out,
+                                                                   uint64_t ld, float *__restrict__ d_weights) {
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t p = static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (p >= pairs) return;
+    float sum = 0.0f;
+    if (static_cast<uint32_t>(ids[p]) < experts) {
+        const uint64_t t = p / k;
+        for (uint32_t c = 8 * lane; c < cols; c += 512) {
+            float a[8], b[8];
+            load8<Y>(y, p * cols + c, cols - c, a);
+            load8<D>(d_out, t * ld + c, cols - c, b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(a[i], b[i], sum);
+        }
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) d_weights[p] = sum;
+}
+
+template <class F>
+void by_experts(uint32_t experts, F &&f) {
+    if (experts <= 64) f(std::integral_constant<int, 1>{});
+    else if (experts <= 128) f(std::integral_constant<int, 2>{});
+    else if (experts <= 256) f(std::integral_constant<int, 4>{});
+    else if (experts <= 512) f(std::integral_constant<int, 8>{});
+    else f(std::integral_constant<int, 16>{});
+}
+
+RouteArgs route_args(const void *logits, uint64_t tokens, uint32_t experts, uint64_t ld, const float *bias, int scoring,
+                     Mx4Type type, uint32_t groups, uint32_t kept, uint32_t k, int renorm, float scale) {
+    BSQ_REQUIRE(experts >= 1 && experts <= kMaxExperts, "moe route: 1 to 1024 experts");
+    BSQ_REQUIRE(k >= 1 && k <= kMaxChosen && k <= experts, "moe route: 1 to 64 experts a token, at most all of them");
+    BSQ_REQUIRE(scoring == 0 || scoring == 1, "moe route: scoring is 0 (softmax) or 1 (sigmoid)");
+    BSQ_REQUIRE(groups >= 1 && groups <= kMaxGroups && experts % groups == 0, "moe route: groups (1 to 64) divide the experts");
+    BSQ_REQUIRE(kept >= 1 && kept <= groups, "moe route: 1 to all groups are kept");
+    BSQ_REQUIRE(ld >= experts, "moe route: rows overlap");
+    BSQ_REQUIRE(tokens <= 0x7FFFFFFFull, "moe route: too many tokens");
+    if (tokens > 0) check_dense(logits, type, "moe route: null logits");
+    return {logits, bias, tokens, ld, experts, k, groups, kept, scoring, renorm != 0, scale};
+}
+
+void plan(const int32_t *ids, uint64_t pairs, uint32_t experts, int32_t *offsets, int32_t *order, hipStream_t stream) {
+    const unsigned threads = pairs > 4096 ? 1024 : 256;
+    moe_plan_kernel<<<experts + 1, threads, 0, stream>>>(ids, static_cast<uint32_t>(pairs), experts, offsets, order);
+    BSQ_HIP(hipGetLastError());
+}
+
+void combine(const void *y, Mx4Type y_type, uint64_t tokens, uint32_t k, uint32_t cols, const int32_t *ids,
+             const float *weights, uint32_t experts, void *out, Mx4Type type, uint64_t ld, hipStream_t stream) {
+    if (tokens == 0 || cols == 0) return;
+    const uint32_t chunks = static_cast<uint32_t>(ceil_div(cols, 8));
+    const uint64_t grid = ceil_div(tokens * chunks, 256);
+    BSQ_REQUIRE(grid <= 0x7FFFFFFFull, "moe combine: too large");
+    by_type(y_type, [&](auto ty) {
+        by_type(type, [&](auto to) {
+            moe_combine_kernel<decltype(ty)::value, decltype(to)::value><<<static_cast<unsigned>(grid), 256, 0, stream>>>(
+                y, tokens, k, cols, chunks, ids, weights, experts, out, ld);
+        });
+    });
+    BSQ_HIP(hipGetLastError());
+}
+
+void weights_backward(const void *y, Mx4Type y_type, uint64_t tokens, uint32_t k, uint32_t cols, const int32_t *ids,
+                      uint32_t experts, const void *d_out, Mx4Type type, uint64_t ld, float *d_weights,
+                      hipStream_t stream) {
+    const uint64_t pairs = tokens * k;
+    if (pairs == 0) return;
+    by_type(y_type, [&](auto ty) {
+        by_type(type, [&](auto td) {
+            moe_weights_backward_kernel<decltype(ty)::value, decltype(td)::value>
+                <<<static_cast<unsigned>(ceil_div(pairs, 4)), 256, 0, stream>>>(y, pairs, k, cols, ids, experts, d_out, ld,
+                                                                               d_weights);
+        });
+    });
+    BSQ_HIP(hipGetLastError());
+}
+
+// Pieces of a workspace, in order.
+struct Arena {
+    uint8_t *at;
+    uint64_t left;
+    uint8_t *take(uint64_t bytes) {
+        bytes = round256(bytes);
+        BSQ_REQUIRE(bytes <= left, "moe: workspace too small");
+        uint8_t *p = at;
+        at += bytes;
+        left -= bytes;
+        return p;
+    }
+};
+
+void check_layer(uint64_t tokens, uint32_t k, uint64_t n, uint64_t inputs, uint32_t experts) {
+    BSQ_REQUIRE(experts >= 1 && experts <= kMaxExperts, "moe linear: 1 to 1024 experts");
+    BSQ_REQUIRE(k >= 1 && k <= kMaxChosen, "moe linear: 1 to 64 experts a token");
+    BSQ_REQUIRE(tokens <= 0x7FFFFFFFull / k, "moe linear: too many tokens");
+    BSQ_REQUIRE(n >= 1 && inputs >= 1 && n <= (1u << 22) && inputs <= (1u << 22), "moe linear: 1 to 2^22 inputs and outputs");
+}
+uint64_t slot_slices(uint64_t pairs, uint32_t experts) { return pairs / kMx4Slice + std::min<uint64_t>(pairs, experts); }
+
+}  // namespace
+}  // namespace bsq
+
+using namespace bsq;
+
+extern "C" {
+
+int bsq_moe_route(const void *d_logits, int type, uint64_t tokens, uint32_t experts, uint64_t ld, const float *d_bias,
+                  int scoring, uint32_t groups, uint32_t kept, uint32_t k, int renormalise, float scale, int32_t *d_ids,
+                  float *d_weights, void *stream) {
+    return entry([&] {
+        const Mx4Type t = type_of(type);
+        const RouteArgs a = route_args(d_logits, tokens, experts, ld, d_bias, scoring, t, groups, kept, k, renormalise, scale);
+        if (tokens == 0) return;
+        BSQ_REQUIRE(d_ids != nullptr && d_weights != nullptr, "moe route: null output");
+        by_type(t, [&](auto ty) {
+            by_experts(experts, [&](auto nv) {
+                moe_route_kernel<decltype(ty)::value, decltype(nv)::value>
+                    <<<static_cast<unsigned>(ceil_div(tokens, 4)), 256, 0, static_cast<hipStream_t>(stream)>>>(a, d_ids,
+                                                                                                            d_weights);
+            });
+        });
+        BSQ_HIP(hipGetLastError());
+    });
+}
+
+int bsq_moe_route_backward(const void *d_logits, int type, uint64_t tokens, uint32_t experts, uint64_t ld, int scoring,
+                           uint32_t k, int renormalise, float scale, const int32_t *d_ids, const float *d_d_weights,
+                           void *d_d_logits, uint64_t ldd, void *stream) {
+    return entry([&] {
+        const Mx4Type t = type_of(type);
+        const RouteArgs a = route_args(d_logits, tokens, experts, ld, nullptr, scoring, t, 1, 1, k, renormalise, scale);
+        BSQ_REQUIRE(ldd >= experts, "moe route: rows overlap");
+        if (tokens == 0) return;
+        BSQ_REQUIRE(d_ids != nullptr && d_d_weights != nullptr, "moe route: null argument");
+        check_dense(d_d_logits, t, "moe route: null gradient");
+        by_type(t, [&](auto ty) {
+            by_experts(experts, [&](auto nv) {
+                moe_route_backward_kernel<decltype(ty)::value, decltype(nv)::value>
+                    <<<static_cast<unsigned>(ceil_div(tokens, 4)), 256, 0, static_cast<hipStream_t>(stream)>>>(
+                        a, d_ids, d_d_weights, d_d_logits, ldd);
+            });
+        });
+        BSQ_HIP(hipGetLastError());
+    });
+}
+
+int bsq_moe_plan(const int32_t *d_ids, uint64_t pairs, uint32_t experts, int32_t *d_offsets, int32_t *d_order,
+                 void *stream) {
+    return entry([&] {
+        BSQ_REQUIRE(experts >= 1 && experts <= kMaxExperts, "moe plan: 1 to 1024 experts");
+        BSQ_REQUIRE(pairs <= 0x7FFFFFFFull, "moe plan: too many pairs");
+        BSQ_REQUIRE(d_offsets != nullptr && (pairs == 0 || (d_ids != nullptr && d_order != nullptr)), "moe plan: null argument");
+        plan(d_ids, pairs, experts, d_offsets, d_order, static_cast<hipStream_t>(stream));
+    });
+}
+
+int bsq_moe_combine(const void *d_y, int y_type, uint64_t tokens, uint32_t k, uint64_t n, const int32_t *d_ids,
+                    const float *d_weights, uint32_t experts, void *d_out, int type, uint64_t ld, void *stream) {
+    return entry([&] {
+        const Mx4Type ty = type_of(y_type), t = type_of(type);
+        check_layer(tokens, k, n, 1, experts);
+        BSQ_REQUIRE(ld >= n, "moe combine: rows overlap");
+        if (tokens == 0) return;
+        BSQ_REQUIRE(d_ids != nullptr && d_weights != nullptr, "moe combine: null argument");
+        check_dense(d_y, ty, "moe combine: null argument");
+        check_dense(d_out, t, "moe combine: null output");
+        combine(d_y, ty, tokens, k, static_cast<uint32_t>(n), d_ids, d_weights, experts, d_out, t, ld,
+                static_cast<hipStream_t>(stream));
+    });
+}
+
+uint64_t bsq_moe_linear_workspace(uint64_t tokens, uint32_t k, uint64_t n, uint64_t inputs, uint32_t experts) {
+    (void)k;
+    (void)n;
+    (void)experts;
+    return packed_bytes(tokens, mx4_slices(inputs));
+}
+
+int bsq_moe_linear(const void *d_x, int x_type, uint64_t tokens, uint64_t inputs, uint64_t ldx, const int32_t *d_ids,
+                   const float *d_weights, uint32_t k, const uint8_t *d_w_codes, const uint8_t *d_w_scales,
+                   uint32_t experts, uint64_t n, int32_t *d_offsets, int32_t *d_order, void *d_y, int y_type, void *d_out,
+                   int out_type, uint64_t ldo, void *d_work, uint64_t work_bytes, void *stream) {
+    return entry([&] {
+        const Mx4Type tx = type_of(x_type), ty = type_of(y_type), to = type_of(out_type);
+        check_layer(tokens, k, n, inputs, experts);
+        BSQ_REQUIRE(ldx >= inputs && ldo >= n, "moe linear: rows overlap");
+        BSQ_REQUIRE(d_offsets != nullptr, "moe linear: null argument");
+        hipStream_t s = static_cast<hipStream_t>(stream);
+        const uint64_t pairs = tokens * k;
+        if (pairs > 0) {
+            BSQ_REQUIRE(d_ids != nullptr && d_weights != nullptr && d_order != nullptr, "moe linear: null argument");
+            check_dense(d_x, tx, "moe linear: null input");
+            check_dense(d_y, ty, "moe linear: null y");
+            check_dense(d_out, to, "moe linear: null output");
+            check_packed(d_w_codes, d_w_scales);
+            check_work(d_work, work_bytes, bsq_moe_linear_workspace(tokens, k, n, inputs, experts));
+        }
+        plan(d_ids, pairs, experts, d_offsets, d_order, s);
+        if (pairs == 0) return;
+        const uint32_t slices = static_cast<uint32_t>(mx4_slices(inputs));
+        Arena arena{static_cast<uint8_t *>(d_work), work_bytes};
+        uint8_t *codes = arena.take(tokens * slices * 128), *scales = arena.take(tokens * slices * 8);
+        launch_mx4_encode(d_x, tx, 1, tokens, inputs, ldx, 0, codes, scales, nullptr, nullptr, s);
+        Mx4Product p;
+        p.a = {codes, scales};
+        p.b = {d_w_codes, d_w_scales};
+        p.M = static_cast<uint32_t>(pairs);
+        p.N = static_cast<uint32_t>(n);
+        p.slices = slices;
+        p.out = d_y;
+        p.type = ty;
+        p.ld = n;
+        p.offsets = d_offsets;
+        p.order = d_order;
+        p.experts = experts;
+        p.per_token = k;
+        launch_mx4_product(p, nullptr, 0, s);
+        combine(d_y, ty, tokens, k, static_cast<uint32_t>(n), d_ids, d_weights, experts, d_out, to, ldo, s);
+    });
+}
+
+uint64_t bsq_moe_linear_backward_workspace(uint64_t tokens, uint32_t k, uint64_t n, uint64_t inputs, uint32_t experts) {
+    const uint64_t slots = slot_slices(tokens * k, experts);
+    return std::max(packed_bytes(tokens, mx4_slices(n)) + round256(tokens * k * inputs * 4),
+                    packed_bytes(n, slots) + packed_bytes(inputs, slots));
+}
+
+int bsq_moe_linear_backward(const void *d_d_out, int d_type, uint64_t tokens, uint64_t n, uint64_t ldd, const void *d_x,
+                            int x_type, uint64_t inputs, uint64_t ldx, const int32_t *d_ids, const float *d_weights,
+                            uint32_t k, const int32_t *d_offsets, const int32_t *d_order, const void *d_y, int y_type,
+                            const uint8_t *d_wt_codes, const uint8_t *d_wt_scales, uint32_t experts, void *d_dx,
+                            uint64_t lddx, float *d_d_weights, void *d_dw, int g_type, void *d_work, uint64_t work_bytes,
+                            void *stream) {
+    return entry([&] {
+        const Mx4Type td = type_of(d_type), tx = type_of(x_type), ty = type_of(y_type), tg = type_of(g_type);
+        check_layer(tokens, k, n, inputs, experts);
+        BSQ_REQUIRE(ldd >= n && ldx >= inputs && lddx >= inputs, "moe linear: rows overlap");
+        const uint64_t pairs = tokens * k;
+        BSQ_REQUIRE(d_offsets != nullptr, "moe linear: null argument");
+        if (pairs > 0) {
+            check_dense(d_d_out, td, "moe linear: null gradient");
+            BSQ_REQUIRE(d_ids != nullptr && d_weights != nullptr && d_order != nullptr, "moe linear: null argument");
+            BSQ_REQUIRE(d_dx == nullptr || (d_wt_codes != nullptr && d_wt_scales != nullptr), "moe linear: dx needs the weights' columns");
+            BSQ_REQUIRE(d_d_weights == nullptr || d_y != nullptr, "moe linear: the weights' gradient needs y");
+            BSQ_REQUIRE(d_dw == nullptr || d_x != nullptr, "moe linear: dw needs x");
+            if (d_dx) check_packed(d_wt_codes, d_wt_scales);
+            if (d_dx) check_dense(d_dx, tg, "");
+            if (d_d_weights) check_dense(d_y, ty, "");
+            if (d_dw) check_dense(d_x, tx, "");
+            check_work(d_work, work_bytes, bsq_moe_linear_backward_workspace(tokens, k, n, inputs, experts));
+        }
+        if (d_dw) check_dense(d_dw, tg, "");
+        hipStream_t s = static_cast<hipStream_t>(stream);
+        if (pairs > 0 && d_dx != nullptr) {
+            // dx[t] = sum of weight * (q(d out[t]) W_e): the layer itself, with
+            // the weights' columns for their rows
+            const uint32_t slices = static_cast<uint32_t>(mx4_slices(n));
+            Arena arena{static_cast<uint8_t *>(d_work), work_bytes};
+            uint8_t *codes = arena.take(tokens * slices * 128), *scales = arena.take(tokens * slices * 8);
+            uint8_t *z = arena.take(pairs * inputs * type_bytes(tg));
+            launch_mx4_encode(d_d_out, td, 1, tokens, n, ldd, 0, codes, scales, nullptr, nullptr, s);
+            Mx4Product p;
+            p.a = {codes, scales};
+            p.b = {d_wt_codes, d_wt_scales};
+            p.M = static_cast<uint32_t>(pairs);
+            p.N = static_cast<uint32_t>(inputs);
+            p.slices = slices;
+            p.out = z;
+            p.type = tg;
+            p.ld = inputs;
+            p.offsets = d_offsets;
+            p.order = d_order;
+            p.experts = experts;
+            p.per_token = k;
+            launch_mx4_product(p, nullptr, 0, s);
+            combine(z, tg, tokens, k, static_cast<uint32_t>(inputs), d_ids, d_weights, experts, d_dx, tg, lddx, s);
+        }
+        if (pairs > 0 && d_d_weights != nullptr)
+            weights_backward(d_y, ty, tokens, k, static_cast<uint32_t>(n), d_ids, experts, d_d_out, td, ldd, d_d_weights, s);
+        if (d_dw != nullptr) {
+            // dw[e] = the sum over the expert's pairs of q(weight d out)^T q(x),
+            // both rounded in blocks of 32 pairs
+            const uint64_t slots = slot_slices(pairs, experts);
+            Arena arena{static_cast<uint8_t *>(d_work), work_bytes};
+            uint8_t *gc = arena.take(n * slots * 128), *gs = arena.take(n * slots * 8);
+            uint8_t *xc = arena.take(inputs * slots * 128), *xs = arena.take(inputs * slots * 8);
+            Mx4Slots of{d_offsets, d_order, d_weights, experts, k};
+            launch_mx4_encode_slots(d_d_out, td, n, ldd, of, slots, gc, gs, s);
+            of.weights = nullptr;
+            launch_mx4_encode_slots(d_x, tx, inputs, ldx, of, slots, xc, xs, s);
+            Mx4Product p;
+            p.a = {gc, gs};
+            p.b = {xc, xs};
+            p.M = static_cast<uint32_t>(n);
+            p.N = static_cast<uint32_t>(inputs);
+            p.slices = static_cast<uint32_t>(slots);
+            p.out = d_dw;
+            p.type = tg;
+            p.ld = inputs;
+            p.offsets = d_offsets;
+            p.experts = experts;
+            p.shared_slots = true;
+            launch_mx4_product(p, nullptr, 0, s);
+        }
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,538 @@
+// MX4 encode and decode (mx4.hpp).
+#include "mx4.hpp"
+
+#include <algorithm>
+#include <type_traits>
+
+#include <bitsqz_llm_c.h>
+
+namespace bsq {
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kThreads = 256;
+
+// Eight consecutive values in their own type.
+template <Mx4Type T>
+struct Eight {
+    static constexpr int kWords = T == Mx4Type::F32 ? 8 : 4;
+    uint32_t w[kWords];
+
+    // values [at, at + 8) of a row of n, zeros past its end; any alignment of
+    // the element's own size
+    __device__ __forceinline__ void load(const uint8_t *row, uint64_t at, uint64_t n) {
+        constexpr int size = T == Mx4Type::F32 ? 4 : 2;
+        if (at + 8 <= n) {
+            __builtin_memcpy(w, row + at * size, 8 * size);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (at + i >= n) continue;
+                if constexpr (T == Mx4Type::F32) w[i] = reinterpret_cast<const uint32_t *>(row)[at + i];
+                else w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(row)[at + i]) << (16 * (i & 1));
+            }
+        }
+    }
+    // bits of the largest magnitude, in the type's own format (they order as
+    // the magnitudes do, infinity and NaN above all)
+    __device__ __forceinline__ uint32_t top() const {
+        if constexpr (T == Mx4Type::F32) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+            return m;
+        } else {
+            u16x2 m = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu));
+            return max(static_cast<uint32_t>(m[0]), static_cast<uint32_t>(m[1]));
+        }
+    }
+    // the eight codes over `scale`
+    __device__ __forceinline__ uint32_t codes(float scale) const {
+        uint32_t c = 0;
+        if constexpr (T == Mx4Type::F32) {
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(w[0]), __uint_as_float(w[1]), scale, 0);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(w[2]), __uint_as_float(w[3]), scale, 1);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(w[4]), __uint_as_float(w[5]), scale, 2);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(w[6]), __uint_as_float(w[7]), scale, 3);
+        } else if constexpr (T == Mx4Type::BF16) {
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, w[0]), scale, 0);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, w[1]), scale, 1);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, w[2]), scale, 2);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, w[3]), scale, 3);
+        } else {
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, w[0]), scale, 0);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, w[1]), scale, 1);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, w[2]), scale, 2);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, w[3]), scale, 3);
+        }
+        return c;
+    }
+};
+
+// the type's magnitude bits as FP32's
+template <Mx4Type T>
+__device__ __forceinline__ uint32_t f32_bits(uint32_t top) {
+    if constexpr (T == Mx4Type::F32) return top;
+    if constexpr (T == Mx4Type::BF16) return top << 16;
+    return __float_as_uint(f16_value(top));
+}
+
+// max over each aligned quad of lanes
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xB1, 0xF, 0xF, true)));
+    return max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x4E, 0xF, 0xF, true)));
+}
+
+// Rows to MX4.  A lane takes eight consecutive values, a quad of lanes a
+// block; loads are 16 bytes a lane (twice for FP32), a wave's codes 256
+// consecutive bytes.
+template <Mx4Type T>
+__global__ __launch_bounds__(kThreads) void mx4_encode_rows_kernel(const uint8_t *__restrict__ x, uint64_t rows,
+                                                                   uint64_t cols, uint64_t ld, uint64_t stride,
+                                                                   uint64_t total, uint32_t chunks,
+                                                                   uint8_t *__restrict__ codes,
+                                                                   uint8_t *__restrict__ scales) {
+    constexpr int size = T == Mx4Type::F32 ? 4 : 2;
+    const uint64_t all = total * chunks;  // a multiple of 32 a row: quads never part
+    for (uint64_t t = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x; t < all;
+         t += static_cast<uint64_t>(gridDim.x) * kThreads) {
+        const uint64_t r = t / chunks, c = t - r * chunks, b = r / rows;
+        Eight<T> v;
+        v.load(x + (b * stride + (r - b * rows) * ld) * size, 8 * c, cols);
+        const uint32_t byte = mx4_scale_byte(f32_bits<T>(quad_max(v.top())));
+        const uint32_t q = byte == 255u ? 0u : v.codes(mx4_power(byte));
+        reinterpret_cast<uint32_t *>(codes)[t] = q;
+        if ((c & 3) == 0) scales[t >> 2] = static_cast<uint8_t>(byte);
+    }
+}
+
+// Columns to MX4, and the rows too if asked.  A workgroup takes a tile of 128
+// rows and 64 words of each: 16 lanes load a row's part (and encode its blocks
+// from registers), the tile goes to LDS, and a lane then takes one block of 32
+// rows of a word's column (two columns of a 16-bit type); the four lanes of a
+// column's four blocks are neighbours, so that their codes are 64 consecutive
+// bytes.  Row r of the tile lies 16 words further along for each block of 32
+// rows before it: sixteen columns of four blocks then read all 64 banks.
+// SLOTS: the rows are those of the experts' slots.  WEIGHTED: each times its
+// weight, staged in FP32, so that a value is rounded once.
+constexpr int kTileRows = 128;
+constexpr int kTileWords = 64;
+
+template <Mx4Type T, bool WEIGHTED>
+constexpr int kTileCols = T == Mx4Type::F32 || WEIGHTED ? 64 : 128;
+
+template <Mx4Type T, bool SLOTS, bool WEIGHTED>
+__global__ __launch_bounds__(kThreads) void mx4_encode_tile_kernel(const uint8_t *__restrict__ x, uint64_t rows,
+                                                                   uint64_t cols, uint64_t ld, uint64_t stride,
+                                                                   uint32_t tiles_c, uint32_t tiles_r,
+                                                                   uint32_t slices_c, uint32_t slices_r, Mx4Slots slots,
+                                                                   uint8_t *__restrict__ codes,
+                                                                   uint8_t *__restrict__ scales,
+                                                                   uint8_t *__restrict__ codes_t,
+                                                                   uint8_t *__restrict__ scales_t) {
+    constexpr Mx4Type S = WEIGHTED ? Mx4Type::F32 : T;  // as staged
+    constexpr int size = T == Mx4Type::F32 ? 4 : 2, kCols = kTileCols<T, WEIGHTED>, kPer = kCols / 16;
+    __shared__ __attribute__((aligned(16))) uint32_t tile[kTileRows * kTileWords + 4 * 16];
+    const int tid = threadIdx.x;
+    const uint32_t tc = blockIdx.x % tiles_c;
+    const uint64_t rest = blockIdx.x / tiles_c;
+    const uint32_t tr = static_cast<uint32_t>(rest % tiles_r);
+    const uint64_t b = rest / tiles_r;
+    const uint64_t c0 = static_cast<uint64_t>(tc) * kCols;
+    uint64_t r0 = static_cast<uint64_t>(tr) * kTileRows, r1 = rows;  // rows of the tile end at r1
+    if constexpr (SLOTS) {
+        // tile tr of the experts' slices, in halves: the expert it belongs to
+        uint32_t first = 0, e = 0;
+        for (; e < slots.experts; ++e) {
+            const uint32_t n = 2 * mx4_slot_slices(slots.offsets, e);
+            if (tr < first + n) break;
+            first += n;
+        }
+        if (e == slots.experts) return;  // uniform: past the last expert's slices
+        r0 = static_cast<uint64_t>(slots.offsets[e]) + static_cast<uint64_t>(tr - first) * kTileRows;
+        r1 = static_cast<uint64_t>(slots.offsets[e + 1]);
+    }
+    const int part = tid & 15;
+    const uint64_t c = c0 + part * kPer;
+#pragma unroll
+    for (int i = 0; i < kTileRows / 16; ++i) {
+        const int r = 16 * i + (tid >> 4);
+        const uint64_t row = r0 + r;
+        constexpr int kWords = kPer * size / 4;
+        uint32_t v[kWords] = {};
+        float w = 1.0f;
+        if (row < r1) {
+            const uint8_t *p = x + b * stride * size;
+            if constexpr (SLOTS) {
+                const uint32_t pair = static_cast<uint32_t>(slots.order[row]);
+                p += static_cast<uint64_t>(pair / slots.per_token) * ld * size;
+                if constexpr (WEIGHTED) w = slots.weights[pair];
+            } else {
+                p += row * ld * size;
+            }
+            if (c + kPer <= cols) {
+                __builtin_memcpy(v, p + c * size, sizeof v);
+            } else {
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) {
+                    if (c + k >= cols) continue;
+                    if constexpr (T == Mx4Type::F32) v[k] = reinterpret_cast<const uint32_t *>(p)[c + k];
+                    else v[k / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(p)[c + k]) << (16 * (k & 1));
+                }
+            }
+        }
+        u32x4 staged;
+        if constexpr (WEIGHTED) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float f;
+                if constexpr (T == Mx4Type::F32) f = __uint_as_float(v[k]);
+                else if constexpr (T == Mx4Type::BF16) f = bf16_value((v[k / 2] >> (16 * (k & 1))) & 0xFFFFu);
+                else f = f16_value((v[k / 2] >> (16 * (k & 1))) & 0xFFFFu);
+                staged[k] = __float_as_uint(f * w);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) staged[k] = v[k];
+            if (codes != nullptr) {  // uniform
+                uint32_t byte, q = 0;
+                if constexpr (T == Mx4Type::F32) {
+                    uint32_t m = 0;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) m = max(m, v[k] & 0x7FFFFFFFu);
+                    m = quad_max(m);
+                    m = max(m, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(m), 0x141, 0xF, 0xF, true)));
+                    byte = mx4_scale_byte(m);
+                    if (byte != 255u) {
+                        const float s = mx4_power(byte);
+                        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, __uint_as_float(v[0]), __uint_as_float(v[1]), s, 0);
+                        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, __uint_as_float(v[2]), __uint_as_float(v[3]), s, 1);
+                    }
+                } else {
+                    Eight<T> e8;
+                    __builtin_memcpy(e8.w, v, 16);
+                    byte = mx4_scale_byte(f32_bits<T>(quad_max(e8.top())));
+                    if (byte != 255u) q = e8.codes(mx4_power(byte));
+                }
+                if (row < rows) {
+                    const uint64_t at = (b * rows + row) * slices_c * kMx4Slice + c;  // padded element
+                    if constexpr (T == Mx4Type::F32) reinterpret_cast<uint16_t *>(codes)[at >> 2] = static_cast<uint16_t>(q);
+                    else reinterpret_cast<uint32_t *>(codes)[at >> 3] = q;
+                    if ((part & (32 / kPer - 1)) == 0) scales[at >> 5] = static_cast<uint8_t>(byte);
+                }
+            }
+        }
+        *reinterpret_cast<u32x4 *>(&tile[r * kTileWords + (r >> 5) * 16 + 4 * part]) = staged;
+    }
+    __syncthreads();
+    const int word = tid >> 2, blk = tid & 3;  // four lanes: the four blocks of a word's column
+    const uint32_t *p = &tile[blk * (32 * kTileWords + 16) + word];
+    uint32_t v[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = p[i * kTileWords];
+    constexpr int kSub = kCols / kTileWords;  // columns in a word
+#pragma unroll
+    for (int h = 0; h < kSub; ++h) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            if constexpr (S == Mx4Type::F32) m = max(m, v[i] & 0x7FFFFFFFu);
+            else m = max(m, (h ? v[i] >> 16 : v[i]) & 0x7FFFu);
+        }
+        const uint32_t byte = mx4_scale_byte(f32_bits<S>(m));
+        const float s = mx4_power(byte);
+        auto val = [&](int i) __attribute__((always_inline)) {
+            if constexpr (S == Mx4Type::F32) return __uint_as_float(v[i]);
+            else if constexpr (S == Mx4Type::BF16) return __uint_as_float(h ? v[i] & 0xFFFF0000u : v[i] << 16);
+            else return f16_value(h ? v[i] >> 16 : v[i] & 0xFFFFu);
+        };
+        u32x4 q = {0, 0, 0, 0};
+        if (byte != 255u) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t o = 0;
+                o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, val(8 * k), val(8 * k + 1), s, 0);
+                o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, val(8 * k + 2), val(8 * k + 3), s, 1);
+                o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, val(8 * k + 4), val(8 * k + 5), s, 2);
+                o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, val(8 * k + 6), val(8 * k + 7), s, 3);
+                q[k] = o;
+            }
+        }
+        const uint64_t col = c0 + static_cast<uint64_t>(word) * kSub + h;
+        if (col < cols) {
+            const uint64_t row = (b * cols + col) * slices_r;  // slices before this column
+            *reinterpret_cast<u32x4 *>(codes_t + row * 128 + static_cast<uint64_t>(tr) * 64 + blk * 16) = q;
+            scales_t[row * 8 + static_cast<uint64_t>(tr) * 4 + blk] = static_cast<uint8_t>(byte);
+        }
+    }
+}
+
+// Values of packed rows.  A lane takes eight codes; the level of a code times
+// its power of two is exact in FP32 and in BF16.
+template <Mx4Type T>
+__global__ __launch_bounds__(kThreads) void mx4_decode_kernel(const uint8_t *__restrict__ codes,
+                                                              const uint8_t *__restrict__ scales, uint64_t rows,
+                                                              uint64_t cols, uint64_t slices, uint32_t chunks,
+                                                              uint8_t *__restrict__ out, uint64_t ld) {
+    constexpr int size = T == Mx4Type::F32 ? 4 : 2;
+    const uint64_t all = rows * chunks;
+    for (uint64_t t = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x; t < all;
+         t += static_cast<uint64_t>(gridDim.x) * kThreads) {
+        const uint64_t r = t / chunks, c = t - r * chunks;
+        const uint32_t q = *reinterpret_cast<const uint32_t *>(codes + r * slices * 128 + 4 * c);
+        const uint32_t byte = scales[r * slices * 8 + (c >> 2)];
+        const float s = byte == 0u ? 0x1p-127f : mx4_power(byte);
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            // E2M1 read as the top of an E8M23 word: the exponent counts from
+            // 2^-126 there, the subnormal half among them
+            const uint32_t k = q >> (4 * i);
+            const float level = __uint_as_float(((k & 8u) << 28) | ((k & 7u) << 22)) * 0x1p126f;
+            v[i] = byte == 255u ? __builtin_nanf("") : level * s;
+        }
+        const uint64_t e = 8 * c;
+        uint8_t *p = out + (r * ld + e) * size;
+        if (e + 8 <= cols) {
+            uint32_t w[T == Mx4Type::F32 ? 8 : 4];
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                if constexpr (T == Mx4Type::F32) {
+                    w[i] = __float_as_uint(v[i]);
+                    w[i + 1] = __float_as_uint(v[i + 1]);
+                } else if constexpr (T == Mx4Type::BF16) {
+                    w[i / 2] = (__float_as_uint(v[i]) >> 16) | (__float_as_uint(v[i + 1]) & 0xFFFF0000u);
+                } else {
+                    w[i / 2] = f16_bits(v[i]) | (f16_bits(v[i + 1]) << 16);
+                }
+            }
+            __builtin_memcpy(p, w, 8 * size);
+        } else {
+            for (int i = 0; i < 8; ++i)
+                if (e + i < cols) store_value<T>(out, r * ld + e + i, v[i]);
+        }
+    }
+}
+
+unsigned grid_for(uint64_t items) {
+    return static_cast<unsigned>(std::min<uint64_t>(ceil_div(items, kThreads), 1u << 20));
+}
+
+}  // namespace
+
+void launch_mx4_encode(const void *x, Mx4Type type, uint64_t batch, uint64_t rows, uint64_t cols, uint64_t ld,
+                       uint64_t stride, uint8_t *codes, uint8_t *scales, uint8_t *codes_t, uint8_t *scales_t,
+                       hipStream_t stream) {
+    if (batch == 0 || rows == 0 || cols == 0 || (codes == nullptr && codes_t == nullptr)) return;
+    const uint32_t slices_c = static_cast<uint32_t>(mx4_slices(cols)), slices_r = static_cast<uint32_t>(mx4_slices(rows));
+    by_type(type, [&](auto t) {
+        constexpr Mx4Type T = decltype(t)::value;
+        const uint8_t *p = static_cast<const uint8_t *>(x);
+        if (codes_t == nullptr) {
+            const uint32_t chunks = slices_c * (kMx4Slice / 8);
+            mx4_encode_rows_kernel<T><<<grid_for(batch * rows * chunks), kThreads, 0, stream>>>(
+                p, rows, cols, ld, stride, batch * rows, chunks, codes, scales);
+        } else {
+            constexpr uint32_t kCols = kTileCols<T, false>;
+            // whole slices both ways, so that the padding is written too
+            const uint32_t tiles_c = slices_c * (kMx4Slice / kCols), tiles_r = 2 * slices_r;
+            const uint64_t grid = batch * tiles_c * tiles_r;
+            BSQ_REQUIRE(grid <= 0x7FFFFFFFull, "mx4 encode: matrix too large");
+            mx4_encode_tile_kernel<T, false, false><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(
+                p, rows, cols, ld, stride, tiles_c, tiles_r, slices_c, slices_r, Mx4Slots{}, codes, scales, codes_t,
+                scales_t);
+        }
+    });
+    BSQ_HIP(hipGetLastError());
+}
+
+void launch_mx4_encode_slots(const void *x, Mx4Type type, uint64_t cols, uint64_t ld, const Mx4Slots &slots,
+                             uint64_t slices, uint8_t *codes_t, uint8_t *scales_t, hipStream_t stream) {
+    if (slices == 0 || cols == 0) return;
+    by_type(type, [&](auto t) {
+        constexpr Mx4Type T = decltype(t)::value;
+        auto go = [&](auto weighted) {
+            constexpr bool W = decltype(weighted)::value;
+            const uint32_t tiles_c = static_cast<uint32_t>(ceil_div(cols, kTileCols<T, W>));
+            const uint64_t grid = 2 * slices * tiles_c;
+            BSQ_REQUIRE(grid <= 0x7FFFFFFFull, "mx4 encode: matrix too large");
+            mx4_encode_tile_kernel<T, true, W><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(
+                static_cast<const uint8_t *>(x), 0, cols, ld, 0, tiles_c, static_cast<uint32_t>(2 * slices), 0,
+                static_cast<uint32_t>(slices), slots, nullptr, nullptr, codes_t, scales_t);
+        };
+        if (slots.weights != nullptr) go(std::true_type{});
+        else go(std::false_type{});
+    });
+    BSQ_HIP(hipGetLastError());
+}
+
+void launch_mx4_decode(const uint8_t *codes, const uint8_t *scales, uint64_t rows, uint64_t cols, void *out,
+                       Mx4Type type, uint64_t ld, hipStream_t stream) {
+    if (rows == 0 || cols == 0) return;
+    by_type(type, [&](auto t) {
+        constexpr Mx4Type T = decltype(t)::value;
+        const uint32_t chunks = static_cast<uint32_t>(ceil_div(cols, 8));
+        mx4_decode_kernel<T><<<grid_for(rows * chunks), kThreads, 0, stream>>>(
+            codes, scales, rows, cols, mx4_slices(cols), chunks, static_cast<uint8_t *>(out), ld);
+    });
+    BSQ_HIP(hipGetLastError());
+}
+
+}  // namespace bsq
+
+using namespace bsq;
+
+namespace {
+
+constexpr uint64_t kMaxSide = 1ull << 31;
+void check_sides(uint64_t m, uint64_t n, uint64_t k) {
+    BSQ_REQUIRE(m < kMaxSide && n < kMaxSide && k <= (1u << 22), "mx4: up to 2^31 rows, 2^22 values a row");
+}
+uint64_t packed(uint64_t rows, uint64_t cols) { return packed_bytes(rows, mx4_slices(cols)); }
+
+void product(Mx4Matrix a, uint64_t m, Mx4Matrix b, uint64_t n, uint64_t k, void *out, Mx4Type type, uint64_t ld,
+             uint8_t *work, uint64_t work_bytes, hipStream_t stream) {
+    Mx4Product p;
+    p.a = a;
+    p.b = b;
+    p.M = static_cast<uint32_t>(m);
+    p.N = static_cast<uint32_t>(n);
+    p.slices = static_cast<uint32_t>(mx4_slices(k));
+    p.out = out;
+    p.type = type;
+    p.ld = ld;
+    launch_mx4_product(p, work, work_bytes, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t bsq_mx4_codes_bytes(uint64_t rows, uint64_t cols) { return rows * mx4_slices(cols) * 128; }
+uint64_t bsq_mx4_scales_bytes(uint64_t rows, uint64_t cols) { return rows * mx4_slices(cols) * 8; }
+
+int bsq_mx4_encode(const void *d_x, int type, uint64_t batch, uint64_t rows, uint64_t cols, uint64_t ld, uint64_t stride,
+                   uint8_t *d_codes, uint8_t *d_scales, uint8_t *d_codes_t, uint8_t *d_scales_t, void *stream) {
+    return entry([&] {
+        const Mx4Type t = type_of(type);
+        check_sides(rows, cols, std::max<uint64_t>(cols, d_codes_t ? rows : 0));
+        BSQ_REQUIRE(batch < kMaxSide, "mx4 encode: batch too large");
+        BSQ_REQUIRE(ld >= cols, "mx4 encode: rows overlap");
+        if (batch == 0 || rows == 0 || cols == 0) return;
+        check_dense(d_x, t, "mx4 encode: null input");
+        BSQ_REQUIRE(d_codes != nullptr || d_codes_t != nullptr, "mx4 encode: null output");
+        BSQ_REQUIRE((d_codes == nullptr) == (d_scales == nullptr) && (d_codes_t == nullptr) == (d_scales_t == nullptr),
+                    "mx4 encode: codes come with their scales");
+        if (d_codes) check_packed(d_codes, d_scales);
+        if (d_codes_t) check_packed(d_codes_t, d_scales_t);
+        launch_mx4_encode(d_x, t, batch, rows, cols, ld, stride, d_codes, d_scales, d_codes_t, d_scales_t,
+                          static_cast<hipStream_t>(stream));
+    });
+}
+
+int bsq_mx4_decode(const uint8_t *d_codes, const uint8_t *d_scales, uint64_t rows, uint64_t cols, void *d_out, int type,
+                   uint64_t ld, void *stream) {
+    return entry([&] {
+        const Mx4Type t = type_of(type);
+        check_sides(rows, cols, cols);
+        BSQ_REQUIRE(ld >= cols, "mx4 decode: rows overlap");
+        if (rows == 0 || cols == 0) return;
+        check_packed(d_codes, d_scales);
+        check_dense(d_out, t, "mx4 decode: null output");
+        launch_mx4_decode(d_codes, d_scales, rows, cols, d_out, t, ld, static_cast<hipStream_t>(stream));
+    });
+}
+
+uint64_t bsq_mx4_product_workspace(uint64_t m, uint64_t n, uint64_t k) {
+    return mx4_product_workspace(static_cast<uint32_t>(m), static_cast<uint32_t>(n), static_cast<uint32_t>(mx4_slices(k)));
+}
+
+int bsq_mx4_product(const uint8_t *d_a_codes, const uint8_t *d_a_scales, uint64_t m, const uint8_t *d_b_codes,
+                    const uint8_t *d_b_scales, uint64_t n, uint64_t k, void *d_out, int type, uint64_t ld, void *d_work,
+                    uint64_t work_bytes, void *stream) {
+    return entry([&] {
+        const Mx4Type t = type_of(type);
+        check_sides(m, n, k);
+        BSQ_REQUIRE(k >= 1, "mx4 product: no values to sum");
+        BSQ_REQUIRE(ld >= n, "mx4 product: rows overlap");
+        if (m == 0 || n == 0) return;
+        check_packed(d_a_codes, d_a_scales);
+        check_packed(d_b_codes, d_b_scales);
+        check_dense(d_out, t, "mx4 product: null output");
+        check_work(d_work, work_bytes, bsq_mx4_product_workspace(m, n, k));
+        product({d_a_codes, d_a_scales}, m, {d_b_codes, d_b_scales}, n, k, d_out, t, ld, static_cast<uint8_t *>(d_work),
+                work_bytes, static_cast<hipStream_t>(stream));
+    });
+}
+
+uint64_t bsq_mx4_linear_workspace(uint64_t m, uint64_t n, uint64_t k) {
+    return packed(m, k) + round256(bsq_mx4_product_workspace(m, n, k));
+}
+
+int bsq_mx4_linear(const void *d_x, int x_type, uint64_t m, uint64_t k, uint64_t ldx, const uint8_t *d_w_codes,
+                   const uint8_t *d_w_scales, uint64_t n, void *d_out, int out_type, uint64_t ldo, uint8_t *d_xt_codes,
+                   uint8_t *d_xt_scales, void *d_work, uint64_t work_bytes, void *stream) {
+    return entry([&] {
+        const Mx4Type tx = type_of(x_type), to = type_of(out_type);
+        check_sides(m, n, std::max<uint64_t>(k, d_xt_codes ? m : 0));
+        BSQ_REQUIRE(k >= 1, "mx4 linear: no inputs");
+        BSQ_REQUIRE(ldx >= k && ldo >= n, "mx4 linear: rows overlap");
+        if (m == 0 || n == 0) return;
+        check_dense(d_x, tx, "mx4 linear: null input");
+        check_dense(d_out, to, "mx4 linear: null output");
+        check_packed(d_w_codes, d_w_scales);
+        BSQ_REQUIRE((d_xt_codes == nullptr) == (d_xt_scales == nullptr), "mx4 linear: codes come with their scales");
+        if (d_xt_codes) check_packed(d_xt_codes, d_xt_scales);
+        check_work(d_work, work_bytes, bsq_mx4_linear_workspace(m, n, k));
+        hipStream_t s = static_cast<hipStream_t>(stream);
+        uint8_t *codes = static_cast<uint8_t *>(d_work), *scales = codes + round256(m * mx4_slices(k) * 128);
+        launch_mx4_encode(d_x, tx, 1, m, k, ldx, 0, codes, scales, d_xt_codes, d_xt_scales, s);
+        product({codes, scales}, m, {d_w_codes, d_w_scales}, n, k, d_out, to, ldo, codes + packed(m, k),
+                work_bytes - packed(m, k), s);
+    });
+}
+
+uint64_t bsq_mx4_linear_backward_workspace(uint64_t m, uint64_t n, uint64_t k) {
+    return packed(m, n) + packed(n, m) +
+           round256(std::max(bsq_mx4_product_workspace(m, k, n), bsq_mx4_product_workspace(n, k, m)));
+}
+
+int bsq_mx4_linear_backward(const void *d_dy, int type, uint64_t m, uint64_t n, uint64_t ldy, const uint8_t *d_xt_codes,
+                            const uint8_t *d_xt_scales, const uint8_t *d_wt_codes, const uint8_t *d_wt_scales, uint64_t k,
+                            void *d_dx, uint64_t lddx, void *d_dw, uint64_t lddw, int g_type, void *d_work,
+                            uint64_t work_bytes, void *stream) {
+    return entry([&] {
+        const Mx4Type t = type_of(type), tg = type_of(g_type);
+        check_sides(m, n, std::max({m, n, k}));
+        BSQ_REQUIRE(m >= 1 && n >= 1, "mx4 linear backward: empty");
+        BSQ_REQUIRE(ldy >= n && (d_dx == nullptr || lddx >= k) && (d_dw == nullptr || lddw >= k), "mx4 linear backward: rows overlap");
+        if (k == 0 || (d_dx == nullptr && d_dw == nullptr)) return;
+        check_dense(d_dy, t, "mx4 linear backward: null gradient");
+        if (d_dx) check_dense(d_dx, tg, "");
+        if (d_dw) check_dense(d_dw, tg, "");
+        if (d_dx) check_packed(d_wt_codes, d_wt_scales);
+        if (d_dw) check_packed(d_xt_codes, d_xt_scales);
+        check_work(d_work, work_bytes, bsq_mx4_linear_backward_workspace(m, n, k));
+        hipStream_t s = static_cast<hipStream_t>(stream);
+        uint8_t *rc = static_cast<uint8_t *>(d_work), *rs = rc + round256(m * mx4_slices(n) * 128);
+        uint8_t *cc = rc + packed(m, n), *cs = cc + round256(n * mx4_slices(m) * 128);
+        uint8_t *rest = cc + packed(n, m);
+        const uint64_t rest_bytes = work_bytes - packed(m, n) - packed(n, m);
+        launch_mx4_encode(d_dy, t, 1, m, n, ldy, 0, d_dx ? rc : nullptr, d_dx ? rs : nullptr, d_dw ? cc : nullptr,
+                          d_dw ? cs : nullptr, s);
+        if (d_dx) product({rc, rs}, m, {d_wt_codes, d_wt_scales}, k, n, d_dx, tg, lddx, rest, rest_bytes, s);
+        if (d_dw) product({cc, cs}, n, {d_xt_codes, d_xt_scales}, k, m, d_dw, tg, lddw, rest, rest_bytes, s);
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,167 @@
+// Microscaled 4-bit matrices (MX4): the packed layout and what its kernels
+// share (mx4.hip, mx4_gemm.hip, moe.hip).
+//
+// Blocks of 32 values along a row share a power of two, the smallest 2^e with
+// e >= -126 at which no value of the block lies above 6 in magnitude; a value
+// over its scale is rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (ties
+// to the even code) and its sign (E2M1).  A block that holds a NaN or an
+// infinity is NaN as a whole: scale byte 255, codes 0.
+//
+// A packed matrix of rows x cols: row-major codes, two a byte with the first
+// in the low half, and row-major scale bytes (e + 127).  Rows are padded with
+// zeros to a multiple of 256 values: 128 bytes of codes (a cache line) and 8 of
+// scales, so that no kernel meets a partial slice or an unaligned row.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "bsq_internal.hpp"
+
+namespace bsq {
+
+constexpr uint32_t kMx4Slice = 256;  // values a row is padded to
+constexpr uint32_t kMx4Block = 32;
+
+__host__ __device__ inline uint64_t mx4_slices(uint64_t cols) { return (cols + kMx4Slice - 1) / kMx4Slice; }
+
+enum class Mx4Type : int { F32 = 0, BF16 = 1, F16 = 2 };
+inline uint32_t type_bytes(Mx4Type t) { return t == Mx4Type::F32 ? 4u : 2u; }
+
+struct Mx4Matrix {
+    const uint8_t *codes = nullptr;
+    const uint8_t *scales = nullptr;
+};
+
+// Where the columns of an encode come from when they are the slots of experts:
+// slot s of the order is row order[s] / per_token of x, scaled by
+// weights[order[s]] if given; expert e has the slots offsets[e] ..
+// offsets[e + 1], and its slices begin at tile tile_of(e) (128 slots each, two
+// a slice).
+struct Mx4Slots {
+    const int32_t *offsets = nullptr;
+    const int32_t *order = nullptr;
+    const float *weights = nullptr;
+    uint32_t experts = 0, per_token = 1;
+};
+
+// x: `batch` matrices of rows x cols, rows `ld` and matrices `stride` elements
+// apart.  rows_out / cols_out (either may be empty): the packed matrices of
+// their rows and of their columns (the transposes'), batch after batch.
+void launch_mx4_encode(const void *x, Mx4Type type, uint64_t batch, uint64_t rows, uint64_t cols, uint64_t ld,
+                       uint64_t stride, uint8_t *codes, uint8_t *scales, uint8_t *codes_t, uint8_t *scales_t,
+                       hipStream_t stream);
+void launch_mx4_decode(const uint8_t *codes, const uint8_t *scales, uint64_t rows, uint64_t cols, void *out,
+                       Mx4Type type, uint64_t ld, hipStream_t stream);
+// The transpose of the slots' rows (cols x slots, `slices` slices of 256 slots
+// a row), every expert's slots from a slice of its own.
+void launch_mx4_encode_slots(const void *x, Mx4Type type, uint64_t cols, uint64_t ld, const Mx4Slots &slots,
+                             uint64_t slices, uint8_t *codes_t, uint8_t *scales_t, hipStream_t stream);
+
+// Products of packed matrices: out[m, n] = sum over the shared axis.
+struct Mx4Product {
+    Mx4Matrix a, b;
+    uint32_t M = 0, N = 0;      // rows of a and b (of one expert's b)
+    uint32_t slices = 0;        // slices of a row of a and b
+    void *out = nullptr;
+    Mx4Type type = Mx4Type::F32;
+    uint64_t ld = 0;
+    // rows of a chosen by the experts' order: slot s multiplies row
+    // order[s] / per_token of a with expert e's b and writes row order[s]
+    const int32_t *offsets = nullptr, *order = nullptr;
+    uint32_t experts = 0, per_token = 1;
+    // the experts' slots are the shared axis instead: out[e] (M x N) sums the
+    // slices of expert e
+    bool shared_slots = false;
+};
+uint64_t mx4_product_workspace(uint32_t M, uint32_t N, uint32_t slices);
+void launch_mx4_product(const Mx4Product &p, void *workspace, uint64_t workspace_bytes, hipStream_t stream);
+
+// First slice of expert e's slots and the number of slices of all.
+__device__ __forceinline__ uint32_t mx4_slot_slices(const int32_t *offsets, uint32_t e) {
+    return (static_cast<uint32_t>(offsets[e + 1] - offsets[e]) + kMx4Slice - 1) / kMx4Slice;
+}
+
+// 2^(b - 127), b in [1, 254]
+__device__ __forceinline__ float mx4_power(uint32_t b) { return __uint_as_float(b << 23); }
+
+// The scale byte of a block whose largest magnitude has the FP32 bits `top`:
+// top / 6 <= 2^e where top / 4 = 1.m 2^e with 1.m <= 1.5, else 2^(e + 1).  NaN
+// and infinity: 255.
+__device__ __forceinline__ uint32_t mx4_scale_byte(uint32_t top) {
+    const uint32_t b = (top + 0x3FFFFFu) >> 23;
+    return top >= 0x7F800000u ? 255u : (b < 3u ? 1u : b - 2u);
+}
+
+__device__ __forceinline__ float bf16_value(uint32_t bits) { return __uint_as_float(bits << 16); }
+// FP32 -> BF16, round to nearest even; NaN stays NaN
+__device__ __forceinline__ uint32_t bf16_bits(float f) {
+    const uint32_t u = __float_as_uint(f);
+    return fabsf(f) <= __builtin_inff() ? (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16 : (u >> 16) | 0x40u;
+}
+__device__ __forceinline__ uint32_t f16_bits(float f) {
+    return static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(f)));
+}
+__device__ __forceinline__ float f16_value(uint32_t bits) {
+    return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+}
+
+template <Mx4Type T>
+__device__ __forceinline__ float load_value(const void *p, uint64_t i) {
+    if constexpr (T == Mx4Type::F32) return static_cast<const float *>(p)[i];
+    const uint32_t b = static_cast<const uint16_t *>(p)[i];
+    return T == Mx4Type::BF16 ? bf16_value(b) : f16_value(b);
+}
+template <Mx4Type T>
+__device__ __forceinline__ void store_value(void *p, uint64_t i, float v) {
+    if constexpr (T == Mx4Type::F32) static_cast<float *>(p)[i] = v;
+    else static_cast<uint16_t *>(p)[i] = static_cast<uint16_t>(T == Mx4Type::BF16 ? bf16_bits(v) : f16_bits(v));
+}
+
+// fn<T>() for the type of a call
+template <class F>
+void by_type(Mx4Type t, F &&fn) {
+    switch (t) {
+        case Mx4Type::F32: fn(std::integral_constant<Mx4Type, Mx4Type::F32>{}); return;
+        case Mx4Type::BF16: fn(std::integral_constant<Mx4Type, Mx4Type::BF16>{}); return;
+        case Mx4Type::F16: fn(std::integral_constant<Mx4Type, Mx4Type::F16>{}); return;
+    }
+    fail("mx4: unknown element type");
+}
+
+// Checks of a call's arguments.
+inline Mx4Type type_of(int t) {
+    BSQ_REQUIRE(t >= 0 && t <= 2, "unknown element type");
+    return static_cast<Mx4Type>(t);
+}
+inline void check_packed(const void *codes, const void *scales) {
+    BSQ_REQUIRE(codes != nullptr && scales != nullptr, "null packed matrix");
+    BSQ_REQUIRE((reinterpret_cast<uintptr_t>(codes) & 15) == 0 && (reinterpret_cast<uintptr_t>(scales) & 7) == 0,
+                "packed codes are 16-byte and scales 8-byte aligned");
+}
+inline void check_dense(const void *p, Mx4Type t, const char *null) {
+    BSQ_REQUIRE(p != nullptr, null);
+    BSQ_REQUIRE((reinterpret_cast<uintptr_t>(p) & (type_bytes(t) - 1)) == 0, "matrix unaligned to its elements");
+}
+inline void check_work(const void *p, uint64_t bytes, uint64_t need) {
+    BSQ_REQUIRE(bytes >= need, "workspace too small");
+    if (need > 0) check_packed(p, p);  // begins with codes
+}
+inline uint64_t round256(uint64_t v) { return (v + 255) & ~255ull; }
+inline uint64_t packed_bytes(uint64_t rows, uint64_t slices) { return round256(rows * slices * 128) + round256(rows * slices * 8); }
+
+// C entry points: exceptions become return codes
+template <class F>
+int entry(F &&f) noexcept {
+    try {
+        f();
+        set_last_error("");
+        return 0;
+    } catch (const std::exception &e) {
+        set_last_error(e.what());
+    } catch (...) {
+        set_last_error("unknown error");
+    }
+    return 1;
+}
+
+}  // namespace bsq

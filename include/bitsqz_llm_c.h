@@ -19,6 +19,8 @@
  *   3. bsq_topk_*, bsq_quant_*, bsq_svd_*, bsq_reconstruct_* -- the four
  *                        module operators the pipeline is built from, each
  *                        mirroring a reference module entry point.
+ * and beside them memory helpers (4), the legacy formats (5), and layers that
+ * compute on 4-bit matrices (6: bsq_mx4_*, bsq_moe_*).
  */
 #ifndef BITSQZ_LLM_C_H
 #define BITSQZ_LLM_C_H
@@ -322,6 +324,111 @@ BSQ_API int bsq_legacy_decode_device(int method, const void *d_payload, uint64_t
  * (2: max norm 448, 3: max norm 6). */
 BSQ_API int bsq_legacy_sweep(int kind, uint64_t lo, uint64_t hi, unsigned long long *d_checksum,
                              void *stream);
+
+/* ---------------------------------------------------------------------------
+ * 6. Microscaled 4-bit matrices (MX4) and layers that compute with them (no
+ *    reference counterpart: its MXFP4 stores flat arrays and only decodes).
+ *
+ *    A packed matrix of rows x cols: blocks of 32 values along a row share a
+ *    power of two, the smallest 2^e, e >= -126, with no value above 6 times it;
+ *    a value over it is rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6
+ *    (ties to the even code) and its sign, E2M1.  A block that holds a NaN or an
+ *    infinity is NaN as a whole.  Row-major codes, two a byte with the first in
+ *    the low half, and row-major scale bytes (e + 127; 255: NaN); rows padded
+ *    with zeros to a multiple of 256 values.  Codes are 16-byte and scales
+ *    8-byte aligned (so is a workspace, 16).
+ *
+ *    Element types: 0 FP32, 1 BF16, 2 FP16.  `ld` counts elements from one row
+ *    to the next.  Sums are held in FP32 and rounded once.  All calls are
+ *    asynchronous on `stream`, keep nothing between calls and take their
+ *    workspace from the caller (its bytes: the function beside them), so they
+ *    can be captured, and run on several streams with a workspace each.
+ * ------------------------------------------------------------------------- */
+BSQ_API uint64_t bsq_mx4_codes_bytes(uint64_t rows, uint64_t cols);
+BSQ_API uint64_t bsq_mx4_scales_bytes(uint64_t rows, uint64_t cols);
+
+/* Packs `batch` matrices of rows x cols (`stride` elements apart): their rows
+ * into d_codes / d_scales, and / or their columns, as the packed cols x rows
+ * transposes, into d_codes_t / d_scales_t, from one read.  Either pair may be
+ * NULL.  The batch's packed matrices follow one another. */
+BSQ_API int bsq_mx4_encode(const void *d_x, int type, uint64_t batch, uint64_t rows, uint64_t cols, uint64_t ld,
+                           uint64_t stride, uint8_t *d_codes, uint8_t *d_scales, uint8_t *d_codes_t,
+                           uint8_t *d_scales_t, void *stream);
+BSQ_API int bsq_mx4_decode(const uint8_t *d_codes, const uint8_t *d_scales, uint64_t rows, uint64_t cols, void *d_out,
+                           int type, uint64_t ld, void *stream);
+
+/* out (m x n) = A B^T of packed A (m x k) and B (n x k). */
+BSQ_API uint64_t bsq_mx4_product_workspace(uint64_t m, uint64_t n, uint64_t k);
+BSQ_API int bsq_mx4_product(const uint8_t *d_a_codes, const uint8_t *d_a_scales, uint64_t m, const uint8_t *d_b_codes,
+                            const uint8_t *d_b_scales, uint64_t n, uint64_t k, void *d_out, int type, uint64_t ld,
+                            void *d_work, uint64_t work_bytes, void *stream);
+
+/* A dense layer: out (m x n) = q(x) W^T, x (m x k) packed on the way, W packed
+ * (n x k).  With d_xt_codes / d_xt_scales (may be NULL) the packed k x m
+ * transpose of x is kept for the backward pass: the activations at 4.25 bits a
+ * value. */
+BSQ_API uint64_t bsq_mx4_linear_workspace(uint64_t m, uint64_t n, uint64_t k);
+BSQ_API int bsq_mx4_linear(const void *d_x, int x_type, uint64_t m, uint64_t k, uint64_t ldx, const uint8_t *d_w_codes,
+                           const uint8_t *d_w_scales, uint64_t n, void *d_out, int out_type, uint64_t ldo,
+                           uint8_t *d_xt_codes, uint8_t *d_xt_scales, void *d_work, uint64_t work_bytes, void *stream);
+/* Its gradients, straight through the rounding: dx (m x k) = q(dy) W with the
+ * weights' columns d_wt_* (k x n packed), dw (n x k) = q(dy^T) q(x^T)^T with
+ * the columns of x that the forward call kept.  d_dx or d_dw may be NULL. */
+BSQ_API uint64_t bsq_mx4_linear_backward_workspace(uint64_t m, uint64_t n, uint64_t k);
+BSQ_API int bsq_mx4_linear_backward(const void *d_dy, int type, uint64_t m, uint64_t n, uint64_t ldy,
+                                    const uint8_t *d_xt_codes, const uint8_t *d_xt_scales, const uint8_t *d_wt_codes,
+                                    const uint8_t *d_wt_scales, uint64_t k, void *d_dx, uint64_t lddx, void *d_dw,
+                                    uint64_t lddw, int g_type, void *d_work, uint64_t work_bytes, void *stream);
+
+/* Routing of tokens to k of `experts` (up to 1024; k up to 64) from their
+ * logits.  Scores: softmax over the experts (scoring 0) or sigmoid (1).  The
+ * choice goes by the logits, or by score + d_bias[expert] where d_bias is not
+ * NULL; with groups > 1 (equal runs of experts, up to 64 groups) only among the
+ * `kept` groups whose largest entry, or with a bias whose two largest entries'
+ * sum, is largest; ties go to the lowest number.  An expert whose logit is NaN
+ * or at or below its type's lowest finite value is closed to the token.  ids:
+ * tokens x k, best first, -1 (weight 0) where no open expert is left; weights:
+ * the scores, over their sum if `renormalise`, times `scale`. */
+BSQ_API int bsq_moe_route(const void *d_logits, int type, uint64_t tokens, uint32_t experts, uint64_t ld,
+                          const float *d_bias, int scoring, uint32_t groups, uint32_t kept, uint32_t k, int renormalise,
+                          float scale, int32_t *d_ids, float *d_weights, void *stream);
+/* d logits (of the logits' type) from d weights and the ids of the choice. */
+BSQ_API int bsq_moe_route_backward(const void *d_logits, int type, uint64_t tokens, uint32_t experts, uint64_t ld,
+                                   int scoring, uint32_t k, int renormalise, float scale, const int32_t *d_ids,
+                                   const float *d_d_weights, void *d_d_logits, uint64_t ldd, void *stream);
+/* The pairs (token, place) = (p / k, p % k) in the experts' order: expert e's
+ * are d_order[d_offsets[e] .. d_offsets[e + 1]), ascending; pairs whose id is
+ * not an expert follow the last.  d_offsets: experts + 1 entries. */
+BSQ_API int bsq_moe_plan(const int32_t *d_ids, uint64_t pairs, uint32_t experts, int32_t *d_offsets, int32_t *d_order,
+                         void *stream);
+/* out[t] = sum over the token's experts of weight * y[t k + j] (y: tokens k x n,
+ * rows side by side). */
+BSQ_API int bsq_moe_combine(const void *d_y, int y_type, uint64_t tokens, uint32_t k, uint64_t n, const int32_t *d_ids,
+                            const float *d_weights, uint32_t experts, void *d_out, int type, uint64_t ld, void *stream);
+
+/* The experts' layer: y[t k + j] = q(x[t]) W_e^T for e = ids[t k + j] and out =
+ * the join of y by the weights.  W: experts packed matrices of n x inputs, one
+ * after another.  d_offsets, d_order (as bsq_moe_plan) and d_y (tokens k x n;
+ * zero rows where a pair has no expert) are written and serve the backward
+ * pass; the gradient of the weights is as fine as y's type. */
+BSQ_API uint64_t bsq_moe_linear_workspace(uint64_t tokens, uint32_t k, uint64_t n, uint64_t inputs, uint32_t experts);
+BSQ_API int bsq_moe_linear(const void *d_x, int x_type, uint64_t tokens, uint64_t inputs, uint64_t ldx,
+                           const int32_t *d_ids, const float *d_weights, uint32_t k, const uint8_t *d_w_codes,
+                           const uint8_t *d_w_scales, uint32_t experts, uint64_t n, int32_t *d_offsets, int32_t *d_order,
+                           void *d_y, int y_type, void *d_out, int out_type, uint64_t ldo, void *d_work,
+                           uint64_t work_bytes, void *stream);
+/* Its gradients, each optional (NULL): dx = sum of weight * q(d out) W_e with
+ * the weights' columns d_wt_* (experts packed matrices of inputs x n), d
+ * weights[t, j] = <d out[t], y[t k + j]>, dw (experts x n x inputs) = the sum
+ * over the expert's pairs of q(weight d out)^T q(x), in blocks of 32 pairs. */
+BSQ_API uint64_t bsq_moe_linear_backward_workspace(uint64_t tokens, uint32_t k, uint64_t n, uint64_t inputs,
+                                                   uint32_t experts);
+BSQ_API int bsq_moe_linear_backward(const void *d_d_out, int d_type, uint64_t tokens, uint64_t n, uint64_t ldd,
+                                    const void *d_x, int x_type, uint64_t inputs, uint64_t ldx, const int32_t *d_ids,
+                                    const float *d_weights, uint32_t k, const int32_t *d_offsets, const int32_t *d_order,
+                                    const void *d_y, int y_type, const uint8_t *d_wt_codes, const uint8_t *d_wt_scales,
+                                    uint32_t experts, void *d_dx, uint64_t lddx, float *d_d_weights, void *d_dw,
+                                    int g_type, void *d_work, uint64_t work_bytes, void *stream);
 
 #ifdef __cplusplus
 }
