@@ -292,47 +292,6 @@ __global__ void moe_plan_kernel(const int32_t *__restrict__ ids, uint32_t pairs,
     }
 }
 
-// Eight consecutive values in FP32
-template <Mx4Type T>
-__device__ __forceinline__ void load8(const void *base, uint64_t at, uint32_t valid, float v[8]) {
-    if (valid >= 8) {
-        if constexpr (T == Mx4Type::F32) {
-            __builtin_memcpy(v, static_cast<const float *>(base) + at, 32);
-        } else {
-            uint32_t w[4];
-            __builtin_memcpy(w, static_cast<const uint16_t *>(base) + at, 16);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t b = (w[i / 2] >> (16 * (i & 1))) & 0xFFFFu;
-                v[i] = T == Mx4Type::BF16 ? bf16_value(b) : f16_value(b);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = static_cast<uint32_t>(i) < valid ? load_value<T>(base, at + i) : 0.0f;
-    }
-}
-template <Mx4Type T>
-__device__ __forceinline__ void store8(void *base, uint64_t at, uint32_t valid, const float v[8]) {
-    if (valid >= 8) {
-        if constexpr (T == Mx4Type::F32) {
-            __builtin_memcpy(static_cast<float *>(base) + at, v, 32);
-        } else {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (T == Mx4Type::BF16) w[i] = bf16_bits(v[2 * i]) | (bf16_bits(v[2 * i + 1]) << 16);
-                else w[i] = f16_bits(v[2 * i]) | (f16_bits(v[2 * i + 1]) << 16);
-            }
-            __builtin_memcpy(static_cast<uint16_t *>(base) + at, w, 16);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (static_cast<uint32_t>(i) < valid) store_value<T>(base, at + i, v[i]);
-    }
-}
-
 // out[t] = sum over the token's experts of weight * y, in the pairs' order; a
 // lane takes eight columns.
 template <Mx4Type Y, Mx4Type O>

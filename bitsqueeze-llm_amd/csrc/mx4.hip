@@ -10,82 +10,8 @@ namespace bsq {
 namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256;
-
-// Eight consecutive values in their own type.
-template <Mx4Type T>
-struct Eight {
-    static constexpr int kWords = T == Mx4Type::F32 ? 8 : 4;
-    uint32_t w[kWords];
-
-    // values [at, at + 8) of a row of n, zeros past its end; any alignment of
-    // the element's own size
-    __device__ __forceinline__ void load(const uint8_t *row, uint64_t at, uint64_t n) {
-        constexpr int size = T == Mx4Type::F32 ? 4 : 2;
-        if (at + 8 <= n) {
-            __builtin_memcpy(w, row + at * size, 8 * size);
-        } else {
-#pragma unroll
-            for (int i = 0; i < kWords; ++i) w[i] = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (at + i >= n) continue;
-                if constexpr (T == Mx4Type::F32) w[i] = reinterpret_cast<const uint32_t *>(row)[at + i];
-                else w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(row)[at + i]) << (16 * (i & 1));
-            }
-        }
-    }
-    // bits of the largest magnitude, in the type's own format (they order as
-    // the magnitudes do, infinity and NaN above all)
-    __device__ __forceinline__ uint32_t top() const {
-        if constexpr (T == Mx4Type::F32) {
-            uint32_t m = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
-            return m;
-        } else {
-            u16x2 m = {0, 0};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu));
-            return max(static_cast<uint32_t>(m[0]), static_cast<uint32_t>(m[1]));
-        }
-    }
-    // the eight codes over `scale`
-    __device__ __forceinline__ uint32_t codes(float scale) const {
-        uint32_t c = 0;
-        if constexpr (T == Mx4Type::F32) {
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(w[0]), __uint_as_float(w[1]), scale, 0);
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(w[2]), __uint_as_float(w[3]), scale, 1);
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(w[4]), __uint_as_float(w[5]), scale, 2);
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(w[6]), __uint_as_float(w[7]), scale, 3);
-        } else if constexpr (T == Mx4Type::BF16) {
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, w[0]), scale, 0);
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, w[1]), scale, 1);
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, w[2]), scale, 2);
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, w[3]), scale, 3);
-        } else {
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, w[0]), scale, 0);
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, w[1]), scale, 1);
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, w[2]), scale, 2);
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2, w[3]), scale, 3);
-        }
-        return c;
-    }
-};
-
-// the type's magnitude bits as FP32's
-template <Mx4Type T>
-__device__ __forceinline__ uint32_t f32_bits(uint32_t top) {
-    if constexpr (T == Mx4Type::F32) return top;
-    if constexpr (T == Mx4Type::BF16) return top << 16;
-    return __float_as_uint(f16_value(top));
-}
 
 // max over each aligned quad of lanes
 __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
@@ -400,8 +326,7 @@ void check_sides(uint64_t m, uint64_t n, uint64_t k) {
 }
 uint64_t packed(uint64_t rows, uint64_t cols) { return packed_bytes(rows, mx4_slices(cols)); }
 
-void product(Mx4Matrix a, uint64_t m, Mx4Matrix b, uint64_t n, uint64_t k, void *out, Mx4Type type, uint64_t ld,
-             uint8_t *work, uint64_t work_bytes, hipStream_t stream) {
+Mx4Product product_of(Mx4Matrix a, uint64_t m, Mx4Matrix b, uint64_t n, uint64_t k, void *out, Mx4Type type, uint64_t ld) {
     Mx4Product p;
     p.a = a;
     p.b = b;
@@ -411,7 +336,7 @@ void product(Mx4Matrix a, uint64_t m, Mx4Matrix b, uint64_t n, uint64_t k, void 
     p.out = out;
     p.type = type;
     p.ld = ld;
-    launch_mx4_product(p, work, work_bytes, stream);
+    return p;
 }
 
 }  // namespace
@@ -470,8 +395,8 @@ int bsq_mx4_product(const uint8_t *d_a_codes, const uint8_t *d_a_scales, uint64_
         check_packed(d_b_codes, d_b_scales);
         check_dense(d_out, t, "mx4 product: null output");
         check_work(d_work, work_bytes, bsq_mx4_product_workspace(m, n, k));
-        product({d_a_codes, d_a_scales}, m, {d_b_codes, d_b_scales}, n, k, d_out, t, ld, static_cast<uint8_t *>(d_work),
-                work_bytes, static_cast<hipStream_t>(stream));
+        launch_mx4_product(product_of({d_a_codes, d_a_scales}, m, {d_b_codes, d_b_scales}, n, k, d_out, t, ld), d_work,
+                           work_bytes, static_cast<hipStream_t>(stream));
     });
 }
 
@@ -496,9 +421,13 @@ int bsq_mx4_linear(const void *d_x, int x_type, uint64_t m, uint64_t k, uint64_t
         check_work(d_work, work_bytes, bsq_mx4_linear_workspace(m, n, k));
         hipStream_t s = static_cast<hipStream_t>(stream);
         uint8_t *codes = static_cast<uint8_t *>(d_work), *scales = codes + round256(m * mx4_slices(k) * 128);
+        const Mx4Product p = product_of({codes, scales}, m, {d_w_codes, d_w_scales}, n, k, d_out, to, ldo);
+        if (mx4_packs_on_the_way(m, p.slices) && d_xt_codes == nullptr) {
+            launch_mx4_product_of(d_x, tx, k, ldx, p, s);
+            return;
+        }
         launch_mx4_encode(d_x, tx, 1, m, k, ldx, 0, codes, scales, d_xt_codes, d_xt_scales, s);
-        product({codes, scales}, m, {d_w_codes, d_w_scales}, n, k, d_out, to, ldo, codes + packed(m, k),
-                work_bytes - packed(m, k), s);
+        launch_mx4_product(p, codes + packed(m, k), work_bytes - packed(m, k), s);
     });
 }
 
@@ -530,8 +459,8 @@ int bsq_mx4_linear_backward(const void *d_dy, int type, uint64_t m, uint64_t n, 
         const uint64_t rest_bytes = work_bytes - packed(m, n) - packed(n, m);
         launch_mx4_encode(d_dy, t, 1, m, n, ldy, 0, d_dx ? rc : nullptr, d_dx ? rs : nullptr, d_dw ? cc : nullptr,
                           d_dw ? cs : nullptr, s);
-        if (d_dx) product({rc, rs}, m, {d_wt_codes, d_wt_scales}, k, n, d_dx, tg, lddx, rest, rest_bytes, s);
-        if (d_dw) product({cc, cs}, n, {d_xt_codes, d_xt_scales}, k, m, d_dw, tg, lddw, rest, rest_bytes, s);
+        if (d_dx) launch_mx4_product(product_of({rc, rs}, m, {d_wt_codes, d_wt_scales}, k, n, d_dx, tg, lddx), rest, rest_bytes, s);
+        if (d_dw) launch_mx4_product(product_of({cc, cs}, n, {d_xt_codes, d_xt_scales}, k, m, d_dw, tg, lddw), rest, rest_bytes, s);
     });
 }
 

@@ -75,6 +75,10 @@ struct Mx4Product {
 };
 uint64_t mx4_product_workspace(uint32_t M, uint32_t N, uint32_t slices);
 void launch_mx4_product(const Mx4Product &p, void *workspace, uint64_t workspace_bytes, hipStream_t stream);
+// The same with a packed from dense x on the way, for m rows where that pays.
+bool mx4_packs_on_the_way(uint64_t m, uint64_t slices);
+void launch_mx4_product_of(const void *x, Mx4Type x_type, uint64_t x_cols, uint64_t ldx, const Mx4Product &p,
+                           hipStream_t stream);
 
 // First slice of expert e's slots and the number of slices of all.
 __device__ __forceinline__ uint32_t mx4_slot_slices(const int32_t *offsets, uint32_t e) {
@@ -115,6 +119,121 @@ template <Mx4Type T>
 __device__ __forceinline__ void store_value(void *p, uint64_t i, float v) {
     if constexpr (T == Mx4Type::F32) static_cast<float *>(p)[i] = v;
     else static_cast<uint16_t *>(p)[i] = static_cast<uint16_t>(T == Mx4Type::BF16 ? bf16_bits(v) : f16_bits(v));
+}
+
+typedef _Float16 mx4_f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 mx4_bf16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t mx4_u16x2 __attribute__((ext_vector_type(2)));
+
+// Eight consecutive values in their own type.
+template <Mx4Type T>
+struct Eight {
+    static constexpr int kWords = T == Mx4Type::F32 ? 8 : 4;
+    uint32_t w[kWords];
+
+    // values [at, at + 8) of a row of n, zeros past its end; any alignment of
+    // the element's own size
+    __device__ __forceinline__ void load(const uint8_t *row, uint64_t at, uint64_t n) {
+        constexpr int size = T == Mx4Type::F32 ? 4 : 2;
+        if (at + 8 <= n) {
+            __builtin_memcpy(w, row + at * size, 8 * size);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (at + i >= n) continue;
+                if constexpr (T == Mx4Type::F32) w[i] = reinterpret_cast<const uint32_t *>(row)[at + i];
+                else w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(row)[at + i]) << (16 * (i & 1));
+            }
+        }
+    }
+    // bits of the largest magnitude, in the type's own format (they order as
+    // the magnitudes do, infinity and NaN above all)
+    __device__ __forceinline__ uint32_t top() const {
+        if constexpr (T == Mx4Type::F32) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+            return m;
+        } else {
+            mx4_u16x2 m = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                m = __builtin_elementwise_max(m, __builtin_bit_cast(mx4_u16x2, w[i] & 0x7FFF7FFFu));
+            return max(static_cast<uint32_t>(m[0]), static_cast<uint32_t>(m[1]));
+        }
+    }
+    // the eight codes over `scale`
+    __device__ __forceinline__ uint32_t codes(float scale) const {
+        uint32_t c = 0;
+        if constexpr (T == Mx4Type::F32) {
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(w[0]), __uint_as_float(w[1]), scale, 0);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(w[2]), __uint_as_float(w[3]), scale, 1);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(w[4]), __uint_as_float(w[5]), scale, 2);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(w[6]), __uint_as_float(w[7]), scale, 3);
+        } else if constexpr (T == Mx4Type::BF16) {
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(mx4_bf16x2, w[0]), scale, 0);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(mx4_bf16x2, w[1]), scale, 1);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(mx4_bf16x2, w[2]), scale, 2);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(mx4_bf16x2, w[3]), scale, 3);
+        } else {
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(mx4_f16x2, w[0]), scale, 0);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(mx4_f16x2, w[1]), scale, 1);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(mx4_f16x2, w[2]), scale, 2);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(mx4_f16x2, w[3]), scale, 3);
+        }
+        return c;
+    }
+};
+
+// the type's magnitude bits as FP32's
+template <Mx4Type T>
+__device__ __forceinline__ uint32_t f32_bits(uint32_t top) {
+    if constexpr (T == Mx4Type::F32) return top;
+    if constexpr (T == Mx4Type::BF16) return top << 16;
+    return __float_as_uint(f16_value(top));
+}
+
+// Eight consecutive values in FP32
+template <Mx4Type T>
+__device__ __forceinline__ void load8(const void *base, uint64_t at, uint32_t valid, float v[8]) {
+    if (valid >= 8) {
+        if constexpr (T == Mx4Type::F32) {
+            __builtin_memcpy(v, static_cast<const float *>(base) + at, 32);
+        } else {
+            uint32_t w[4];
+            __builtin_memcpy(w, static_cast<const uint16_t *>(base) + at, 16);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t b = (w[i / 2] >> (16 * (i & 1))) & 0xFFFFu;
+                v[i] = T == Mx4Type::BF16 ? bf16_value(b) : f16_value(b);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = static_cast<uint32_t>(i) < valid ? load_value<T>(base, at + i) : 0.0f;
+    }
+}
+template <Mx4Type T>
+__device__ __forceinline__ void store8(void *base, uint64_t at, uint32_t valid, const float v[8]) {
+    if (valid >= 8) {
+        if constexpr (T == Mx4Type::F32) {
+            __builtin_memcpy(static_cast<float *>(base) + at, v, 32);
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (T == Mx4Type::BF16) w[i] = bf16_bits(v[2 * i]) | (bf16_bits(v[2 * i + 1]) << 16);
+                else w[i] = f16_bits(v[2 * i]) | (f16_bits(v[2 * i + 1]) << 16);
+            }
+            __builtin_memcpy(static_cast<uint16_t *>(base) + at, w, 16);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (static_cast<uint32_t>(i) < valid) store_value<T>(base, at + i, v[i]);
+    }
 }
 
 // fn<T>() for the type of a call

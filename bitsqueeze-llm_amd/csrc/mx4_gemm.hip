@@ -8,6 +8,7 @@
 // lane's four scale bytes of a slice are one aligned word and the instruction
 // picks byte s itself.
 #include "mx4.hpp"
+#include "tile_map.hpp"
 
 #include <algorithm>
 #include <type_traits>
@@ -53,13 +54,16 @@ __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c, uint32_t sa, 
 
 enum Mode { kDense, kRows, kShared };
 
-// The tile of BM slots number t of the experts' tiles: the expert (experts
+// The tile of `tile` slots number t of the experts' tiles: the expert (experts
 // itself for the slots of none, `experts + 1` past the last tile) and its slots.
 struct SlotTile {
     uint32_t expert, begin, end;
 };
+// Without t: the number of tiles, in `begin`.
+constexpr uint32_t kCount = 0xFFFFFFFFu;
 __device__ __forceinline__ SlotTile slot_tile(const Mx4Product &p, uint32_t pairs, uint32_t t, uint32_t tile) {
     const uint32_t lane = threadIdx.x & 63;
+    uint32_t count = 0;
     for (uint32_t e0 = 0; e0 <= p.experts; e0 += 64) {
         const uint32_t e = e0 + lane;
         uint32_t lo = 0, hi = 0;
@@ -74,7 +78,7 @@ __device__ __forceinline__ SlotTile slot_tile(const Mx4Product &p, uint32_t pair
             const uint32_t v = __shfl_up(sum, d);
             sum += lane >= static_cast<uint32_t>(d) ? v : 0u;
         }
-        const uint64_t over = __ballot(sum > t);
+        const uint64_t over = t == kCount ? 0 : __ballot(sum > t);
         if (over != 0) {
             const int at = __builtin_ctzll(over);
             const uint32_t before = __builtin_amdgcn_readlane(sum - n, at);
@@ -82,31 +86,68 @@ __device__ __forceinline__ SlotTile slot_tile(const Mx4Product &p, uint32_t pair
             const uint32_t end = __builtin_amdgcn_readlane(hi, at);
             return {e0 + at, begin, min(begin + tile, end)};
         }
-        t -= __builtin_amdgcn_readlane(sum, 63);
+        const uint32_t all = __builtin_amdgcn_readlane(sum, 63);
+        if (t != kCount) t -= all;
+        count += all;
     }
-    return {p.experts + 1, 0, 0};
+    return {p.experts + 1, count, 0};
 }
 
-// T x T tiles, four waves of T/2 x T/2, slices of 256 values: the codes and
-// scales of a slice's rows go global -> LDS directly, two slices deep.  A
-// row's eight 16-byte blocks are stored in the order block ^ (row % 8), so that
-// eight neighbouring rows' reads of one block cover all banks; the permutation
-// is made by the lanes' source addresses.
-template <int T, Mode MODE, Mx4Type O>
-__global__ __launch_bounds__(kThreads) void mx4_product_kernel(Mx4Product p, uint32_t tiles_n, uint32_t pairs) {
-    constexpr int B = T / 64;          // 32 x 32 blocks of a wave, each way
-    constexpr int kRowLoads = T / 32;  // 16-byte transfers of a lane per operand and slice
-    struct Stage {
-        uint8_t a[T * kCodeBytes], b[T * kCodeBytes], sa[T * kScaleBytes], sb[T * kScaleBytes];
-    };
-    // an object each, so that reads of one are not held for transfers to the other
-    __shared__ __attribute__((aligned(1024))) Stage s0, s1;
+// T x T tiles, four waves of T/2 x T/2 (256: eight of 128 x 64), slices of 256
+// values: a slice's codes go global -> LDS directly, one slice ahead, with one
+// barrier a slice, some of the next slice's transfers behind each of the steps'
+// matrix instructions (all of them first, and the waves wait for their issue).
+// What bounds the kernel is the lines that the transfers touch (16384-byte
+// pieces of whole lines arrive at 30 TB/s, of half lines at 15), so a row's
+// scales, 8 bytes a slice, come four slices at a time: a line for each slice of
+// scales as for each of codes took 314 us with the products left out (8192^3),
+// where the products alone take 196.
+// A row's eight 16-byte blocks are stored in the order block ^ (row / 2 % 8):
+// sixteen neighbouring rows' reads of one block cover all 64 banks.  The lanes'
+// source addresses make the permutation.
+// G > 1: G teams of four waves take a share of the tile's slices each, from
+// stages of their own, and join their sums in LDS in the teams' order: tiles
+// that leave CUs idle take 1 / G of the time (300 x 1000 x 4000 in tiles of 64:
+// 10.4 us with one team, 8.0 with four; through a workspace and a launch
+// of its own 10.9 to 15.7).
+// With `splits` > 1 (dense products) workgroup z sums the slices [z, z + 1)
+// slices / splits and writes part z of the output (FP32 parts in the
+// workspace).
+template <int T>
+constexpr int kTeam = T == 256 ? 8 : 4;  // waves
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t tn = blockIdx.x % tiles_n, tm = blockIdx.x / tiles_n;
-    uint32_t m0 = tm * T, m_end = p.M, expert = 0, slice0 = 0, slices = p.slices;
+template <int T, int G, Mode MODE, Mx4Type O>
+__global__ __launch_bounds__(64 * G * kTeam<T>, T == 64 ? G : 2) void mx4_product_kernel(Mx4Product p, uint32_t tiles_m, uint32_t tiles_n,
+                                                                         uint32_t splits) {
+    constexpr int kWaves = kTeam<T>, kWavesN = kWaves / 2;
+    constexpr int WM = T / 2, WN = T / kWavesN;     // a wave's part
+    constexpr int BM = WM / 32, BN = WN / 32;       // in blocks of 32 x 32
+    constexpr int kRowLoads = T / (8 * kWaves);     // 16-byte transfers of a lane per operand and slice
+    struct Stage {
+        uint8_t a[T * kCodeBytes], b[T * kCodeBytes];
+    };
+    constexpr int kGroup = 4 * kScaleBytes;  // a row's scales of four slices
+    // an object each, so that reads of one are not held for transfers to another
+    __shared__ __attribute__((aligned(1024))) Stage stage0[G], stage1[G];
+    __shared__ __attribute__((aligned(1024))) uint8_t scale_words[G * 4 * T * kGroup];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) % kWaves;
+    const int team = G == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6) / kWaves;
+    const Stage &s0 = stage0[team], &s1 = stage1[team];
+    const uint8_t *scales_a = scale_words + team * 4 * T * kGroup, *scales_b = scales_a + 2 * T * kGroup;
     if constexpr (MODE == kRows) {
-        const SlotTile s = slot_tile(p, pairs, tm, T);
+        // the tiles that there are, evenly over the XCDs
+        tiles_m = slot_tile(p, p.M, kCount, T).begin;
+        if (blockIdx.x >= tiles_m * tiles_n) return;
+    }
+    int tm, tn, z;
+    xcd_tile(static_cast<int>(tiles_m), static_cast<int>(tiles_n), static_cast<int>(splits), tm, tn, z);
+    uint32_t m0 = tm * T, m_end = p.M, expert = 0, slice0 = 0, slices = p.slices;
+    if constexpr (MODE == kDense) {
+        slice0 = static_cast<uint32_t>(static_cast<uint64_t>(z) * p.slices / splits);
+        slices = static_cast<uint32_t>(static_cast<uint64_t>(z + 1) * p.slices / splits) - slice0;
+    } else if constexpr (MODE == kRows) {
+        const SlotTile s = slot_tile(p, p.M, tm, T);
         if (s.expert > p.experts) return;  // uniform
         expert = s.expert;
         m0 = s.begin;
@@ -121,141 +162,474 @@ __global__ __launch_bounds__(kThreads) void mx4_product_kernel(Mx4Product p, uin
         slice0 = __builtin_amdgcn_readfirstlane(before);
         slices = __builtin_amdgcn_readfirstlane(mx4_slot_slices(p.offsets, expert));
     }
+    // every team passes the same barriers, `turns` of them
+    const uint32_t turns = (slices + G - 1) / G;
+    if constexpr (G > 1) {
+        const uint32_t from = min(team * turns, slices), to = min(from + turns, slices);
+        slice0 += from;
+        slices = to - from;
+    }
     const uint32_t n0 = tn * T;
-    const uint32_t b_first = MODE == kRows ? min(expert, p.experts - 1) * p.N : 0u;
+    const uint64_t b_first = MODE == kRows ? static_cast<uint64_t>(min(expert, p.experts - 1)) * p.N : 0u;
 
-    // this lane's rows and blocks of the transfers (rows past the end repeat
-    // the last one; their results are not stored)
-    const uint8_t *ga[kRowLoads], *gb[kRowLoads];
+    // This lane's rows and blocks of the transfers, as offsets from the tile's
+    // first row (rows past the end repeat the last one; their results are not
+    // stored).  Rows that the order chooses lie anywhere: 64 bits.
+    const uint32_t pitch = p.slices * kCodeBytes, pitch_s = p.slices * kScaleBytes;
+    const uint8_t *base_a = p.a.codes + static_cast<uint64_t>(slice0) * kCodeBytes;
+    const uint8_t *base_sa = p.a.scales + static_cast<uint64_t>(slice0) * kScaleBytes;
+    if constexpr (MODE != kRows) {
+        base_a += static_cast<uint64_t>(m0) * pitch;
+        base_sa += static_cast<uint64_t>(m0) * pitch_s;
+    }
+    const uint8_t *base_b = p.b.codes + (b_first + n0) * pitch + static_cast<uint64_t>(slice0) * kCodeBytes;
+    const uint8_t *base_sb = p.b.scales + (b_first + n0) * pitch_s + static_cast<uint64_t>(slice0) * kScaleBytes;
+    using Offset = std::conditional_t<MODE == kRows, uint64_t, uint32_t>;
+    auto row_a = [&](uint32_t r) __attribute__((always_inline)) {
+        const uint32_t row = min(m0 + r, m_end - 1);
+        if constexpr (MODE == kRows) return static_cast<Offset>(static_cast<uint32_t>(p.order[row]) / p.per_token);
+        else return static_cast<Offset>(row - m0);
+    };
+    auto row_b = [&](uint32_t r) __attribute__((always_inline)) { return min(n0 + r, p.N - 1) - n0; };
+    const uint32_t block = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
+    Offset oa[kRowLoads];
+    uint32_t ob[kRowLoads];
 #pragma unroll
     for (int i = 0; i < kRowLoads; ++i) {
-        const uint32_t r = 8 * (4 * i + wave) + (lane >> 3), block = (lane & 7) ^ (r & 7);
-        uint64_t ra = min(m0 + r, m_end - 1);
-        if constexpr (MODE == kRows) ra = static_cast<uint32_t>(p.order[ra]) / p.per_token;
-        const uint64_t rb = static_cast<uint64_t>(b_first) + min(n0 + r, p.N - 1);
-        ga[i] = p.a.codes + (ra * p.slices + slice0) * kCodeBytes + 16 * block;
-        gb[i] = p.b.codes + (rb * p.slices + slice0) * kCodeBytes + 16 * block;
+        const uint32_t r = 8 * (kWaves * i + wave) + (lane >> 3);
+        oa[i] = row_a(r) * pitch + 16 * block;
+        ob[i] = row_b(r) * pitch + 16 * block;
     }
-    constexpr int kScaleLoads = T / 128;  // 4-byte transfers of a lane per operand and slice
-    const uint8_t *gsa[kScaleLoads], *gsb[kScaleLoads];
-#pragma unroll
-    for (int i = 0; i < kScaleLoads; ++i) {
-        const uint32_t r = 32 * (4 * i + wave) + (lane >> 1);
-        uint64_t ra = min(m0 + r, m_end - 1);
-        if constexpr (MODE == kRows) ra = static_cast<uint32_t>(p.order[ra]) / p.per_token;
-        const uint64_t rb = static_cast<uint64_t>(b_first) + min(n0 + r, p.N - 1);
-        gsa[i] = p.a.scales + (ra * p.slices + slice0) * kScaleBytes + 4 * (lane & 1);
-        gsb[i] = p.b.scales + (rb * p.slices + slice0) * kScaleBytes + 4 * (lane & 1);
-    }
-    auto fetch = [&](const Stage &s, uint32_t k) __attribute__((always_inline)) {
+    // part 0 to 2 of the codes of slice k (past the end the last one's again,
+    // which is not read: a branch here would part the matrix instructions from
+    // their operands' reads)
+    auto fetch_part = [&](const Stage &s, uint32_t k, int part) __attribute__((always_inline)) {
         asm volatile("" ::: "memory");
-        const uint64_t c = static_cast<uint64_t>(k) * kCodeBytes, f = static_cast<uint64_t>(k) * kScaleBytes;
+        const uint64_t c = static_cast<uint64_t>(min(k, slices - 1)) * kCodeBytes;
 #pragma unroll
         for (int i = 0; i < kRowLoads; ++i) {
-            dma16(ga[i] + c, s.a + 1024 * (4 * i + wave));
-            dma16(gb[i] + c, s.b + 1024 * (4 * i + wave));
-        }
-#pragma unroll
-        for (int i = 0; i < kScaleLoads; ++i) {
-            dma4(gsa[i] + f, s.sa + 256 * (4 * i + wave));
-            dma4(gsb[i] + f, s.sb + 256 * (4 * i + wave));
+            if (i * 3 / kRowLoads != part) continue;
+            dma16(base_a + c + oa[i], s.a + 1024 * (kWaves * i + wave));
+            dma16(base_b + c + ob[i], s.b + 1024 * (kWaves * i + wave));
         }
         asm volatile("" ::: "memory");
     };
-    constexpr int kLoads = 2 * (kRowLoads + kScaleLoads);
-
-    f32x16 acc[B][B] = {};
-    const int wm = (wave >> 1) * (T / 2), wn = (wave & 1) * (T / 2), row = lane & 31, half = lane >> 5;
-    auto multiply = [&](const Stage &s) __attribute__((always_inline)) {
-        uint32_t sa[B], sb[B];
+    // the scales of the four slices from k on, a lane four bytes of the row
+    // whose codes it transfers (its offset in scales is a sixteenth); words past
+    // the row's end repeat the last.  Rows eight apart hold their words in
+    // another order, or they would share banks.
+    auto fetch_scales = [&](uint32_t k) __attribute__((always_inline)) {
+        asm volatile("" ::: "memory");
+        const uint32_t word = 4 * min(2 * k + ((lane & 7) ^ (2 * (wave & 3))), 2 * slices - 1);
+        const uint32_t to = (k & 4) / 4 * (T * kGroup) + 256 * wave;
 #pragma unroll
-        for (int i = 0; i < B; ++i) {
-            sa[i] = *reinterpret_cast<const uint32_t *>(s.sa + (wm + 32 * i + row) * kScaleBytes + 4 * half);
-            sb[i] = *reinterpret_cast<const uint32_t *>(s.sb + (wn + 32 * i + row) * kScaleBytes + 4 * half);
+        for (int i = 0; i < kRowLoads; ++i) {
+            dma4(base_sa + (oa[i] >> 4) - block + word, scales_a + to + 256 * kWaves * i);
+            dma4(base_sb + (ob[i] >> 4) - block + word, scales_b + to + 256 * kWaves * i);
         }
+        asm volatile("" ::: "memory");
+    };
+
+    f32x16 acc[BM][BN] = {};
+    const int wm = (wave / kWavesN) * WM, wn = (wave % kWavesN) * WN, row = lane & 31, half = lane >> 5;
+    struct Frags {
+        u32x4 a[BM], b[BN];
+    };
+    auto read = [&](Frags &f, const Stage &s, int step) __attribute__((always_inline)) {
+        const int unit = 16 * ((4 * half + step) ^ ((row >> 1) & 7));
+#pragma unroll
+        for (int i = 0; i < BM; ++i) f.a[i] = *reinterpret_cast<const u32x4 *>(s.a + (wm + 32 * i + row) * kCodeBytes + unit);
+#pragma unroll
+        for (int j = 0; j < BN; ++j) f.b[j] = *reinterpret_cast<const u32x4 *>(s.b + (wn + 32 * j + row) * kCodeBytes + unit);
+    };
+    // slice k is in `here` once every wave has passed the barrier, which also
+    // frees the other stage for slice k + 1
+    auto slice = [&](const Stage &here, const Stage &freed, uint32_t k) __attribute__((always_inline)) {
+        stage_barrier<0>();
+        if (G > 1 && k >= slices) return;  // uniform in a wave
+        if ((k & 3) == 3 && k + 1 < slices) fetch_scales(k + 1);
+        uint32_t sa[BM], sb[BN];
+        Frags f[2];
+        read(f[0], here, 0);
+        const uint32_t at = (k & 4) / 4 * (T * kGroup) + 4 * ((2 * (k & 3) + half) ^ (2 * ((row >> 3) & 3)));
+#pragma unroll
+        for (int i = 0; i < BM; ++i) sa[i] = *reinterpret_cast<const uint32_t *>(scales_a + at + (wm + 32 * i + row) * kGroup);
+#pragma unroll
+        for (int j = 0; j < BN; ++j) sb[j] = *reinterpret_cast<const uint32_t *>(scales_b + at + (wn + 32 * j + row) * kGroup);
         auto step = [&](auto st) __attribute__((always_inline)) {
             constexpr int S = decltype(st)::value;
-            const int unit = 16 * ((4 * half + S) ^ (row & 7));
-            u32x4 a[B], b[B];
+            if constexpr (S < 3) read(f[(S + 1) & 1], here, S + 1);
+            const Frags &h = f[S & 1];
 #pragma unroll
-            for (int i = 0; i < B; ++i) {
-                a[i] = *reinterpret_cast<const u32x4 *>(s.a + (wm + 32 * i + row) * kCodeBytes + unit);
-                b[i] = *reinterpret_cast<const u32x4 *>(s.b + (wn + 32 * i + row) * kCodeBytes + unit);
-            }
+            for (int i = 0; i < BM; ++i)
 #pragma unroll
-            for (int i = 0; i < B; ++i)
-#pragma unroll
-                for (int j = 0; j < B; ++j) acc[i][j] = mfma<S>(a[i], b[j], acc[i][j], sa[i], sb[j]);
+                for (int j = 0; j < BN; ++j) acc[i][j] = mfma<S>(h.a[i], h.b[j], acc[i][j], sa[i], sb[j]);
+            if constexpr (S < 3) fetch_part(freed, k + 1, S);
+            __builtin_amdgcn_sched_barrier(0);
         };
         step(std::integral_constant<int, 0>{});
         step(std::integral_constant<int, 1>{});
         step(std::integral_constant<int, 2>{});
         step(std::integral_constant<int, 3>{});
     };
-
-    auto slice = [&](const Stage &here, const Stage &next, uint32_t k) __attribute__((always_inline)) {
-        if (k + 1 < slices) {
-            fetch(next, k + 1);
-            stage_barrier<kLoads>();
-        } else {
-            stage_barrier<0>();
-        }
-        multiply(here);
-        stage_barrier<63>();  // its LDS reads are done before the stage is filled again
-    };
     if (slices > 0) {
-        fetch(s0, 0);
-        for (uint32_t k = 0; k < slices; k += 2) {
-            slice(s0, s1, k);
-            if (k + 1 < slices) slice(s1, s0, k + 1);
-        }
+        fetch_scales(0);
+#pragma unroll
+        for (int part = 0; part < 3; ++part) fetch_part(s0, 0, part);
     }
-    // lane: column n = lane % 32 of a block, rows 8 (q / 4) + 4 (lane / 32) + q % 4
-    const uint64_t out0 = MODE == kShared ? static_cast<uint64_t>(expert) * p.M : 0u;
+    for (uint32_t k = 0; k < turns; k += 2) {
+        slice(s0, s1, k);
+        if (k + 1 < turns) slice(s1, s0, k + 1);
+    }
+    const uint64_t out0 = MODE == kShared ? static_cast<uint64_t>(expert) * p.M : static_cast<uint64_t>(z) * p.M;
+    auto put = [&](uint32_t m, uint32_t n, const float v[8]) __attribute__((always_inline)) {
+        uint64_t at = out0 + m;
+        if constexpr (MODE == kRows) at = static_cast<uint32_t>(p.order[m]);
+        store8<O>(p.out, at * p.ld + n, p.N - n, v);
+    };
+    // Out through LDS, 32 rows of the wave's at a time, so that a store covers
+    // whole 16-byte pieces of a row.  The accumulators hold column lane % 32 of
+    // a block and rows 8 (q / 4) + 4 (lane / 32) + q % 4; rows of the upper
+    // half-wave have their columns' 32s swapped, or both would write one bank.
+    constexpr int W = WN, swap = W >= 64 ? 32 : 0;
+    constexpr int kPart = 32 * W;  // floats; half of a team's waves in either stage
+    static_assert(kPart * 4 * kWaves <= 2 * sizeof(Stage), "the output's parts fit the stages");
+    auto part_of = [&](int t, int w) __attribute__((always_inline)) {
+        return reinterpret_cast<float *>((w < kWaves / 2 ? stage0[t].a : stage1[t].a)) + w % (kWaves / 2) * kPart;
+    };
+    stage_barrier<0>();
+    float *stage = part_of(team, wave);
 #pragma unroll
-    for (int i = 0; i < B; ++i)
+    for (int i = 0; i < BM; ++i) {
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-            const uint32_t m = m0 + wm + 32 * i + 8 * (q >> 2) + 4 * half + (q & 3);
-            if (m >= m_end) continue;
-            uint64_t at = out0 + m;
-            if constexpr (MODE == kRows) at = static_cast<uint32_t>(p.order[m]);
+        for (int j = 0; j < BN; ++j)
 #pragma unroll
-            for (int j = 0; j < B; ++j) {
-                const uint32_t n = n0 + wn + 32 * j + row;
-                if (n < p.N) store_value<O>(p.out, at * p.ld + n, acc[i][j][q]);
+            for (int q = 0; q < 16; ++q)
+                stage[(8 * (q >> 2) + 4 * half + (q & 3)) * W + ((32 * j + row) ^ (swap * half))] = acc[i][j][q];
+        if constexpr (G > 1) __syncthreads();
+        // the teams share a wave's rows out
+        for (int c = lane + 64 * team; c < kPart / 8; c += 64 * G) {
+            const int r = c / (W / 8), col = c % (W / 8) * 8, from = r * W + (col ^ (swap * ((r >> 2) & 1)));
+            const uint32_t m = m0 + wm + 32 * i + r, n = n0 + wn + col;
+            if (m >= m_end || n >= p.N) continue;
+            float v[8];
+            __builtin_memcpy(v, part_of(0, wave) + from, 32);
+#pragma unroll
+            for (int t = 1; t < G; ++t) {
+                float u[8];
+                __builtin_memcpy(u, part_of(t, wave) + from, 32);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += u[e];
             }
+            put(m, n, v);
         }
+        if (G > 1 && i + 1 < BM) __syncthreads();
+    }
+}
+
+// The sum of the parts in order, rounded to the output's type.
+template <Mx4Type O>
+__global__ __launch_bounds__(kThreads) void mx4_join_kernel(const float *__restrict__ parts, uint32_t splits, uint32_t M,
+                                                            uint32_t N, void *__restrict__ out, uint64_t ld) {
+    const uint32_t chunks = (N + 7) / 8;
+    const uint64_t size = static_cast<uint64_t>(M) * N;
+    const uint64_t t = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x, m = t / chunks;
+    if (m >= M) return;
+    const uint32_t n = 8 * static_cast<uint32_t>(t - m * chunks);
+    float sum[8];
+    load8<Mx4Type::F32>(parts, m * N + n, N - n, sum);
+#pragma unroll 4
+    for (uint32_t z = 1; z < splits; ++z) {
+        float v[8];
+        load8<Mx4Type::F32>(parts, z * size + m * N + n, N - n, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += v[e];
+    }
+    store8<O>(out, m * ld + n, N - n, sum);
+}
+
+// ---------------------------------------------------------------------------
+// few rows
+// ---------------------------------------------------------------------------
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// A row's slice as v_mfma_scale_f32_16x16x128_f8f6f4 takes it: lane l has row
+// l % 16 and, in step s of two, block 4 s + l / 16.
+struct Slice16 {
+    u32x4 codes[2];
+    u32x2 scales;
+    __device__ __forceinline__ void load(const Mx4Matrix &m, uint64_t row_slice, int g) {
+        const uint8_t *p = m.codes + row_slice * kCodeBytes + 16 * g;
+        codes[0] = *reinterpret_cast<const u32x4 *>(p);
+        codes[1] = *reinterpret_cast<const u32x4 *>(p + 64);
+        scales = *reinterpret_cast<const u32x2 *>(m.scales + row_slice * kScaleBytes);
+    }
+    __device__ __forceinline__ uint32_t scale(int s, int g) const { return scales[s] >> (8 * g); }
+};
+
+__device__ __forceinline__ f32x4_t mfma16(u32x4 a, u32x4 b, f32x4_t c, uint32_t sa, uint32_t sb) {
+    const i32x8 a8 = {static_cast<int>(a[0]), static_cast<int>(a[1]), static_cast<int>(a[2]), static_cast<int>(a[3]), 0, 0, 0, 0};
+    const i32x8 b8 = {static_cast<int>(b[0]), static_cast<int>(b[1]), static_cast<int>(b[2]), static_cast<int>(b[3]), 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, c, 4, 4, 0, static_cast<int>(sa), 0, static_cast<int>(sb));
+}
+
+// Up to 16 MT rows of a: b is read once, straight into registers, by
+// workgroups of 16 NT of its rows whose waves share the slices out in turn (a
+// wave issues the loads of AHEAD slices before it uses the first), and the
+// waves' sums are joined in LDS in the waves' order.
+// X: the type of a dense x that every workgroup packs into LDS for itself while
+// its first loads of b are in flight (kPacked: a is packed already).
+constexpr int kPacked = -1;
+// waves of a workgroup: their sums fit 64 KB
+constexpr int most_waves(int tiles) { return tiles <= 4 ? 16 : 64 / tiles; }
+
+template <int MT, int NT, int AHEAD, Mode MODE, Mx4Type O, int X>
+__global__ __launch_bounds__(64 * most_waves(MT * NT)) void mx4_few_rows_kernel(Mx4Product p, uint32_t tiles_n,
+                                                                                uint32_t pairs, const void *x,
+                                                                                uint64_t x_cols, uint64_t ldx) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
+    const int r = lane & 15, g = lane >> 4;
+    const uint32_t tn = blockIdx.x % tiles_n, tm = blockIdx.x / tiles_n;
+    uint32_t m0 = tm * 16 * MT, m_end = p.M, expert = 0, slices = p.slices;
+    if constexpr (MODE == kRows) {
+        const SlotTile s = slot_tile(p, pairs, tm, 16 * MT);
+        if (s.expert > p.experts) return;  // uniform
+        expert = s.expert;
+        m0 = s.begin;
+        m_end = s.end;
+        if (expert == p.experts) slices = 0;  // slots of no expert: zero rows
+    }
+    const uint32_t n0 = tn * 16 * NT;
+    const uint64_t b_first = MODE == kRows ? static_cast<uint64_t>(min(expert, p.experts - 1)) * p.N : 0u;
+    uint64_t a_row[MT], b_row[NT];  // first slices
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        uint64_t row = min(m0 + 16 * i + r, m_end - 1);
+        if constexpr (MODE == kRows) row = static_cast<uint32_t>(p.order[row]) / p.per_token;
+        a_row[i] = row * p.slices;
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) b_row[j] = (b_first + min(n0 + 16 * j + r, p.N - 1)) * p.slices;
+
+    Slice16 a[AHEAD][MT], b[AHEAD][NT];
+    auto load = [&](uint32_t k0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const uint32_t k = min(k0 + u * waves, slices - 1);  // past the end: the last slice again, not used
+#pragma unroll
+            for (int j = 0; j < NT; ++j) b[u][j].load(p.b, b_row[j] + k, g);
+            if constexpr (X == kPacked)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) a[u][i].load(p.a, a_row[i] + k, g);
+        }
+    };
+    uint32_t k0 = wave;
+    if (k0 < slices) load(k0);
+    if constexpr (X != kPacked) {
+        constexpr Mx4Type T = static_cast<Mx4Type>(X == kPacked ? 0 : X);
+        constexpr int size = T == Mx4Type::F32 ? 4 : 2;
+        const uint32_t blocks = p.slices * 8, all = p.M * blocks;
+        for (uint32_t t = tid; t < all; t += blockDim.x) {
+            const uint32_t row = t / blocks, blk = t - row * blocks;
+            const uint8_t *from = static_cast<const uint8_t *>(x) + static_cast<uint64_t>(row) * ldx * size;
+            Eight<T> v[4];
+            if (32ull * blk + 32 <= x_cols) {
+                __builtin_memcpy(v, from + 32ull * blk * size, sizeof v);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) v[q].load(from, 32ull * blk + 8 * q, x_cols);
+            }
+            const uint32_t byte = mx4_scale_byte(f32_bits<T>(max(max(v[0].top(), v[1].top()), max(v[2].top(), v[3].top()))));
+            u32x4 c = {0, 0, 0, 0};
+            if (byte != 255u) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) c[q] = v[q].codes(mx4_power(byte));
+            }
+            *reinterpret_cast<u32x4 *>(lds + 16 * t) = c;
+            lds[16 * all + t] = static_cast<uint8_t>(byte);
+        }
+        __syncthreads();
+    }
+    f32x4_t acc[MT][NT] = {};
+    while (k0 < slices) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const uint32_t k = k0 + u * waves;
+            if (k >= slices) break;  // uniform
+            if constexpr (X != kPacked) {
+                const Mx4Matrix packed{lds, lds + 16 * 8 * p.M * p.slices};
+                a[u][0].load(packed, a_row[0] + k, g);
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        acc[i][j] = mfma16(a[u][i].codes[s], b[u][j].codes[s], acc[i][j], a[u][i].scale(s, g), b[u][j].scale(s, g));
+        }
+        k0 += AHEAD * waves;
+        if (k0 < slices) load(k0);
+    }
+    if constexpr (X != kPacked) __syncthreads();  // the packed x is done with
+    // lane: column n = lane % 16 of a tile, rows 4 (lane / 16) + q
+    float *part = reinterpret_cast<float *>(lds);  // [wave][16 MT][16 NT]
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                part[(wave * 16 * MT + 16 * i + 4 * g + q) * (16 * NT) + 16 * j + r] = acc[i][j][q];
+    __syncthreads();
+    for (uint32_t t = tid; t < 16 * MT * 16 * NT; t += blockDim.x) {
+        const uint32_t m = m0 + t / (16 * NT), n = n0 + t % (16 * NT);
+        if (m >= m_end || n >= p.N) continue;
+        float sum = part[t];
+        for (int w = 1; w < waves; ++w) sum += part[w * 16 * MT * 16 * NT + t];
+        uint64_t at = m;
+        if constexpr (MODE == kRows) at = static_cast<uint32_t>(p.order[m]);
+        store_value<O>(p.out, at * p.ld + n, sum);
+    }
+}
+
+// Rows of x, and bytes of them packed, that are worth packing again in every
+// workgroup rather than once in a launch of their own.
+constexpr uint32_t kPackRows = 4, kPackBytes = 32768;
+// Rows up to which b is streamed (16 x 4096 x 11008: 10.1 us; in tiles of 64 37
+// rows take 12.7).
+constexpr uint32_t kFewRows = 16;
+
+template <int MT, int NT, int AHEAD, Mode MODE, int X>
+void few_rows(const Mx4Product &p, uint64_t tiles_m, uint32_t pairs, const void *x, uint64_t x_cols, uint64_t ldx,
+              hipStream_t stream) {
+    const uint64_t tiles_n = ceil_div(p.N, 16 * NT);
+    const unsigned waves = std::min<unsigned>(most_waves(MT * NT), std::max(1u, (p.slices + AHEAD - 1) / AHEAD));
+    const uint64_t grid = tiles_n * tiles_m;
+    BSQ_REQUIRE(grid <= 0x7FFFFFFFull, "mx4 product: too large");
+    const unsigned lds = std::max(waves * MT * NT * 1024, X == kPacked ? 0u : p.M * p.slices * 136);
+    by_type(p.type, [&](auto t) {
+        mx4_few_rows_kernel<MT, NT, AHEAD, MODE, decltype(t)::value, X>
+            <<<static_cast<unsigned>(grid), 64 * waves, lds, stream>>>(p, static_cast<uint32_t>(tiles_n), pairs, x, x_cols, ldx);
+    });
 }
 
 }  // namespace
 
-uint64_t mx4_product_workspace(uint32_t, uint32_t, uint32_t) { return 0; }
+bool mx4_packs_on_the_way(uint64_t m, uint64_t slices) { return m <= kPackRows && m * slices * 136 <= kPackBytes; }
 
-void launch_mx4_product(const Mx4Product &p, void *, uint64_t, hipStream_t stream) {
+void launch_mx4_product_of(const void *x, Mx4Type x_type, uint64_t x_cols, uint64_t ldx, const Mx4Product &p,
+                           hipStream_t stream) {
     if (p.M == 0 || p.N == 0) return;
-    constexpr uint32_t T = 128;
-    const uint64_t tiles_n = ceil_div(p.N, T);
-    by_type(p.type, [&](auto t) {
-        constexpr Mx4Type O = decltype(t)::value;
-        if (p.shared_slots) {
-            const uint64_t grid = tiles_n * ceil_div(p.M, T);
-            BSQ_REQUIRE(grid <= 0x7FFFFFFFull && p.experts <= 65535, "mx4 product: too large");
-            mx4_product_kernel<T, kShared, O><<<dim3(static_cast<unsigned>(grid), p.experts), kThreads, 0, stream>>>(
-                p, static_cast<uint32_t>(tiles_n), 0);
-        } else if (p.offsets != nullptr) {
-            // M: the pairs
-            const uint64_t grid = tiles_n * (ceil_div(p.M, T) + p.experts + 1);
-            BSQ_REQUIRE(grid <= 0x7FFFFFFFull, "mx4 product: too large");
-            mx4_product_kernel<T, kRows, O><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(
-                p, static_cast<uint32_t>(tiles_n), p.M);
-        } else {
-            const uint64_t grid = tiles_n * ceil_div(p.M, T);
-            BSQ_REQUIRE(grid <= 0x7FFFFFFFull, "mx4 product: too large");
-            mx4_product_kernel<T, kDense, O><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(
-                p, static_cast<uint32_t>(tiles_n), 0);
-        }
+    by_type(x_type, [&](auto t) {
+        few_rows<1, 1, 4, kDense, static_cast<int>(decltype(t)::value)>(p, 1, 0, x, x_cols, ldx, stream);
     });
+    BSQ_HIP(hipGetLastError());
+}
+
+namespace {
+
+// How a product is cut.  Measured in us (M x N x K, tile . teams):
+//   2048 x 4096 x 4096    64.1 33.6   128.1 27.4   128.2 31.6   256 38.7
+//   1024 x 4096 x 4096    64.1 18.8   64.2 20.6    128.1 18.0   128.2 17.1
+//    512 x 4096 x 4096    64.1 12.5   64.2 11.8    64.4 16.1    128.2 15.3
+//    256 x 4096 x 4096    64.1 11.1   64.2 8.9     64.4 8.7
+//   2000 x  300 x  512    64.1 4.5    64.2 4.4     64.4 5.2
+// Teams as long as every workgroup still finds a CU of its own; tiles of 256
+// where their rounds over the CUs cost less (a round of one a CU 2.4 us a
+// slice, of two 128s a CU 1.44).
+struct Plan {
+    uint32_t tile, tiles_m, tiles_n, teams, splits;
+    uint64_t bytes;
+};
+Plan plan_of(uint32_t M, uint32_t N, uint32_t slices) {
+    const uint64_t cus = static_cast<uint64_t>(cu_count());
+    auto tiles = [&](uint64_t t) { return ceil_div(M, t) * ceil_div(N, t); };
+    Plan q{128, 0, 0, 1, 1, 0};
+    if (tiles(128) > 2 * cus) {
+        if (2.4 * ceil_div(tiles(256), cus) < 1.44 * ceil_div(tiles(128), 2 * cus)) q.tile = 256;
+    } else if (tiles(64) > 2 * cus) {
+        q.teams = tiles(128) <= cus && slices > 1 ? 2 : 1;
+    } else {
+        q.tile = 64;
+        q.teams = slices == 1 ? 1 : tiles(64) > cus || slices < 8 ? 2 : 4;
+    }
+    if (q.tile == 64 && q.teams == 4) {
+        // more workgroups for a long shared axis: a turn of four slices 1.6 us,
+        // against the join's launch and the parts' way to memory and back (37
+        // x 4096 x 11008: 19.5 us with one split, 12.7 with 4; 128 x 128 x
+        // 60000: 70 and, with 8, 15.8)
+        double best = 0.0;
+        for (uint32_t s = 1; s <= 16 && tiles(64) * s <= 2 * cus; s *= 2) {
+            const double t = 1.6 * ceil_div(slices, 4 * s) + (s > 1 ? 4.0 + s * (8.0 * M * N / 2.5e6) : 0.0);
+            if (s == 1 || t < best) {
+                best = t;
+                q.splits = s;
+            }
+        }
+    }
+    q.tiles_m = static_cast<uint32_t>(ceil_div(M, q.tile));
+    q.tiles_n = static_cast<uint32_t>(ceil_div(N, q.tile));
+    q.bytes = q.splits > 1 ? static_cast<uint64_t>(q.splits) * M * N * 4 : 0;
+    return q;
+}
+
+template <int T, int G, Mode MODE>
+void tiles(const Mx4Product &p, uint64_t tiles_m, uint64_t tiles_n, uint32_t splits, hipStream_t stream) {
+    const uint64_t grid = tiles_m * tiles_n * splits;
+    BSQ_REQUIRE(grid <= 0x7FFFFFFFull, "mx4 product: too large");
+    const dim3 g(static_cast<unsigned>(grid), MODE == kShared ? p.experts : 1);
+    by_type(p.type, [&](auto t) {
+        mx4_product_kernel<T, G, MODE, decltype(t)::value><<<g, 64 * G * kTeam<T>, 0, stream>>>(
+            p, static_cast<uint32_t>(tiles_m), static_cast<uint32_t>(tiles_n), splits);
+    });
+}
+
+}  // namespace
+
+uint64_t mx4_product_workspace(uint32_t M, uint32_t N, uint32_t slices) {
+    return M <= kFewRows || N == 0 ? 0 : plan_of(M, N, slices).bytes;
+}
+
+void launch_mx4_product(const Mx4Product &p, void *workspace, uint64_t workspace_bytes, hipStream_t stream) {
+    if (p.M == 0 || p.N == 0) return;
+    if (p.shared_slots) {
+        tiles<256, 1, kShared>(p, ceil_div(p.M, 256), ceil_div(p.N, 256), 1, stream);
+    } else if (p.offsets != nullptr) {
+        // M: the pairs; every expert's tiles, and those of the pairs of none
+        auto of = [&](uint64_t t) { return ceil_div(p.M, t) + p.experts + 1; };
+        // (16384 pairs of 32 experts, 2752 x 4096: 64 250 us, 128 208, 256 221)
+        const uint64_t each = p.M / p.experts;
+        if (each <= 16) few_rows<1, 1, 4, kRows, kPacked>(p, of(16), p.M, nullptr, 0, 0, stream);
+        else if (each <= 64) tiles<64, 1, kRows>(p, of(64), ceil_div(p.N, 64), 1, stream);
+        else tiles<128, 1, kRows>(p, of(128), ceil_div(p.N, 128), 1, stream);
+    } else if (p.M <= kFewRows) {
+        few_rows<1, 1, 4, kDense, kPacked>(p, 1, 0, nullptr, 0, 0, stream);
+    } else {
+        const Plan q = plan_of(p.M, p.N, p.slices);
+        BSQ_REQUIRE(workspace_bytes >= q.bytes, "mx4 product: workspace too small");
+        Mx4Product part = p;
+        if (q.splits > 1) {
+            part.out = workspace;
+            part.type = Mx4Type::F32;
+            part.ld = p.N;
+        }
+        if (q.tile == 256) tiles<256, 1, kDense>(part, q.tiles_m, q.tiles_n, q.splits, stream);
+        else if (q.tile == 128 && q.teams == 2) tiles<128, 2, kDense>(part, q.tiles_m, q.tiles_n, q.splits, stream);
+        else if (q.tile == 128) tiles<128, 1, kDense>(part, q.tiles_m, q.tiles_n, q.splits, stream);
+        else if (q.teams == 4) tiles<64, 4, kDense>(part, q.tiles_m, q.tiles_n, q.splits, stream);
+        else if (q.teams == 2) tiles<64, 2, kDense>(part, q.tiles_m, q.tiles_n, q.splits, stream);
+        else tiles<64, 1, kDense>(part, q.tiles_m, q.tiles_n, q.splits, stream);
+        if (q.splits > 1) {
+            by_type(p.type, [&](auto t) {
+                const uint64_t grid = ceil_div(p.M * ceil_div(p.N, 8), kThreads);
+                mx4_join_kernel<decltype(t)::value><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(
+                    static_cast<const float *>(workspace), q.splits, p.M, p.N, p.out, p.ld);
+            });
+        }
+    }
     BSQ_HIP(hipGetLastError());
 }
 
