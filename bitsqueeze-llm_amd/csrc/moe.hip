@@ -20,20 +20,34 @@ constexpr uint32_t kMaxExperts = 1024, kMaxChosen = 64, kMaxGroups = 64;
 // one wave's reductions through DPP moves; the result in every lane
 // ---------------------------------------------------------------------------
 template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or(int other, int v) {
+    return __builtin_amdgcn_update_dpp(other, v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
 __device__ __forceinline__ float dpp_or(float other, float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(other), __float_as_int(v), CTRL, ROWS, 0xF, false));
+    return __int_as_float(dpp_or<CTRL, ROWS>(__float_as_int(other), __float_as_int(v)));
 }
 __device__ __forceinline__ float from_lane(float v, int lane) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
 }
-__device__ __forceinline__ float wave_max(float v) {
-    v = fmaxf(v, dpp_or<0xB1, 0xF>(v, v));
-    v = fmaxf(v, dpp_or<0x4E, 0xF>(v, v));
-    v = fmaxf(v, dpp_or<0x141, 0xF>(v, v));
-    v = fmaxf(v, dpp_or<0x140, 0xF>(v, v));
-    v = fmaxf(v, dpp_or<0x142, 0xA>(v, v));
-    v = fmaxf(v, dpp_or<0x143, 0xC>(v, v));
-    return from_lane(v, 63);
+__device__ __forceinline__ int wave_max(int v) {
+    v = max(v, dpp_or<0xB1, 0xF>(v, v));
+    v = max(v, dpp_or<0x4E, 0xF>(v, v));
+    v = max(v, dpp_or<0x141, 0xF>(v, v));
+    v = max(v, dpp_or<0x140, 0xF>(v, v));
+    v = max(v, dpp_or<0x142, 0xA>(v, v));
+    v = max(v, dpp_or<0x143, 0xC>(v, v));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+// over each aligned run of `lanes` (a power of two), in every lane of it
+__device__ __forceinline__ int run_max(int v, uint32_t lanes) {
+    if (lanes > 1) v = max(v, dpp_or<0xB1, 0xF>(v, v));
+    if (lanes > 2) v = max(v, dpp_or<0x4E, 0xF>(v, v));
+    if (lanes > 4) v = max(v, dpp_or<0x141, 0xF>(v, v));
+    if (lanes > 8) v = max(v, dpp_or<0x140, 0xF>(v, v));
+    if (lanes > 16) v = max(v, __shfl_xor(v, 16));
+    if (lanes > 32) v = max(v, __shfl_xor(v, 32));
+    return v;
 }
 __device__ __forceinline__ float wave_sum(float v) {
     v += dpp_or<0xB1, 0xF>(0.0f, v);
@@ -44,6 +58,14 @@ __device__ __forceinline__ float wave_sum(float v) {
     v += dpp_or<0x143, 0xC>(0.0f, v);
     return from_lane(v, 63);
 }
+
+// Keys as integers that order as the floats do (-0 as 0), and back.
+constexpr int kShut = static_cast<int>(0x807FFFFFu);  // -infinity
+__device__ __forceinline__ int key_of(float f) {
+    const int b = __float_as_int(f + 0.0f);
+    return b ^ ((b >> 31) & 0x7FFFFFFF);
+}
+__device__ __forceinline__ float value_of(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7FFFFFFF)); }
 
 template <Mx4Type T>
 constexpr float kLowest = T == Mx4Type::F32 ? -FLT_MAX : T == Mx4Type::BF16 ? -0x1.FEp127f : -65504.0f;
@@ -60,17 +82,29 @@ struct RouteArgs {
 // A token's logits: expert e = lane * NV + i.  Experts that are closed to the
 // token (at or below the type's lowest value, or NaN) and those past the end
 // read -infinity.
+template <Mx4Type T>
+__device__ __forceinline__ float open_logit(float v) {
+    return v > kLowest<T> ? fminf(v, FLT_MAX) : -INFINITY;
+}
 template <Mx4Type T, int NV>
 __device__ __forceinline__ void load_logits(const RouteArgs &a, uint64_t t, uint32_t lane, float x[NV]) {
     const uint32_t e0 = lane * NV;
     const uint64_t at = t * a.ld + e0;
+    if (e0 + NV <= a.experts) {
+        if constexpr (T == Mx4Type::F32) {
+            __builtin_memcpy(x, static_cast<const float *>(a.logits) + at, 4 * NV);
+        } else {
+            uint16_t h[NV];
+            __builtin_memcpy(h, static_cast<const uint16_t *>(a.logits) + at, 2 * NV);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        x[i] = -INFINITY;
-        if (e0 + i < a.experts) {
-            const float v = load_value<T>(a.logits, at + i);
-            x[i] = v > kLowest<T> ? fminf(v, FLT_MAX) : -INFINITY;
+            for (int i = 0; i < NV; ++i) x[i] = T == Mx4Type::BF16 ? bf16_value(h[i]) : f16_value(h[i]);
         }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) x[i] = open_logit<T>(x[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            x[i] = e0 + i < a.experts ? open_logit<T>(load_value<T>(a.logits, at + i)) : -INFINITY;
     }
 }
 
@@ -83,7 +117,7 @@ __device__ __forceinline__ void softmax_of(const float x[NV], float e[NV], float
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < NV; ++i) m = fmaxf(m, x[i]);
-    top = wave_max(m);
+    top = value_of(wave_max(key_of(m)));
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -93,156 +127,248 @@ __device__ __forceinline__ void softmax_of(const float x[NV], float e[NV], float
     sum = fmaxf(wave_sum(s), 1.0f);
 }
 
-// One wave a token, its scores and keys in registers.  The largest key of the
-// wave is a DPP reduction; the lowest lane that holds it (and its lowest
-// index) is the expert, so that ties go to the lowest.
+// A lane's keys in descending order, equal ones by their index: value q of the
+// list and its index in the q-th four bits of `where`.  Only neighbours change
+// places, so that equal keys keep their order.  Lists longer than four are not
+// sorted: their largest is found again each time.
+template <int NV>
+struct Keys {
+    int key[NV];
+    uint32_t where = 0;
+    static constexpr bool kSorted = NV <= 4;
+    __device__ __forceinline__ void sort() {
+        if constexpr (kSorted) {
+            uint32_t at[NV];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) at[i] = i;
+#pragma unroll
+            for (int r = 0; r < NV; ++r)
+#pragma unroll
+                for (int i = r & 1; i + 1 < NV; i += 2) {
+                    const bool swap = key[i + 1] > key[i];
+                    const int hi = max(key[i], key[i + 1]), lo = min(key[i], key[i + 1]);
+                    const uint32_t a = at[i], b = at[i + 1];
+                    at[i] = swap ? b : a;
+                    at[i + 1] = swap ? a : b;
+                    key[i] = hi;
+                    key[i + 1] = lo;
+                }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) where |= at[i] << (4 * i);
+        }
+    }
+    // the largest key and its index
+    __device__ __forceinline__ int head(uint32_t &at) const {
+        if constexpr (kSorted) {
+            at = where & 15u;
+            return key[0];
+        }
+        int m = key[0];
+        at = 0;
+#pragma unroll
+        for (int i = 1; i < NV; ++i) {
+            at = key[i] > m ? i : at;
+            m = max(m, key[i]);
+        }
+        return m;
+    }
+    __device__ __forceinline__ void drop(bool mine, uint32_t at) {
+        if constexpr (kSorted) {
+#pragma unroll
+            for (int i = 0; i + 1 < NV; ++i) key[i] = mine ? key[i + 1] : key[i];
+            key[NV - 1] = mine ? kShut : key[NV - 1];
+            where = mine ? where >> 4 : where;
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) key[i] = mine && at == static_cast<uint32_t>(i) ? kShut : key[i];
+        }
+    }
+};
+
+// Lane l's keys of groups that are not among the `kept` best become kShut.
+// A group's score: its largest key, with a bias the sum of its two largest.
+template <int NV>
+__device__ __forceinline__ void keep_groups(const RouteArgs &a, uint32_t lane, Keys<NV> &keys) {
+    const uint32_t each = a.experts / a.groups, run = each / NV;
+    const bool two = a.bias != nullptr;
+    if (Keys<NV>::kSorted && each % NV == 0 && (run & (run - 1)) == 0) {
+        // a group is an aligned run of lanes: all groups at once
+        const int best = run_max(keys.key[0], run);
+        int score = best;
+        if (two) {
+            const bool top = keys.key[0] == best;
+            const int other = top ? (NV > 1 ? keys.key[NV > 1 ? 1 : 0] : kShut) : keys.key[0];
+            int next = run_max(other, run);
+            const uint64_t tied = (__ballot(top) >> (lane & ~(run - 1))) & (run == 64 ? ~0ull : (1ull << run) - 1);
+            next = __builtin_popcountll(tied) > 1 ? best : next;
+            score = next > kShut ? key_of(value_of(best) + value_of(next)) : best;
+        }
+        // its rank: groups above it, and equal ones of a lower number
+        const uint32_t mine = lane / run;
+        uint32_t rank = 0;
+        for (uint32_t g = 0; g < a.groups; ++g) {
+            const int s = __builtin_amdgcn_readlane(score, static_cast<int>(g * run));
+            rank += s > score - (g < mine ? 1 : 0);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) keys.key[i] = rank < a.kept ? keys.key[i] : kShut;
+        return;
+    }
+    uint32_t group[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) group[i] = (lane * NV + (Keys<NV>::kSorted ? (keys.where >> (4 * i)) & 15u : i)) / each;
+    int of_group = kShut;
+    for (uint32_t g = 0; g < a.groups; ++g) {
+        int m = kShut;
+        uint32_t at = NV;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const bool more = group[i] == g && keys.key[i] > m;
+            m = more ? keys.key[i] : m;
+            at = more ? i : at;
+        }
+        const int best = wave_max(m);
+        int s = best;
+        if (two && best > kShut) {
+            const bool first = lane == static_cast<uint32_t>(__builtin_ctzll(__ballot(m == best)));
+            m = kShut;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (group[i] == g && !(first && at == static_cast<uint32_t>(i))) m = max(m, keys.key[i]);
+            const int next = wave_max(m);
+            s = next > kShut ? key_of(value_of(best) + value_of(next)) : best;
+        }
+        of_group = lane == g ? s : of_group;
+    }
+    uint64_t chosen = 0;
+    bool taken = lane >= a.groups;
+    for (uint32_t j = 0; j < a.kept; ++j) {
+        const int best = wave_max(taken ? kShut : of_group);
+        const uint64_t at = __ballot(!taken && of_group == best);
+        if (at == 0) break;
+        const int g = __builtin_ctzll(at);
+        chosen |= 1ull << g;
+        taken |= lane == static_cast<uint32_t>(g);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) keys.key[i] = group[i] < 64 && ((chosen >> group[i]) & 1) ? keys.key[i] : kShut;
+}
+
+// One wave a token, NV experts a lane.  The largest of the lanes' largest keys
+// is a DPP reduction of integers; the lowest lane that holds it gives the
+// expert, so that ties go to the lowest.  Lane j then forms the weight of the
+// j-th choice from that expert's own logit.
 template <Mx4Type T, int NV>
 __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a, int32_t *__restrict__ ids,
                                                         float *__restrict__ weights) {
     const uint32_t lane = threadIdx.x & 63;
     const uint64_t t = static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (t >= a.tokens) return;  // whole waves
-    float x[NV], score[NV], key[NV];
+    float x[NV], score[NV], top = 0.0f, sum = 1.0f;
     load_logits<T, NV>(a, t, lane, x);
-    if (a.sigmoid) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) score[i] = sigmoid_of(x[i]);
-    } else {
-        float top, sum;
+    Keys<NV> keys;
+    if (!a.sigmoid) {
         softmax_of<NV>(x, score, top, sum);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) score[i] /= sum;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        key[i] = x[i];
+        keys.key[i] = key_of(x[i]);
         if (a.bias != nullptr && x[i] > -INFINITY) {
-            const float v = score[i] + a.bias[lane * NV + i];
-            key[i] = v > -INFINITY ? v : -INFINITY;
+            const float v = (a.sigmoid ? sigmoid_of(x[i]) : score[i] / sum) + a.bias[lane * NV + i];
+            keys.key[i] = v > -INFINITY ? key_of(v) : kShut;
         }
     }
-    if (a.groups > 1) {
-        const uint32_t each = a.experts / a.groups;
-        uint32_t group[NV];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) group[i] = (lane * NV + i) / each;
-        float of_group = -INFINITY;
-        for (uint32_t g = 0; g < a.groups; ++g) {
-            float m = -INFINITY;
-            uint32_t at = NV;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const bool more = group[i] == g && key[i] > m;
-                m = more ? key[i] : m;
-                at = more ? i : at;
-            }
-            const float best = wave_max(m);
-            float s = best;
-            if (a.bias != nullptr && best > -INFINITY) {  // and the second largest
-                const bool first = lane == static_cast<uint32_t>(__builtin_ctzll(__ballot(m == best)));
-                m = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    if (group[i] == g && !(first && at == static_cast<uint32_t>(i))) m = fmaxf(m, key[i]);
-                const float next = wave_max(m);
-                s = next > -INFINITY ? best + next : best;
-            }
-            of_group = lane == g ? s : of_group;
-        }
-        uint64_t chosen = 0;
-        bool taken = lane >= a.groups;
-        for (uint32_t j = 0; j < a.kept; ++j) {
-            const float best = wave_max(taken ? -INFINITY : of_group);
-            const uint64_t at = __ballot(!taken && of_group == best);
-            if (at == 0) break;
-            const int g = __builtin_ctzll(at);
-            chosen |= 1ull << g;
-            taken |= lane == static_cast<uint32_t>(g);
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) key[i] = group[i] < 64 && ((chosen >> group[i]) & 1) ? key[i] : -INFINITY;
-    }
+    keys.sort();
+    if (a.groups > 1) keep_groups<NV>(a, lane, keys);
     int32_t id = -1;
-    float mine = 0.0f, total = 0.0f;
     for (uint32_t j = 0; j < a.k; ++j) {
-        float m = key[0], s = score[0];
-        uint32_t at = 0;
-#pragma unroll
-        for (int i = 1; i < NV; ++i) {
-            const bool more = key[i] > m;
-            m = more ? key[i] : m;
-            s = more ? score[i] : s;
-            at = more ? i : at;
-        }
-        const float best = wave_max(m);
-        if (!(best > -INFINITY)) break;  // uniform: no expert is left
+        uint32_t at;
+        const int m = keys.head(at);
+        const int best = wave_max(m);
+        if (best == kShut) break;  // uniform: no expert is left
         const int from = __builtin_ctzll(__ballot(m == best));
-        const float w = from_lane(s, from);
         const int32_t e = from * NV + __builtin_amdgcn_readlane(static_cast<int>(at), from);
-        total += w;
         id = lane == j ? e : id;
-        mine = lane == j ? w : mine;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) key[i] = lane == static_cast<uint32_t>(from) && at == static_cast<uint32_t>(i) ? -INFINITY : key[i];
+        keys.drop(lane == static_cast<uint32_t>(from), at);
     }
+    float mine = 0.0f;
+    if (id >= 0) {
+        const float v = open_logit<T>(load_value<T>(a.logits, t * a.ld + id));
+        mine = a.sigmoid ? sigmoid_of(v) : expf(v - top) / sum;
+    }
+    const float total = a.renorm ? fmaxf(wave_sum(mine), FLT_MIN) : 1.0f;
     if (lane < a.k) {
         ids[t * a.k + lane] = id;
-        weights[t * a.k + lane] = (a.renorm ? mine / fmaxf(total, FLT_MIN) : mine) * a.scale;
+        weights[t * a.k + lane] = mine / total * a.scale;
     }
 }
 
 // d logits from d weights.  Lane j forms the score of the token's j-th expert
 // again from its own logit; with w_j = scale s_j / S the scores' gradient is
-// (g_j - sum g w / scale) / S, g = scale dw, and the scores' own rule follows.
+// (g_j - sum g w / scale) / S, g = scale dw, and the scores' own rule follows:
+// only the chosen for sigmoid, every expert for softmax.  The chosen reach
+// their experts' lanes through a row in LDS.
 template <Mx4Type T, int NV>
 __global__ __launch_bounds__(256) void moe_route_backward_kernel(RouteArgs a, const int32_t *__restrict__ ids,
                                                                  const float *__restrict__ d_weights,
                                                                  void *__restrict__ d_logits, uint64_t ldd) {
+    __shared__ float rows[4][64 * NV];
     const uint32_t lane = threadIdx.x & 63;
     const uint64_t t = static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (t >= a.tokens) return;
-    float x[NV], score[NV], top = 0.0f, sum = 1.0f;
-    load_logits<T, NV>(a, t, lane, x);
-    if (a.sigmoid) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) score[i] = sigmoid_of(x[i]);
-    } else {
+    if (t >= a.tokens) return;  // whole waves, which share nothing
+    float *row = rows[threadIdx.x >> 6];
+    float score[NV], top = 0.0f, sum = 1.0f;
+    if (!a.sigmoid) {
+        float x[NV];
+        load_logits<T, NV>(a, t, lane, x);
         softmax_of<NV>(x, score, top, sum);
 #pragma unroll
         for (int i = 0; i < NV; ++i) score[i] /= sum;
     }
-    int32_t id = lane < a.k ? ids[t * a.k + lane] : -1;
-    float s = 0.0f, d = 0.0f;
-    if (static_cast<uint32_t>(id) < a.experts) {
-        const float v = load_value<T>(a.logits, t * a.ld + id);
-        if (v > kLowest<T>) {
-            const float c = fminf(v, FLT_MAX);
-            s = a.sigmoid ? sigmoid_of(c) : expf(c - top) / sum;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) row[lane * NV + i] = 0.0f;
+    const int32_t id = lane < a.k ? ids[t * a.k + lane] : -1;
+    float s = 0.0f, rest = 0.0f, d = 0.0f;
+    bool real = static_cast<uint32_t>(id) < a.experts;
+    if (real) {
+        const float v = open_logit<T>(load_value<T>(a.logits, t * a.ld + id));
+        real = v > -INFINITY;
+        if (real) {
+            s = a.sigmoid ? sigmoid_of(v) : expf(v - top) / sum;
+            rest = a.sigmoid ? sigmoid_of(-v) : 0.0f;  // 1 - s, without the difference
             d = d_weights[t * a.k + lane] * a.scale;
-        } else {
-            id = -1;
         }
     }
     if (a.renorm) {
         const float total = fmaxf(wave_sum(s), FLT_MIN);
         const float mean = wave_sum(d * (s / total));
-        d = static_cast<uint32_t>(id) < a.experts ? (d - mean) / total : 0.0f;
+        d = real ? (d - mean) / total : 0.0f;
     }
     const float mean = a.sigmoid ? 0.0f : wave_sum(d * s);
-    float g[NV] = {};
-    for (uint32_t j = 0; j < a.k; ++j) {
-        const uint32_t e = static_cast<uint32_t>(__builtin_amdgcn_readlane(id, static_cast<int>(j)));
-        const float v = from_lane(d, static_cast<int>(j));
-#pragma unroll
-        for (int i = 0; i < NV; ++i) g[i] += lane * NV + i == e ? v : 0.0f;
-    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (real) row[id] = a.sigmoid ? d * s * rest : d;  // a choice has an expert once
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    float g[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const uint32_t e = lane * NV + i;
-        if (e >= a.experts) continue;
-        // 1 - sigmoid(x) = sigmoid(-x), without the difference
-        const float v = a.sigmoid ? g[i] * score[i] * sigmoid_of(-x[i]) : score[i] * (g[i] - mean);
-        store_value<T>(d_logits, t * ldd + e, x[i] > -INFINITY ? v : 0.0f);
+        g[i] = row[lane * NV + i];
+        if (!a.sigmoid) g[i] = score[i] * (g[i] - mean);
+    }
+    const uint32_t e0 = lane * NV;
+    const uint64_t at = t * ldd + e0;
+    if (e0 + NV <= a.experts) {
+        if constexpr (T == Mx4Type::F32) {
+            __builtin_memcpy(static_cast<float *>(d_logits) + at, g, 4 * NV);
+        } else {
+            uint16_t h[NV];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) h[i] = static_cast<uint16_t>(T == Mx4Type::BF16 ? bf16_bits(g[i]) : f16_bits(g[i]));
+            __builtin_memcpy(static_cast<uint16_t *>(d_logits) + at, h, 2 * NV);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (e0 + i < a.experts) store_value<T>(d_logits, at + i, g[i]);
     }
 }
 
