@@ -374,48 +374,76 @@ __global__ __launch_bounds__(256) void moe_route_backward_kernel(RouteArgs a, co
 
 // Pairs in the experts' order, the pairs of one expert by their number; those
 // of no expert last.  Workgroup e counts the pairs of lower experts and its own
-// (each wave a contiguous share), then writes its own in order: two reads of
-// the ids from cache a workgroup, no workspace and no atomics.
-__global__ void moe_plan_kernel(const int32_t *__restrict__ ids, uint32_t pairs, uint32_t experts,
-                                int32_t *__restrict__ offsets, int32_t *__restrict__ order) {
-    __shared__ uint32_t lower[16], own[16];
-    const uint32_t e = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const uint32_t share = ((pairs + waves - 1) / waves + 63) / 64 * 64;
-    const uint32_t from = min(wave * share, pairs), to = min(from + share, pairs);
-    auto expert = [&](uint32_t p) {
-        const uint32_t v = static_cast<uint32_t>(ids[p]);
-        return v < experts ? v : experts;
-    };
-    uint32_t lt = 0, eq = 0;
-    for (uint32_t p = from + lane; p < to; p += 64) {
-        const uint32_t v = expert(p);
-        lt += v < e;
-        eq += v == e;
-    }
+// (each wave a contiguous share), then writes its own in order: reads from
+// cache only, no workspace and no atomics.  The ids of up to 16384 pairs (16 a
+// lane) stay in registers; more are read again a tile at a time.
+constexpr uint32_t kPlanThreads = 1024, kPlanEach = 16, kPlanTile = kPlanThreads * kPlanEach;
+
+__device__ __forceinline__ void plan_expert(const int32_t *__restrict__ ids, uint32_t pairs, uint32_t experts, uint32_t e,
+                                            int32_t *__restrict__ offsets, int32_t *__restrict__ order) {
+    constexpr uint32_t kWaves = kPlanThreads / 64;
+    __shared__ uint32_t lower[kWaves], own[2][kWaves];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t v[kPlanEach];
+    auto load = [&](uint32_t base) __attribute__((always_inline)) {
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        lt += __shfl_xor(lt, d);
-        eq += __shfl_xor(eq, d);
+        for (uint32_t i = 0; i < kPlanEach; ++i) {
+            const uint32_t p = base + wave * (64 * kPlanEach) + 64 * i + lane;
+            const uint32_t id = p < pairs ? static_cast<uint32_t>(ids[p]) : 0u;
+            v[i] = p < pairs ? min(id, experts) : 0xFFFFFFFFu;
+        }
+    };
+    uint32_t lt = 0;
+    for (uint32_t base = 0; base < pairs; base += kPlanTile) {
+        load(base);
+#pragma unroll
+        for (uint32_t i = 0; i < kPlanEach; ++i) lt += __builtin_popcountll(__ballot(v[i] < e));
     }
-    if (lane == 0) {
-        lower[wave] = lt;
-        own[wave] = eq;
-    }
+    if (lane == 0) lower[wave] = lt;
     __syncthreads();
-    uint32_t begin = 0, at = 0;
-    for (uint32_t w = 0; w < waves; ++w) {
-        begin += lower[w];
-        at += w < wave ? own[w] : 0u;
+    uint32_t at = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kWaves; ++w) at += lower[w];
+    if (threadIdx.x == 0) offsets[e] = static_cast<int32_t>(at);
+    uint32_t turn = 0;
+    for (uint32_t base = 0; base < pairs; base += kPlanTile, turn ^= 1) {
+        if (pairs > kPlanTile) load(base);
+        uint32_t eq = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kPlanEach; ++i) eq += __builtin_popcountll(__ballot(v[i] == e));
+        if (lane == 0) own[turn][wave] = eq;
+        __syncthreads();
+        uint32_t to = at;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; ++w) {
+            to += w < wave ? own[turn][w] : 0u;
+            at += own[turn][w];
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kPlanEach; ++i) {
+            const uint64_t who = __ballot(v[i] == e);
+            if (v[i] == e)
+                order[to + __builtin_popcountll(who & ((1ull << lane) - 1))] =
+                    static_cast<int32_t>(base + wave * (64 * kPlanEach) + 64 * i + lane);
+            to += __builtin_popcountll(who);
+        }
     }
-    if (threadIdx.x == 0) offsets[e] = static_cast<int32_t>(begin);
-    at += begin;
-    for (uint32_t p0 = from; p0 < to; p0 += 64) {
-        const uint32_t p = p0 + lane;
-        const bool mine = p < to && expert(p) == e;
-        const uint64_t who = __ballot(mine);
-        if (mine) order[at + __builtin_popcountll(who & ((1ull << lane) - 1))] = static_cast<int32_t>(p);
-        at += __builtin_popcountll(who);
-    }
+}
+
+__global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t *__restrict__ ids, uint32_t pairs,
+                                                                uint32_t experts, int32_t *__restrict__ offsets,
+                                                                int32_t *__restrict__ order) {
+    plan_expert(ids, pairs, experts, blockIdx.x, offsets, order);
+}
+
+// The plan by the first experts + 1 workgroups and the tokens' rows to MX4 by
+// the others: neither needs the other, and a launch of its own costs more.
+template <Mx4Type T>
+__global__ __launch_bounds__(kPlanThreads) void moe_begin_kernel(const int32_t *__restrict__ ids, uint32_t pairs,
+                                                                 uint32_t experts, int32_t *__restrict__ offsets,
+                                                                 int32_t *__restrict__ order, Mx4Rows rows) {
+    if (blockIdx.x <= experts) plan_expert(ids, pairs, experts, blockIdx.x, offsets, order);
+    else encode_rows<T, kPlanThreads>(rows, blockIdx.x - experts - 1, gridDim.x - experts - 1);
 }
 
 // out[t] = sum over the token's experts of weight * y, in the pairs' order; a
@@ -431,14 +459,16 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const void *__restrict
     if (t >= tokens) return;
     const uint32_t c = 8 * static_cast<uint32_t>(item - t * chunks), valid = cols - c;
     float sum[8] = {};
+#pragma unroll 4
     for (uint32_t j = 0; j < k; ++j) {
+        // loads without a branch, so that several pairs' are in flight
         const uint64_t p = t * k + j;
-        if (static_cast<uint32_t>(ids[p]) >= experts) continue;
+        const bool real = static_cast<uint32_t>(ids[p]) < experts;
         const float w = weights[p];
         float v[8];
         load8<Y>(y, p * cols + c, valid, v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum[i] = __builtin_fmaf(w, v[i], sum[i]);
+        for (int i = 0; i < 8; ++i) sum[i] = real ? __builtin_fmaf(w, v[i], sum[i]) : sum[i];
     }
     store8<O>(out, t * ld + c, valid, sum);
 }
@@ -490,8 +520,7 @@ RouteArgs route_args(const void *logits, uint64_t tokens, uint32_t experts, uint
 }
 
 void plan(const int32_t *ids, uint64_t pairs, uint32_t experts, int32_t *offsets, int32_t *order, hipStream_t stream) {
-    const unsigned threads = pairs > 4096 ? 1024 : 256;
-    moe_plan_kernel<<<experts + 1, threads, 0, stream>>>(ids, static_cast<uint32_t>(pairs), experts, offsets, order);
+    moe_plan_kernel<<<experts + 1, kPlanThreads, 0, stream>>>(ids, static_cast<uint32_t>(pairs), experts, offsets, order);
     BSQ_HIP(hipGetLastError());
 }
 
@@ -645,12 +674,21 @@ int bsq_moe_linear(const void *d_x, int x_type, uint64_t tokens, uint64_t inputs
             check_packed(d_w_codes, d_w_scales);
             check_work(d_work, work_bytes, bsq_moe_linear_workspace(tokens, k, n, inputs, experts));
         }
-        plan(d_ids, pairs, experts, d_offsets, d_order, s);
-        if (pairs == 0) return;
+        if (pairs == 0) {
+            plan(d_ids, pairs, experts, d_offsets, d_order, s);
+            return;
+        }
         const uint32_t slices = static_cast<uint32_t>(mx4_slices(inputs));
         Arena arena{static_cast<uint8_t *>(d_work), work_bytes};
         uint8_t *codes = arena.take(tokens * slices * 128), *scales = arena.take(tokens * slices * 8);
-        launch_mx4_encode(d_x, tx, 1, tokens, inputs, ldx, 0, codes, scales, nullptr, nullptr, s);
+        const Mx4Rows rows{static_cast<const uint8_t *>(d_x), tokens, inputs, ldx, 0, tokens, slices * (kMx4Slice / 8),
+                           codes, scales};
+        const uint64_t groups = std::min<uint64_t>(ceil_div(tokens * rows.chunks, kPlanThreads), 1u << 20);
+        by_type(tx, [&](auto t) {
+            moe_begin_kernel<decltype(t)::value><<<static_cast<unsigned>(experts + 1 + groups), kPlanThreads, 0, s>>>(
+                d_ids, static_cast<uint32_t>(pairs), experts, d_offsets, d_order, rows);
+        });
+        BSQ_HIP(hipGetLastError());
         Mx4Product p;
         p.a = {codes, scales};
         p.b = {d_w_codes, d_w_scales};

@@ -13,74 +13,58 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
 
-// max over each aligned quad of lanes
-__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
-    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xB1, 0xF, 0xF, true)));
-    return max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x4E, 0xF, 0xF, true)));
-}
-
-// Rows to MX4.  A lane takes eight consecutive values, a quad of lanes a
-// block; loads are 16 bytes a lane (twice for FP32), a wave's codes 256
-// consecutive bytes.
 template <Mx4Type T>
-__global__ __launch_bounds__(kThreads) void mx4_encode_rows_kernel(const uint8_t *__restrict__ x, uint64_t rows,
-                                                                   uint64_t cols, uint64_t ld, uint64_t stride,
-                                                                   uint64_t total, uint32_t chunks,
-                                                                   uint8_t *__restrict__ codes,
-                                                                   uint8_t *__restrict__ scales) {
-    constexpr int size = T == Mx4Type::F32 ? 4 : 2;
-    const uint64_t all = total * chunks;  // a multiple of 32 a row: quads never part
-    for (uint64_t t = static_cast<uint64_t>(blockIdx.x) * kThreads + threadIdx.x; t < all;
-         t += static_cast<uint64_t>(gridDim.x) * kThreads) {
-        const uint64_t r = t / chunks, c = t - r * chunks, b = r / rows;
-        Eight<T> v;
-        v.load(x + (b * stride + (r - b * rows) * ld) * size, 8 * c, cols);
-        const uint32_t byte = mx4_scale_byte(f32_bits<T>(quad_max(v.top())));
-        const uint32_t q = byte == 255u ? 0u : v.codes(mx4_power(byte));
-        reinterpret_cast<uint32_t *>(codes)[t] = q;
-        if ((c & 3) == 0) scales[t >> 2] = static_cast<uint8_t>(byte);
-    }
+__global__ __launch_bounds__(kThreads) void mx4_encode_rows_kernel(Mx4Rows r) {
+    encode_rows<T, kThreads>(r, blockIdx.x, gridDim.x);
 }
 
-// Columns to MX4, and the rows too if asked.  A workgroup takes a tile of 128
+// Columns to MX4, and the rows too if asked.  A workgroup takes a tile of 256
 // rows and 64 words of each: 16 lanes load a row's part (and encode its blocks
 // from registers), the tile goes to LDS, and a lane then takes one block of 32
-// rows of a word's column (two columns of a 16-bit type); the four lanes of a
-// column's four blocks are neighbours, so that their codes are 64 consecutive
-// bytes.  Row r of the tile lies 16 words further along for each block of 32
-// rows before it: sixteen columns of four blocks then read all 64 banks.
+// rows of a word's column (two columns of a 16-bit type); the eight lanes of a
+// column's eight blocks are neighbours, so that their codes are a whole line.
+// Row r of the tile lies 8 words further along for each block of 32 rows
+// before it: eight columns of eight blocks then read all 64 banks.  Tiles that
+// write the halves of a line of row codes run on one XCD.
 // SLOTS: the rows are those of the experts' slots.  WEIGHTED: each times its
 // weight, staged in FP32, so that a value is rounded once.
-constexpr int kTileRows = 128;
+// HBM bound: 4096 x 11008 BF16 both ways, 32 us (read once, two packed
+// matrices written: 27 us at the rate of a large copy).
+constexpr int kTileRows = 256;
 constexpr int kTileWords = 64;
+constexpr int kTileThreads = 512;
 
 template <Mx4Type T, bool WEIGHTED>
 constexpr int kTileCols = T == Mx4Type::F32 || WEIGHTED ? 64 : 128;
 
 template <Mx4Type T, bool SLOTS, bool WEIGHTED>
-__global__ __launch_bounds__(kThreads) void mx4_encode_tile_kernel(const uint8_t *__restrict__ x, uint64_t rows,
-                                                                   uint64_t cols, uint64_t ld, uint64_t stride,
-                                                                   uint32_t tiles_c, uint32_t tiles_r,
-                                                                   uint32_t slices_c, uint32_t slices_r, Mx4Slots slots,
-                                                                   uint8_t *__restrict__ codes,
-                                                                   uint8_t *__restrict__ scales,
-                                                                   uint8_t *__restrict__ codes_t,
-                                                                   uint8_t *__restrict__ scales_t) {
+__global__ __launch_bounds__(kTileThreads) void mx4_encode_tile_kernel(const uint8_t *__restrict__ x, uint64_t rows,
+                                                                       uint64_t cols, uint64_t ld, uint64_t stride,
+                                                                       uint32_t tiles_c, uint32_t tiles_r,
+                                                                       uint32_t slices_c, uint32_t slices_r,
+                                                                       Mx4Slots slots, uint8_t *__restrict__ codes,
+                                                                       uint8_t *__restrict__ scales,
+                                                                       uint8_t *__restrict__ codes_t,
+                                                                       uint8_t *__restrict__ scales_t) {
     constexpr Mx4Type S = WEIGHTED ? Mx4Type::F32 : T;  // as staged
     constexpr int size = T == Mx4Type::F32 ? 4 : 2, kCols = kTileCols<T, WEIGHTED>, kPer = kCols / 16;
-    __shared__ __attribute__((aligned(16))) uint32_t tile[kTileRows * kTileWords + 4 * 16];
+    constexpr int kPad = 8, kPasses = kTileRows / 32;
+    __shared__ __attribute__((aligned(16))) uint32_t tile[kTileRows * kTileWords + 8 * kPad];
     const int tid = threadIdx.x;
-    const uint32_t tc = blockIdx.x % tiles_c;
-    const uint64_t rest = blockIdx.x / tiles_c;
+    // each XCD a contiguous run of the tiles
+    const uint32_t xcd = blockIdx.x % 8, per = gridDim.x / 8, extra = gridDim.x % 8;
+    const uint32_t number = xcd * per + min(xcd, extra) + blockIdx.x / 8;
+    const uint32_t tc = number % tiles_c;
+    const uint64_t rest = number / tiles_c;
     const uint32_t tr = static_cast<uint32_t>(rest % tiles_r);
     const uint64_t b = rest / tiles_r;
     const uint64_t c0 = static_cast<uint64_t>(tc) * kCols;
     uint64_t r0 = static_cast<uint64_t>(tr) * kTileRows, r1 = rows;  // rows of the tile end at r1
     if constexpr (SLOTS) {
-        // tile tr of the experts' slices, in halves: the expert it belongs to
+        // tile tr of the experts' slices: the expert it belongs to
         uint32_t first = 0, e = 0;
         for (; e < slots.experts; ++e) {
-            const uint32_t n = 2 * mx4_slot_slices(slots.offsets, e);
+            const uint32_t n = mx4_slot_slices(slots.offsets, e);
             if (tr < first + n) break;
             first += n;
         }
@@ -90,63 +74,75 @@ __global__ __launch_bounds__(kThreads) void mx4_encode_tile_kernel(const uint8_t
     }
     const int part = tid & 15;
     const uint64_t c = c0 + part * kPer;
+    constexpr int kWords = kPer * size / 4;
+    uint32_t v[kPasses][kWords];
+    float w[kPasses];
+    const uint8_t *from[kPasses];
 #pragma unroll
-    for (int i = 0; i < kTileRows / 16; ++i) {
-        const int r = 16 * i + (tid >> 4);
-        const uint64_t row = r0 + r;
-        constexpr int kWords = kPer * size / 4;
-        uint32_t v[kWords] = {};
-        float w = 1.0f;
-        if (row < r1) {
-            const uint8_t *p = x + b * stride * size;
-            if constexpr (SLOTS) {
-                const uint32_t pair = static_cast<uint32_t>(slots.order[row]);
-                p += static_cast<uint64_t>(pair / slots.per_token) * ld * size;
-                if constexpr (WEIGHTED) w = slots.weights[pair];
-            } else {
-                p += row * ld * size;
-            }
-            if (c + kPer <= cols) {
-                __builtin_memcpy(v, p + c * size, sizeof v);
-            } else {
+    for (int i = 0; i < kPasses; ++i) {
+        const uint64_t row = min(r0 + 32 * i + (tid >> 4), r1 - 1);  // past the end: the last row, not used
+        from[i] = x + b * stride * size;
+        w[i] = 1.0f;
+        if constexpr (SLOTS) {
+            const uint32_t pair = static_cast<uint32_t>(slots.order[row]);
+            from[i] += static_cast<uint64_t>(pair / slots.per_token) * ld * size;
+            if constexpr (WEIGHTED) w[i] = slots.weights[pair];
+        } else {
+            from[i] += row * ld * size;
+        }
+    }
+    if (c + kPer <= cols) {
 #pragma unroll
-                for (int k = 0; k < kPer; ++k) {
-                    if (c + k >= cols) continue;
-                    if constexpr (T == Mx4Type::F32) v[k] = reinterpret_cast<const uint32_t *>(p)[c + k];
-                    else v[k / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(p)[c + k]) << (16 * (k & 1));
-                }
+        for (int i = 0; i < kPasses; ++i) __builtin_memcpy(v[i], from[i] + c * size, sizeof v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+#pragma unroll
+            for (int k = 0; k < kWords; ++k) v[i][k] = 0;
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+                if (c + k >= cols) continue;
+                if constexpr (T == Mx4Type::F32) v[i][k] = reinterpret_cast<const uint32_t *>(from[i])[c + k];
+                else v[i][k / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(from[i])[c + k]) << (16 * (k & 1));
             }
         }
+    }
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+        const int r = 32 * i + (tid >> 4);
+        const uint64_t row = r0 + r;
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) v[i][k] = row < r1 ? v[i][k] : 0u;
         u32x4 staged;
         if constexpr (WEIGHTED) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 float f;
-                if constexpr (T == Mx4Type::F32) f = __uint_as_float(v[k]);
-                else if constexpr (T == Mx4Type::BF16) f = bf16_value((v[k / 2] >> (16 * (k & 1))) & 0xFFFFu);
-                else f = f16_value((v[k / 2] >> (16 * (k & 1))) & 0xFFFFu);
-                staged[k] = __float_as_uint(f * w);
+                if constexpr (T == Mx4Type::F32) f = __uint_as_float(v[i][k]);
+                else if constexpr (T == Mx4Type::BF16) f = bf16_value((v[i][k / 2] >> (16 * (k & 1))) & 0xFFFFu);
+                else f = f16_value((v[i][k / 2] >> (16 * (k & 1))) & 0xFFFFu);
+                staged[k] = row < r1 ? __float_as_uint(f * w[i]) : 0u;
             }
         } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) staged[k] = v[k];
+            for (int k = 0; k < 4; ++k) staged[k] = v[i][k];
             if (codes != nullptr) {  // uniform
                 uint32_t byte, q = 0;
                 if constexpr (T == Mx4Type::F32) {
                     uint32_t m = 0;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) m = max(m, v[k] & 0x7FFFFFFFu);
+                    for (int k = 0; k < 4; ++k) m = max(m, v[i][k] & 0x7FFFFFFFu);
                     m = quad_max(m);
                     m = max(m, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(m), 0x141, 0xF, 0xF, true)));
                     byte = mx4_scale_byte(m);
                     if (byte != 255u) {
                         const float s = mx4_power(byte);
-                        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, __uint_as_float(v[0]), __uint_as_float(v[1]), s, 0);
-                        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, __uint_as_float(v[2]), __uint_as_float(v[3]), s, 1);
+                        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, __uint_as_float(v[i][0]), __uint_as_float(v[i][1]), s, 0);
+                        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, __uint_as_float(v[i][2]), __uint_as_float(v[i][3]), s, 1);
                     }
                 } else {
                     Eight<T> e8;
-                    __builtin_memcpy(e8.w, v, 16);
+                    __builtin_memcpy(e8.w, v[i], 16);
                     byte = mx4_scale_byte(f32_bits<T>(quad_max(e8.top())));
                     if (byte != 255u) q = e8.codes(mx4_power(byte));
                 }
@@ -158,29 +154,29 @@ __global__ __launch_bounds__(kThreads) void mx4_encode_tile_kernel(const uint8_t
                 }
             }
         }
-        *reinterpret_cast<u32x4 *>(&tile[r * kTileWords + (r >> 5) * 16 + 4 * part]) = staged;
+        *reinterpret_cast<u32x4 *>(&tile[r * kTileWords + i * kPad + 4 * part]) = staged;
     }
     __syncthreads();
-    const int word = tid >> 2, blk = tid & 3;  // four lanes: the four blocks of a word's column
-    const uint32_t *p = &tile[blk * (32 * kTileWords + 16) + word];
-    uint32_t v[32];
+    const int word = tid >> 3, blk = tid & 7;  // eight lanes: the eight blocks of a word's column
+    const uint32_t *p = &tile[blk * (32 * kTileWords + kPad) + word];
+    uint32_t u[32];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = p[i * kTileWords];
+    for (int i = 0; i < 32; ++i) u[i] = p[i * kTileWords];
     constexpr int kSub = kCols / kTileWords;  // columns in a word
 #pragma unroll
     for (int h = 0; h < kSub; ++h) {
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-            if constexpr (S == Mx4Type::F32) m = max(m, v[i] & 0x7FFFFFFFu);
-            else m = max(m, (h ? v[i] >> 16 : v[i]) & 0x7FFFu);
+            if constexpr (S == Mx4Type::F32) m = max(m, u[i] & 0x7FFFFFFFu);
+            else m = max(m, (h ? u[i] >> 16 : u[i]) & 0x7FFFu);
         }
         const uint32_t byte = mx4_scale_byte(f32_bits<S>(m));
         const float s = mx4_power(byte);
         auto val = [&](int i) __attribute__((always_inline)) {
-            if constexpr (S == Mx4Type::F32) return __uint_as_float(v[i]);
-            else if constexpr (S == Mx4Type::BF16) return __uint_as_float(h ? v[i] & 0xFFFF0000u : v[i] << 16);
-            else return f16_value(h ? v[i] >> 16 : v[i] & 0xFFFFu);
+            if constexpr (S == Mx4Type::F32) return __uint_as_float(u[i]);
+            else if constexpr (S == Mx4Type::BF16) return __uint_as_float(h ? u[i] & 0xFFFF0000u : u[i] << 16);
+            else return f16_value(h ? u[i] >> 16 : u[i] & 0xFFFFu);
         };
         u32x4 q = {0, 0, 0, 0};
         if (byte != 255u) {
@@ -196,9 +192,9 @@ __global__ __launch_bounds__(kThreads) void mx4_encode_tile_kernel(const uint8_t
         }
         const uint64_t col = c0 + static_cast<uint64_t>(word) * kSub + h;
         if (col < cols) {
-            const uint64_t row = (b * cols + col) * slices_r;  // slices before this column
-            *reinterpret_cast<u32x4 *>(codes_t + row * 128 + static_cast<uint64_t>(tr) * 64 + blk * 16) = q;
-            scales_t[row * 8 + static_cast<uint64_t>(tr) * 4 + blk] = static_cast<uint8_t>(byte);
+            const uint64_t at = (b * cols + col) * slices_r + tr;  // slices before this one
+            *reinterpret_cast<u32x4 *>(codes_t + at * 128 + blk * 16) = q;
+            scales_t[at * 8 + blk] = static_cast<uint8_t>(byte);
         }
     }
 }
@@ -267,14 +263,14 @@ void launch_mx4_encode(const void *x, Mx4Type type, uint64_t batch, uint64_t row
         if (codes_t == nullptr) {
             const uint32_t chunks = slices_c * (kMx4Slice / 8);
             mx4_encode_rows_kernel<T><<<grid_for(batch * rows * chunks), kThreads, 0, stream>>>(
-                p, rows, cols, ld, stride, batch * rows, chunks, codes, scales);
+                Mx4Rows{p, rows, cols, ld, stride, batch * rows, chunks, codes, scales});
         } else {
             constexpr uint32_t kCols = kTileCols<T, false>;
             // whole slices both ways, so that the padding is written too
-            const uint32_t tiles_c = slices_c * (kMx4Slice / kCols), tiles_r = 2 * slices_r;
+            const uint32_t tiles_c = slices_c * (kMx4Slice / kCols), tiles_r = slices_r;
             const uint64_t grid = batch * tiles_c * tiles_r;
             BSQ_REQUIRE(grid <= 0x7FFFFFFFull, "mx4 encode: matrix too large");
-            mx4_encode_tile_kernel<T, false, false><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(
+            mx4_encode_tile_kernel<T, false, false><<<static_cast<unsigned>(grid), kTileThreads, 0, stream>>>(
                 p, rows, cols, ld, stride, tiles_c, tiles_r, slices_c, slices_r, Mx4Slots{}, codes, scales, codes_t,
                 scales_t);
         }
@@ -290,10 +286,10 @@ void launch_mx4_encode_slots(const void *x, Mx4Type type, uint64_t cols, uint64_
         auto go = [&](auto weighted) {
             constexpr bool W = decltype(weighted)::value;
             const uint32_t tiles_c = static_cast<uint32_t>(ceil_div(cols, kTileCols<T, W>));
-            const uint64_t grid = 2 * slices * tiles_c;
+            const uint64_t grid = slices * tiles_c;
             BSQ_REQUIRE(grid <= 0x7FFFFFFFull, "mx4 encode: matrix too large");
-            mx4_encode_tile_kernel<T, true, W><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(
-                static_cast<const uint8_t *>(x), 0, cols, ld, 0, tiles_c, static_cast<uint32_t>(2 * slices), 0,
+            mx4_encode_tile_kernel<T, true, W><<<static_cast<unsigned>(grid), kTileThreads, 0, stream>>>(
+                static_cast<const uint8_t *>(x), 0, cols, ld, 0, tiles_c, static_cast<uint32_t>(slices), 0,
                 static_cast<uint32_t>(slices), slots, nullptr, nullptr, codes_t, scales_t);
         };
         if (slots.weights != nullptr) go(std::true_type{});

@@ -35,8 +35,7 @@ struct Mx4Matrix {
 // Where the columns of an encode come from when they are the slots of experts:
 // slot s of the order is row order[s] / per_token of x, scaled by
 // weights[order[s]] if given; expert e has the slots offsets[e] ..
-// offsets[e + 1], and its slices begin at tile tile_of(e) (128 slots each, two
-// a slice).
+// offsets[e + 1], padded to whole slices of its own.
 struct Mx4Slots {
     const int32_t *offsets = nullptr;
     const int32_t *order = nullptr;
@@ -233,6 +232,36 @@ __device__ __forceinline__ void store8(void *base, uint64_t at, uint32_t valid, 
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (static_cast<uint32_t>(i) < valid) store_value<T>(base, at + i, v[i]);
+    }
+}
+
+// max over each aligned quad of lanes
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xB1, 0xF, 0xF, true)));
+    return max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x4E, 0xF, 0xF, true)));
+}
+
+// Rows to MX4.  A lane takes eight consecutive values, a quad of lanes a
+// block; loads are 16 bytes a lane (twice for FP32), a wave's codes 256
+// consecutive bytes.  Workgroup `group` of `groups` of THREADS.
+struct Mx4Rows {
+    const uint8_t *x;
+    uint64_t rows, cols, ld, stride, total;  // total: the batch's rows
+    uint32_t chunks;                         // of eight values in a padded row
+    uint8_t *codes, *scales;
+};
+template <Mx4Type T, int THREADS>
+__device__ __forceinline__ void encode_rows(const Mx4Rows &r, uint32_t group, uint32_t groups) {
+    constexpr int size = T == Mx4Type::F32 ? 4 : 2;
+    const uint64_t all = r.total * r.chunks;  // a multiple of 32 a row: quads never part
+    for (uint64_t t = static_cast<uint64_t>(group) * THREADS + threadIdx.x; t < all;
+         t += static_cast<uint64_t>(groups) * THREADS) {
+        const uint64_t row = t / r.chunks, c = t - row * r.chunks, b = row / r.rows;
+        Eight<T> v;
+        v.load(r.x + (b * r.stride + (row - b * r.rows) * r.ld) * size, 8 * c, r.cols);
+        const uint32_t byte = mx4_scale_byte(f32_bits<T>(quad_max(v.top())));
+        reinterpret_cast<uint32_t *>(r.codes)[t] = byte == 255u ? 0u : v.codes(mx4_power(byte));
+        if ((c & 3) == 0) r.scales[t >> 2] = static_cast<uint8_t>(byte);
     }
 }
 
