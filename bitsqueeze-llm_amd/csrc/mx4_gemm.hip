@@ -52,6 +52,14 @@ __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c, uint32_t sa, 
                                                            static_cast<int>(sb));
 }
 
+// A uniform address that stays in scalar registers: added to the lanes' offsets
+// ahead of a loop it would take two vector registers for each of them.
+template <int G>
+__device__ __forceinline__ const uint8_t *scalar(const uint8_t *p) {
+    if constexpr (G == 1) asm volatile("" : "+s"(p));  // teams differ within a workgroup
+    return p;
+}
+
 enum Mode { kDense, kRows, kShared };
 
 // The tile of `tile` slots number t of the experts' tiles: the expert (experts
@@ -162,12 +170,27 @@ __global__ __launch_bounds__(64 * G * kTeam<T>, T == 64 ? G : 2) void mx4_produc
         slice0 = __builtin_amdgcn_readfirstlane(before);
         slices = __builtin_amdgcn_readfirstlane(mx4_slot_slices(p.offsets, expert));
     }
-    // every team passes the same barriers, `turns` of them
+    if (MODE != kDense && slices == 0) {  // uniform: nothing to sum, zeros
+        const uint64_t first = MODE == kShared ? static_cast<uint64_t>(expert) * p.M : 0u;
+        const float zero[8] = {};
+        for (uint32_t c = tid; c < T * T / 8; c += blockDim.x) {
+            const uint32_t m = m0 + c / (T / 8), n = tn * T + c % (T / 8) * 8;
+            if (m >= m_end || n >= p.N) continue;
+            uint64_t at = first + m;
+            if constexpr (MODE == kRows) at = static_cast<uint32_t>(p.order[m]);
+            store8<O>(p.out, at * p.ld + n, p.N - n, zero);
+        }
+        return;
+    }
+    // every team passes the same barriers, `turns` of them; one without a slice
+    // transfers the last and multiplies none
     const uint32_t turns = (slices + G - 1) / G;
+    uint32_t mine = slices;
     if constexpr (G > 1) {
         const uint32_t from = min(team * turns, slices), to = min(from + turns, slices);
-        slice0 += from;
-        slices = to - from;
+        mine = to - from;
+        slice0 += min(from, slices - 1);
+        slices = max(mine, 1u);
     }
     const uint32_t n0 = tn * T;
     const uint64_t b_first = MODE == kRows ? static_cast<uint64_t>(min(expert, p.experts - 1)) * p.N : 0u;
@@ -200,34 +223,44 @@ __global__ __launch_bounds__(64 * G * kTeam<T>, T == 64 ? G : 2) void mx4_produc
         oa[i] = row_a(r) * pitch + 16 * block;
         ob[i] = row_b(r) * pitch + 16 * block;
     }
-    // part 0 to 2 of the codes of slice k (past the end the last one's again,
+    // part 0 or 1 of the codes of slice k (past the end the last one's again,
     // which is not read: a branch here would part the matrix instructions from
     // their operands' reads)
     auto fetch_part = [&](const Stage &s, uint32_t k, int part) __attribute__((always_inline)) {
         asm volatile("" ::: "memory");
         const uint64_t c = static_cast<uint64_t>(min(k, slices - 1)) * kCodeBytes;
+        const uint8_t *pa = scalar<G>(base_a + c), *pb = scalar<G>(base_b + c);
 #pragma unroll
         for (int i = 0; i < kRowLoads; ++i) {
-            if (i * 3 / kRowLoads != part) continue;
-            dma16(base_a + c + oa[i], s.a + 1024 * (kWaves * i + wave));
-            dma16(base_b + c + ob[i], s.b + 1024 * (kWaves * i + wave));
+            if (i / 3 != part) continue;
+            dma16(pa + oa[i], s.a + 1024 * (kWaves * i + wave));
+            dma16(pb + ob[i], s.b + 1024 * (kWaves * i + wave));
         }
         asm volatile("" ::: "memory");
     };
-    // the scales of the four slices from k on, a lane four bytes of the row
-    // whose codes it transfers (its offset in scales is a sixteenth); words past
-    // the row's end repeat the last.  Rows eight apart hold their words in
-    // another order, or they would share banks.
-    auto fetch_scales = [&](uint32_t k) __attribute__((always_inline)) {
+    // rows' part i of the scales of the four slices from k on, a lane four bytes
+    // of the row whose codes it transfers (its offset in scales is a
+    // sixteenth); words past the row's end repeat the last.  Rows eight apart
+    // hold their words in another order, or they would share banks.
+    auto fetch_scales = [&](uint32_t k, uint32_t i, Offset a, uint32_t b) __attribute__((always_inline)) {
         asm volatile("" ::: "memory");
         const uint32_t word = 4 * min(2 * k + ((lane & 7) ^ (2 * (wave & 3))), 2 * slices - 1);
-        const uint32_t to = (k & 4) / 4 * (T * kGroup) + 256 * wave;
-#pragma unroll
-        for (int i = 0; i < kRowLoads; ++i) {
-            dma4(base_sa + (oa[i] >> 4) - block + word, scales_a + to + 256 * kWaves * i);
-            dma4(base_sb + (ob[i] >> 4) - block + word, scales_b + to + 256 * kWaves * i);
-        }
+        const uint32_t to = (k & 4) / 4 * (T * kGroup) + 256 * (kWaves * i + wave);
+        dma4(scalar<G>(base_sa) + ((a >> 4) - block + word), scales_a + to);
+        dma4(scalar<G>(base_sb) + ((b >> 4) - block + word), scales_b + to);
         asm volatile("" ::: "memory");
+    };
+    // a part of the next four slices' with each slice
+    auto next_scales = [&](uint32_t k) __attribute__((always_inline)) {
+        const uint32_t i = k % kRowLoads;
+        Offset a = oa[0];
+        uint32_t b = ob[0];
+#pragma unroll
+        for (uint32_t j = 1; j < kRowLoads; ++j) {
+            a = i == j ? oa[j] : a;
+            b = i == j ? ob[j] : b;
+        }
+        fetch_scales((k & ~3u) + 4, i, a, b);
     };
 
     f32x16 acc[BM][BN] = {};
@@ -235,52 +268,81 @@ __global__ __launch_bounds__(64 * G * kTeam<T>, T == 64 ? G : 2) void mx4_produc
     struct Frags {
         u32x4 a[BM], b[BN];
     };
+    // A lane's block of step s lies at its first step's place xor 16 s, and its
+    // scale word of slice k at that of slice 0 xor 8 (k % 4).  The places are
+    // formed anew each time: kept, all steps' and stages' would not fit the
+    // registers.
+    const uint32_t place = row * kCodeBytes + 16 * ((4 * half) ^ ((row >> 1) & 7));
+    const uint32_t place_s = row * kGroup + 4 * (half ^ (2 * ((row >> 3) & 3)));
     auto read = [&](Frags &f, const Stage &s, int step) __attribute__((always_inline)) {
-        const int unit = 16 * ((4 * half + step) ^ ((row >> 1) & 7));
+        uint32_t at = place ^ (16 * step);
+        asm volatile("" : "+v"(at));
+        const uint8_t *pa = s.a + wm * kCodeBytes + at, *pb = s.b + wn * kCodeBytes + at;
 #pragma unroll
-        for (int i = 0; i < BM; ++i) f.a[i] = *reinterpret_cast<const u32x4 *>(s.a + (wm + 32 * i + row) * kCodeBytes + unit);
+        for (int i = 0; i < BM; ++i) f.a[i] = *reinterpret_cast<const u32x4 *>(pa + 32 * i * kCodeBytes);
 #pragma unroll
-        for (int j = 0; j < BN; ++j) f.b[j] = *reinterpret_cast<const u32x4 *>(s.b + (wn + 32 * j + row) * kCodeBytes + unit);
+        for (int j = 0; j < BN; ++j) f.b[j] = *reinterpret_cast<const u32x4 *>(pb + 32 * j * kCodeBytes);
     };
-    // slice k is in `here` once every wave has passed the barrier, which also
-    // frees the other stage for slice k + 1
-    auto slice = [&](const Stage &here, const Stage &freed, uint32_t k) __attribute__((always_inline)) {
-        stage_barrier<0>();
-        if (G > 1 && k >= slices) return;  // uniform in a wave
-        if ((k & 3) == 3 && k + 1 < slices) fetch_scales(k + 1);
-        uint32_t sa[BM], sb[BN];
-        Frags f[2];
-        read(f[0], here, 0);
-        const uint32_t at = (k & 4) / 4 * (T * kGroup) + 4 * ((2 * (k & 3) + half) ^ (2 * ((row >> 3) & 3)));
+    uint32_t sa[2][BM], sb[2][BN];  // the scales of slice k in [k % 2]
+    auto read_scales = [&](uint32_t k, int to) __attribute__((always_inline)) {
+        uint32_t at = (k & 4) / 4 * (T * kGroup) + (place_s ^ (8 * (k & 3)));
+        asm volatile("" : "+v"(at));
+        const uint8_t *pa = scales_a + wm * kGroup + at, *pb = scales_b + wn * kGroup + at;
 #pragma unroll
-        for (int i = 0; i < BM; ++i) sa[i] = *reinterpret_cast<const uint32_t *>(scales_a + at + (wm + 32 * i + row) * kGroup);
+        for (int i = 0; i < BM; ++i) sa[to][i] = *reinterpret_cast<const uint32_t *>(pa + 32 * i * kGroup);
 #pragma unroll
-        for (int j = 0; j < BN; ++j) sb[j] = *reinterpret_cast<const uint32_t *>(scales_b + at + (wn + 32 * j + row) * kGroup);
-        auto step = [&](auto st) __attribute__((always_inline)) {
+        for (int j = 0; j < BN; ++j) sb[to][j] = *reinterpret_cast<const uint32_t *>(pb + 32 * j * kGroup);
+    };
+    Frags f[2];
+    // Slice k from `here`, whose first fragments and scales are in registers.
+    // The barrier stands before the last step's products: once a wave has read
+    // its fragments the stage is free for slice k + 2, and slice k + 1, whose
+    // transfers have had a whole slice's time, is read while they run.
+    auto slice = [&](const Stage &here, const Stage &other, uint32_t k, auto parity) __attribute__((always_inline)) {
+        constexpr int P = decltype(parity)::value;
+        if (G > 1 && k >= mine) {  // uniform in a wave
+            stage_barrier<0>();
+            return;
+        }
+        auto multiply = [&](auto st) __attribute__((always_inline)) {
             constexpr int S = decltype(st)::value;
-            if constexpr (S < 3) read(f[(S + 1) & 1], here, S + 1);
-            const Frags &h = f[S & 1];
 #pragma unroll
             for (int i = 0; i < BM; ++i)
 #pragma unroll
-                for (int j = 0; j < BN; ++j) acc[i][j] = mfma<S>(h.a[i], h.b[j], acc[i][j], sa[i], sb[j]);
-            if constexpr (S < 3) fetch_part(freed, k + 1, S);
-            __builtin_amdgcn_sched_barrier(0);
+                for (int j = 0; j < BN; ++j) acc[i][j] = mfma<S>(f[S & 1].a[i], f[S & 1].b[j], acc[i][j], sa[P][i], sb[P][j]);
         };
-        step(std::integral_constant<int, 0>{});
-        step(std::integral_constant<int, 1>{});
-        step(std::integral_constant<int, 2>{});
-        step(std::integral_constant<int, 3>{});
+        read(f[1], here, 1);
+        multiply(std::integral_constant<int, 0>{});
+        fetch_part(other, k + 1, 1);
+        next_scales(k);
+        __builtin_amdgcn_sched_barrier(0);
+        read(f[0], here, 2);
+        multiply(std::integral_constant<int, 1>{});
+        __builtin_amdgcn_sched_barrier(0);
+        read(f[1], here, 3);
+        multiply(std::integral_constant<int, 2>{});
+        __builtin_amdgcn_sched_barrier(0);
+        stage_barrier<0>();
+        read(f[0], other, 0);
+        read_scales(k + 1, P ^ 1);
+        multiply(std::integral_constant<int, 3>{});
+        fetch_part(here, k + 2, 0);
+        __builtin_amdgcn_sched_barrier(0);
     };
-    if (slices > 0) {
-        fetch_scales(0);
 #pragma unroll
-        for (int part = 0; part < 3; ++part) fetch_part(s0, 0, part);
+    for (uint32_t i = 0; i < kRowLoads; ++i) fetch_scales(0, i, oa[i], ob[i]);
+    fetch_part(s0, 0, 0);
+    fetch_part(s0, 0, 1);
+    stage_barrier<0>();
+    read(f[0], s0, 0);
+    read_scales(0, 0);
+    fetch_part(s1, 1, 0);
+    uint32_t k = 0;
+    for (; k + 2 <= turns; k += 2) {
+        slice(s0, s1, k, std::integral_constant<int, 0>{});
+        slice(s1, s0, k + 1, std::integral_constant<int, 1>{});
     }
-    for (uint32_t k = 0; k < turns; k += 2) {
-        slice(s0, s1, k);
-        if (k + 1 < turns) slice(s1, s0, k + 1);
-    }
+    if (k < turns) slice(s0, s1, k, std::integral_constant<int, 0>{});
     const uint64_t out0 = MODE == kShared ? static_cast<uint64_t>(expert) * p.M : static_cast<uint64_t>(z) * p.M;
     auto put = [&](uint32_t m, uint32_t n, const float v[8]) __attribute__((always_inline)) {
         uint64_t at = out0 + m;
