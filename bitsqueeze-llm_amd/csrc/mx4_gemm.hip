@@ -326,17 +326,22 @@ __global__ __launch_bounds__(64 * G * kTeam<T>, T == 64 ? G : 2) void mx4_produc
         read(f[0], other, 0);
         read_scales(k + 1, P ^ 1);
         multiply(std::integral_constant<int, 3>{});
-        fetch_part(here, k + 2, 0);
         __builtin_amdgcn_sched_barrier(0);
+        // the sums stay on this side of the branch
+#pragma unroll
+        for (int i = 0; i < BM; ++i)
+#pragma unroll
+            for (int j = 0; j < BN; ++j) asm volatile("" : "+v"(acc[i][j]));
+        if (k + 2 < slices) fetch_part(here, k + 2, 0);
     };
 #pragma unroll
     for (uint32_t i = 0; i < kRowLoads; ++i) fetch_scales(0, i, oa[i], ob[i]);
     fetch_part(s0, 0, 0);
     fetch_part(s0, 0, 1);
-    stage_barrier<0>();
+    fetch_part(s1, 1, 0);
+    stage_barrier<2 * (kRowLoads < 3 ? kRowLoads : 3)>();  // all but slice 1's
     read(f[0], s0, 0);
     read_scales(0, 0);
-    fetch_part(s1, 1, 0);
     uint32_t k = 0;
     for (; k + 2 <= turns; k += 2) {
         slice(s0, s1, k, std::integral_constant<int, 0>{});
@@ -602,6 +607,11 @@ namespace {
 // Teams as long as every workgroup still finds a CU of its own; tiles of 256
 // where their rounds over the CUs cost less (a round of one a CU 2.4 us a
 // slice, of two 128s a CU 1.44).
+bool large_tiles(uint64_t rows128, uint64_t rows256, uint64_t N) {
+    const uint64_t cus = static_cast<uint64_t>(cu_count());
+    return 2.4 * ceil_div(ceil_div(rows256, 256) * ceil_div(N, 256), cus) <
+           1.44 * ceil_div(ceil_div(rows128, 128) * ceil_div(N, 128), 2 * cus);
+}
 struct Plan {
     uint32_t tile, tiles_m, tiles_n, teams, splits;
     uint64_t bytes;
@@ -611,7 +621,7 @@ Plan plan_of(uint32_t M, uint32_t N, uint32_t slices) {
     auto tiles = [&](uint64_t t) { return ceil_div(M, t) * ceil_div(N, t); };
     Plan q{128, 0, 0, 1, 1, 0};
     if (tiles(128) > 2 * cus) {
-        if (2.4 * ceil_div(tiles(256), cus) < 1.44 * ceil_div(tiles(128), 2 * cus)) q.tile = 256;
+        if (large_tiles(M, M, N)) q.tile = 256;
     } else if (tiles(64) > 2 * cus) {
         q.teams = tiles(128) <= cus && slices > 1 ? 2 : 1;
     } else {
@@ -662,10 +672,14 @@ void launch_mx4_product(const Mx4Product &p, void *workspace, uint64_t workspace
     } else if (p.offsets != nullptr) {
         // M: the pairs; every expert's tiles, and those of the pairs of none
         auto of = [&](uint64_t t) { return ceil_div(p.M, t) + p.experts + 1; };
-        // (16384 pairs of 32 experts, 2752 x 4096: 64 250 us, 128 208, 256 221)
         const uint64_t each = p.M / p.experts;
         if (each <= 16) few_rows<1, 1, 4, kRows, kPacked>(p, of(16), p.M, nullptr, 0, 0, stream);
         else if (each <= 64) tiles<64, 1, kRows>(p, of(64), ceil_div(p.N, 64), 1, stream);
+        // with half a tile an expert left over, as for dense products (us: 16384
+        // pairs of 32 experts, 2752 x 4096 with 128 199, with 256 179; 4096 of
+        // 16, 2752 x 2048 46 and 54, 2048 x 2752 43 and 37)
+        else if (large_tiles(p.M + 64ull * p.experts, p.M + 128ull * p.experts, p.N))
+            tiles<256, 1, kRows>(p, of(256), ceil_div(p.N, 256), 1, stream);
         else tiles<128, 1, kRows>(p, of(128), ceil_div(p.N, 128), 1, stream);
     } else if (p.M <= kFewRows) {
         few_rows<1, 1, 4, kDense, kPacked>(p, 1, 0, nullptr, 0, 0, stream);

@@ -187,6 +187,42 @@ def test_layer(type, out, tokens, k, experts, inputs, n):
         assert (np.abs(gw[e] - dw[e]) <= bound + ROUNDING[out] * np.abs(dw[e]) + 1e-30).all()
 
 
+@pytest.mark.parametrize("tokens,k,experts,inputs,n", [(1500, 2, 4, 300, 520), (3000, 2, 3, 256, 1400), (2600, 4, 40, 130, 300)])
+def test_layer_in_large_tiles(tokens, k, experts, inputs, n):
+    # integers whose sums are exact: the forward pass, the gradient of x and the
+    # weights' own, element by element
+    rng = np.random.default_rng(tokens)
+
+    def of(*shape):
+        a = rng.integers(-2, 3, shape).astype(np.float32)
+        a[..., ::32] = 4.0
+        return a
+
+    x, w, dy = of(tokens, inputs), of(experts, n, inputs), of(tokens, n)
+    w[:, ::32], dy[::1, ::32] = 4.0, 4.0
+    ids, _ = choices(rng, tokens, k, experts)
+    weights = rng.choice([0.5, 1.0, 2.0], (tokens, k)).astype(np.float32)
+    layer = B.MoeLinear(*B.mx4_encode(w, columns=True))
+    got = layer.forward(x, ids, weights)
+    gx, gweights, gw = layer.backward(dy)
+    y, z = np.zeros((tokens, k, n)), np.zeros((tokens, k, inputs))
+    for e in range(experts):
+        t, j = np.nonzero(ids == e)
+        y[t, j] = x[t] @ w[e].T
+        z[t, j] = dy[t] @ w[e]
+        g = (weights[t, j, None] * dy[t]).astype(np.float64)
+        if len(t):
+            want = R.rounded(np.ascontiguousarray(g.T)) @ R.rounded(np.ascontiguousarray(x[t].T.astype(np.float64))).T
+            assert np.array_equal(gw[e], want.astype(np.float32)), e
+        else:
+            assert (gw[e] == 0).all()
+    real = (ids >= 0) & (ids < experts)
+    wt = np.where(real, weights, 0.0)[..., None]
+    assert np.array_equal(got, (y * wt).sum(1).astype(np.float32))
+    assert np.array_equal(gx, (z * wt).sum(1).astype(np.float32))
+    assert (np.abs(gweights - (y * dy[:, None]).sum(2)) <= n * 2.0**-23 * (np.abs(y) * np.abs(dy[:, None])).sum(2)).all()
+
+
 def test_layer_of_no_tokens():
     layer = B.MoeLinear(*B.mx4_encode(np.ones((3, 40, 50), np.float32), columns=True))
     out = layer.forward(np.zeros((0, 50), np.float32), np.zeros((0, 2), np.int32), np.zeros((0, 2), np.float32))

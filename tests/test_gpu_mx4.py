@@ -185,6 +185,23 @@ def test_product(out, m, n, k):
     assert (np.abs(got - want) <= bound).all(), np.abs(got - want).max()
 
 
+@pytest.mark.parametrize("m,n,k", [(600, 600, 200), (400, 500, 1800), (900, 700, 3000), (2100, 1000, 513), (2100, 1000, 256),
+                                   (2300, 2000, 300), (2300, 2000, 1100), (2950, 2948, 256), (2950, 2948, 900),
+                                   (5000, 1800, 2049), (120, 70, 20000), (130, 300, 9000)])
+def test_product_of_every_cut(m, n, k):
+    # the tiles and teams that these sizes take on 256 CUs: 64 alone, in twos and
+    # fours, 128 alone and in twos, 256; odd and even slices; split shared axes.
+    # Every element against a sum over integers that is exact in FP32.
+    rng = np.random.default_rng(m + n + k)
+    x = rng.integers(-2, 3, (m, k)).astype(np.float32)
+    w = rng.integers(-2, 3, (n, k)).astype(np.float32)
+    x[:, ::32], w[:, ::32] = 4.0, 4.0  # scale 1 in every block
+    want = x @ w.T  # below 2^24: exact
+    a, b = B.mx4_encode(x), B.mx4_encode(w)
+    assert np.array_equal(B.mx4_product(a, b), want)
+    assert np.array_equal(B.mx4_product(a, b, B.TYPE_BF16), B.to_bf16(want))
+
+
 def test_product_is_exact_where_sums_are():
     # integers: every partial sum is exact in FP32, so the result is too, in any
     # order, and a misplaced block or scale shows
