@@ -709,8 +709,8 @@ int bsq_moe_linear(const void *d_x, int x_type, uint64_t tokens, uint64_t inputs
 
 uint64_t bsq_moe_linear_backward_workspace(uint64_t tokens, uint32_t k, uint64_t n, uint64_t inputs, uint32_t experts) {
     const uint64_t slots = slot_slices(tokens * k, experts);
-    return std::max(packed_bytes(tokens, mx4_slices(n)) + round256(tokens * k * inputs * 4),
-                    packed_bytes(n, slots) + packed_bytes(inputs, slots));
+    return packed_bytes(tokens, mx4_slices(n)) + round256(tokens * k * inputs * 4) + packed_bytes(n, slots) +
+           packed_bytes(inputs, slots);
 }
 
 int bsq_moe_linear_backward(const void *d_d_out, int d_type, uint64_t tokens, uint64_t n, uint64_t ldd, const void *d_x,
@@ -739,14 +739,31 @@ int bsq_moe_linear_backward(const void *d_d_out, int d_type, uint64_t tokens, ui
         }
         if (d_dw) check_dense(d_dw, tg, "");
         hipStream_t s = static_cast<hipStream_t>(stream);
+        const uint64_t slots = slot_slices(pairs, experts);
+        const uint32_t slices = static_cast<uint32_t>(mx4_slices(n));
+        Arena arena{static_cast<uint8_t *>(d_work), work_bytes};
+        uint8_t *codes = nullptr, *scales = nullptr, *z = nullptr, *gc = nullptr, *gs = nullptr, *xc = nullptr, *xs = nullptr;
+        if (pairs > 0) {
+            codes = arena.take(tokens * slices * 128), scales = arena.take(tokens * slices * 8);
+            z = arena.take(pairs * inputs * type_bytes(tg));
+            gc = arena.take(n * slots * 128), gs = arena.take(n * slots * 8);
+            xc = arena.take(inputs * slots * 128), xs = arena.take(inputs * slots * 8);
+            Mx4Slots of{d_offsets, d_order, d_weights, experts, k};
+            if (d_dx != nullptr && d_dw != nullptr && td == tx) {
+                launch_mx4_encode_backward(d_d_out, n, ldd, d_x, inputs, ldx, td, tokens, of, slots, gc, gs, xc, xs, codes,
+                                           scales, s);
+            } else {
+                if (d_dx != nullptr) launch_mx4_encode(d_d_out, td, 1, tokens, n, ldd, 0, codes, scales, nullptr, nullptr, s);
+                if (d_dw != nullptr) {
+                    launch_mx4_encode_slots(d_d_out, td, n, ldd, of, slots, gc, gs, s);
+                    of.weights = nullptr;
+                    launch_mx4_encode_slots(d_x, tx, inputs, ldx, of, slots, xc, xs, s);
+                }
+            }
+        }
         if (pairs > 0 && d_dx != nullptr) {
             // dx[t] = sum of weight * (q(d out[t]) W_e): the layer itself, with
             // the weights' columns for their rows
-            const uint32_t slices = static_cast<uint32_t>(mx4_slices(n));
-            Arena arena{static_cast<uint8_t *>(d_work), work_bytes};
-            uint8_t *codes = arena.take(tokens * slices * 128), *scales = arena.take(tokens * slices * 8);
-            uint8_t *z = arena.take(pairs * inputs * type_bytes(tg));
-            launch_mx4_encode(d_d_out, td, 1, tokens, n, ldd, 0, codes, scales, nullptr, nullptr, s);
             Mx4Product p;
             p.a = {codes, scales};
             p.b = {d_wt_codes, d_wt_scales};
@@ -768,14 +785,6 @@ int bsq_moe_linear_backward(const void *d_d_out, int d_type, uint64_t tokens, ui
         if (d_dw != nullptr) {
             // dw[e] = the sum over the expert's pairs of q(weight d out)^T q(x),
             // both rounded in blocks of 32 pairs
-            const uint64_t slots = slot_slices(pairs, experts);
-            Arena arena{static_cast<uint8_t *>(d_work), work_bytes};
-            uint8_t *gc = arena.take(n * slots * 128), *gs = arena.take(n * slots * 8);
-            uint8_t *xc = arena.take(inputs * slots * 128), *xs = arena.take(inputs * slots * 8);
-            Mx4Slots of{d_offsets, d_order, d_weights, experts, k};
-            launch_mx4_encode_slots(d_d_out, td, n, ldd, of, slots, gc, gs, s);
-            of.weights = nullptr;
-            launch_mx4_encode_slots(d_x, tx, inputs, ldx, of, slots, xc, xs, s);
             Mx4Product p;
             p.a = {gc, gs};
             p.b = {xc, xs};

@@ -33,27 +33,30 @@ __global__ __launch_bounds__(kThreads) void mx4_encode_rows_kernel(Mx4Rows r) {
 constexpr int kTileRows = 256;
 constexpr int kTileWords = 64;
 constexpr int kTileThreads = 512;
+constexpr int kPad = 8, kPasses = kTileRows / 32;
+constexpr int kTileLds = kTileRows * kTileWords + 8 * kPad;
 
 template <Mx4Type T, bool WEIGHTED>
 constexpr int kTileCols = T == Mx4Type::F32 || WEIGHTED ? 64 : 128;
 
+struct EncodeTiles {
+    const uint8_t *x;
+    uint64_t rows, cols, ld, stride;
+    uint32_t tiles_c, tiles_r, slices_c, slices_r;
+    Mx4Slots slots;
+    uint8_t *codes, *scales, *codes_t, *scales_t;
+};
+
+// Tile number `group` of `groups`.
 template <Mx4Type T, bool SLOTS, bool WEIGHTED>
-__global__ __launch_bounds__(kTileThreads) void mx4_encode_tile_kernel(const uint8_t *__restrict__ x, uint64_t rows,
-                                                                       uint64_t cols, uint64_t ld, uint64_t stride,
-                                                                       uint32_t tiles_c, uint32_t tiles_r,
-                                                                       uint32_t slices_c, uint32_t slices_r,
-                                                                       Mx4Slots slots, uint8_t *__restrict__ codes,
-                                                                       uint8_t *__restrict__ scales,
-                                                                       uint8_t *__restrict__ codes_t,
-                                                                       uint8_t *__restrict__ scales_t) {
+__device__ __forceinline__ void encode_tile(const EncodeTiles &job, uint32_t *tile, uint32_t group, uint32_t groups) {
+    const auto [x, rows, cols, ld, stride, tiles_c, tiles_r, slices_c, slices_r, slots, codes, scales, codes_t, scales_t] = job;
     constexpr Mx4Type S = WEIGHTED ? Mx4Type::F32 : T;  // as staged
     constexpr int size = T == Mx4Type::F32 ? 4 : 2, kCols = kTileCols<T, WEIGHTED>, kPer = kCols / 16;
-    constexpr int kPad = 8, kPasses = kTileRows / 32;
-    __shared__ __attribute__((aligned(16))) uint32_t tile[kTileRows * kTileWords + 8 * kPad];
     const int tid = threadIdx.x;
     // each XCD a contiguous run of the tiles
-    const uint32_t xcd = blockIdx.x % 8, per = gridDim.x / 8, extra = gridDim.x % 8;
-    const uint32_t number = xcd * per + min(xcd, extra) + blockIdx.x / 8;
+    const uint32_t xcd = group % 8, per = groups / 8, extra = groups % 8;
+    const uint32_t number = xcd * per + min(xcd, extra) + group / 8;
     const uint32_t tc = number % tiles_c;
     const uint64_t rest = number / tiles_c;
     const uint32_t tr = static_cast<uint32_t>(rest % tiles_r);
@@ -199,6 +202,25 @@ __global__ __launch_bounds__(kTileThreads) void mx4_encode_tile_kernel(const uin
     }
 }
 
+template <Mx4Type T, bool SLOTS, bool WEIGHTED>
+__global__ __launch_bounds__(kTileThreads) void mx4_encode_tile_kernel(EncodeTiles job) {
+    __shared__ __attribute__((aligned(16))) uint32_t tile[kTileLds];
+    encode_tile<T, SLOTS, WEIGHTED>(job, tile, blockIdx.x, gridDim.x);
+}
+
+// What the gradients of the experts' layer multiply, in one launch: the
+// weighted gradients' and the inputs' columns by experts, and the gradients'
+// rows.  None needs another; three launches took 8 us more.
+template <Mx4Type T>
+__global__ __launch_bounds__(kTileThreads) void mx4_encode_backward_kernel(EncodeTiles d, uint32_t d_groups, EncodeTiles x,
+                                                                           uint32_t x_groups, Mx4Rows rows) {
+    __shared__ __attribute__((aligned(16))) uint32_t tile[kTileLds];
+    const uint32_t g = blockIdx.x;
+    if (g < d_groups) encode_tile<T, true, true>(d, tile, g, d_groups);
+    else if (g < d_groups + x_groups) encode_tile<T, true, false>(x, tile, g - d_groups, x_groups);
+    else encode_rows<T, kTileThreads>(rows, g - d_groups - x_groups, gridDim.x - d_groups - x_groups);
+}
+
 // Values of packed rows.  A lane takes eight codes; the level of a code times
 // its power of two is exact in FP32 and in BF16.
 template <Mx4Type T>
@@ -271,12 +293,26 @@ void launch_mx4_encode(const void *x, Mx4Type type, uint64_t batch, uint64_t row
             const uint64_t grid = batch * tiles_c * tiles_r;
             BSQ_REQUIRE(grid <= 0x7FFFFFFFull, "mx4 encode: matrix too large");
             mx4_encode_tile_kernel<T, false, false><<<static_cast<unsigned>(grid), kTileThreads, 0, stream>>>(
-                p, rows, cols, ld, stride, tiles_c, tiles_r, slices_c, slices_r, Mx4Slots{}, codes, scales, codes_t,
-                scales_t);
+                EncodeTiles{p, rows, cols, ld, stride, tiles_c, tiles_r, slices_c, slices_r, Mx4Slots{}, codes, scales,
+                            codes_t, scales_t});
         }
     });
     BSQ_HIP(hipGetLastError());
 }
+
+namespace {
+
+template <Mx4Type T, bool WEIGHTED>
+EncodeTiles slot_tiles(const void *x, uint64_t cols, uint64_t ld, const Mx4Slots &slots, uint64_t slices, uint8_t *codes_t,
+                       uint8_t *scales_t, uint64_t &grid) {
+    const uint32_t tiles_c = static_cast<uint32_t>(ceil_div(cols, kTileCols<T, WEIGHTED>));
+    grid = slices * tiles_c;
+    BSQ_REQUIRE(grid <= 0x7FFFFFFFull, "mx4 encode: matrix too large");
+    return {static_cast<const uint8_t *>(x), 0, cols, ld, 0, tiles_c, static_cast<uint32_t>(slices), 0,
+            static_cast<uint32_t>(slices), slots, nullptr, nullptr, codes_t, scales_t};
+}
+
+}  // namespace
 
 void launch_mx4_encode_slots(const void *x, Mx4Type type, uint64_t cols, uint64_t ld, const Mx4Slots &slots,
                              uint64_t slices, uint8_t *codes_t, uint8_t *scales_t, hipStream_t stream) {
@@ -285,15 +321,31 @@ void launch_mx4_encode_slots(const void *x, Mx4Type type, uint64_t cols, uint64_
         constexpr Mx4Type T = decltype(t)::value;
         auto go = [&](auto weighted) {
             constexpr bool W = decltype(weighted)::value;
-            const uint32_t tiles_c = static_cast<uint32_t>(ceil_div(cols, kTileCols<T, W>));
-            const uint64_t grid = slices * tiles_c;
-            BSQ_REQUIRE(grid <= 0x7FFFFFFFull, "mx4 encode: matrix too large");
-            mx4_encode_tile_kernel<T, true, W><<<static_cast<unsigned>(grid), kTileThreads, 0, stream>>>(
-                static_cast<const uint8_t *>(x), 0, cols, ld, 0, tiles_c, static_cast<uint32_t>(slices), 0,
-                static_cast<uint32_t>(slices), slots, nullptr, nullptr, codes_t, scales_t);
+            uint64_t grid;
+            const EncodeTiles job = slot_tiles<T, W>(x, cols, ld, slots, slices, codes_t, scales_t, grid);
+            mx4_encode_tile_kernel<T, true, W><<<static_cast<unsigned>(grid), kTileThreads, 0, stream>>>(job);
         };
         if (slots.weights != nullptr) go(std::true_type{});
         else go(std::false_type{});
+    });
+    BSQ_HIP(hipGetLastError());
+}
+
+void launch_mx4_encode_backward(const void *d, uint64_t n, uint64_t ldd, const void *x, uint64_t inputs, uint64_t ldx,
+                                Mx4Type type, uint64_t tokens, Mx4Slots slots, uint64_t slices, uint8_t *dc, uint8_t *ds,
+                                uint8_t *xc, uint8_t *xs, uint8_t *rc, uint8_t *rs, hipStream_t stream) {
+    by_type(type, [&](auto t) {
+        constexpr Mx4Type T = decltype(t)::value;
+        uint64_t d_groups, x_groups;
+        const EncodeTiles of_d = slot_tiles<T, true>(d, n, ldd, slots, slices, dc, ds, d_groups);
+        slots.weights = nullptr;
+        const EncodeTiles of_x = slot_tiles<T, false>(x, inputs, ldx, slots, slices, xc, xs, x_groups);
+        const Mx4Rows rows{static_cast<const uint8_t *>(d), tokens, n, ldd, 0, tokens,
+                           static_cast<uint32_t>(mx4_slices(n)) * (kMx4Slice / 8), rc, rs};
+        const uint64_t groups = std::min<uint64_t>(ceil_div(tokens * rows.chunks, kTileThreads), 1u << 20);
+        BSQ_REQUIRE(d_groups + x_groups + groups <= 0x7FFFFFFFull, "mx4 encode: matrix too large");
+        mx4_encode_backward_kernel<T><<<static_cast<unsigned>(d_groups + x_groups + groups), kTileThreads, 0, stream>>>(
+            of_d, static_cast<uint32_t>(d_groups), of_x, static_cast<uint32_t>(x_groups), rows);
     });
     BSQ_HIP(hipGetLastError());
 }
@@ -418,7 +470,7 @@ int bsq_mx4_linear(const void *d_x, int x_type, uint64_t m, uint64_t k, uint64_t
         hipStream_t s = static_cast<hipStream_t>(stream);
         uint8_t *codes = static_cast<uint8_t *>(d_work), *scales = codes + round256(m * mx4_slices(k) * 128);
         const Mx4Product p = product_of({codes, scales}, m, {d_w_codes, d_w_scales}, n, k, d_out, to, ldo);
-        if (mx4_packs_on_the_way(m, p.slices) && d_xt_codes == nullptr) {
+        if (mx4_packs_on_the_way(m, n, p.slices) && d_xt_codes == nullptr) {
             launch_mx4_product_of(d_x, tx, k, ldx, p, s);
             return;
         }

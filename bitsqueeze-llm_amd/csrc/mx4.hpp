@@ -56,6 +56,12 @@ void launch_mx4_decode(const uint8_t *codes, const uint8_t *scales, uint64_t row
 void launch_mx4_encode_slots(const void *x, Mx4Type type, uint64_t cols, uint64_t ld, const Mx4Slots &slots,
                              uint64_t slices, uint8_t *codes_t, uint8_t *scales_t, hipStream_t stream);
 
+// Both of those for the weighted gradients d (tokens x n) and the inputs x, and
+// the rows of d, in one launch; d and x of one type.
+void launch_mx4_encode_backward(const void *d, uint64_t n, uint64_t ldd, const void *x, uint64_t inputs, uint64_t ldx,
+                                Mx4Type type, uint64_t tokens, Mx4Slots slots, uint64_t slices, uint8_t *dc, uint8_t *ds,
+                                uint8_t *xc, uint8_t *xs, uint8_t *rc, uint8_t *rs, hipStream_t stream);
+
 // Products of packed matrices: out[m, n] = sum over the shared axis.
 struct Mx4Product {
     Mx4Matrix a, b;
@@ -75,7 +81,7 @@ struct Mx4Product {
 uint64_t mx4_product_workspace(uint32_t M, uint32_t N, uint32_t slices);
 void launch_mx4_product(const Mx4Product &p, void *workspace, uint64_t workspace_bytes, hipStream_t stream);
 // The same with a packed from dense x on the way, for m rows where that pays.
-bool mx4_packs_on_the_way(uint64_t m, uint64_t slices);
+bool mx4_packs_on_the_way(uint64_t m, uint64_t n, uint64_t slices);
 void launch_mx4_product_of(const void *x, Mx4Type x_type, uint64_t x_cols, uint64_t ldx, const Mx4Product &p,
                            hipStream_t stream);
 

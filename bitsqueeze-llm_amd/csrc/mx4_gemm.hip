@@ -562,9 +562,11 @@ __global__ __launch_bounds__(64 * most_waves(MT * NT)) void mx4_few_rows_kernel(
     }
 }
 
-// Rows of x, and bytes of them packed, that are worth packing again in every
-// workgroup rather than once in a launch of their own.
-constexpr uint32_t kPackRows = 4, kPackBytes = 32768;
+// x is packed again in every workgroup rather than once in a launch of its own
+// (some 3 us) as long as it fits their LDS and what they read of it together
+// (`kPackReads` values) comes from L2 in less than that.
+constexpr uint32_t kPackRows = 16, kPackBytes = 32768;
+constexpr uint64_t kPackReads = 4ull << 20;
 // Rows up to which b is streamed (16 x 4096 x 11008: 10.1 us; in tiles of 64 37
 // rows take 12.7).
 constexpr uint32_t kFewRows = 16;
@@ -585,7 +587,9 @@ void few_rows(const Mx4Product &p, uint64_t tiles_m, uint32_t pairs, const void 
 
 }  // namespace
 
-bool mx4_packs_on_the_way(uint64_t m, uint64_t slices) { return m <= kPackRows && m * slices * 136 <= kPackBytes; }
+bool mx4_packs_on_the_way(uint64_t m, uint64_t n, uint64_t slices) {
+    return m <= kPackRows && m * slices * 136 <= kPackBytes && m * slices * kMx4Slice * ceil_div(n, 16) <= kPackReads;
+}
 
 void launch_mx4_product_of(const void *x, Mx4Type x_type, uint64_t x_cols, uint64_t ldx, const Mx4Product &p,
                            hipStream_t stream) {

@@ -223,6 +223,34 @@ def test_layer_in_large_tiles(tokens, k, experts, inputs, n):
     assert (np.abs(gweights - (y * dy[:, None]).sum(2)) <= n * 2.0**-23 * (np.abs(y) * np.abs(dy[:, None])).sum(2)).all()
 
 
+def test_layer_types_and_parts_of_the_backward_pass():
+    # gradients of another type than the inputs, and each gradient asked for by
+    # itself, give what the whole call gives on the same values
+    rng = np.random.default_rng(77)
+    tokens, k, experts, inputs, n = 90, 2, 5, 140, 75
+    x, w = B.to_bf16(normal(rng, tokens, inputs)), normal(rng, experts, n, inputs)
+    dy16 = B.to_bf16(normal(rng, tokens, n) * 0.01)
+    dy32 = B.from_bf16(dy16)
+    ids, weights = choices(rng, tokens, k, experts)
+    layer = B.MoeLinear(*B.mx4_encode(w, columns=True))
+    layer.forward(x, ids, weights, B.TYPE_BF16)
+    whole = layer.backward(dy16, B.TYPE_BF16)
+    for got, want in zip(layer.backward(dy32, B.TYPE_F32), whole):
+        assert np.array_equal(got, want)
+    L, d = B.lib(), B.DeviceBuffer.from_array(dy16)
+    work = B.DeviceBuffer(L.bsq_moe_linear_backward_workspace(tokens, k, n, inputs, experts))
+    outs = [B.DeviceBuffer(v.nbytes) for v in whole]
+    for only in range(3):
+        dx, dweights, dw = (outs[i].ptr if i == only else None for i in range(3))
+        B.check(L.bsq_moe_linear_backward(d.ptr, B.TYPE_BF16, tokens, n, n, layer.x.ptr, B.TYPE_BF16, inputs, inputs,
+                                          layer.ids.ptr, layer.weights.ptr, k, layer.offsets.ptr, layer.order.ptr,
+                                          layer.y.ptr, 0, layer.wt.codes.ptr, layer.wt.scales.ptr, experts, dx, inputs,
+                                          dweights, dw, 0, work.ptr, work.nbytes, None), "backward")
+        B.check(L.bsq_stream_synchronize(None), "sync")
+        got = outs[only].download(np.float32, whole[only].size).reshape(whole[only].shape)
+        assert np.array_equal(got, whole[only]), only
+
+
 def test_layer_of_no_tokens():
     layer = B.MoeLinear(*B.mx4_encode(np.ones((3, 40, 50), np.float32), columns=True))
     out = layer.forward(np.zeros((0, 50), np.float32), np.zeros((0, 2), np.int32), np.zeros((0, 2), np.float32))
