@@ -30,21 +30,24 @@ __device__ __forceinline__ float dpp_or(float other, float v) {
 __device__ __forceinline__ float from_lane(float v, int lane) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
 }
+// (the least integer, which max takes for nothing, for lanes that read none: the
+// move then folds into the max)
+constexpr int kLeast = static_cast<int>(0x80000000u);
 __device__ __forceinline__ int wave_max(int v) {
-    v = max(v, dpp_or<0xB1, 0xF>(v, v));
-    v = max(v, dpp_or<0x4E, 0xF>(v, v));
-    v = max(v, dpp_or<0x141, 0xF>(v, v));
-    v = max(v, dpp_or<0x140, 0xF>(v, v));
-    v = max(v, dpp_or<0x142, 0xA>(v, v));
-    v = max(v, dpp_or<0x143, 0xC>(v, v));
+    v = max(v, dpp_or<0xB1, 0xF>(kLeast, v));
+    v = max(v, dpp_or<0x4E, 0xF>(kLeast, v));
+    v = max(v, dpp_or<0x141, 0xF>(kLeast, v));
+    v = max(v, dpp_or<0x140, 0xF>(kLeast, v));
+    v = max(v, dpp_or<0x142, 0xA>(kLeast, v));
+    v = max(v, dpp_or<0x143, 0xC>(kLeast, v));
     return __builtin_amdgcn_readlane(v, 63);
 }
 // over each aligned run of `lanes` (a power of two), in every lane of it
 __device__ __forceinline__ int run_max(int v, uint32_t lanes) {
-    if (lanes > 1) v = max(v, dpp_or<0xB1, 0xF>(v, v));
-    if (lanes > 2) v = max(v, dpp_or<0x4E, 0xF>(v, v));
-    if (lanes > 4) v = max(v, dpp_or<0x141, 0xF>(v, v));
-    if (lanes > 8) v = max(v, dpp_or<0x140, 0xF>(v, v));
+    if (lanes > 1) v = max(v, dpp_or<0xB1, 0xF>(kLeast, v));
+    if (lanes > 2) v = max(v, dpp_or<0x4E, 0xF>(kLeast, v));
+    if (lanes > 4) v = max(v, dpp_or<0x141, 0xF>(kLeast, v));
+    if (lanes > 8) v = max(v, dpp_or<0x140, 0xF>(kLeast, v));
     if (lanes > 16) v = max(v, __shfl_xor(v, 16));
     if (lanes > 32) v = max(v, __shfl_xor(v, 32));
     return v;
@@ -54,8 +57,8 @@ __device__ __forceinline__ float wave_sum(float v) {
     v += dpp_or<0x4E, 0xF>(0.0f, v);
     v += dpp_or<0x141, 0xF>(0.0f, v);
     v += dpp_or<0x140, 0xF>(0.0f, v);
-    v += dpp_or<0x142, 0xA>(0.0f, v);
-    v += dpp_or<0x143, 0xC>(0.0f, v);
+    v += dpp_or<0x142, 0xA>(-0.0f, v);
+    v += dpp_or<0x143, 0xC>(-0.0f, v);
     return from_lane(v, 63);
 }
 
