@@ -260,7 +260,11 @@ __device__ __forceinline__ void keep_groups(const RouteArgs &a, uint32_t lane, K
 // One wave a token, NV experts a lane.  The largest of the lanes' largest keys
 // is a DPP reduction of integers; the lowest lane that holds it gives the
 // expert, so that ties go to the lowest.  Lane j then forms the weight of the
-// j-th choice from that expert's own logit.
+// j-th choice from that expert's own logit.  Scores and sums are FP32.
+// Instructions bound it: 16384 tokens, 256 experts BF16, 8 groups, 8 chosen by
+// sigmoid and bias 17.7 us (9 MB), half of it the eight rounds of a maximum;
+// one wave a token as its logits are then in registers, and no round waits for
+// a barrier.
 template <Mx4Type T, int NV>
 __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a, int32_t *__restrict__ ids,
                                                         float *__restrict__ weights) {
@@ -310,7 +314,8 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a, int32_t *__
 // again from its own logit; with w_j = scale s_j / S the scores' gradient is
 // (g_j - sum g w / scale) / S, g = scale dw, and the scores' own rule follows:
 // only the chosen for sigmoid, every expert for softmax.  The chosen reach
-// their experts' lanes through a row in LDS.
+// their experts' lanes through a row in LDS.  The same tokens: 7.2 us (9.4 MB
+// written, as much read for softmax), launch and latency.
 template <Mx4Type T, int NV>
 __global__ __launch_bounds__(256) void moe_route_backward_kernel(RouteArgs a, const int32_t *__restrict__ ids,
                                                                  const float *__restrict__ d_weights,
@@ -379,7 +384,8 @@ __global__ __launch_bounds__(256) void moe_route_backward_kernel(RouteArgs a, co
 // of no expert last.  Workgroup e counts the pairs of lower experts and its own
 // (each wave a contiguous share), then writes its own in order: reads from
 // cache only, no workspace and no atomics.  The ids of up to 16384 pairs (16 a
-// lane) stay in registers; more are read again a tile at a time.
+// lane) stay in registers; more are read again a tile at a time.  Latency bound
+// (16384 pairs of 32 experts: 6 us, behind the encode of the tokens 0).
 constexpr uint32_t kPlanThreads = 1024, kPlanEach = 16, kPlanTile = kPlanThreads * kPlanEach;
 
 __device__ __forceinline__ void plan_expert(const int32_t *__restrict__ ids, uint32_t pairs, uint32_t experts, uint32_t e,
@@ -440,7 +446,8 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t *_
 }
 
 // The plan by the first experts + 1 workgroups and the tokens' rows to MX4 by
-// the others: neither needs the other, and a launch of its own costs more.
+// the others: neither needs the other, and a launch of its own costs more (4096
+// x 4096 BF16 and 16384 pairs: 16.8 us).
 template <Mx4Type T>
 __global__ __launch_bounds__(kPlanThreads) void moe_begin_kernel(const int32_t *__restrict__ ids, uint32_t pairs,
                                                                  uint32_t experts, int32_t *__restrict__ offsets,
@@ -450,7 +457,11 @@ __global__ __launch_bounds__(kPlanThreads) void moe_begin_kernel(const int32_t *
 }
 
 // out[t] = sum over the token's experts of weight * y, in the pairs' order; a
-// lane takes eight columns.
+// lane takes eight columns.  HBM bound: 16384 rows of 2752 BF16 to 4096 19.8 us
+// (113 MB; 21.8 at the rate of a large copy, part of y is still in cache).  y
+// itself is of the type the caller asks for: in BF16 its rounding is as large
+// as the output's own and independent of it, so the error grows by up to the
+// square root of two, and half the bytes are moved.
 template <Mx4Type Y, Mx4Type O>
 __global__ __launch_bounds__(256) void moe_combine_kernel(const void *__restrict__ y, uint64_t tokens, uint32_t k,
                                                           uint32_t cols, uint32_t chunks,
@@ -476,7 +487,9 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const void *__restrict
     store8<O>(out, t * ld + c, valid, sum);
 }
 
-// d weights: a wave takes a pair's dot product with the token's d out.
+// d weights: a wave takes a pair's dot product with the token's d out.  4096
+// pairs of 2752 BF16: 10.4 us (23 MB of y, d out from L2), bound by a wave's
+// own chain of loads.
 template <Mx4Type Y, Mx4Type D>
 __global__ __launch_bounds__(256) void moe_weights_backward_kernel(const void *__restrict__ y, uint64_t pairs, uint32_t k,
                                                                    uint32_t cols, const int32_t *__restrict__ ids,
@@ -738,6 +751,9 @@ int bsq_moe_linear_backward(const void *d_d_out, int d_type, uint64_t tokens, ui
             if (d_dx) check_dense(d_dx, tg, "");
             if (d_d_weights) check_dense(d_y, ty, "");
             if (d_dw) check_dense(d_x, tx, "");
+            // its rows of slots are 128 bytes a slice, and a tile's 256 of them lie
+            // within 32 bits
+            BSQ_REQUIRE(d_dw == nullptr || slot_slices(pairs, experts) <= 1u << 17, "moe linear: too many pairs for dw");
             check_work(d_work, work_bytes, bsq_moe_linear_backward_workspace(tokens, k, n, inputs, experts));
         }
         if (d_dw) check_dense(d_dw, tg, "");

@@ -105,11 +105,14 @@ __device__ __forceinline__ SlotTile slot_tile(const Mx4Product &p, uint32_t pair
 // values: a slice's codes go global -> LDS directly, one slice ahead, with one
 // barrier a slice, some of the next slice's transfers behind each of the steps'
 // matrix instructions (all of them first, and the waves wait for their issue).
-// What bounds the kernel is the lines that the transfers touch (16384-byte
-// pieces of whole lines arrive at 30 TB/s, of half lines at 15), so a row's
-// scales, 8 bytes a slice, come four slices at a time: a line for each slice of
-// scales as for each of codes took 314 us with the products left out (8192^3),
-// where the products alone take 196.
+// The transfers are of whole lines (four times as many half lines arrive at 15
+// TB/s, whole ones at 30), and a row's scales, 8 bytes a slice, come four slices
+// at a time, or they would touch as many lines as the codes.
+// 8192 x 8192 x 8192: 291 us, 3.78 PFLOP/s, the matrix cores busy in 0.48 of the
+// cycles (as in a library's product of that size in BF16) at the 1.86 GHz that
+// the card then runs at; 228 us with the transfers left out, 242 with the
+// products, 259 with every line in L2: what bounds it is both together, and the
+// power.
 // A row's eight 16-byte blocks are stored in the order block ^ (row / 2 % 8):
 // sixteen neighbouring rows' reads of one block cover all 64 banks.  The lanes'
 // source addresses make the permutation.
@@ -394,7 +397,9 @@ __global__ __launch_bounds__(64 * G * kTeam<T>, T == 64 ? G : 2) void mx4_produc
     }
 }
 
-// The sum of the parts in order, rounded to the output's type.
+// The sum of the parts in order, rounded to the output's type; a lane takes
+// eight columns.  A launch's time for the sizes that are split (37 x 4096, four
+// parts of 606 KB, from L2: 2.5 us).
 template <Mx4Type O>
 __global__ __launch_bounds__(kThreads) void mx4_join_kernel(const float *__restrict__ parts, uint32_t splits, uint32_t M,
                                                             uint32_t N, void *__restrict__ out, uint64_t ld) {
@@ -441,55 +446,47 @@ __device__ __forceinline__ f32x4_t mfma16(u32x4 a, u32x4 b, f32x4_t c, uint32_t 
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, c, 4, 4, 0, static_cast<int>(sa), 0, static_cast<int>(sb));
 }
 
-// Up to 16 MT rows of a: b is read once, straight into registers, by
-// workgroups of 16 NT of its rows whose waves share the slices out in turn (a
-// wave issues the loads of AHEAD slices before it uses the first), and the
-// waves' sums are joined in LDS in the waves' order.
+// Up to 16 rows of a: b is read once, straight into registers, by workgroups of
+// 16 of its rows whose waves share the slices out in turn (a wave issues the
+// loads of four slices before it uses the first), and the waves' sums are
+// joined in LDS in the waves' order.
 // X: the type of a dense x that every workgroup packs into LDS for itself while
 // its first loads of b are in flight (kPacked: a is packed already).
-constexpr int kPacked = -1;
-// waves of a workgroup: their sums fit 64 KB
-constexpr int most_waves(int tiles) { return tiles <= 4 ? 16 : 64 / tiles; }
+// One row x 11008 x 4096: 8 us (24 MB, 4.7 us at the rate of a large copy), the
+// launch and a wave's two rounds of loads; 64 pairs of 32 experts of 2752 x
+// 4096: 33 to 36 us for the 160 MB of those that have any, HBM bound.
+constexpr int kPacked = -1, kAhead = 4, kMostWaves = 16;  // the waves' sums: 16 KB
 
-template <int MT, int NT, int AHEAD, Mode MODE, Mx4Type O, int X>
-__global__ __launch_bounds__(64 * most_waves(MT * NT)) void mx4_few_rows_kernel(Mx4Product p, uint32_t tiles_n,
-                                                                                uint32_t pairs, const void *x,
-                                                                                uint64_t x_cols, uint64_t ldx) {
+template <Mode MODE, Mx4Type O, int X>
+__global__ __launch_bounds__(64 * kMostWaves) void mx4_few_rows_kernel(Mx4Product p, uint32_t tiles_n, uint32_t pairs,
+                                                                       const void *x, uint64_t x_cols, uint64_t ldx) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
     const int r = lane & 15, g = lane >> 4;
     const uint32_t tn = blockIdx.x % tiles_n, tm = blockIdx.x / tiles_n;
-    uint32_t m0 = tm * 16 * MT, m_end = p.M, expert = 0, slices = p.slices;
+    uint32_t m0 = tm * 16, m_end = p.M, expert = 0, slices = p.slices;
     if constexpr (MODE == kRows) {
-        const SlotTile s = slot_tile(p, pairs, tm, 16 * MT);
+        const SlotTile s = slot_tile(p, pairs, tm, 16);
         if (s.expert > p.experts) return;  // uniform
         expert = s.expert;
         m0 = s.begin;
         m_end = s.end;
         if (expert == p.experts) slices = 0;  // slots of no expert: zero rows
     }
-    const uint32_t n0 = tn * 16 * NT;
+    const uint32_t n0 = tn * 16;
     const uint64_t b_first = MODE == kRows ? static_cast<uint64_t>(min(expert, p.experts - 1)) * p.N : 0u;
-    uint64_t a_row[MT], b_row[NT];  // first slices
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        uint64_t row = min(m0 + 16 * i + r, m_end - 1);
-        if constexpr (MODE == kRows) row = static_cast<uint32_t>(p.order[row]) / p.per_token;
-        a_row[i] = row * p.slices;
-    }
-#pragma unroll
-    for (int j = 0; j < NT; ++j) b_row[j] = (b_first + min(n0 + 16 * j + r, p.N - 1)) * p.slices;
+    uint64_t a_row = min(m0 + r, m_end - 1);  // its first slice, as b's
+    if constexpr (MODE == kRows) a_row = static_cast<uint32_t>(p.order[a_row]) / p.per_token;
+    a_row *= p.slices;
+    const uint64_t b_row = (b_first + min(n0 + r, p.N - 1)) * p.slices;
 
-    Slice16 a[AHEAD][MT], b[AHEAD][NT];
+    Slice16 a[kAhead], b[kAhead];
     auto load = [&](uint32_t k0) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
+        for (int u = 0; u < kAhead; ++u) {
             const uint32_t k = min(k0 + u * waves, slices - 1);  // past the end: the last slice again, not used
-#pragma unroll
-            for (int j = 0; j < NT; ++j) b[u][j].load(p.b, b_row[j] + k, g);
-            if constexpr (X == kPacked)
-#pragma unroll
-                for (int i = 0; i < MT; ++i) a[u][i].load(p.a, a_row[i] + k, g);
+            b[u].load(p.b, b_row + k, g);
+            if constexpr (X == kPacked) a[u].load(p.a, a_row + k, g);
         }
     };
     uint32_t k0 = wave;
@@ -519,43 +516,33 @@ __global__ __launch_bounds__(64 * most_waves(MT * NT)) void mx4_few_rows_kernel(
         }
         __syncthreads();
     }
-    f32x4_t acc[MT][NT] = {};
+    f32x4_t acc = {};
     while (k0 < slices) {
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
+        for (int u = 0; u < kAhead; ++u) {
             const uint32_t k = k0 + u * waves;
             if (k >= slices) break;  // uniform
             if constexpr (X != kPacked) {
                 const Mx4Matrix packed{lds, lds + 16 * 8 * p.M * p.slices};
-                a[u][0].load(packed, a_row[0] + k, g);
+                a[u].load(packed, a_row + k, g);
             }
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-                        acc[i][j] = mfma16(a[u][i].codes[s], b[u][j].codes[s], acc[i][j], a[u][i].scale(s, g), b[u][j].scale(s, g));
+            for (int s = 0; s < 2; ++s) acc = mfma16(a[u].codes[s], b[u].codes[s], acc, a[u].scale(s, g), b[u].scale(s, g));
         }
-        k0 += AHEAD * waves;
+        k0 += kAhead * waves;
         if (k0 < slices) load(k0);
     }
     if constexpr (X != kPacked) __syncthreads();  // the packed x is done with
-    // lane: column n = lane % 16 of a tile, rows 4 (lane / 16) + q
-    float *part = reinterpret_cast<float *>(lds);  // [wave][16 MT][16 NT]
+    // lane: column n = lane % 16, rows 4 (lane / 16) + q
+    float *part = reinterpret_cast<float *>(lds);  // [wave][16][16]
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                part[(wave * 16 * MT + 16 * i + 4 * g + q) * (16 * NT) + 16 * j + r] = acc[i][j][q];
+    for (int q = 0; q < 4; ++q) part[(wave * 16 + 4 * g + q) * 16 + r] = acc[q];
     __syncthreads();
-    for (uint32_t t = tid; t < 16 * MT * 16 * NT; t += blockDim.x) {
-        const uint32_t m = m0 + t / (16 * NT), n = n0 + t % (16 * NT);
+    for (uint32_t t = tid; t < 256; t += blockDim.x) {
+        const uint32_t m = m0 + t / 16, n = n0 + t % 16;
         if (m >= m_end || n >= p.N) continue;
         float sum = part[t];
-        for (int w = 1; w < waves; ++w) sum += part[w * 16 * MT * 16 * NT + t];
+        for (int w = 1; w < waves; ++w) sum += part[w * 256 + t];
         uint64_t at = m;
         if constexpr (MODE == kRows) at = static_cast<uint32_t>(p.order[m]);
         store_value<O>(p.out, at * p.ld + n, sum);
@@ -571,16 +558,16 @@ constexpr uint64_t kPackReads = 4ull << 20;
 // rows take 12.7).
 constexpr uint32_t kFewRows = 16;
 
-template <int MT, int NT, int AHEAD, Mode MODE, int X>
+template <Mode MODE, int X>
 void few_rows(const Mx4Product &p, uint64_t tiles_m, uint32_t pairs, const void *x, uint64_t x_cols, uint64_t ldx,
               hipStream_t stream) {
-    const uint64_t tiles_n = ceil_div(p.N, 16 * NT);
-    const unsigned waves = std::min<unsigned>(most_waves(MT * NT), std::max(1u, (p.slices + AHEAD - 1) / AHEAD));
+    const uint64_t tiles_n = ceil_div(p.N, 16);
+    const unsigned waves = std::min<unsigned>(kMostWaves, std::max(1u, (p.slices + kAhead - 1) / kAhead));
     const uint64_t grid = tiles_n * tiles_m;
     BSQ_REQUIRE(grid <= 0x7FFFFFFFull, "mx4 product: too large");
-    const unsigned lds = std::max(waves * MT * NT * 1024, X == kPacked ? 0u : p.M * p.slices * 136);
+    const unsigned lds = std::max(waves * 1024, X == kPacked ? 0u : p.M * p.slices * 136);
     by_type(p.type, [&](auto t) {
-        mx4_few_rows_kernel<MT, NT, AHEAD, MODE, decltype(t)::value, X>
+        mx4_few_rows_kernel<MODE, decltype(t)::value, X>
             <<<static_cast<unsigned>(grid), 64 * waves, lds, stream>>>(p, static_cast<uint32_t>(tiles_n), pairs, x, x_cols, ldx);
     });
 }
@@ -595,7 +582,7 @@ void launch_mx4_product_of(const void *x, Mx4Type x_type, uint64_t x_cols, uint6
                            hipStream_t stream) {
     if (p.M == 0 || p.N == 0) return;
     by_type(x_type, [&](auto t) {
-        few_rows<1, 1, 4, kDense, static_cast<int>(decltype(t)::value)>(p, 1, 0, x, x_cols, ldx, stream);
+        few_rows<kDense, static_cast<int>(decltype(t)::value)>(p, 1, 0, x, x_cols, ldx, stream);
     });
     BSQ_HIP(hipGetLastError());
 }
@@ -684,7 +671,7 @@ void launch_mx4_product(const Mx4Product &p, void *workspace, uint64_t workspace
         auto of = [&](uint64_t t) { return ceil_div(p.M, t) + p.experts + 1; };
         auto rows = [&](uint64_t t) { return p.M + t / 2 * p.experts; };
         auto count = [&](uint64_t t) { return ceil_div(rows(t), t) * ceil_div(p.N, t); };
-        if (p.M / p.experts <= 16) few_rows<1, 1, 4, kRows, kPacked>(p, of(16), p.M, nullptr, 0, 0, stream);
+        if (p.M / p.experts <= 16) few_rows<kRows, kPacked>(p, of(16), p.M, nullptr, 0, 0, stream);
         else if (count(64) <= 2 * cus && p.slices > 1) tiles<64, 2, kRows>(p, of(64), ceil_div(p.N, 64), 1, stream);
         else if (count(128) <= cus || p.M / p.experts <= 64) tiles<64, 1, kRows>(p, of(64), ceil_div(p.N, 64), 1, stream);
         // (us: 16384 pairs of 32 experts, 2752 x 4096 with 128 199, with 256
@@ -692,7 +679,7 @@ void launch_mx4_product(const Mx4Product &p, void *workspace, uint64_t workspace
         else if (large_tiles(rows(128), rows(256), p.N)) tiles<256, 1, kRows>(p, of(256), ceil_div(p.N, 256), 1, stream);
         else tiles<128, 1, kRows>(p, of(128), ceil_div(p.N, 128), 1, stream);
     } else if (p.M <= kFewRows) {
-        few_rows<1, 1, 4, kDense, kPacked>(p, 1, 0, nullptr, 0, 0, stream);
+        few_rows<kDense, kPacked>(p, 1, 0, nullptr, 0, 0, stream);
     } else {
         const Plan q = plan_of(p.M, p.N, p.slices);
         BSQ_REQUIRE(workspace_bytes >= q.bytes, "mx4 product: workspace too small");

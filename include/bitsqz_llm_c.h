@@ -420,7 +420,8 @@ BSQ_API int bsq_moe_linear(const void *d_x, int x_type, uint64_t tokens, uint64_
 /* Its gradients, each optional (NULL): dx = sum of weight * q(d out) W_e with
  * the weights' columns d_wt_* (experts packed matrices of inputs x n), d
  * weights[t, j] = <d out[t], y[t k + j]>, dw (experts x n x inputs) = the sum
- * over the expert's pairs of q(weight d out)^T q(x), in blocks of 32 pairs. */
+ * over the expert's pairs of q(weight d out)^T q(x), in blocks of 32 pairs (up
+ * to some 33 million pairs: tokens k / 256 + experts <= 2^17). */
 BSQ_API uint64_t bsq_moe_linear_backward_workspace(uint64_t tokens, uint32_t k, uint64_t n, uint64_t inputs,
                                                    uint32_t experts);
 BSQ_API int bsq_moe_linear_backward(const void *d_d_out, int d_type, uint64_t tokens, uint64_t n, uint64_t ldd,

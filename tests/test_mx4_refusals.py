@@ -186,3 +186,16 @@ def test_bf16_conversion_of_the_binding():
     b = B.to_bf16(x)
     assert b.tolist()[:4] == [0x3F80, 0x3F80, 0x3F82, 0x8000] and b[4] == 0x7F80 and b[5] == 0x7F80 and b[6] == 0xFF80
     assert np.isnan(B.from_bf16(B.to_bf16(np.array([np.nan], np.float32)))).all()
+
+
+def test_the_experts_weight_gradient_takes_so_many_pairs():
+    """A row of its operands is 128 bytes a slice of 256 pairs, and 256 of them lie within 32 bits."""
+    L = B.lib()
+
+    def back(tokens, dw):
+        return L.bsq_moe_linear_backward(D, 0, tokens, 8, 8, D, 0, 300, 300, D, D, 16, D, D, D, 0, D, D, 5, None, 300, None, dw,
+                                         0, D, 0, None)
+
+    refused(back(1 << 21, D), "too many pairs")
+    refused(back((1 << 21) - 80, D), "workspace")  # within the limit: the next check's turn
+    refused(back(1 << 21, None), "workspace")
