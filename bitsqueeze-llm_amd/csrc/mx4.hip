@@ -30,7 +30,7 @@ __global__ __launch_bounds__(kThreads) void mx4_encode_rows_kernel(Mx4Rows r) {
 // before it: eight columns of eight blocks then read all 64 banks.  Tiles that
 // write the halves of a line of row codes run on one XCD.
 // SLOTS: the rows are those of the experts' slots.  WEIGHTED: each times its
-// weight, staged in FP32, so that a value is rounded once.
+// weight, in FP32 as its block is encoded, so that a value is rounded once.
 // HBM bound: 4096 x 11008 BF16 both ways, 32 us (read once, two packed
 // matrices written: 27 us at the rate of a large copy); 16 matrices of 2752 x
 // 2048 65 (53).
@@ -38,10 +38,11 @@ constexpr int kTileRows = 256;
 constexpr int kTileWords = 64;
 constexpr int kTileThreads = 512;
 constexpr int kPad = 8, kPasses = kTileRows / 32;
-constexpr int kTileLds = kTileRows * kTileWords + 8 * kPad;
+constexpr int kTileWeights = kTileRows * kTileWords + 8 * kPad;  // where the rows' weights lie
+constexpr int kTileLds = kTileWeights + kTileRows;
 
-template <Mx4Type T, bool WEIGHTED>
-constexpr int kTileCols = T == Mx4Type::F32 || WEIGHTED ? 64 : 128;
+template <Mx4Type T>
+constexpr int kTileCols = T == Mx4Type::F32 ? 64 : 128;
 
 struct EncodeTiles {
     const uint8_t *x;
@@ -55,8 +56,7 @@ struct EncodeTiles {
 template <Mx4Type T, bool SLOTS, bool WEIGHTED>
 __device__ __forceinline__ void encode_tile(const EncodeTiles &job, uint32_t *tile, uint32_t group, uint32_t groups) {
     const auto [x, rows, cols, ld, stride, tiles_c, tiles_r, slices_c, slices_r, slots, codes, scales, codes_t, scales_t] = job;
-    constexpr Mx4Type S = WEIGHTED ? Mx4Type::F32 : T;  // as staged
-    constexpr int size = T == Mx4Type::F32 ? 4 : 2, kCols = kTileCols<T, WEIGHTED>, kPer = kCols / 16;
+    constexpr int size = T == Mx4Type::F32 ? 4 : 2, kCols = kTileCols<T>, kPer = kCols / 16;
     const int tid = threadIdx.x;
     // each XCD a contiguous run of the tiles
     const uint32_t xcd = group % 8, per = groups / 8, extra = groups % 8;
@@ -68,16 +68,31 @@ __device__ __forceinline__ void encode_tile(const EncodeTiles &job, uint32_t *ti
     const uint64_t c0 = static_cast<uint64_t>(tc) * kCols;
     uint64_t r0 = static_cast<uint64_t>(tr) * kTileRows, r1 = rows;  // rows of the tile end at r1
     if constexpr (SLOTS) {
-        // tile tr of the experts' slices: the expert it belongs to
-        uint32_t first = 0, e = 0;
-        for (; e < slots.experts; ++e) {
-            const uint32_t n = mx4_slot_slices(slots.offsets, e);
-            if (tr < first + n) break;
-            first += n;
+        // tile tr of the experts' slices: the expert it belongs to, 64 at a time
+        const uint32_t lane = tid & 63;
+        uint32_t before = 0;
+        r1 = 0;
+        for (uint32_t e0 = 0; e0 < slots.experts; e0 += 64) {
+            const uint32_t e = min(e0 + lane, slots.experts - 1);
+            const uint32_t lo = static_cast<uint32_t>(slots.offsets[e]), hi = static_cast<uint32_t>(slots.offsets[e + 1]);
+            const uint32_t n = e0 + lane < slots.experts ? (hi - lo + kMx4Slice - 1) / kMx4Slice : 0u;
+            uint32_t sum = n;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t up = __shfl_up(sum, d);
+                sum += lane >= static_cast<uint32_t>(d) ? up : 0u;
+            }
+            const uint64_t over = __ballot(before + sum > tr);
+            if (over != 0) {
+                const int at = __builtin_ctzll(over);
+                r0 = __builtin_amdgcn_readlane(lo, at) +
+                     (tr - before - __builtin_amdgcn_readlane(sum - n, at)) * static_cast<uint64_t>(kTileRows);
+                r1 = __builtin_amdgcn_readlane(hi, at);
+                break;
+            }
+            before += __builtin_amdgcn_readlane(sum, 63);
         }
-        if (e == slots.experts) return;  // uniform: past the last expert's slices
-        r0 = static_cast<uint64_t>(slots.offsets[e]) + static_cast<uint64_t>(tr - first) * kTileRows;
-        r1 = static_cast<uint64_t>(slots.offsets[e + 1]);
+        if (r1 == 0) return;  // uniform: past the last expert's slices
     }
     const int part = tid & 15;
     const uint64_t c = c0 + part * kPer;
@@ -121,44 +136,34 @@ __device__ __forceinline__ void encode_tile(const EncodeTiles &job, uint32_t *ti
 #pragma unroll
         for (int k = 0; k < kWords; ++k) v[i][k] = row < r1 ? v[i][k] : 0u;
         u32x4 staged;
-        if constexpr (WEIGHTED) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float f;
-                if constexpr (T == Mx4Type::F32) f = __uint_as_float(v[i][k]);
-                else if constexpr (T == Mx4Type::BF16) f = bf16_value((v[i][k / 2] >> (16 * (k & 1))) & 0xFFFFu);
-                else f = f16_value((v[i][k / 2] >> (16 * (k & 1))) & 0xFFFFu);
-                staged[k] = row < r1 ? __float_as_uint(f * w[i]) : 0u;
+        for (int k = 0; k < 4; ++k) staged[k] = v[i][k];
+        if (WEIGHTED && part == 0) tile[kTileWeights + r] = row < r1 ? __float_as_uint(w[i]) : 0u;
+        if (!SLOTS && codes != nullptr) {  // uniform
+            uint32_t byte, q = 0;
+            if constexpr (T == Mx4Type::F32) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) m = max(m, v[i][k] & 0x7FFFFFFFu);
+                m = quad_max(m);
+                m = max(m, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(m), 0x141, 0xF, 0xF, true)));
+                byte = mx4_scale_byte(m);
+                if (byte != 255u) {
+                    const float s = mx4_power(byte);
+                    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, __uint_as_float(v[i][0]), __uint_as_float(v[i][1]), s, 0);
+                    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, __uint_as_float(v[i][2]), __uint_as_float(v[i][3]), s, 1);
+                }
+            } else {
+                Eight<T> e8;
+                __builtin_memcpy(e8.w, v[i], 16);
+                byte = mx4_scale_byte(f32_bits<T>(quad_max(e8.top())));
+                if (byte != 255u) q = e8.codes(mx4_power(byte));
             }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) staged[k] = v[i][k];
-            if (codes != nullptr) {  // uniform
-                uint32_t byte, q = 0;
-                if constexpr (T == Mx4Type::F32) {
-                    uint32_t m = 0;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) m = max(m, v[i][k] & 0x7FFFFFFFu);
-                    m = quad_max(m);
-                    m = max(m, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(m), 0x141, 0xF, 0xF, true)));
-                    byte = mx4_scale_byte(m);
-                    if (byte != 255u) {
-                        const float s = mx4_power(byte);
-                        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, __uint_as_float(v[i][0]), __uint_as_float(v[i][1]), s, 0);
-                        q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, __uint_as_float(v[i][2]), __uint_as_float(v[i][3]), s, 1);
-                    }
-                } else {
-                    Eight<T> e8;
-                    __builtin_memcpy(e8.w, v[i], 16);
-                    byte = mx4_scale_byte(f32_bits<T>(quad_max(e8.top())));
-                    if (byte != 255u) q = e8.codes(mx4_power(byte));
-                }
-                if (row < rows) {
-                    const uint64_t at = (b * rows + row) * slices_c * kMx4Slice + c;  // padded element
-                    if constexpr (T == Mx4Type::F32) reinterpret_cast<uint16_t *>(codes)[at >> 2] = static_cast<uint16_t>(q);
-                    else reinterpret_cast<uint32_t *>(codes)[at >> 3] = q;
-                    if ((part & (32 / kPer - 1)) == 0) scales[at >> 5] = static_cast<uint8_t>(byte);
-                }
+            if (row < rows) {
+                const uint64_t at = (b * rows + row) * slices_c * kMx4Slice + c;  // padded element
+                if constexpr (T == Mx4Type::F32) reinterpret_cast<uint16_t *>(codes)[at >> 2] = static_cast<uint16_t>(q);
+                else reinterpret_cast<uint32_t *>(codes)[at >> 3] = q;
+                if ((part & (32 / kPer - 1)) == 0) scales[at >> 5] = static_cast<uint8_t>(byte);
             }
         }
         *reinterpret_cast<u32x4 *>(&tile[r * kTileWords + i * kPad + 4 * part]) = staged;
@@ -169,22 +174,26 @@ __device__ __forceinline__ void encode_tile(const EncodeTiles &job, uint32_t *ti
     uint32_t u[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) u[i] = p[i * kTileWords];
+    float by[32];
+    if constexpr (WEIGHTED) __builtin_memcpy(by, &tile[kTileWeights + 32 * blk], sizeof by);
     constexpr int kSub = kCols / kTileWords;  // columns in a word
 #pragma unroll
     for (int h = 0; h < kSub; ++h) {
+        auto val = [&](int i) __attribute__((always_inline)) {
+            float f;
+            if constexpr (T == Mx4Type::F32) f = __uint_as_float(u[i]);
+            else if constexpr (T == Mx4Type::BF16) f = __uint_as_float(h ? u[i] & 0xFFFF0000u : u[i] << 16);
+            else f = f16_value(h ? u[i] >> 16 : u[i] & 0xFFFFu);
+            return WEIGHTED ? f * by[i] : f;
+        };
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-            if constexpr (S == Mx4Type::F32) m = max(m, u[i] & 0x7FFFFFFFu);
+            if constexpr (T == Mx4Type::F32 || WEIGHTED) m = max(m, __float_as_uint(val(i)) & 0x7FFFFFFFu);
             else m = max(m, (h ? u[i] >> 16 : u[i]) & 0x7FFFu);
         }
-        const uint32_t byte = mx4_scale_byte(f32_bits<S>(m));
+        const uint32_t byte = mx4_scale_byte(WEIGHTED ? m : f32_bits<T>(m));
         const float s = mx4_power(byte);
-        auto val = [&](int i) __attribute__((always_inline)) {
-            if constexpr (S == Mx4Type::F32) return __uint_as_float(u[i]);
-            else if constexpr (S == Mx4Type::BF16) return __uint_as_float(h ? u[i] & 0xFFFF0000u : u[i] << 16);
-            else return f16_value(h ? u[i] >> 16 : u[i] & 0xFFFFu);
-        };
         u32x4 q = {0, 0, 0, 0};
         if (byte != 255u) {
 #pragma unroll
@@ -295,7 +304,7 @@ void launch_mx4_encode(const void *x, Mx4Type type, uint64_t batch, uint64_t row
             mx4_encode_rows_kernel<T><<<grid_for(batch * rows * chunks), kThreads, 0, stream>>>(
                 Mx4Rows{p, rows, cols, ld, stride, batch * rows, chunks, codes, scales});
         } else {
-            constexpr uint32_t kCols = kTileCols<T, false>;
+            constexpr uint32_t kCols = kTileCols<T>;
             // whole slices both ways, so that the padding is written too
             const uint32_t tiles_c = slices_c * (kMx4Slice / kCols), tiles_r = slices_r;
             const uint64_t grid = batch * tiles_c * tiles_r;
@@ -310,10 +319,10 @@ void launch_mx4_encode(const void *x, Mx4Type type, uint64_t batch, uint64_t row
 
 namespace {
 
-template <Mx4Type T, bool WEIGHTED>
+template <Mx4Type T>
 EncodeTiles slot_tiles(const void *x, uint64_t cols, uint64_t ld, const Mx4Slots &slots, uint64_t slices, uint8_t *codes_t,
                        uint8_t *scales_t, uint64_t &grid) {
-    const uint32_t tiles_c = static_cast<uint32_t>(ceil_div(cols, kTileCols<T, WEIGHTED>));
+    const uint32_t tiles_c = static_cast<uint32_t>(ceil_div(cols, kTileCols<T>));
     grid = slices * tiles_c;
     BSQ_REQUIRE(grid <= 0x7FFFFFFFull, "mx4 encode: matrix too large");
     return {static_cast<const uint8_t *>(x), 0, cols, ld, 0, tiles_c, static_cast<uint32_t>(slices), 0,
@@ -330,7 +339,7 @@ void launch_mx4_encode_slots(const void *x, Mx4Type type, uint64_t cols, uint64_
         auto go = [&](auto weighted) {
             constexpr bool W = decltype(weighted)::value;
             uint64_t grid;
-            const EncodeTiles job = slot_tiles<T, W>(x, cols, ld, slots, slices, codes_t, scales_t, grid);
+            const EncodeTiles job = slot_tiles<T>(x, cols, ld, slots, slices, codes_t, scales_t, grid);
             mx4_encode_tile_kernel<T, true, W><<<static_cast<unsigned>(grid), kTileThreads, 0, stream>>>(job);
         };
         if (slots.weights != nullptr) go(std::true_type{});
@@ -345,9 +354,9 @@ void launch_mx4_encode_backward(const void *d, uint64_t n, uint64_t ldd, const v
     by_type(type, [&](auto t) {
         constexpr Mx4Type T = decltype(t)::value;
         uint64_t d_groups, x_groups;
-        const EncodeTiles of_d = slot_tiles<T, true>(d, n, ldd, slots, slices, dc, ds, d_groups);
+        const EncodeTiles of_d = slot_tiles<T>(d, n, ldd, slots, slices, dc, ds, d_groups);
         slots.weights = nullptr;
-        const EncodeTiles of_x = slot_tiles<T, false>(x, inputs, ldx, slots, slices, xc, xs, x_groups);
+        const EncodeTiles of_x = slot_tiles<T>(x, inputs, ldx, slots, slices, xc, xs, x_groups);
         const Mx4Rows rows{static_cast<const uint8_t *>(d), tokens, n, ldd, 0, tokens,
                            static_cast<uint32_t>(mx4_slices(n)) * (kMx4Slice / 8), rc, rs};
         const uint64_t groups = std::min<uint64_t>(ceil_div(tokens * rows.chunks, kTileThreads), 1u << 20);
