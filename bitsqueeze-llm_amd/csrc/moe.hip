@@ -262,9 +262,9 @@ __device__ __forceinline__ void keep_groups(const RouteArgs &a, uint32_t lane, K
 // expert, so that ties go to the lowest.  Lane j then forms the weight of the
 // j-th choice from that expert's own logit.  Scores and sums are FP32.
 // Instructions bound it: 16384 tokens, 256 experts BF16, 8 groups, 8 chosen by
-// sigmoid and bias 17.7 us (9 MB), half of it the eight rounds of a maximum;
-// one wave a token as its logits are then in registers, and no round waits for
-// a barrier.
+// sigmoid and bias 17 us (9 MB), half of it the eight rounds of a maximum; one
+// wave a token as its logits are then in registers, and no round waits for a
+// barrier.
 template <Mx4Type T, int NV>
 __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a, int32_t *__restrict__ ids,
                                                         float *__restrict__ weights) {
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a, int32_t *__
 // (g_j - sum g w / scale) / S, g = scale dw, and the scores' own rule follows:
 // only the chosen for sigmoid, every expert for softmax.  The chosen reach
 // their experts' lanes through a row in LDS.  The same tokens: 7.2 us (9.4 MB
-// written, as much read for softmax), launch and latency.
+// written; softmax reads as much), launch and latency.
 template <Mx4Type T, int NV>
 __global__ __launch_bounds__(256) void moe_route_backward_kernel(RouteArgs a, const int32_t *__restrict__ ids,
                                                                  const float *__restrict__ d_weights,

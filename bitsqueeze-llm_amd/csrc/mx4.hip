@@ -31,9 +31,9 @@ __global__ __launch_bounds__(kThreads) void mx4_encode_rows_kernel(Mx4Rows r) {
 // write the halves of a line of row codes run on one XCD.
 // SLOTS: the rows are those of the experts' slots.  WEIGHTED: each times its
 // weight, in FP32 as its block is encoded, so that a value is rounded once.
-// HBM bound: 4096 x 11008 BF16 both ways, 32 us (read once, two packed
-// matrices written: 27 us at the rate of a large copy); 16 matrices of 2752 x
-// 2048 65 (53).
+// HBM bound: 4096 x 11008 BF16 both ways, 32 us with x in the last cache, 45
+// from HBM among other writes (read once, two packed matrices written: 27 us at
+// the rate of a large copy); 16 matrices of 2752 x 2048 64 (53).
 constexpr int kTileRows = 256;
 constexpr int kTileWords = 64;
 constexpr int kTileThreads = 512;
@@ -224,8 +224,8 @@ __global__ __launch_bounds__(kTileThreads) void mx4_encode_tile_kernel(EncodeTil
 // What the gradients of the experts' layer multiply, in one launch: the
 // weighted gradients' and the inputs' columns by experts, and the gradients'
 // rows.  None needs another; three launches took 8 us more.  2048 tokens of
-// two pairs each, 2752 and 2048 BF16: 25 us, 60 MB mostly from L2, and short
-// tiles at the experts' ends.
+// two pairs each, 2752 and 2048 BF16: 25 us for 75 MB, mostly from the caches:
+// the chain of a tile's loads (its expert, its pairs, their rows) bounds it.
 template <Mx4Type T>
 __global__ __launch_bounds__(kTileThreads) void mx4_encode_backward_kernel(EncodeTiles d, uint32_t d_groups, EncodeTiles x,
                                                                            uint32_t x_groups, Mx4Rows rows) {
