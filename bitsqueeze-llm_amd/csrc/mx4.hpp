@@ -220,6 +220,16 @@ __device__ __forceinline__ void load8(const void *base, uint64_t at, uint32_t va
         for (int i = 0; i < 8; ++i) v[i] = static_cast<uint32_t>(i) < valid ? load_value<T>(base, at + i) : 0.0f;
     }
 }
+// Two values rounded to the nearest of a 16-bit type (BF16 in one instruction).
+template <Mx4Type T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (T == Mx4Type::BF16) {
+        const mx4_bf16x2 v = {static_cast<__bf16>(lo), static_cast<__bf16>(hi)};
+        return __builtin_bit_cast(uint32_t, v);
+    } else {
+        return f16_bits(lo) | (f16_bits(hi) << 16);
+    }
+}
 template <Mx4Type T>
 __device__ __forceinline__ void store8(void *base, uint64_t at, uint32_t valid, const float v[8]) {
     if (valid >= 8) {
@@ -228,10 +238,7 @@ __device__ __forceinline__ void store8(void *base, uint64_t at, uint32_t valid, 
         } else {
             uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (T == Mx4Type::BF16) w[i] = bf16_bits(v[2 * i]) | (bf16_bits(v[2 * i + 1]) << 16);
-                else w[i] = f16_bits(v[2 * i]) | (f16_bits(v[2 * i + 1]) << 16);
-            }
+            for (int i = 0; i < 4; ++i) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
             __builtin_memcpy(static_cast<uint16_t *>(base) + at, w, 16);
         }
     } else {

@@ -352,11 +352,6 @@ __global__ __launch_bounds__(64 * G * kTeam<T>, T == 64 ? G : 2) void mx4_produc
     }
     if (k < turns) slice(s0, s1, k, std::integral_constant<int, 0>{});
     const uint64_t out0 = MODE == kShared ? static_cast<uint64_t>(expert) * p.M : static_cast<uint64_t>(z) * p.M;
-    auto put = [&](uint32_t m, uint32_t n, const float v[8]) __attribute__((always_inline)) {
-        uint64_t at = out0 + m;
-        if constexpr (MODE == kRows) at = static_cast<uint32_t>(p.order[m]);
-        store8<O>(p.out, at * p.ld + n, p.N - n, v);
-    };
     // Out through LDS, 32 rows of the wave's at a time, so that a store covers
     // whole 16-byte pieces of a row.  The accumulators hold column lane % 32 of
     // a block and rows 8 (q / 4) + 4 (lane / 32) + q % 4; rows of the upper
@@ -377,21 +372,39 @@ __global__ __launch_bounds__(64 * G * kTeam<T>, T == 64 ? G : 2) void mx4_produc
             for (int q = 0; q < 16; ++q)
                 stage[(8 * (q >> 2) + 4 * half + (q & 3)) * W + ((32 * j + row) ^ (swap * half))] = acc[i][j][q];
         if constexpr (G > 1) __syncthreads();
-        // the teams share a wave's rows out
-        for (int c = lane + 64 * team; c < kPart / 8; c += 64 * G) {
-            const int r = c / (W / 8), col = c % (W / 8) * 8, from = r * W + (col ^ (swap * ((r >> 2) & 1)));
-            const uint32_t m = m0 + wm + 32 * i + r, n = n0 + wn + col;
-            if (m >= m_end || n >= p.N) continue;
-            float v[8];
-            __builtin_memcpy(v, part_of(0, wave) + from, 32);
+        // The teams share a wave's rows out.  All of a lane's reads go out before
+        // its first store, and no store waits for another (one piece after the
+        // other took a third of the time of 16 products of 2752 x 2048 x 256).
+        constexpr int kPieces = (kPart / 8 + 64 * G - 1) / (64 * G);
+        auto piece = [&](int j) __attribute__((always_inline)) { return (lane + 64 * (team + G * j)) % (kPart / 8); };
+        const bool some = 64 * team < kPart / 8;  // four teams have a piece for two
+        float v[kPieces][8];
+        uint64_t to[kPieces];
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) {
+            const int c = piece(j), r = c / (W / 8);
+            const uint32_t m = min(m0 + wm + 32 * i + r, m_end - 1);
+            if constexpr (MODE == kRows) to[j] = static_cast<uint32_t>(p.order[m]);
+            else to[j] = out0 + m;
+        }
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) {
+            const int c = piece(j), r = c / (W / 8), col = c % (W / 8) * 8;
+            const int from = r * W + (col ^ (swap * ((r >> 2) & 1)));
+            __builtin_memcpy(v[j], part_of(0, wave) + from, 32);
 #pragma unroll
             for (int t = 1; t < G; ++t) {
                 float u[8];
                 __builtin_memcpy(u, part_of(t, wave) + from, 32);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] += u[e];
+                for (int e = 0; e < 8; ++e) v[j][e] += u[e];
             }
-            put(m, n, v);
+        }
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) {
+            const int c = piece(j), r = c / (W / 8), col = c % (W / 8) * 8;
+            const uint32_t m = m0 + wm + 32 * i + r, n = n0 + wn + col;
+            if (some && m < m_end && n < p.N) store8<O>(p.out, to[j] * p.ld + n, p.N - n, v[j]);
         }
         if (G > 1 && i + 1 < BM) __syncthreads();
     }
