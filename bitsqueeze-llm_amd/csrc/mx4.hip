@@ -76,12 +76,7 @@ __device__ __forceinline__ void encode_tile(const EncodeTiles &job, uint32_t *ti
             const uint32_t e = min(e0 + lane, slots.experts - 1);
             const uint32_t lo = static_cast<uint32_t>(slots.offsets[e]), hi = static_cast<uint32_t>(slots.offsets[e + 1]);
             const uint32_t n = e0 + lane < slots.experts ? (hi - lo + kMx4Slice - 1) / kMx4Slice : 0u;
-            uint32_t sum = n;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const uint32_t up = __shfl_up(sum, d);
-                sum += lane >= static_cast<uint32_t>(d) ? up : 0u;
-            }
+            const uint32_t sum = wave_prefix(n);
             const uint64_t over = __ballot(before + sum > tr);
             if (over != 0) {
                 const int at = __builtin_ctzll(over);

@@ -15,6 +15,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "bsq_internal.hpp"
 
 namespace bsq {
@@ -88,6 +90,23 @@ void launch_mx4_product_of(const void *x, Mx4Type x_type, uint64_t x_cols, uint6
 // First slice of expert e's slots and the number of slices of all.
 __device__ __forceinline__ uint32_t mx4_slot_slices(const int32_t *offsets, uint32_t e) {
     return (static_cast<uint32_t>(offsets[e + 1] - offsets[e]) + kMx4Slice - 1) / kMx4Slice;
+}
+
+// The sum of v over the lanes up to this one, by moves within rows of 16 lanes
+// and of the rows' last lanes.
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {
+    auto moved = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+        return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(ctrl)::value,
+                                                                 decltype(rows)::value, 0xF, false));
+    };
+    using All = std::integral_constant<int, 0xF>;
+    v += moved(std::integral_constant<int, 0x111>{}, All{});
+    v += moved(std::integral_constant<int, 0x112>{}, All{});
+    v += moved(std::integral_constant<int, 0x114>{}, All{});
+    v += moved(std::integral_constant<int, 0x118>{}, All{});
+    v += moved(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});
+    v += moved(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});
+    return v;
 }
 
 // 2^(b - 127), b in [1, 254]

@@ -62,43 +62,49 @@ __device__ __forceinline__ const uint8_t *scalar(const uint8_t *p) {
 
 enum Mode { kDense, kRows, kShared };
 
-// The tile of `tile` slots number t of the experts' tiles: the expert (experts
-// itself for the slots of none, `experts + 1` past the last tile) and its slots.
+// The slots of 64 experts from e0 on, one a lane (`experts` itself: the slots of
+// none), and their tiles of `tile` slots: how many, and up to this lane.
+struct SlotScan {
+    uint32_t begin, end, tiles, sum;
+};
+__device__ __forceinline__ SlotScan scan_slots(const Mx4Product &p, uint32_t pairs, uint32_t e0, uint32_t tile) {
+    const uint32_t e = e0 + (threadIdx.x & 63);
+    SlotScan s{0, 0, 0, 0};
+    if (e <= p.experts) {
+        s.begin = static_cast<uint32_t>(p.offsets[e]);
+        s.end = e < p.experts ? static_cast<uint32_t>(p.offsets[e + 1]) : pairs;
+    }
+    s.tiles = (s.end - s.begin + tile - 1) / tile;
+    s.sum = wave_prefix(s.tiles);
+    return s;
+}
+// `first`: the scan of the first 64 experts, which is all of it for most layers.
+__device__ __forceinline__ uint32_t slot_tiles(const Mx4Product &p, uint32_t pairs, uint32_t tile, const SlotScan &first) {
+    uint32_t count = __builtin_amdgcn_readlane(first.sum, 63);
+    for (uint32_t e0 = 64; e0 <= p.experts; e0 += 64)
+        count += __builtin_amdgcn_readlane(scan_slots(p, pairs, e0, tile).sum, 63);
+    return count;
+}
+// Tile number t of the experts' tiles: the expert (`experts + 1` past the last
+// tile) and the tile's slots.
 struct SlotTile {
     uint32_t expert, begin, end;
 };
-// Without t: the number of tiles, in `begin`.
-constexpr uint32_t kCount = 0xFFFFFFFFu;
-__device__ __forceinline__ SlotTile slot_tile(const Mx4Product &p, uint32_t pairs, uint32_t t, uint32_t tile) {
-    const uint32_t lane = threadIdx.x & 63;
-    uint32_t count = 0;
-    for (uint32_t e0 = 0; e0 <= p.experts; e0 += 64) {
-        const uint32_t e = e0 + lane;
-        uint32_t lo = 0, hi = 0;
-        if (e <= p.experts) {
-            lo = static_cast<uint32_t>(p.offsets[e]);
-            hi = e < p.experts ? static_cast<uint32_t>(p.offsets[e + 1]) : pairs;
-        }
-        const uint32_t n = (hi - lo + tile - 1) / tile;
-        uint32_t sum = n;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t v = __shfl_up(sum, d);
-            sum += lane >= static_cast<uint32_t>(d) ? v : 0u;
-        }
-        const uint64_t over = t == kCount ? 0 : __ballot(sum > t);
+__device__ __forceinline__ SlotTile slot_tile(const Mx4Product &p, uint32_t pairs, uint32_t t, uint32_t tile, SlotScan s) {
+    for (uint32_t e0 = 0;;) {
+        const uint64_t over = __ballot(s.sum > t);
         if (over != 0) {
             const int at = __builtin_ctzll(over);
-            const uint32_t before = __builtin_amdgcn_readlane(sum - n, at);
-            const uint32_t begin = __builtin_amdgcn_readlane(lo, at) + (t - before) * tile;
-            const uint32_t end = __builtin_amdgcn_readlane(hi, at);
+            const uint32_t before = __builtin_amdgcn_readlane(s.sum - s.tiles, at);
+            const uint32_t begin = __builtin_amdgcn_readlane(s.begin, at) + (t - before) * tile;
+            const uint32_t end = __builtin_amdgcn_readlane(s.end, at);
             return {e0 + at, begin, min(begin + tile, end)};
         }
-        const uint32_t all = __builtin_amdgcn_readlane(sum, 63);
-        if (t != kCount) t -= all;
-        count += all;
+        t -= __builtin_amdgcn_readlane(s.sum, 63);
+        e0 += 64;
+        if (e0 > p.experts) return {p.experts + 1, 0, 0};
+        s = scan_slots(p, pairs, e0, tile);
     }
-    return {p.experts + 1, count, 0};
 }
 
 // T x T tiles, four waves of T/2 x T/2 (256: eight of 128 x 64), slices of 256
@@ -146,9 +152,11 @@ __global__ __launch_bounds__(64 * G * kTeam<T>, T == 64 ? G : 2) void mx4_produc
     const int team = G == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6) / kWaves;
     const Stage &s0 = stage0[team], &s1 = stage1[team];
     const uint8_t *scales_a = scale_words + team * 4 * T * kGroup, *scales_b = scales_a + 2 * T * kGroup;
+    SlotScan scan;
     if constexpr (MODE == kRows) {
         // the tiles that there are, evenly over the XCDs
-        tiles_m = slot_tile(p, p.M, kCount, T).begin;
+        scan = scan_slots(p, p.M, 0, T);
+        tiles_m = slot_tiles(p, p.M, T, scan);
         if (blockIdx.x >= tiles_m * tiles_n) return;
     }
     int tm, tn, z;
@@ -158,7 +166,7 @@ __global__ __launch_bounds__(64 * G * kTeam<T>, T == 64 ? G : 2) void mx4_produc
         slice0 = static_cast<uint32_t>(static_cast<uint64_t>(z) * p.slices / splits);
         slices = static_cast<uint32_t>(static_cast<uint64_t>(z + 1) * p.slices / splits) - slice0;
     } else if constexpr (MODE == kRows) {
-        const SlotTile s = slot_tile(p, p.M, tm, T);
+        const SlotTile s = slot_tile(p, p.M, tm, T, scan);
         if (s.expert > p.experts) return;  // uniform
         expert = s.expert;
         m0 = s.begin;
@@ -479,7 +487,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void mx4_few_rows_kernel(Mx4Produc
     const uint32_t tn = blockIdx.x % tiles_n, tm = blockIdx.x / tiles_n;
     uint32_t m0 = tm * 16, m_end = p.M, expert = 0, slices = p.slices;
     if constexpr (MODE == kRows) {
-        const SlotTile s = slot_tile(p, pairs, tm, 16);
+        const SlotTile s = slot_tile(p, pairs, tm, 16, scan_slots(p, pairs, 0, 16));
         if (s.expert > p.experts) return;  // uniform
         expert = s.expert;
         m0 = s.begin;
