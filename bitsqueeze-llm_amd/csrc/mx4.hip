@@ -219,7 +219,7 @@ __global__ __launch_bounds__(kTileThreads) void mx4_encode_tile_kernel(EncodeTil
 // What the gradients of the experts' layer multiply, in one launch: the
 // weighted gradients' and the inputs' columns by experts, and the gradients'
 // rows.  None needs another; three launches took 8 us more.  2048 tokens of
-// two pairs each, 2752 and 2048 BF16: 25 us for 75 MB, mostly from the caches:
+// two pairs each, 2752 and 2048 BF16: 24 us for 75 MB, mostly from the caches:
 // the chain of a tile's loads (its expert, its pairs, their rows) bounds it.
 template <Mx4Type T>
 __global__ __launch_bounds__(kTileThreads) void mx4_encode_backward_kernel(EncodeTiles d, uint32_t d_groups, EncodeTiles x,

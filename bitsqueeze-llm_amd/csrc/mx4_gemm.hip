@@ -114,18 +114,18 @@ __device__ __forceinline__ SlotTile slot_tile(const Mx4Product &p, uint32_t pair
 // The transfers are of whole lines (four times as many half lines arrive at 15
 // TB/s, whole ones at 30), and a row's scales, 8 bytes a slice, come four slices
 // at a time, or they would touch as many lines as the codes.
-// 8192 x 8192 x 8192: 291 us, 3.78 PFLOP/s, the matrix cores busy in 0.48 of the
+// 8192 x 8192 x 8192: 267 us, 4.11 PFLOP/s, the matrix cores busy in half of the
 // cycles (as in a library's product of that size in BF16) at the 1.86 GHz that
-// the card then runs at; 228 us with the transfers left out, 242 with the
-// products, 259 with every line in L2: what bounds it is both together, and the
-// power.
+// the card then runs at.  Left out of an earlier form of 291 us, the transfers
+// gave 228, the products 242, and every line from L2 259: what bounds it is both
+// together, and the power.
 // A row's eight 16-byte blocks are stored in the order block ^ (row / 2 % 8):
 // sixteen neighbouring rows' reads of one block cover all 64 banks.  The lanes'
 // source addresses make the permutation.
 // G > 1: G teams of four waves take a share of the tile's slices each, from
 // stages of their own, and join their sums in LDS in the teams' order: tiles
 // that leave CUs idle take 1 / G of the time (300 x 1000 x 4000 in tiles of 64:
-// 10.4 us with one team, 8.0 with four; through a workspace and a launch
+// 10.8 us with one team, 7.7 with four; through a workspace and a launch
 // of its own 10.9 to 15.7).
 // With `splits` > 1 (dense products) workgroup z sums the slices [z, z + 1)
 // slices / splits and writes part z of the output (FP32 parts in the
@@ -576,7 +576,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void mx4_few_rows_kernel(Mx4Produc
 constexpr uint32_t kPackRows = 16, kPackBytes = 32768;
 constexpr uint64_t kPackReads = 4ull << 20;
 // Rows up to which b is streamed (16 x 4096 x 11008: 10.1 us; in tiles of 64 37
-// rows take 12.7).
+// rows take 13.3).
 constexpr uint32_t kFewRows = 16;
 
 template <Mode MODE, int X>
@@ -611,11 +611,12 @@ void launch_mx4_product_of(const void *x, Mx4Type x_type, uint64_t x_cols, uint6
 namespace {
 
 // How a product is cut.  Measured in us (M x N x K, tile . teams):
-//   2048 x 4096 x 4096    64.1 33.6   128.1 27.4   128.2 31.6   256 38.7
-//   1024 x 4096 x 4096    64.1 18.8   64.2 20.6    128.1 18.0   128.2 17.1
-//    512 x 4096 x 4096    64.1 12.5   64.2 11.8    64.4 16.1    128.2 15.3
-//    256 x 4096 x 4096    64.1 11.1   64.2 8.9     64.4 8.7
-//   2000 x  300 x  512    64.1 4.5    64.2 4.4     64.4 5.2
+//   8192 x 4096 x 4096    128.1 91.4  128.2 113    256 75.4
+//   2048 x 4096 x 4096    64.1 36.8   128.1 24.6   128.2 28.9   256 31.4
+//   1024 x 4096 x 4096    64.1 21.1   64.2 21.3    128.1 16.7   128.2 15.8
+//    512 x 4096 x 4096    64.1 13.5   64.2 12.3    64.4 15.7    128.2 14.1
+//    256 x 4096 x 4096    64.1 11.8   64.2 9.0     64.4 8.7     128.2 13.6
+//   2000 x  300 x  512    64.1 4.0    64.2 4.0     64.4 4.9     128.2 6.3
 // Teams as long as every workgroup still finds a CU of its own; tiles of 256
 // where their rounds over the CUs cost less (a round of one a CU 2.4 us a
 // slice, of two 128s a CU 1.44).
@@ -643,7 +644,7 @@ Plan plan_of(uint32_t M, uint32_t N, uint32_t slices) {
     if (q.tile == 64 && q.teams == 4) {
         // more workgroups for a long shared axis: a turn of four slices 1.6 us,
         // against the join's launch and the parts' way to memory and back (37
-        // x 4096 x 11008: 19.5 us with one split, 12.7 with 4; 128 x 128 x
+        // x 4096 x 11008: 21.2 us with one split, 13.3 with 4; 128 x 128 x
         // 60000: 70 and, with 8, 15.8)
         double best = 0.0;
         for (uint32_t s = 1; s <= 16 && tiles(64) * s <= 2 * cus; s *= 2) {
@@ -682,8 +683,8 @@ void launch_mx4_product(const Mx4Product &p, void *workspace, uint64_t workspace
     const uint64_t cus = static_cast<uint64_t>(cu_count());
     if (p.shared_slots) {
         // (480 tokens to 4 experts, 176 x 338: 256 14.2 us, 64 4.9; 4096 pairs of
-        // 16 experts, 2752 x 2048: 256 82, 128 87, 64 102, where the 180 MB
-        // written alone take 39)
+        // 16 experts, 2752 x 2048: 256 66, 128 70, where the 180 MB written take
+        // some 35)
         auto of = [&](uint64_t t) { return p.experts * ceil_div(p.M, t) * ceil_div(p.N, t); };
         if (of(128) <= cus) tiles<64, 1, kShared>(p, ceil_div(p.M, 64), ceil_div(p.N, 64), 1, stream);
         else if (of(256) <= 2 * cus) tiles<128, 1, kShared>(p, ceil_div(p.M, 128), ceil_div(p.N, 128), 1, stream);
@@ -697,8 +698,9 @@ void launch_mx4_product(const Mx4Product &p, void *workspace, uint64_t workspace
         if (p.M / p.experts <= 16) few_rows<kRows, kPacked>(p, of(16), p.M, nullptr, 0, 0, stream);
         else if (count(64) <= 2 * cus && p.slices > 1) tiles<64, 2, kRows>(p, of(64), ceil_div(p.N, 64), 1, stream);
         else if (count(128) <= cus || p.M / p.experts <= 64) tiles<64, 1, kRows>(p, of(64), ceil_div(p.N, 64), 1, stream);
-        // (us: 16384 pairs of 32 experts, 2752 x 4096 with 128 199, with 256
-        // 179; 4096 of 16, 2752 x 2048 46 and 54, 2048 x 2752 43 and 37)
+        // (us: 16384 pairs of 32 experts, 2752 x 4096 with 256 159, before the
+        // last changes 179 against 199 with 128; 4096 of 16, 2752 x 2048 with
+        // 128 45, with 256 60, 2048 x 2752 41 and 33)
         else if (large_tiles(rows(128), rows(256), p.N)) tiles<256, 1, kRows>(p, of(256), ceil_div(p.N, 256), 1, stream);
         else tiles<128, 1, kRows>(p, of(128), ceil_div(p.N, 128), 1, stream);
     } else if (p.M <= kFewRows) {

@@ -187,7 +187,8 @@ def test_layer(type, out, tokens, k, experts, inputs, n):
         assert (np.abs(gw[e] - dw[e]) <= bound + ROUNDING[out] * np.abs(dw[e]) + 1e-30).all()
 
 
-@pytest.mark.parametrize("tokens,k,experts,inputs,n", [(1500, 2, 4, 300, 520), (3000, 2, 3, 256, 1400), (2600, 4, 40, 130, 300)])
+@pytest.mark.parametrize("tokens,k,experts,inputs,n", [(1500, 2, 4, 300, 520), (3000, 2, 3, 256, 1400), (2600, 4, 40, 130, 300),
+                                                       (2000, 2, 64, 130, 200), (1500, 4, 150, 130, 260)])
 def test_layer_in_large_tiles(tokens, k, experts, inputs, n):
     # integers whose sums are exact: the forward pass, the gradient of x and the
     # weights' own, element by element
