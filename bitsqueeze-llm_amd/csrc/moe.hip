@@ -488,8 +488,8 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const void *__restrict
 }
 
 // d weights: a wave takes a pair's dot product with the token's d out.  4096
-// pairs of 2752 BF16: 10.4 us (23 MB of y, d out from L2), bound by a wave's
-// own chain of loads.
+// pairs of 2752 BF16: 10.6 us for 34 MB (6.5 at the rate of a large copy); loads of
+// several pieces in flight take 10.4.
 template <Mx4Type Y, Mx4Type D>
 __global__ __launch_bounds__(256) void moe_weights_backward_kernel(const void *__restrict__ y, uint64_t pairs, uint32_t k,
                                                                    uint32_t cols, const int32_t *__restrict__ ids,
