@@ -142,20 +142,29 @@ def abi_leg(src, ddst, n, wl, reps=5):
     return 4.0 * n / (ms * 1e-3) / 1e9, ms
 
 
-def sources_sha256() -> str:
-    """SHA-256 over the kernel and runtime sources, the public headers and the
-    build script (file names and contents, in name order): the identity of
-    the code a profile summary was collected from."""
-    import hashlib
+# Sources of operators that no workload here runs.
+OTHER_SOURCES = {"mx4.hip", "mx4.hpp", "mx4_gemm.hip", "moe.hip"}
 
+
+def sources_sha256() -> str:
+    """SHA-256 over the sources of the workloads' kernels and runtime, the C++
+    headers (file names and contents, in name order) and the flags that they are
+    built with: the identity of the code a profile summary was collected from."""
+    import hashlib
+    import importlib.util
+
+    spec = importlib.util.spec_from_file_location("bsq_build", os.path.join(PKG, "build.py"))
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
     h = hashlib.sha256()
     files = []
-    for d, exts in ((os.path.join(PKG, "csrc"), (".hip", ".hpp")), (os.path.join(ROOT, "include"), (".h", ".hpp"))):
-        files += [os.path.join(d, f) for f in sorted(os.listdir(d)) if f.endswith(exts)]
-    files.append(os.path.join(PKG, "build.py"))
+    for d, exts in ((os.path.join(PKG, "csrc"), (".hip", ".hpp")), (os.path.join(ROOT, "include"), (".hpp",))):
+        files += [os.path.join(d, f) for f in sorted(os.listdir(d)) if f.endswith(exts) and f not in OTHER_SOURCES]
     for f in files:
         h.update(os.path.relpath(f, ROOT).encode())
         h.update(open(f, "rb").read())
+    flags = [f.replace(ROOT, "") for f in build.COMMON]
+    h.update(repr((flags, build.EXTRA, sorted(build.NO_CONTRACT - OTHER_SOURCES))).encode())
     return h.hexdigest()
 
 
