@@ -137,13 +137,15 @@ __device__ __forceinline__ void softmax_of(const float x[NV], float e[NV], float
 template <int NV>
 struct Keys {
     int key[NV];
-    uint32_t where = 0;
+    uint32_t where = 0x3210u;
     static constexpr bool kSorted = NV <= 4;
+    // from any order: again where keys of the list were closed
     __device__ __forceinline__ void sort() {
         if constexpr (kSorted) {
             uint32_t at[NV];
 #pragma unroll
-            for (int i = 0; i < NV; ++i) at[i] = i;
+            for (int i = 0; i < NV; ++i) at[i] = (where >> (4 * i)) & 15u;
+            where = 0;
 #pragma unroll
             for (int r = 0; r < NV; ++r)
 #pragma unroll
@@ -255,6 +257,7 @@ __device__ __forceinline__ void keep_groups(const RouteArgs &a, uint32_t lane, K
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) keys.key[i] = group[i] < 64 && ((chosen >> group[i]) & 1) ? keys.key[i] : kShut;
+    keys.sort();  // a lane's keys may be of two groups: the open ones to the front
 }
 
 // One wave a token, NV experts a lane.  The largest of the lanes' largest keys
