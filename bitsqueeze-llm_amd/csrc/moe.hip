@@ -767,7 +767,7 @@ int bsq_moe_linear_backward(const void *d_d_out, int d_type, uint64_t tokens, ui
         uint8_t *codes = nullptr, *scales = nullptr, *z = nullptr, *gc = nullptr, *gs = nullptr, *xc = nullptr, *xs = nullptr;
         if (pairs > 0) {
             codes = arena.take(tokens * slices * 128), scales = arena.take(tokens * slices * 8);
-            z = arena.take(pairs * inputs * type_bytes(tg));
+            z = arena.take(pairs * inputs * 4);
             gc = arena.take(n * slots * 128), gs = arena.take(n * slots * 8);
             xc = arena.take(inputs * slots * 128), xs = arena.take(inputs * slots * 8);
             Mx4Slots of{d_offsets, d_order, d_weights, experts, k};
@@ -785,7 +785,10 @@ int bsq_moe_linear_backward(const void *d_d_out, int d_type, uint64_t tokens, ui
         }
         if (pairs > 0 && d_dx != nullptr) {
             // dx[t] = sum of weight * (q(d out[t]) W_e): the layer itself, with
-            // the weights' columns for their rows
+            // the weights' columns for their rows.  The terms are FP32 until they
+            // are summed, whatever the gradients' type: a pair's product may lie
+            // above FP16's range where its weight brings it back, and in BF16
+            // dx was off by 0.0024 in place of 0.0017.
             Mx4Product p;
             p.a = {codes, scales};
             p.b = {d_wt_codes, d_wt_scales};
@@ -793,14 +796,14 @@ int bsq_moe_linear_backward(const void *d_d_out, int d_type, uint64_t tokens, ui
             p.N = static_cast<uint32_t>(inputs);
             p.slices = slices;
             p.out = z;
-            p.type = tg;
+            p.type = Mx4Type::F32;
             p.ld = inputs;
             p.offsets = d_offsets;
             p.order = d_order;
             p.experts = experts;
             p.per_token = k;
             launch_mx4_product(p, nullptr, 0, s);
-            combine(z, tg, tokens, k, static_cast<uint32_t>(inputs), d_ids, d_weights, experts, d_dx, tg, lddx, s);
+            combine(z, Mx4Type::F32, tokens, k, static_cast<uint32_t>(inputs), d_ids, d_weights, experts, d_dx, tg, lddx, s);
         }
         if (pairs > 0 && d_d_weights != nullptr)
             weights_backward(d_y, ty, tokens, k, static_cast<uint32_t>(n), d_ids, experts, d_d_out, td, ldd, d_d_weights, s);
