@@ -314,11 +314,14 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a, int32_t *__
 }
 
 // d logits from d weights.  Lane j forms the score of the token's j-th expert
-// again from its own logit; with w_j = scale s_j / S the scores' gradient is
-// (g_j - sum g w / scale) / S, g = scale dw, and the scores' own rule follows:
-// only the chosen for sigmoid, every expert for softmax.  The chosen reach
-// their experts' lanes through a row in LDS.  The same tokens: 7.2 us (9.4 MB
-// written; softmax reads as much), launch and latency.
+// again from its own logit.  With g = scale dw and w_j = s_j / S (S = 1 without
+// the renormalisation) the gradient of the j-th expert's own logit is w_j h_j,
+// h_j = g_j - sum g w, for sigmoid times 1 - s_j; for softmax every expert of
+// score s loses s sum w h, which is 0 where the weights are renormalised.  Where
+// S is held at the smallest normal number it does not depend on the scores, and
+// h_j = g_j.  Nothing is divided by S but the scores, so no quotient overflows.
+// The chosen reach their experts' lanes through a row in LDS.  The same tokens:
+// 7.2 us (9.4 MB written; softmax reads as much), launch and latency.
 template <Mx4Type T, int NV>
 __global__ __launch_bounds__(256) void moe_route_backward_kernel(RouteArgs a, const int32_t *__restrict__ ids,
                                                                  const float *__restrict__ d_weights,
@@ -350,20 +353,24 @@ __global__ __launch_bounds__(256) void moe_route_backward_kernel(RouteArgs a, co
             d = d_weights[t * a.k + lane] * a.scale;
         }
     }
+    float share = s, mean = 0.0f;
+    bool whole = false;  // the shares sum to one whatever the scores
     if (a.renorm) {
-        const float total = fmaxf(wave_sum(s), FLT_MIN);
-        const float mean = wave_sum(d * (s / total));
-        d = real ? (d - mean) / total : 0.0f;
+        const float total = wave_sum(s);
+        whole = total > FLT_MIN;
+        share = s / fmaxf(total, FLT_MIN);
+        const float common = wave_sum(d * share);
+        d = real && whole ? d - common : d;
     }
-    const float mean = a.sigmoid ? 0.0f : wave_sum(d * s);
+    if (!a.sigmoid && !whole) mean = wave_sum(d * share);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (real) row[id] = a.sigmoid ? d * s * rest : d;  // a choice has an expert once
+    if (real) row[id] = d * share * (a.sigmoid ? rest : 1.0f);  // a choice has an expert once
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     float g[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         g[i] = row[lane * NV + i];
-        if (!a.sigmoid) g[i] = score[i] * (g[i] - mean);
+        if (!a.sigmoid) g[i] -= score[i] * mean;
     }
     const uint32_t e0 = lane * NV;
     const uint64_t at = t * ldd + e0;

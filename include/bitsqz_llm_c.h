@@ -388,7 +388,8 @@ BSQ_API int bsq_mx4_linear_backward(const void *d_dy, int type, uint64_t m, uint
  * sum, is largest; ties go to the lowest number.  An expert whose logit is NaN
  * or at or below its type's lowest finite value is closed to the token.  ids:
  * tokens x k, best first, -1 (weight 0) where no open expert is left; weights:
- * the scores, over their sum if `renormalise`, times `scale`. */
+ * the scores, over their sum if `renormalise` (over the smallest normal FP32
+ * number where the sum is below it), times `scale`. */
 BSQ_API int bsq_moe_route(const void *d_logits, int type, uint64_t tokens, uint32_t experts, uint64_t ld,
                           const float *d_bias, int scoring, uint32_t groups, uint32_t kept, uint32_t k, int renormalise,
                           float scale, int32_t *d_ids, float *d_weights, void *stream);
