@@ -657,6 +657,14 @@ def _typed(x: np.ndarray, type: int) -> np.ndarray:
     return np.ascontiguousarray(x, _TYPE_NUMPY[type])
 
 
+def workspace(query: str, *sizes: int) -> int:
+    """The bytes that a bsq_*_workspace query gives; raises where there is no size."""
+    n = getattr(lib(), query)(*sizes)
+    if n == 2**64 - 1:
+        raise BsqError(f"{query} failed: {lib().bsq_last_error().decode()}")
+    return n
+
+
 class Mx4:
     """A packed matrix of rows x cols (or several, one after another) on the GPU."""
 
@@ -696,7 +704,7 @@ def mx4_encode(x: np.ndarray, type: int = TYPE_F32, rows: bool = True, columns: 
 
 def mx4_product(a: Mx4, b: Mx4, type: int = TYPE_F32) -> np.ndarray:
     out = DeviceBuffer(a.rows * b.rows * _TYPE_NUMPY[type].itemsize)
-    work = DeviceBuffer(lib().bsq_mx4_product_workspace(a.rows, b.rows, a.cols))
+    work = DeviceBuffer(workspace("bsq_mx4_product_workspace", a.rows, b.rows, a.cols))
     check(lib().bsq_mx4_product(a.codes.ptr, a.scales.ptr, a.rows, b.codes.ptr, b.scales.ptr, b.rows, a.cols, out.ptr,
                                 type, b.rows, work.ptr, work.nbytes, None), "mx4_product")
     check(lib().bsq_stream_synchronize(None), "sync")
@@ -708,7 +716,7 @@ def mx4_linear(x: np.ndarray, w: Mx4, type: int = TYPE_F32, out_type: int = TYPE
     x = _typed(x, type)
     m, k = x.shape
     d, out = DeviceBuffer.from_array(x), DeviceBuffer(m * w.rows * _TYPE_NUMPY[out_type].itemsize)
-    work = DeviceBuffer(lib().bsq_mx4_linear_workspace(m, w.rows, k))
+    work = DeviceBuffer(workspace("bsq_mx4_linear_workspace", m, w.rows, k))
     xt = Mx4(k, m) if keep else None
     check(lib().bsq_mx4_linear(d.ptr, type, m, k, k, w.codes.ptr, w.scales.ptr, w.rows, out.ptr, out_type, w.rows,
                                xt.codes.ptr if keep else None, xt.scales.ptr if keep else None, work.ptr, work.nbytes,
@@ -724,7 +732,7 @@ def mx4_linear_backward(dy: np.ndarray, xt: Mx4, wt: Mx4, type: int = TYPE_F32, 
     (m, n), k = dy.shape, wt.rows
     size = _TYPE_NUMPY[g_type].itemsize
     d, dx, dw = DeviceBuffer.from_array(dy), DeviceBuffer(m * k * size), DeviceBuffer(n * k * size)
-    work = DeviceBuffer(lib().bsq_mx4_linear_backward_workspace(m, n, k))
+    work = DeviceBuffer(workspace("bsq_mx4_linear_backward_workspace", m, n, k))
     check(lib().bsq_mx4_linear_backward(d.ptr, type, m, n, n, xt.codes.ptr, xt.scales.ptr, wt.codes.ptr, wt.scales.ptr,
                                         k, dx.ptr, k, dw.ptr, k, g_type, work.ptr, work.nbytes, None),
           "mx4_linear_backward")
@@ -785,7 +793,7 @@ class MoeLinear:
         self.offsets, self.order = DeviceBuffer(4 * (e + 1)), DeviceBuffer(4 * m * k)
         self.y = DeviceBuffer(m * k * n * _TYPE_NUMPY[y_type].itemsize)
         out = DeviceBuffer(m * n * _TYPE_NUMPY[out_type].itemsize)
-        work = DeviceBuffer(lib().bsq_moe_linear_workspace(m, k, n, self.inputs, e))
+        work = DeviceBuffer(workspace("bsq_moe_linear_workspace", m, k, n, self.inputs, e))
         check(lib().bsq_moe_linear(self.x.ptr, type, m, self.inputs, self.inputs, self.ids.ptr, self.weights.ptr, k,
                                    self.w.codes.ptr, self.w.scales.ptr, e, n, self.offsets.ptr, self.order.ptr,
                                    self.y.ptr, y_type, out.ptr, out_type, n, work.ptr, work.nbytes, None), "moe_linear")
@@ -799,7 +807,7 @@ class MoeLinear:
         t = _TYPE_NUMPY[g_type]
         d, dx, dw = DeviceBuffer.from_array(d_out), DeviceBuffer(m * inputs * t.itemsize), DeviceBuffer(e * n * inputs * t.itemsize)
         dweights = DeviceBuffer(4 * m * k)
-        work = DeviceBuffer(lib().bsq_moe_linear_backward_workspace(m, k, n, inputs, e))
+        work = DeviceBuffer(workspace("bsq_moe_linear_backward_workspace", m, k, n, inputs, e))
         check(lib().bsq_moe_linear_backward(d.ptr, type, m, n, n, self.x.ptr, self.type, inputs, inputs, self.ids.ptr,
                                             self.weights.ptr, k, self.offsets.ptr, self.order.ptr, self.y.ptr,
                                             self.y_type, self.wt.codes.ptr, self.wt.scales.ptr, e, dx.ptr, inputs,

@@ -601,6 +601,12 @@ void check_layer(uint64_t tokens, uint32_t k, uint64_t n, uint64_t inputs, uint3
     BSQ_REQUIRE(n >= 1 && inputs >= 1 && n <= (1u << 22) && inputs <= (1u << 22), "moe linear: 1 to 2^22 inputs and outputs");
 }
 uint64_t slot_slices(uint64_t pairs, uint32_t experts) { return pairs / kMx4Slice + std::min<uint64_t>(pairs, experts); }
+uint64_t linear_work(uint64_t tokens, uint64_t inputs) { return packed_bytes(tokens, mx4_slices(inputs)); }
+uint64_t linear_backward_work(uint64_t tokens, uint32_t k, uint64_t n, uint64_t inputs, uint32_t experts) {
+    const uint64_t slots = slot_slices(tokens * k, experts);
+    return packed_bytes(tokens, mx4_slices(n)) + round256(tokens * k * inputs * 4) + packed_bytes(n, slots) +
+           packed_bytes(inputs, slots);
+}
 
 }  // namespace
 }  // namespace bsq
@@ -675,10 +681,10 @@ int bsq_moe_combine(const void *d_y, int y_type, uint64_t tokens, uint32_t k, ui
 }
 
 uint64_t bsq_moe_linear_workspace(uint64_t tokens, uint32_t k, uint64_t n, uint64_t inputs, uint32_t experts) {
-    (void)k;
-    (void)n;
-    (void)experts;
-    return packed_bytes(tokens, mx4_slices(inputs));
+    return size_query([&] {
+        check_layer(tokens, k, n, inputs, experts);
+        return linear_work(tokens, inputs);
+    });
 }
 
 int bsq_moe_linear(const void *d_x, int x_type, uint64_t tokens, uint64_t inputs, uint64_t ldx, const int32_t *d_ids,
@@ -698,7 +704,7 @@ int bsq_moe_linear(const void *d_x, int x_type, uint64_t tokens, uint64_t inputs
             check_dense(d_y, ty, "moe linear: null y");
             check_dense(d_out, to, "moe linear: null output");
             check_packed(d_w_codes, d_w_scales);
-            check_work(d_work, work_bytes, bsq_moe_linear_workspace(tokens, k, n, inputs, experts));
+            check_work(d_work, work_bytes, linear_work(tokens, inputs));
         }
         if (pairs == 0) {
             plan(d_ids, pairs, experts, d_offsets, d_order, s);
@@ -734,9 +740,10 @@ int bsq_moe_linear(const void *d_x, int x_type, uint64_t tokens, uint64_t inputs
 }
 
 uint64_t bsq_moe_linear_backward_workspace(uint64_t tokens, uint32_t k, uint64_t n, uint64_t inputs, uint32_t experts) {
-    const uint64_t slots = slot_slices(tokens * k, experts);
-    return packed_bytes(tokens, mx4_slices(n)) + round256(tokens * k * inputs * 4) + packed_bytes(n, slots) +
-           packed_bytes(inputs, slots);
+    return size_query([&] {
+        check_layer(tokens, k, n, inputs, experts);
+        return linear_backward_work(tokens, k, n, inputs, experts);
+    });
 }
 
 int bsq_moe_linear_backward(const void *d_d_out, int d_type, uint64_t tokens, uint64_t n, uint64_t ldd, const void *d_x,
@@ -764,7 +771,7 @@ int bsq_moe_linear_backward(const void *d_d_out, int d_type, uint64_t tokens, ui
             // its rows of slots are 128 bytes a slice, and a tile's 256 of them lie
             // within 32 bits
             BSQ_REQUIRE(d_dw == nullptr || slot_slices(pairs, experts) <= 1u << 17, "moe linear: too many pairs for dw");
-            check_work(d_work, work_bytes, bsq_moe_linear_backward_workspace(tokens, k, n, inputs, experts));
+            check_work(d_work, work_bytes, linear_backward_work(tokens, k, n, inputs, experts));
         }
         if (d_dw) check_dense(d_dw, tg, "");
         hipStream_t s = static_cast<hipStream_t>(stream);

@@ -386,6 +386,15 @@ void check_sides(uint64_t m, uint64_t n, uint64_t k) {
 }
 uint64_t packed(uint64_t rows, uint64_t cols) { return packed_bytes(rows, mx4_slices(cols)); }
 
+// Workspaces of sizes that are checked; they ask the device for its CUs.
+uint64_t product_work(uint64_t m, uint64_t n, uint64_t k) {
+    return mx4_product_workspace(static_cast<uint32_t>(m), static_cast<uint32_t>(n), static_cast<uint32_t>(mx4_slices(k)));
+}
+uint64_t linear_work(uint64_t m, uint64_t n, uint64_t k) { return packed(m, k) + round256(product_work(m, n, k)); }
+uint64_t linear_backward_work(uint64_t m, uint64_t n, uint64_t k) {
+    return packed(m, n) + packed(n, m) + round256(std::max(product_work(m, k, n), product_work(n, k, m)));
+}
+
 Mx4Product product_of(Mx4Matrix a, uint64_t m, Mx4Matrix b, uint64_t n, uint64_t k, void *out, Mx4Type type, uint64_t ld) {
     Mx4Product p;
     p.a = a;
@@ -439,7 +448,10 @@ int bsq_mx4_decode(const uint8_t *d_codes, const uint8_t *d_scales, uint64_t row
 }
 
 uint64_t bsq_mx4_product_workspace(uint64_t m, uint64_t n, uint64_t k) {
-    return mx4_product_workspace(static_cast<uint32_t>(m), static_cast<uint32_t>(n), static_cast<uint32_t>(mx4_slices(k)));
+    return size_query([&] {
+        check_sides(m, n, k);
+        return product_work(m, n, k);
+    });
 }
 
 int bsq_mx4_product(const uint8_t *d_a_codes, const uint8_t *d_a_scales, uint64_t m, const uint8_t *d_b_codes,
@@ -454,14 +466,17 @@ int bsq_mx4_product(const uint8_t *d_a_codes, const uint8_t *d_a_scales, uint64_
         check_packed(d_a_codes, d_a_scales);
         check_packed(d_b_codes, d_b_scales);
         check_dense(d_out, t, "mx4 product: null output");
-        check_work(d_work, work_bytes, bsq_mx4_product_workspace(m, n, k));
+        check_work(d_work, work_bytes, product_work(m, n, k));
         launch_mx4_product(product_of({d_a_codes, d_a_scales}, m, {d_b_codes, d_b_scales}, n, k, d_out, t, ld), d_work,
                            work_bytes, static_cast<hipStream_t>(stream));
     });
 }
 
 uint64_t bsq_mx4_linear_workspace(uint64_t m, uint64_t n, uint64_t k) {
-    return packed(m, k) + round256(bsq_mx4_product_workspace(m, n, k));
+    return size_query([&] {
+        check_sides(m, n, k);
+        return linear_work(m, n, k);
+    });
 }
 
 int bsq_mx4_linear(const void *d_x, int x_type, uint64_t m, uint64_t k, uint64_t ldx, const uint8_t *d_w_codes,
@@ -478,7 +493,7 @@ int bsq_mx4_linear(const void *d_x, int x_type, uint64_t m, uint64_t k, uint64_t
         check_packed(d_w_codes, d_w_scales);
         BSQ_REQUIRE((d_xt_codes == nullptr) == (d_xt_scales == nullptr), "mx4 linear: codes come with their scales");
         if (d_xt_codes) check_packed(d_xt_codes, d_xt_scales);
-        check_work(d_work, work_bytes, bsq_mx4_linear_workspace(m, n, k));
+        check_work(d_work, work_bytes, linear_work(m, n, k));
         hipStream_t s = static_cast<hipStream_t>(stream);
         uint8_t *codes = static_cast<uint8_t *>(d_work), *scales = codes + round256(m * mx4_slices(k) * 128);
         const Mx4Product p = product_of({codes, scales}, m, {d_w_codes, d_w_scales}, n, k, d_out, to, ldo);
@@ -492,8 +507,10 @@ int bsq_mx4_linear(const void *d_x, int x_type, uint64_t m, uint64_t k, uint64_t
 }
 
 uint64_t bsq_mx4_linear_backward_workspace(uint64_t m, uint64_t n, uint64_t k) {
-    return packed(m, n) + packed(n, m) +
-           round256(std::max(bsq_mx4_product_workspace(m, k, n), bsq_mx4_product_workspace(n, k, m)));
+    return size_query([&] {
+        check_sides(m, n, std::max({m, n, k}));
+        return linear_backward_work(m, n, k);
+    });
 }
 
 int bsq_mx4_linear_backward(const void *d_dy, int type, uint64_t m, uint64_t n, uint64_t ldy, const uint8_t *d_xt_codes,
@@ -511,7 +528,7 @@ int bsq_mx4_linear_backward(const void *d_dy, int type, uint64_t m, uint64_t n, 
         if (d_dw) check_dense(d_dw, tg, "");
         if (d_dx) check_packed(d_wt_codes, d_wt_scales);
         if (d_dw) check_packed(d_xt_codes, d_xt_scales);
-        check_work(d_work, work_bytes, bsq_mx4_linear_backward_workspace(m, n, k));
+        check_work(d_work, work_bytes, linear_backward_work(m, n, k));
         hipStream_t s = static_cast<hipStream_t>(stream);
         uint8_t *rc = static_cast<uint8_t *>(d_work), *rs = rc + round256(m * mx4_slices(n) * 128);
         uint8_t *cc = rc + packed(m, n), *cs = cc + round256(n * mx4_slices(m) * 128);

@@ -344,4 +344,12 @@ int entry(F &&f) noexcept {
     return 1;
 }
 
+// Size queries: UINT64_MAX where there is no size, with the reason as the last
+// error
+template <class F>
+uint64_t size_query(F &&f) noexcept {
+    uint64_t size = UINT64_MAX;
+    return entry([&] { size = f(); }) == 0 ? size : UINT64_MAX;
+}
+
 }  // namespace bsq

@@ -342,7 +342,10 @@ BSQ_API int bsq_legacy_sweep(int kind, uint64_t lo, uint64_t hi, unsigned long l
  *    to the next.  Sums are held in FP32 and rounded once.  All calls are
  *    asynchronous on `stream`, keep nothing between calls and take their
  *    workspace from the caller (its bytes: the function beside them), so they
- *    can be captured, and run on several streams with a workspace each.
+ *    can be captured, and run on several streams with a workspace each.  The
+ *    workspace functions give UINT64_MAX, with the reason in bsq_last_error(),
+ *    for sizes that the call refuses, or without a device where the size hangs
+ *    on its CUs.
  * ------------------------------------------------------------------------- */
 BSQ_API uint64_t bsq_mx4_codes_bytes(uint64_t rows, uint64_t cols);
 BSQ_API uint64_t bsq_mx4_scales_bytes(uint64_t rows, uint64_t cols);
