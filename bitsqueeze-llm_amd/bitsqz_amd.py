@@ -657,6 +657,13 @@ def _typed(x: np.ndarray, type: int) -> np.ndarray:
     return np.ascontiguousarray(x, _TYPE_NUMPY[type])
 
 
+def _agree(ok: bool, what: str):
+    """The calls see only pointers: sizes that do not agree are refused here,
+    before anything is uploaded."""
+    if not ok:
+        raise ValueError(what)
+
+
 def workspace(query: str, *sizes: int) -> int:
     """The bytes that a bsq_*_workspace query gives; raises where there is no size."""
     n = getattr(lib(), query)(*sizes)
@@ -691,6 +698,7 @@ class Mx4:
 def mx4_encode(x: np.ndarray, type: int = TYPE_F32, rows: bool = True, columns: bool = False):
     """The packed rows and / or columns of x (rows x cols, or a batch of those)."""
     x = _typed(x, type)
+    _agree(x.ndim in (2, 3), "mx4_encode: x is rows x cols or a batch of those")
     batch, r, c = (1, *x.shape) if x.ndim == 2 else x.shape
     by_row = Mx4(r, c, batch) if rows else None
     by_col = Mx4(c, r, batch) if columns else None
@@ -703,6 +711,8 @@ def mx4_encode(x: np.ndarray, type: int = TYPE_F32, rows: bool = True, columns: 
 
 
 def mx4_product(a: Mx4, b: Mx4, type: int = TYPE_F32) -> np.ndarray:
+    _agree(a.batch == b.batch == 1, "mx4_product: a batch of matrices")
+    _agree(a.cols == b.cols, f"mx4_product: {a.cols} and {b.cols} columns")
     out = DeviceBuffer(a.rows * b.rows * _TYPE_NUMPY[type].itemsize)
     work = DeviceBuffer(workspace("bsq_mx4_product_workspace", a.rows, b.rows, a.cols))
     check(lib().bsq_mx4_product(a.codes.ptr, a.scales.ptr, a.rows, b.codes.ptr, b.scales.ptr, b.rows, a.cols, out.ptr,
@@ -714,6 +724,9 @@ def mx4_product(a: Mx4, b: Mx4, type: int = TYPE_F32) -> np.ndarray:
 def mx4_linear(x: np.ndarray, w: Mx4, type: int = TYPE_F32, out_type: int = TYPE_F32, keep: bool = False):
     """out = q(x) W^T; with `keep` also the packed transpose of x."""
     x = _typed(x, type)
+    _agree(x.ndim == 2, "mx4_linear: x is a matrix")
+    _agree(w.batch == 1, "mx4_linear: a batch of weights")
+    _agree(x.shape[1] == w.cols, f"mx4_linear: x has {x.shape[1]} columns, the weights {w.cols}")
     m, k = x.shape
     d, out = DeviceBuffer.from_array(x), DeviceBuffer(m * w.rows * _TYPE_NUMPY[out_type].itemsize)
     work = DeviceBuffer(workspace("bsq_mx4_linear_workspace", m, w.rows, k))
@@ -729,7 +742,12 @@ def mx4_linear(x: np.ndarray, w: Mx4, type: int = TYPE_F32, out_type: int = TYPE
 def mx4_linear_backward(dy: np.ndarray, xt: Mx4, wt: Mx4, type: int = TYPE_F32, g_type: int = TYPE_F32):
     """(dx, dw) of mx4_linear from the packed columns of x and of the weights."""
     dy = _typed(dy, type)
+    _agree(dy.ndim == 2, "mx4_linear_backward: dy is a matrix")
+    _agree(xt.batch == wt.batch == 1, "mx4_linear_backward: a batch of matrices")
     (m, n), k = dy.shape, wt.rows
+    _agree(xt.cols == m, f"mx4_linear_backward: dy has {m} rows, the kept columns of x {xt.cols}")
+    _agree(wt.cols == n, f"mx4_linear_backward: dy has {n} columns, the weights' columns {wt.cols}")
+    _agree(xt.rows == k, f"mx4_linear_backward: x has {xt.rows} inputs, the weights {k}")
     size = _TYPE_NUMPY[g_type].itemsize
     d, dx, dw = DeviceBuffer.from_array(dy), DeviceBuffer(m * k * size), DeviceBuffer(n * k * size)
     work = DeviceBuffer(workspace("bsq_mx4_linear_backward_workspace", m, n, k))
@@ -744,7 +762,9 @@ def moe_route(logits: np.ndarray, k: int, type: int = TYPE_F32, bias: np.ndarray
               scoring: int = SCORE_SOFTMAX, groups: int = 1, kept: int = 1, renormalise: bool = True, scale: float = 1.0):
     """(ids, weights), tokens x k."""
     logits = _typed(logits, type)
+    _agree(logits.ndim == 2, "moe_route: the logits are a matrix")
     tokens, experts = logits.shape
+    _agree(bias is None or np.shape(bias) == (experts,), f"moe_route: a bias for each of {experts} experts")
     d = DeviceBuffer.from_array(logits)
     db = DeviceBuffer.from_array(np.ascontiguousarray(bias, np.float32)) if bias is not None else None
     ids, weights = DeviceBuffer(tokens * k * 4), DeviceBuffer(tokens * k * 4)
@@ -757,9 +777,12 @@ def moe_route(logits: np.ndarray, k: int, type: int = TYPE_F32, bias: np.ndarray
 
 def moe_route_backward(logits: np.ndarray, ids: np.ndarray, d_weights: np.ndarray, type: int = TYPE_F32,
                        scoring: int = SCORE_SOFTMAX, renormalise: bool = True, scale: float = 1.0) -> np.ndarray:
-    logits = _typed(logits, type)
+    logits, ids = _typed(logits, type), np.ascontiguousarray(ids, np.int32)
+    _agree(logits.ndim == 2, "moe_route_backward: the logits are a matrix")
+    _agree(ids.ndim == 2 and len(ids) == len(logits), f"moe_route_backward: ids of {len(logits)} tokens")
+    _agree(np.shape(d_weights) == ids.shape, "moe_route_backward: a gradient of weights for every id")
     (tokens, experts), k = logits.shape, ids.shape[1]
-    d, di = DeviceBuffer.from_array(logits), DeviceBuffer.from_array(np.ascontiguousarray(ids, np.int32))
+    d, di = DeviceBuffer.from_array(logits), DeviceBuffer.from_array(ids)
     dw, out = DeviceBuffer.from_array(np.ascontiguousarray(d_weights, np.float32)), DeviceBuffer(logits.nbytes)
     check(lib().bsq_moe_route_backward(d.ptr, type, tokens, experts, experts, scoring, k, int(renormalise), scale, di.ptr,
                                        dw.ptr, out.ptr, experts, None), "moe_route_backward")
@@ -782,14 +805,21 @@ class MoeLinear:
     def __init__(self, w: Mx4, wt: Mx4 | None = None):
         """w: a batch of n x inputs; wt: the batch of its columns (inputs x n),
         for the gradient of x."""
+        _agree(wt is None or (wt.batch, wt.rows, wt.cols) == (w.batch, w.cols, w.rows),
+               "MoeLinear: wt are the weights' columns, experts x inputs x n")
+        self.done = False  # a forward call has left what backward() reads
         self.w, self.wt, self.experts, self.n, self.inputs = w, wt, w.batch, w.rows, w.cols
 
     def forward(self, x, ids, weights, type: int = TYPE_F32, out_type: int = TYPE_F32, y_type: int = TYPE_F32):
-        x, ids = _typed(x, type), np.ascontiguousarray(ids, np.int32)
-        (m, _), k, e, n = x.shape, ids.shape[1], self.experts, self.n
+        self.done = False
+        x, ids, weights = _typed(x, type), np.ascontiguousarray(ids, np.int32), np.ascontiguousarray(weights, np.float32)
+        _agree(x.ndim == 2, "MoeLinear: x is a matrix")
+        _agree(x.shape[1] == self.inputs, f"MoeLinear: x has {x.shape[1]} columns, the weights {self.inputs}")
+        _agree(ids.ndim == 2 and len(ids) == len(x), f"MoeLinear: ids of {len(x)} tokens")
+        _agree(weights.shape == ids.shape, "MoeLinear: routing weights for every id")
+        m, k, e, n = len(x), ids.shape[1], self.experts, self.n
         self.type, self.m, self.k, self.y_type = type, m, k, y_type
-        self.x, self.ids = DeviceBuffer.from_array(x), DeviceBuffer.from_array(ids)
-        self.weights = DeviceBuffer.from_array(np.ascontiguousarray(weights, np.float32))
+        self.x, self.ids, self.weights = (DeviceBuffer.from_array(v) for v in (x, ids, weights))
         self.offsets, self.order = DeviceBuffer(4 * (e + 1)), DeviceBuffer(4 * m * k)
         self.y = DeviceBuffer(m * k * n * _TYPE_NUMPY[y_type].itemsize)
         out = DeviceBuffer(m * n * _TYPE_NUMPY[out_type].itemsize)
@@ -798,11 +828,16 @@ class MoeLinear:
                                    self.w.codes.ptr, self.w.scales.ptr, e, n, self.offsets.ptr, self.order.ptr,
                                    self.y.ptr, y_type, out.ptr, out_type, n, work.ptr, work.nbytes, None), "moe_linear")
         check(lib().bsq_stream_synchronize(None), "sync")
+        self.done = True
         return out.download(_TYPE_NUMPY[out_type], m * n).reshape(m, n)
 
     def backward(self, d_out, type: int = TYPE_F32, g_type: int = TYPE_F32):
         """(dx, d weights, dw)."""
         d_out = _typed(d_out, type)
+        _agree(self.done, "MoeLinear: backward() goes back through a forward() call")
+        _agree(self.wt is not None, "MoeLinear: backward() needs the weights' columns")
+        _agree(d_out.ndim == 2, "MoeLinear: d_out is a matrix")
+        _agree(d_out.shape == (self.m, self.n), f"MoeLinear: d_out is {self.m} x {self.n}")
         m, k, n, e, inputs = self.m, self.k, self.n, self.experts, self.inputs
         t = _TYPE_NUMPY[g_type]
         d, dx, dw = DeviceBuffer.from_array(d_out), DeviceBuffer(m * inputs * t.itemsize), DeviceBuffer(e * n * inputs * t.itemsize)
