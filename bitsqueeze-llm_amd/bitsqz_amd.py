@@ -748,6 +748,8 @@ def mx4_linear_backward(dy: np.ndarray, xt: Mx4, wt: Mx4, type: int = TYPE_F32, 
     _agree(xt.cols == m, f"mx4_linear_backward: dy has {m} rows, the kept columns of x {xt.cols}")
     _agree(wt.cols == n, f"mx4_linear_backward: dy has {n} columns, the weights' columns {wt.cols}")
     _agree(xt.rows == k, f"mx4_linear_backward: x has {xt.rows} inputs, the weights {k}")
+    if m == 0 or n == 0:  # an empty batch: the call itself wants one to sum over
+        return np.zeros((m, k), _TYPE_NUMPY[g_type]), np.zeros((n, k), _TYPE_NUMPY[g_type])
     size = _TYPE_NUMPY[g_type].itemsize
     d, dx, dw = DeviceBuffer.from_array(dy), DeviceBuffer(m * k * size), DeviceBuffer(n * k * size)
     work = DeviceBuffer(workspace("bsq_mx4_linear_backward_workspace", m, n, k))

@@ -376,7 +376,9 @@ BSQ_API int bsq_mx4_linear(const void *d_x, int x_type, uint64_t m, uint64_t k, 
                            uint8_t *d_xt_codes, uint8_t *d_xt_scales, void *d_work, uint64_t work_bytes, void *stream);
 /* Its gradients, straight through the rounding: dx (m x k) = q(dy) W with the
  * weights' columns d_wt_* (k x n packed), dw (n x k) = q(dy^T) q(x^T)^T with
- * the columns of x that the forward call kept.  d_dx or d_dw may be NULL. */
+ * the columns of x that the forward call kept.  d_dx or d_dw may be NULL.  m
+ * and n are at least 1: unlike the forward call it refuses an empty batch, whose
+ * dw, all zeros, is the caller's to write. */
 BSQ_API uint64_t bsq_mx4_linear_backward_workspace(uint64_t m, uint64_t n, uint64_t k);
 BSQ_API int bsq_mx4_linear_backward(const void *d_dy, int type, uint64_t m, uint64_t n, uint64_t ldy,
                                     const uint8_t *d_xt_codes, const uint8_t *d_xt_scales, const uint8_t *d_wt_codes,
