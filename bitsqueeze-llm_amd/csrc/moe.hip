@@ -755,7 +755,8 @@ int bsq_moe_linear_backward(const void *d_d_out, int d_type, uint64_t tokens, ui
     return entry([&] {
         const Mx4Type td = type_of(d_type), tx = type_of(x_type), ty = type_of(y_type), tg = type_of(g_type);
         check_layer(tokens, k, n, inputs, experts);
-        BSQ_REQUIRE(ldd >= n && ldx >= inputs && lddx >= inputs, "moe linear: rows overlap");
+        BSQ_REQUIRE(ldd >= n && (d_dw == nullptr || ldx >= inputs) && (d_dx == nullptr || lddx >= inputs),
+                    "moe linear: rows overlap");
         const uint64_t pairs = tokens * k;
         BSQ_REQUIRE(d_offsets != nullptr, "moe linear: null argument");
         if (pairs > 0) {
