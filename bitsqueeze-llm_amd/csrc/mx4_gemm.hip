@@ -379,7 +379,9 @@ __global__ __launch_bounds__(64 * G * kTeam<T>, T == 64 ? G : 2) void mx4_produc
 #pragma unroll
             for (int q = 0; q < 16; ++q)
                 stage[(8 * (q >> 2) + 4 * half + (q & 3)) * W + ((32 * j + row) ^ (swap * half))] = acc[i][j][q];
+        // other lanes read what this one wrote: with one team only the wave's own
         if constexpr (G > 1) __syncthreads();
+        else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         // The teams share a wave's rows out.  All of a lane's reads go out before
         // its first store, and no store waits for another (one piece after the
         // other took a third of the time of 16 products of 2752 x 2048 x 256).
@@ -414,7 +416,9 @@ __global__ __launch_bounds__(64 * G * kTeam<T>, T == 64 ? G : 2) void mx4_produc
             const uint32_t m = m0 + wm + 32 * i + r, n = n0 + wn + col;
             if (some && m < m_end && n < p.N) store8<O>(p.out, to[j] * p.ld + n, p.N - n, v[j]);
         }
-        if (G > 1 && i + 1 < BM) __syncthreads();
+        // and all have read before the next rows take the place
+        if constexpr (G == 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        else if (i + 1 < BM) __syncthreads();
     }
 }
 
