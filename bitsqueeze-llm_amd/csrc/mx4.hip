@@ -280,11 +280,30 @@ __global__ __launch_bounds__(kThreads) void mx4_decode_kernel(const uint8_t *__r
     }
 }
 
-unsigned grid_for(uint64_t items) {
-    return static_cast<unsigned>(std::min<uint64_t>(ceil_div(items, kThreads), 1u << 20));
+unsigned grid_for(uint64_t items) { return grid_over(ceil_div(items, kThreads)); }
+
+constexpr const char *kTooLarge = "mx4 encode: matrix too large";
+uint64_t tile_cols(Mx4Type type) { return type == Mx4Type::F32 ? kTileCols<Mx4Type::F32> : kTileCols<Mx4Type::BF16>; }
+// whole slices both ways, so that the padding is written too
+uint64_t encode_tiles(Mx4Type type, uint64_t batch, uint64_t rows, uint64_t cols) {
+    return batch * mx4_slices(cols) * (kMx4Slice / tile_cols(type)) * mx4_slices(rows);
+}
+uint64_t slot_groups(Mx4Type type, uint64_t cols, uint64_t slices) { return slices * ceil_div(cols, tile_cols(type)); }
+uint64_t row_groups(uint64_t tokens, uint64_t n) {
+    return grid_over(ceil_div(tokens * mx4_slices(n) * (kMx4Slice / 8), kTileThreads));
 }
 
 }  // namespace
+
+void check_mx4_encode(Mx4Type type, uint64_t batch, uint64_t rows, uint64_t cols) {
+    grid_of(encode_tiles(type, batch, rows, cols), kTileThreads, kTooLarge);
+}
+void check_mx4_encode_slots(Mx4Type type, uint64_t cols, uint64_t slices) {
+    grid_of(slot_groups(type, cols, slices), kTileThreads, kTooLarge);
+}
+void check_mx4_encode_backward(Mx4Type type, uint64_t n, uint64_t inputs, uint64_t tokens, uint64_t slices) {
+    grid_of(slot_groups(type, n, slices) + slot_groups(type, inputs, slices) + row_groups(tokens, n), kTileThreads, kTooLarge);
+}
 
 void launch_mx4_encode(const void *x, Mx4Type type, uint64_t batch, uint64_t rows, uint64_t cols, uint64_t ld,
                        uint64_t stride, uint8_t *codes, uint8_t *scales, uint8_t *codes_t, uint8_t *scales_t,
@@ -300,13 +319,10 @@ void launch_mx4_encode(const void *x, Mx4Type type, uint64_t batch, uint64_t row
                 Mx4Rows{p, rows, cols, ld, stride, batch * rows, chunks, codes, scales});
         } else {
             constexpr uint32_t kCols = kTileCols<T>;
-            // whole slices both ways, so that the padding is written too
-            const uint32_t tiles_c = slices_c * (kMx4Slice / kCols), tiles_r = slices_r;
-            const uint64_t grid = batch * tiles_c * tiles_r;
-            BSQ_REQUIRE(grid <= 0x7FFFFFFFull, "mx4 encode: matrix too large");
-            mx4_encode_tile_kernel<T, false, false><<<static_cast<unsigned>(grid), kTileThreads, 0, stream>>>(
-                EncodeTiles{p, rows, cols, ld, stride, tiles_c, tiles_r, slices_c, slices_r, Mx4Slots{}, codes, scales,
-                            codes_t, scales_t});
+            const unsigned grid = grid_of(encode_tiles(type, batch, rows, cols), kTileThreads, kTooLarge);
+            mx4_encode_tile_kernel<T, false, false><<<grid, kTileThreads, 0, stream>>>(
+                EncodeTiles{p, rows, cols, ld, stride, slices_c * (kMx4Slice / kCols), slices_r, slices_c, slices_r,
+                            Mx4Slots{}, codes, scales, codes_t, scales_t});
         }
     });
     BSQ_HIP(hipGetLastError());
@@ -316,10 +332,8 @@ namespace {
 
 template <Mx4Type T>
 EncodeTiles slot_tiles(const void *x, uint64_t cols, uint64_t ld, const Mx4Slots &slots, uint64_t slices, uint8_t *codes_t,
-                       uint8_t *scales_t, uint64_t &grid) {
+                       uint8_t *scales_t) {
     const uint32_t tiles_c = static_cast<uint32_t>(ceil_div(cols, kTileCols<T>));
-    grid = slices * tiles_c;
-    BSQ_REQUIRE(grid <= 0x7FFFFFFFull, "mx4 encode: matrix too large");
     return {static_cast<const uint8_t *>(x), 0, cols, ld, 0, tiles_c, static_cast<uint32_t>(slices), 0,
             static_cast<uint32_t>(slices), slots, nullptr, nullptr, codes_t, scales_t};
 }
@@ -333,9 +347,9 @@ void launch_mx4_encode_slots(const void *x, Mx4Type type, uint64_t cols, uint64_
         constexpr Mx4Type T = decltype(t)::value;
         auto go = [&](auto weighted) {
             constexpr bool W = decltype(weighted)::value;
-            uint64_t grid;
-            const EncodeTiles job = slot_tiles<T>(x, cols, ld, slots, slices, codes_t, scales_t, grid);
-            mx4_encode_tile_kernel<T, true, W><<<static_cast<unsigned>(grid), kTileThreads, 0, stream>>>(job);
+            const unsigned grid = grid_of(slot_groups(type, cols, slices), kTileThreads, kTooLarge);
+            mx4_encode_tile_kernel<T, true, W><<<grid, kTileThreads, 0, stream>>>(
+                slot_tiles<T>(x, cols, ld, slots, slices, codes_t, scales_t));
         };
         if (slots.weights != nullptr) go(std::true_type{});
         else go(std::false_type{});
@@ -348,15 +362,14 @@ void launch_mx4_encode_backward(const void *d, uint64_t n, uint64_t ldd, const v
                                 uint8_t *xc, uint8_t *xs, uint8_t *rc, uint8_t *rs, hipStream_t stream) {
     by_type(type, [&](auto t) {
         constexpr Mx4Type T = decltype(t)::value;
-        uint64_t d_groups, x_groups;
-        const EncodeTiles of_d = slot_tiles<T>(d, n, ldd, slots, slices, dc, ds, d_groups);
+        const uint64_t d_groups = slot_groups(type, n, slices), x_groups = slot_groups(type, inputs, slices);
+        const EncodeTiles of_d = slot_tiles<T>(d, n, ldd, slots, slices, dc, ds);
         slots.weights = nullptr;
-        const EncodeTiles of_x = slot_tiles<T>(x, inputs, ldx, slots, slices, xc, xs, x_groups);
+        const EncodeTiles of_x = slot_tiles<T>(x, inputs, ldx, slots, slices, xc, xs);
         const Mx4Rows rows{static_cast<const uint8_t *>(d), tokens, n, ldd, 0, tokens,
                            static_cast<uint32_t>(mx4_slices(n)) * (kMx4Slice / 8), rc, rs};
-        const uint64_t groups = std::min<uint64_t>(ceil_div(tokens * rows.chunks, kTileThreads), 1u << 20);
-        BSQ_REQUIRE(d_groups + x_groups + groups <= 0x7FFFFFFFull, "mx4 encode: matrix too large");
-        mx4_encode_backward_kernel<T><<<static_cast<unsigned>(d_groups + x_groups + groups), kTileThreads, 0, stream>>>(
+        const unsigned grid = grid_of(d_groups + x_groups + row_groups(tokens, n), kTileThreads, kTooLarge);
+        mx4_encode_backward_kernel<T><<<grid, kTileThreads, 0, stream>>>(
             of_d, static_cast<uint32_t>(d_groups), of_x, static_cast<uint32_t>(x_groups), rows);
     });
     BSQ_HIP(hipGetLastError());
@@ -501,6 +514,8 @@ int bsq_mx4_linear(const void *d_x, int x_type, uint64_t m, uint64_t k, uint64_t
             launch_mx4_product_of(d_x, tx, k, ldx, p, s);
             return;
         }
+        if (d_xt_codes != nullptr) check_mx4_encode(tx, 1, m, k);
+        check_mx4_product(p);
         launch_mx4_encode(d_x, tx, 1, m, k, ldx, 0, codes, scales, d_xt_codes, d_xt_scales, s);
         launch_mx4_product(p, codes + packed(m, k), work_bytes - packed(m, k), s);
     });
@@ -534,10 +549,15 @@ int bsq_mx4_linear_backward(const void *d_dy, int type, uint64_t m, uint64_t n, 
         uint8_t *cc = rc + packed(m, n), *cs = cc + round256(n * mx4_slices(m) * 128);
         uint8_t *rest = cc + packed(n, m);
         const uint64_t rest_bytes = work_bytes - packed(m, n) - packed(n, m);
+        const Mx4Product dx = product_of({rc, rs}, m, {d_wt_codes, d_wt_scales}, k, n, d_dx, tg, lddx);
+        const Mx4Product dw = product_of({cc, cs}, n, {d_xt_codes, d_xt_scales}, k, m, d_dw, tg, lddw);
+        if (d_dw) check_mx4_encode(t, 1, m, n);
+        if (d_dx) check_mx4_product(dx);
+        if (d_dw) check_mx4_product(dw);
         launch_mx4_encode(d_dy, t, 1, m, n, ldy, 0, d_dx ? rc : nullptr, d_dx ? rs : nullptr, d_dw ? cc : nullptr,
                           d_dw ? cs : nullptr, s);
-        if (d_dx) launch_mx4_product(product_of({rc, rs}, m, {d_wt_codes, d_wt_scales}, k, n, d_dx, tg, lddx), rest, rest_bytes, s);
-        if (d_dw) launch_mx4_product(product_of({cc, cs}, n, {d_xt_codes, d_xt_scales}, k, m, d_dw, tg, lddw), rest, rest_bytes, s);
+        if (d_dx) launch_mx4_product(dx, rest, rest_bytes, s);
+        if (d_dw) launch_mx4_product(dw, rest, rest_bytes, s);
     });
 }
 

@@ -51,18 +51,23 @@ struct Mx4Slots {
 void launch_mx4_encode(const void *x, Mx4Type type, uint64_t batch, uint64_t rows, uint64_t cols, uint64_t ld,
                        uint64_t stride, uint8_t *codes, uint8_t *scales, uint8_t *codes_t, uint8_t *scales_t,
                        hipStream_t stream);
+// Whether the tiles of an encode that writes the columns fit a launch; for calls
+// that queue other work before it, and likewise the checks below.
+void check_mx4_encode(Mx4Type type, uint64_t batch, uint64_t rows, uint64_t cols);
 void launch_mx4_decode(const uint8_t *codes, const uint8_t *scales, uint64_t rows, uint64_t cols, void *out,
                        Mx4Type type, uint64_t ld, hipStream_t stream);
 // The transpose of the slots' rows (cols x slots, `slices` slices of 256 slots
 // a row), every expert's slots from a slice of its own.
 void launch_mx4_encode_slots(const void *x, Mx4Type type, uint64_t cols, uint64_t ld, const Mx4Slots &slots,
                              uint64_t slices, uint8_t *codes_t, uint8_t *scales_t, hipStream_t stream);
+void check_mx4_encode_slots(Mx4Type type, uint64_t cols, uint64_t slices);
 
 // Both of those for the weighted gradients d (tokens x n) and the inputs x, and
 // the rows of d, in one launch; d and x of one type.
 void launch_mx4_encode_backward(const void *d, uint64_t n, uint64_t ldd, const void *x, uint64_t inputs, uint64_t ldx,
                                 Mx4Type type, uint64_t tokens, Mx4Slots slots, uint64_t slices, uint8_t *dc, uint8_t *ds,
                                 uint8_t *xc, uint8_t *xs, uint8_t *rc, uint8_t *rs, hipStream_t stream);
+void check_mx4_encode_backward(Mx4Type type, uint64_t n, uint64_t inputs, uint64_t tokens, uint64_t slices);
 
 // Products of packed matrices: out[m, n] = sum over the shared axis.
 struct Mx4Product {
@@ -82,6 +87,7 @@ struct Mx4Product {
 };
 uint64_t mx4_product_workspace(uint32_t M, uint32_t N, uint32_t slices);
 void launch_mx4_product(const Mx4Product &p, void *workspace, uint64_t workspace_bytes, hipStream_t stream);
+void check_mx4_product(const Mx4Product &p);
 // The same with a packed from dense x on the way, for m rows where that pays.
 bool mx4_packs_on_the_way(uint64_t m, uint64_t n, uint64_t slices);
 void launch_mx4_product_of(const void *x, Mx4Type x_type, uint64_t x_cols, uint64_t ldx, const Mx4Product &p,
@@ -307,6 +313,15 @@ void by_type(Mx4Type t, F &&fn) {
     }
     fail("mx4: unknown element type");
 }
+
+// The grid of a launch.  Its threads are counted in 32 bits: past those the
+// runtime cuts the grid without an error.
+inline unsigned grid_of(uint64_t groups, uint64_t threads, const char *too_large) {
+    BSQ_REQUIRE(groups <= 0xFFFFFFFFull / threads, too_large);
+    return static_cast<unsigned>(groups);
+}
+// The same for kernels whose workgroups go on from item to item.
+inline unsigned grid_over(uint64_t groups) { return static_cast<unsigned>(groups < (1u << 20) ? groups : 1u << 20); }
 
 // Checks of a call's arguments.
 inline Mx4Type type_of(int t) {

@@ -583,17 +583,20 @@ constexpr uint64_t kPackReads = 4ull << 20;
 // rows take 13.3).
 constexpr uint32_t kFewRows = 16;
 
+constexpr const char *kTooLarge = "mx4 product: too large";
+unsigned few_rows_waves(const Mx4Product &p) {
+    return std::min<unsigned>(kMostWaves, std::max(1u, (p.slices + kAhead - 1) / kAhead));
+}
+
 template <Mode MODE, int X>
 void few_rows(const Mx4Product &p, uint64_t tiles_m, uint32_t pairs, const void *x, uint64_t x_cols, uint64_t ldx,
               hipStream_t stream) {
     const uint64_t tiles_n = ceil_div(p.N, 16);
-    const unsigned waves = std::min<unsigned>(kMostWaves, std::max(1u, (p.slices + kAhead - 1) / kAhead));
-    const uint64_t grid = tiles_n * tiles_m;
-    BSQ_REQUIRE(grid <= 0x7FFFFFFFull, "mx4 product: too large");
+    const unsigned waves = few_rows_waves(p), grid = grid_of(tiles_n * tiles_m, 64 * waves, kTooLarge);
     const unsigned lds = std::max(waves * 1024, X == kPacked ? 0u : p.M * p.slices * 136);
     by_type(p.type, [&](auto t) {
         mx4_few_rows_kernel<MODE, decltype(t)::value, X>
-            <<<static_cast<unsigned>(grid), 64 * waves, lds, stream>>>(p, static_cast<uint32_t>(tiles_n), pairs, x, x_cols, ldx);
+            <<<grid, 64 * waves, lds, stream>>>(p, static_cast<uint32_t>(tiles_n), pairs, x, x_cols, ldx);
     });
 }
 
@@ -665,14 +668,55 @@ Plan plan_of(uint32_t M, uint32_t N, uint32_t slices) {
     return q;
 }
 
+// A product's kernel and its grid; a tile of 16 stands for few rows.
+struct Cut {
+    uint32_t tile, teams, splits;
+    uint64_t tiles_m, tiles_n, bytes;
+};
+Cut cut_of(const Mx4Product &p) {
+    auto cut = [&](uint32_t tile, uint32_t teams, uint64_t tiles_m) {
+        return Cut{tile, teams, 1, tiles_m, ceil_div(p.N, tile), 0};
+    };
+    if (p.shared_slots) {
+        // (480 tokens to 4 experts, 176 x 338: 256 14.2 us, 64 4.9; 4096 pairs of
+        // 16 experts, 2752 x 2048: 256 66, 128 70, where the 180 MB written take
+        // some 35)
+        const uint64_t cus = static_cast<uint64_t>(cu_count());
+        auto of = [&](uint64_t t) { return p.experts * ceil_div(p.M, t) * ceil_div(p.N, t); };
+        const uint32_t tile = of(128) <= cus ? 64 : of(256) <= 2 * cus ? 128 : 256;
+        return cut(tile, 1, ceil_div(p.M, tile));
+    }
+    if (p.offsets != nullptr) {
+        // M: the pairs; every expert's tiles, and those of the pairs of none, none
+        // of them empty.  What the cut goes by: half a tile an expert left over.
+        auto of = [&](uint64_t t) { return std::min<uint64_t>(p.M, ceil_div(p.M, t) + p.experts + 1); };
+        if (p.M / p.experts <= 16) return cut(16, 1, of(16));
+        const uint64_t cus = static_cast<uint64_t>(cu_count());
+        auto rows = [&](uint64_t t) { return p.M + t / 2 * p.experts; };
+        auto count = [&](uint64_t t) { return ceil_div(rows(t), t) * ceil_div(p.N, t); };
+        if (count(64) <= 2 * cus && p.slices > 1) return cut(64, 2, of(64));
+        if (count(128) <= cus || p.M / p.experts <= 64) return cut(64, 1, of(64));
+        // (us: 16384 pairs of 32 experts, 2752 x 4096 with 256 159, before the
+        // last changes 179 against 199 with 128; 4096 of 16, 2752 x 2048 with
+        // 128 45, with 256 60, 2048 x 2752 41 and 33)
+        const uint32_t tile = large_tiles(rows(128), rows(256), p.N) ? 256 : 128;
+        return cut(tile, 1, of(tile));
+    }
+    if (p.M <= kFewRows) return cut(16, 1, 1);
+    const Plan q = plan_of(p.M, p.N, p.slices);
+    return {q.tile, q.teams, q.splits, q.tiles_m, q.tiles_n, q.bytes};
+}
+uint32_t threads_of(const Cut &c, const Mx4Product &p) {
+    return 64 * (c.tile == 16 ? few_rows_waves(p) : c.teams * (c.tile == 256 ? kTeam<256> : kTeam<64>));
+}
+
 template <int T, int G, Mode MODE>
-void tiles(const Mx4Product &p, uint64_t tiles_m, uint64_t tiles_n, uint32_t splits, hipStream_t stream) {
-    const uint64_t grid = tiles_m * tiles_n * splits;
-    BSQ_REQUIRE(grid <= 0x7FFFFFFFull, "mx4 product: too large");
-    const dim3 g(static_cast<unsigned>(grid), MODE == kShared ? p.experts : 1);
+void tiles(const Mx4Product &p, const Cut &c, hipStream_t stream) {
+    const unsigned groups = grid_of(c.tiles_m * c.tiles_n * c.splits, 64 * G * kTeam<T>, kTooLarge);
+    const dim3 g(groups, MODE == kShared ? p.experts : 1);
     by_type(p.type, [&](auto t) {
         mx4_product_kernel<T, G, MODE, decltype(t)::value><<<g, 64 * G * kTeam<T>, 0, stream>>>(
-            p, static_cast<uint32_t>(tiles_m), static_cast<uint32_t>(tiles_n), splits);
+            p, static_cast<uint32_t>(c.tiles_m), static_cast<uint32_t>(c.tiles_n), c.splits);
     });
 }
 
@@ -682,53 +726,46 @@ uint64_t mx4_product_workspace(uint32_t M, uint32_t N, uint32_t slices) {
     return M <= kFewRows || N == 0 ? 0 : plan_of(M, N, slices).bytes;
 }
 
+void check_mx4_product(const Mx4Product &p) {
+    if (p.M == 0 || p.N == 0) return;
+    const Cut c = cut_of(p);
+    grid_of(c.tiles_m * c.tiles_n * c.splits, threads_of(c, p), kTooLarge);
+}
+
 void launch_mx4_product(const Mx4Product &p, void *workspace, uint64_t workspace_bytes, hipStream_t stream) {
     if (p.M == 0 || p.N == 0) return;
-    const uint64_t cus = static_cast<uint64_t>(cu_count());
+    const Cut c = cut_of(p);
     if (p.shared_slots) {
-        // (480 tokens to 4 experts, 176 x 338: 256 14.2 us, 64 4.9; 4096 pairs of
-        // 16 experts, 2752 x 2048: 256 66, 128 70, where the 180 MB written take
-        // some 35)
-        auto of = [&](uint64_t t) { return p.experts * ceil_div(p.M, t) * ceil_div(p.N, t); };
-        if (of(128) <= cus) tiles<64, 1, kShared>(p, ceil_div(p.M, 64), ceil_div(p.N, 64), 1, stream);
-        else if (of(256) <= 2 * cus) tiles<128, 1, kShared>(p, ceil_div(p.M, 128), ceil_div(p.N, 128), 1, stream);
-        else tiles<256, 1, kShared>(p, ceil_div(p.M, 256), ceil_div(p.N, 256), 1, stream);
+        if (c.tile == 64) tiles<64, 1, kShared>(p, c, stream);
+        else if (c.tile == 128) tiles<128, 1, kShared>(p, c, stream);
+        else tiles<256, 1, kShared>(p, c, stream);
     } else if (p.offsets != nullptr) {
-        // M: the pairs; every expert's tiles, and those of the pairs of none.
-        // What the cut goes by: half a tile an expert left over.
-        auto of = [&](uint64_t t) { return ceil_div(p.M, t) + p.experts + 1; };
-        auto rows = [&](uint64_t t) { return p.M + t / 2 * p.experts; };
-        auto count = [&](uint64_t t) { return ceil_div(rows(t), t) * ceil_div(p.N, t); };
-        if (p.M / p.experts <= 16) few_rows<kRows, kPacked>(p, of(16), p.M, nullptr, 0, 0, stream);
-        else if (count(64) <= 2 * cus && p.slices > 1) tiles<64, 2, kRows>(p, of(64), ceil_div(p.N, 64), 1, stream);
-        else if (count(128) <= cus || p.M / p.experts <= 64) tiles<64, 1, kRows>(p, of(64), ceil_div(p.N, 64), 1, stream);
-        // (us: 16384 pairs of 32 experts, 2752 x 4096 with 256 159, before the
-        // last changes 179 against 199 with 128; 4096 of 16, 2752 x 2048 with
-        // 128 45, with 256 60, 2048 x 2752 41 and 33)
-        else if (large_tiles(rows(128), rows(256), p.N)) tiles<256, 1, kRows>(p, of(256), ceil_div(p.N, 256), 1, stream);
-        else tiles<128, 1, kRows>(p, of(128), ceil_div(p.N, 128), 1, stream);
-    } else if (p.M <= kFewRows) {
+        if (c.tile == 16) few_rows<kRows, kPacked>(p, c.tiles_m, p.M, nullptr, 0, 0, stream);
+        else if (c.tile == 64 && c.teams == 2) tiles<64, 2, kRows>(p, c, stream);
+        else if (c.tile == 64) tiles<64, 1, kRows>(p, c, stream);
+        else if (c.tile == 128) tiles<128, 1, kRows>(p, c, stream);
+        else tiles<256, 1, kRows>(p, c, stream);
+    } else if (c.tile == 16) {
         few_rows<kDense, kPacked>(p, 1, 0, nullptr, 0, 0, stream);
     } else {
-        const Plan q = plan_of(p.M, p.N, p.slices);
-        BSQ_REQUIRE(workspace_bytes >= q.bytes, "mx4 product: workspace too small");
+        BSQ_REQUIRE(workspace_bytes >= c.bytes, "mx4 product: workspace too small");
         Mx4Product part = p;
-        if (q.splits > 1) {
+        if (c.splits > 1) {
             part.out = workspace;
             part.type = Mx4Type::F32;
             part.ld = p.N;
         }
-        if (q.tile == 256) tiles<256, 1, kDense>(part, q.tiles_m, q.tiles_n, q.splits, stream);
-        else if (q.tile == 128 && q.teams == 2) tiles<128, 2, kDense>(part, q.tiles_m, q.tiles_n, q.splits, stream);
-        else if (q.tile == 128) tiles<128, 1, kDense>(part, q.tiles_m, q.tiles_n, q.splits, stream);
-        else if (q.teams == 4) tiles<64, 4, kDense>(part, q.tiles_m, q.tiles_n, q.splits, stream);
-        else if (q.teams == 2) tiles<64, 2, kDense>(part, q.tiles_m, q.tiles_n, q.splits, stream);
-        else tiles<64, 1, kDense>(part, q.tiles_m, q.tiles_n, q.splits, stream);
-        if (q.splits > 1) {
+        if (c.tile == 256) tiles<256, 1, kDense>(part, c, stream);
+        else if (c.tile == 128 && c.teams == 2) tiles<128, 2, kDense>(part, c, stream);
+        else if (c.tile == 128) tiles<128, 1, kDense>(part, c, stream);
+        else if (c.teams == 4) tiles<64, 4, kDense>(part, c, stream);
+        else if (c.teams == 2) tiles<64, 2, kDense>(part, c, stream);
+        else tiles<64, 1, kDense>(part, c, stream);
+        if (c.splits > 1) {
             by_type(p.type, [&](auto t) {
                 const uint64_t grid = ceil_div(p.M * ceil_div(p.N, 8), kThreads);
                 mx4_join_kernel<decltype(t)::value><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(
-                    static_cast<const float *>(workspace), q.splits, p.M, p.N, p.out, p.ld);
+                    static_cast<const float *>(workspace), c.splits, p.M, p.N, p.out, p.ld);
             });
         }
     }
