@@ -321,7 +321,7 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a, int32_t *__
 // S is held at the smallest normal number it does not depend on the scores, and
 // h_j = g_j.  Nothing is divided by S but the scores, so no quotient overflows.
 // The chosen reach their experts' lanes through a row in LDS.  The same tokens:
-// 7.2 us (9.4 MB written; softmax reads as much), launch and latency.
+// 7.0 us (9.4 MB written; softmax reads as much), launch and latency.
 template <Mx4Type T, int NV>
 __global__ __launch_bounds__(256) void moe_route_backward_kernel(RouteArgs a, const int32_t *__restrict__ ids,
                                                                  const float *__restrict__ d_weights,
@@ -471,7 +471,8 @@ __global__ __launch_bounds__(kPlanThreads) void moe_begin_kernel(const int32_t *
 // (113 MB; 21.8 at the rate of a large copy, part of y is still in cache).  y
 // itself is of the type the caller asks for: in BF16 its rounding is as large
 // as the output's own and independent of it, so the error grows by up to the
-// square root of two, and half the bytes are moved.
+// square root of two, and half the bytes are moved; in FP16 a product above
+// 65504 is infinite here whatever its weight.
 template <Mx4Type Y, Mx4Type O>
 __global__ __launch_bounds__(256) void moe_combine_kernel(const void *__restrict__ y, uint64_t tokens, uint32_t k,
                                                           uint32_t cols, uint32_t chunks,
@@ -498,8 +499,9 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const void *__restrict
 }
 
 // d weights: a wave takes a pair's dot product with the token's d out.  4096
-// pairs of 2752 BF16: 10.6 us for 34 MB (6.5 at the rate of a large copy); loads of
-// several pieces in flight take 10.4.
+// pairs of 2752, y FP32 and d out BF16: 10.7 us for 56 MB (10.9 at the rate of a
+// large copy; y comes in part from the last cache); loads of several pieces in
+// flight take 10.4.
 template <Mx4Type Y, Mx4Type D>
 __global__ __launch_bounds__(256) void moe_weights_backward_kernel(const void *__restrict__ y, uint64_t pairs, uint32_t k,
                                                                    uint32_t cols, const int32_t *__restrict__ ids,
@@ -821,7 +823,9 @@ int bsq_moe_linear_backward(const void *d_d_out, int d_type, uint64_t tokens, ui
         // the weights' columns for their rows.  The terms are FP32 until they
         // are summed, whatever the gradients' type: a pair's product may lie
         // above FP16's range where its weight brings it back, and in BF16
-        // dx was off by 0.0024 in place of 0.0017.
+        // dx was off by 0.0024 in place of 0.0017 (2048 tokens to 2 of 16
+        // experts, 2752 and 2048: product and join 42 and 7.7 us, of BF16 terms
+        // 32 and 6.1).
         dx.a = {codes, scales};
         dx.b = {d_wt_codes, d_wt_scales};
         dx.M = static_cast<uint32_t>(pairs);

@@ -690,15 +690,18 @@ Cut cut_of(const Mx4Product &p) {
         // M: the pairs; every expert's tiles, and those of the pairs of none, none
         // of them empty.  What the cut goes by: half a tile an expert left over.
         auto of = [&](uint64_t t) { return std::min<uint64_t>(p.M, ceil_div(p.M, t) + p.experts + 1); };
+        // (us of the layer, 2752 x 4096, with 16 and with 64: 16 pairs of 32 experts
+        // 26 and 26, of one 13 and 18; 128 of 32 56 and 54, of one 26 and 19; 512 of
+        // 32 90 and 60, of one 71 and 23)
         if (p.M / p.experts <= 16) return cut(16, 1, of(16));
         const uint64_t cus = static_cast<uint64_t>(cu_count());
         auto rows = [&](uint64_t t) { return p.M + t / 2 * p.experts; };
         auto count = [&](uint64_t t) { return ceil_div(rows(t), t) * ceil_div(p.N, t); };
         if (count(64) <= 2 * cus && p.slices > 1) return cut(64, 2, of(64));
         if (count(128) <= cus || p.M / p.experts <= 64) return cut(64, 1, of(64));
-        // (us: 16384 pairs of 32 experts, 2752 x 4096 with 256 159, before the
-        // last changes 179 against 199 with 128; 4096 of 16, 2752 x 2048 with
-        // 128 45, with 256 60, 2048 x 2752 41 and 33)
+        // (us: 16384 pairs of 32 experts, 2752 x 4096 to BF16 with 256 156 to 168,
+        // with 128 177 to 193; 4096 of 16 to FP32, 2752 x 2048 with 128 45, with
+        // 256 57, 2048 x 2752 47 and 42)
         const uint32_t tile = large_tiles(rows(128), rows(256), p.N) ? 256 : 128;
         return cut(tile, 1, of(tile));
     }

@@ -339,7 +339,9 @@ BSQ_API int bsq_legacy_sweep(int kind, uint64_t lo, uint64_t hi, unsigned long l
  *    8-byte aligned (so is a workspace, 16).
  *
  *    Element types: 0 FP32, 1 BF16, 2 FP16.  `ld` counts elements from one row
- *    to the next.  Sums are held in FP32 and rounded once.  All calls are
+ *    to the next.  Sums are held in FP32 (in the order of the matrix
+ *    instructions, the tiles and the splits: the same from run to run) and
+ *    rounded once; the join of experts sums y as it is stored.  All calls are
  *    asynchronous on `stream`, keep nothing between calls and take their
  *    workspace from the caller (its bytes: the function beside them), so they
  *    can be captured, and run on several streams with a workspace each.  The
@@ -416,7 +418,11 @@ BSQ_API int bsq_moe_combine(const void *d_y, int y_type, uint64_t tokens, uint32
  * the join of y by the weights.  W: experts packed matrices of n x inputs, one
  * after another.  d_offsets, d_order (as bsq_moe_plan) and d_y (tokens k x n;
  * zero rows where a pair has no expert) are written and serve the backward
- * pass; the gradient of the weights is as fine as y's type. */
+ * pass.  out and the gradient of the weights are as fine as y's type, which is
+ * the caller's choice: FP32 y leaves out one rounding, BF16 y halves the bytes
+ * and rounds each pair's product once more (0.0024 in place of 0.0017 of a BF16
+ * out), FP16 y is infinite above 65504.  Gradients by the backward call sum FP32
+ * products whatever their type. */
 BSQ_API uint64_t bsq_moe_linear_workspace(uint64_t tokens, uint32_t k, uint64_t n, uint64_t inputs, uint32_t experts);
 BSQ_API int bsq_moe_linear(const void *d_x, int x_type, uint64_t tokens, uint64_t inputs, uint64_t ldx,
                            const int32_t *d_ids, const float *d_weights, uint32_t k, const uint8_t *d_w_codes,
