@@ -146,10 +146,9 @@ def abi_leg(src, ddst, n, wl, reps=5):
 OTHER_SOURCES = {"mx4.hip", "mx4.hpp", "mx4_gemm.hip", "moe.hip"}
 
 
-def sources_sha256() -> str:
-    """SHA-256 over the sources of the workloads' kernels and runtime, the C++
-    headers (file names and contents, in name order) and the flags that they are
-    built with: the identity of the code a profile summary was collected from."""
+def _sha256_of(files, names):
+    """SHA-256 over files (names and contents) and the flags that those named
+    `names` are built with."""
     import hashlib
     import importlib.util
 
@@ -157,15 +156,29 @@ def sources_sha256() -> str:
     build = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(build)
     h = hashlib.sha256()
-    files = []
-    for d, exts in ((os.path.join(PKG, "csrc"), (".hip", ".hpp")), (os.path.join(ROOT, "include"), (".hpp",))):
-        files += [os.path.join(d, f) for f in sorted(os.listdir(d)) if f.endswith(exts) and f not in OTHER_SOURCES]
     for f in files:
         h.update(os.path.relpath(f, ROOT).encode())
         h.update(open(f, "rb").read())
     flags = [f.replace(ROOT, "") for f in build.COMMON]
-    h.update(repr((flags, build.EXTRA, sorted(build.NO_CONTRACT - OTHER_SOURCES))).encode())
+    h.update(repr((flags, build.EXTRA, sorted(n for n in build.NO_CONTRACT if names(n)))).encode())
     return h.hexdigest()
+
+
+def sources_sha256() -> str:
+    """The identity of the code that the workloads' profile summaries were
+    collected from: the sources of their kernels and runtime, the C++ headers (in
+    name order) and the flags that they are built with."""
+    files = []
+    for d, exts in ((os.path.join(PKG, "csrc"), (".hip", ".hpp")), (os.path.join(ROOT, "include"), (".hpp",))):
+        files += [os.path.join(d, f) for f in sorted(os.listdir(d)) if f.endswith(exts) and f not in OTHER_SOURCES]
+    return _sha256_of(files, lambda n: n not in OTHER_SOURCES)
+
+
+def operators_sha256() -> str:
+    """The same for profiles/operators_kernel_stats.md: the operators' sources and
+    what they share with others."""
+    names = sorted(OTHER_SOURCES | {"bsq_internal.hpp", "tile_map.hpp"})
+    return _sha256_of([os.path.join(PKG, "csrc", f) for f in names], lambda n: n in OTHER_SOURCES)
 
 
 def committed_traffic(workload: str, cls: str):
