@@ -142,8 +142,11 @@ def abi_leg(src, ddst, n, wl, reps=5):
     return 4.0 * n / (ms * 1e-3) / 1e9, ms
 
 
-# Sources of operators that no workload here runs.
-OTHER_SOURCES = {"mx4.hip", "mx4.hpp", "mx4_gemm.hip", "moe.hip"}
+# Sources of operators that no workload here runs: layers on 4-bit matrices, and
+# attention over a 4-bit cache.
+MX4_SOURCES = {"mx4.hip", "mx4.hpp", "mx4_gemm.hip", "moe.hip"}
+KV4_SOURCES = {"kv4.hip", "kv4.hpp", "kv4_attention.hip"}
+OTHER_SOURCES = MX4_SOURCES | KV4_SOURCES
 
 
 def _sha256_of(files, names):
@@ -177,8 +180,14 @@ def sources_sha256() -> str:
 def operators_sha256() -> str:
     """The same for profiles/operators_kernel_stats.md: the operators' sources and
     what they share with others."""
-    names = sorted(OTHER_SOURCES | {"bsq_internal.hpp", "tile_map.hpp"})
-    return _sha256_of([os.path.join(PKG, "csrc", f) for f in names], lambda n: n in OTHER_SOURCES)
+    names = sorted(MX4_SOURCES | {"bsq_internal.hpp", "tile_map.hpp"})
+    return _sha256_of([os.path.join(PKG, "csrc", f) for f in names], lambda n: n in MX4_SOURCES)
+
+
+def more_operators_sha256() -> str:
+    """The same for profiles/more_operators_kernel_stats.md."""
+    names = sorted(KV4_SOURCES | {"bsq_internal.hpp", "mx4.hpp"})
+    return _sha256_of([os.path.join(PKG, "csrc", f) for f in names], lambda n: n in KV4_SOURCES)
 
 
 def committed_traffic(workload: str, cls: str):

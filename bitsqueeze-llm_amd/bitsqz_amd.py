@@ -71,6 +71,17 @@ class DevicePacked(C.Structure):
     ]
 
 
+class Kv4Pages(C.Structure):
+    """bsq_kv4_cache_t (include/bitsqz_llm_c.h)."""
+    _fields_ = [("d_pages", C.c_void_p), ("pages", C.c_uint64), ("page", C.c_uint32), ("heads", C.c_uint32),
+                ("dim", C.c_uint32)]
+
+
+class Rope(C.Structure):
+    """bsq_rope_t (include/bitsqz_llm_c.h)."""
+    _fields_ = [("d_frequencies", C.c_void_p), ("dims", C.c_uint32), ("interleaved", C.c_int), ("factor", C.c_float)]
+
+
 _lib = None
 P = C.c_void_p
 
@@ -83,7 +94,7 @@ def lib():
     if not os.path.exists(LIB_PATH):
         raise RuntimeError(f"{LIB_PATH} missing: run `python bitsqueeze-llm_amd/build.py`")
     L = C.CDLL(LIB_PATH)
-    u16, u32, u64, f32, i32 = C.c_uint16, C.c_uint32, C.c_uint64, C.c_float, C.c_int
+    u16, u32, u64, f32, f64, i32 = C.c_uint16, C.c_uint32, C.c_uint64, C.c_float, C.c_double, C.c_int
     sig = {
         "bsq_last_error": (C.c_char_p, []),
         "bsq_version": (C.c_char_p, []),
@@ -167,6 +178,17 @@ def lib():
         "bsq_moe_linear_backward_workspace": (u64, [u64, u32, u64, u64, u32]),
         "bsq_moe_linear_backward": (i32, [P, i32, u64, u64, u64, P, i32, u64, u64, P, P, u32, P, P, P, i32, P, P, u32, P,
                                           u64, P, P, i32, P, u64, P]),
+        "bsq_kv4_cache_bytes": (u64, [u64, u32, u32, u32]),
+        "bsq_kv4_plan_workspace": (u64, [u32]),
+        "bsq_kv4_plan": (i32, [P, P, u32, P, u32, u32, P, u64, P, P, P, P, u64, P, P, P, P, u64, P]),
+        "bsq_rope_frequencies": (i32, [u32, f64, i32, f64, f64, P, C.POINTER(f32)]),
+        "bsq_rope": (i32, [C.POINTER(Rope), P, P, i32, u64, u32, u32, u64, i32, P, u64, P]),
+        "bsq_kv4_append": (i32, [C.POINTER(Kv4Pages), C.POINTER(Rope), P, P, u64, i32, P, u32, u64, P, u64, P, u64, P, u64,
+                                 P]),
+        "bsq_kv4_read": (i32, [C.POINTER(Kv4Pages), P, u64, i32, P, u64, P, u64, P]),
+        "bsq_kv4_attention_workspace": (u64, [C.POINTER(Kv4Pages), u32, u32, u64, u32, u32]),
+        "bsq_kv4_attention": (i32, [C.POINTER(Kv4Pages), P, u32, P, P, u32, P, i32, u64, u32, u32, u64, f32, i32, u32, P,
+                                    i32, u64, P, P, u64, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -853,3 +875,142 @@ class MoeLinear:
         check(lib().bsq_stream_synchronize(None), "sync")
         return (dx.download(t, m * inputs).reshape(m, inputs), dweights.download(np.float32, m * k).reshape(m, k),
                 dw.download(t, e * n * inputs).reshape(e, n, inputs))
+
+
+# ---------------------------------------------------------------------------
+# attention over a paged cache of keys and values in MX4, rotary positions
+# (include/bitsqz_llm_c.h, group 7)
+# ---------------------------------------------------------------------------
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS = 0, 1, 2, 3
+
+
+def rope_frequencies(dims: int, base: float = 10000.0, scaling: int = ROPE_PLAIN, stretch: float = 1.0,
+                     length: float = 0.0):
+    """(frequencies, factor) of a head's turning `dims` values."""
+    f, factor = np.zeros(max(dims // 2, 0)), C.c_float()
+    check(lib().bsq_rope_frequencies(dims, base, scaling, stretch, length, _ptr(f), C.byref(factor)), "rope_frequencies")
+    return f, factor.value
+
+
+class Turn:
+    """What turns queries and keys: frequencies on the GPU, one a pair of the
+    head's first values, the factor, and how the pairs lie."""
+
+    def __init__(self, frequencies: np.ndarray, factor: float = 1.0, interleaved: bool = False):
+        frequencies = np.ascontiguousarray(frequencies, np.float64)
+        _agree(frequencies.ndim == 1 and frequencies.size > 0, "Turn: a row of frequencies")
+        self.dims, self.buffer = 2 * frequencies.size, DeviceBuffer.from_array(frequencies)
+        self.rope = Rope(self.buffer.value, self.dims, int(interleaved), factor)
+
+
+def rope(x: np.ndarray, positions: np.ndarray, turn: Turn, type: int = TYPE_F32, back: bool = False) -> np.ndarray:
+    """x (tokens x heads x dim) turned by its positions, or a gradient turned back;
+    rows whose position is below zero come back as they are."""
+    x, positions = _typed(x, type), np.ascontiguousarray(positions, np.int32)
+    _agree(x.ndim == 3, "rope: x is tokens x heads x dim")
+    _agree(positions.shape == x.shape[:1], "rope: a position for every token")
+    _agree(turn.dims <= x.shape[2], f"rope: {turn.dims} turning values in a head of {x.shape[2]}")
+    tokens, heads, dim = x.shape
+    d, p = DeviceBuffer.from_array(x), DeviceBuffer.from_array(positions)
+    check(lib().bsq_rope(turn.rope, p.ptr, d.ptr, type, tokens, heads, dim, heads * dim, int(back), d.ptr, heads * dim,
+                         None), "rope")
+    check(lib().bsq_stream_synchronize(None), "sync")
+    return d.download(x.dtype, x.size).reshape(x.shape)
+
+
+class Kv4Cache:
+    """A paged cache of one layer with its bookkeeping: step(), then append() and
+    attend() of that step's tokens.  All pages are free at first, all requests
+    empty."""
+
+    def __init__(self, pages: int, page: int, heads: int, dim: int, requests: int, width: int):
+        """width: the most pages of a request."""
+        _agree(min(pages, heads, dim, requests, width) >= 1, "Kv4Cache: sizes of at least 1")
+        size = lib().bsq_kv4_cache_bytes(pages, page, heads, dim)
+        if size == 2**64 - 1:
+            raise BsqError(f"kv4 cache failed: {lib().bsq_last_error().decode()}")
+        self.pages, self.page, self.heads, self.dim, self.requests, self.width = pages, page, heads, dim, requests, width
+        self.buffer = DeviceBuffer(size)
+        self.cache = Kv4Pages(self.buffer.value, pages, page, heads, dim)
+        self.table = DeviceBuffer.from_array(np.full((requests, width), -1, np.int32))
+        self.free = DeviceBuffer.from_array(np.arange(pages - 1, -1, -1, dtype=np.int32))
+        self.left = DeviceBuffer.from_array(np.array([pages, 0], np.int32))
+        self.lengths = DeviceBuffer.from_array(np.zeros(requests, np.int32))
+        self.work = DeviceBuffer(workspace("bsq_kv4_plan_workspace", requests))
+        self.tokens = None
+
+    def step(self, new: np.ndarray, tokens: int | None = None) -> dict:
+        """The places of the requests' new tokens (below zero: the request has
+        ended), `tokens` of them where given; as host arrays."""
+        new = np.ascontiguousarray(new, np.int32)
+        _agree(new.shape == (self.requests,), f"Kv4Cache: new tokens of {self.requests} requests")
+        tokens = int(np.maximum(new, 0).sum()) if tokens is None else tokens
+        d = DeviceBuffer.from_array(new)
+        self.starts = DeviceBuffer(4 * (self.requests + 1))
+        of, self.positions, self.slots = (DeviceBuffer(4 * tokens) for _ in range(3))
+        check(lib().bsq_kv4_plan(self.lengths.ptr, d.ptr, self.requests, self.table.ptr, self.width, self.page,
+                                 self.free.ptr, self.pages, self.left.ptr, self.lengths.ptr, self.left.ptr,
+                                 self.starts.ptr, tokens, of.ptr, self.positions.ptr, self.slots.ptr, self.work.ptr,
+                                 self.work.nbytes, None), "kv4_plan")
+        check(lib().bsq_stream_synchronize(None), "sync")
+        self.tokens, self.most = tokens, int(max(new.max(), 1))
+        left = self.left.download(np.int32, 2)
+        return {"starts": self.starts.download(np.int32, self.requests + 1), "requests": of.download(np.int32, tokens),
+                "positions": self.positions.download(np.int32, tokens), "slots": self.slots.download(np.int32, tokens),
+                "lengths": self.lengths.download(np.int32, self.requests), "left": int(left[0]), "unserved": int(left[1])}
+
+    def _step_of(self, x: np.ndarray, heads: int | None, what: str):
+        _agree(self.tokens is not None, f"Kv4Cache: {what} of a step()")
+        _agree(x.ndim == 3 and len(x) == self.tokens and x.shape[2] == self.dim and heads in (None, x.shape[1]),
+               f"Kv4Cache: {what} are {self.tokens} tokens of {heads or 'any'} heads of {self.dim}")
+
+    def append(self, k: np.ndarray, v: np.ndarray, q: np.ndarray | None = None, turn: Turn | None = None,
+               type: int = TYPE_F32):
+        """The step's keys (turned, if `turn`) and values into their slots; returns
+        the queries, turned, if given."""
+        k, v = _typed(k, type), _typed(v, type)
+        self._step_of(k, self.heads, "keys")
+        self._step_of(v, self.heads, "values")
+        _agree(turn is None or turn.dims <= self.dim, "Kv4Cache: more turning values than a head has")
+        if q is not None:
+            q = _typed(q, type)
+            self._step_of(q, None, "queries")
+        dk, dv = DeviceBuffer.from_array(k), DeviceBuffer.from_array(v)
+        dq = DeviceBuffer.from_array(q) if q is not None else None
+        wide, row = q.shape[1] if q is not None else 0, self.heads * self.dim
+        check(lib().bsq_kv4_append(self.cache, turn.rope if turn is not None else None, self.positions.ptr, self.slots.ptr,
+                                   self.tokens, type, dq.ptr if dq else None, wide, wide * self.dim,
+                                   dq.ptr if dq else None, wide * self.dim, dk.ptr, row, dv.ptr, row, None), "kv4_append")
+        check(lib().bsq_stream_synchronize(None), "sync")
+        return dq.download(q.dtype, q.size).reshape(q.shape) if q is not None else None
+
+    def read(self, slots: np.ndarray, type: int = TYPE_F32):
+        """(keys, values) at the slots; zeros where a slot is none."""
+        slots = np.ascontiguousarray(slots, np.int32)
+        _agree(slots.ndim == 1, "Kv4Cache: a row of slots")
+        n, row, t = len(slots), self.heads * self.dim, _TYPE_NUMPY[type]
+        d, out = DeviceBuffer.from_array(slots), [DeviceBuffer(n * row * t.itemsize) for _ in range(2)]
+        for b in out:
+            b.zero()
+        check(lib().bsq_kv4_read(self.cache, d.ptr, n, type, out[0].ptr, row, out[1].ptr, row, None), "kv4_read")
+        check(lib().bsq_stream_synchronize(None), "sync")
+        return tuple(b.download(t, n * row).reshape(n, self.heads, self.dim) for b in out)
+
+    def attend(self, q: np.ndarray, scale: float | None = None, type: int = TYPE_F32, out_type: int = TYPE_F32,
+               causal: bool = True, window: int = 0):
+        """(out, lse) of the step's queries over their requests' keys and values;
+        zeros and minus infinity for places that are no token."""
+        q = _typed(q, type)
+        self._step_of(q, None, "queries")
+        _agree(q.shape[1] % self.heads == 0, f"Kv4Cache: queries of a multiple of {self.heads} heads")
+        n, heads, t = self.tokens, q.shape[1], _TYPE_NUMPY[out_type]
+        d, out = DeviceBuffer.from_array(q), DeviceBuffer(q.size * t.itemsize)
+        lse = DeviceBuffer.from_array(np.full((n, heads), -np.inf, np.float32))
+        out.zero()
+        work = DeviceBuffer(workspace("bsq_kv4_attention_workspace", self.cache, self.width, self.requests, n, self.most, heads))
+        check(lib().bsq_kv4_attention(self.cache, self.table.ptr, self.width, self.lengths.ptr, self.starts.ptr,
+                                      self.requests, d.ptr, type, n, self.most, heads, heads * self.dim,
+                                      self.dim**-0.5 if scale is None else scale, int(causal), window, out.ptr, out_type,
+                                      heads * self.dim, lse.ptr, work.ptr, work.nbytes, None), "kv4_attention")
+        check(lib().bsq_stream_synchronize(None), "sync")
+        return out.download(t, q.size).reshape(q.shape), lse.download(np.float32, n * heads).reshape(n, heads)

@@ -34,7 +34,8 @@ COMMON = [
     "-Wno-unused-command-line-argument",
 ]
 # Sources whose arithmetic must round operation by operation (bit-exact codecs).
-NO_CONTRACT = {"quant.hip", "topk.hip", "runtime.hip", "recon.hip", "legacy.hip", "mx4.hip", "moe.hip"}
+NO_CONTRACT = {"quant.hip", "topk.hip", "runtime.hip", "recon.hip", "legacy.hip", "mx4.hip", "moe.hip",
+               "kv4.hip"}
 # Per-file extra flags: the register-resident FP64 factorisations need their
 # fully unrolled loops kept unrolled so the per-thread matrix stays in VGPRs.
 EXTRA = {"linalg.hip": ["-mllvm", "-pragma-unroll-threshold=200000"],

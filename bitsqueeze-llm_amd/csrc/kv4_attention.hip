@@ -1,0 +1,701 @@
+// Attention over the paged MX4 cache (kv4.hpp).
+//
+// out_i = sum_j p_ij v_j / sum_j p_ij, p_ij = 2^(x_ij - m_i), x_ij = scale log2(e)
+// q_i . k_j, in one pass over the keys with m_i a running reference.  m_i is
+// raised only where some x_ij lies more than 8 above it: the sums are FP32, so a
+// reference that is up to 2^8 low costs nothing, and most tiles need no rescale
+// and no exchange between lanes.
+//
+// Keys and values are converted to BF16, which holds E2M1 times a power of two
+// exactly, and multiplied on the BF16 matrix instructions; queries that BF16 does
+// not hold are split into two (FP16) or three (FP32) BF16 pieces, so that products
+// are those of FP32.  The weights p go in the same number of pieces.
+#include "kv4.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace bsq {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr uint32_t kRows = 16;                   // (token, head of the group) pairs of a tile of queries
+constexpr uint32_t kStep = 32;                   // keys a wave takes at once
+constexpr uint32_t kSpan = kStep * kWaves;       // keys a workgroup takes at once
+constexpr float kSlack = 8.0f;
+
+struct AttentionArgs {
+    Kv4Cache cache;
+    const int32_t *table, *lengths, *starts;
+    uint32_t width, requests;
+    const uint8_t *q;
+    Mx4Type q_type, out_type;
+    uint64_t ldq, ldo;
+    uint32_t tokens, most, group;  // group: query heads to a head of keys
+    float factor;                  // scale log2(e), not below zero
+    bool negate;                   // the scale is below zero
+    bool causal;
+    uint32_t window;
+    uint8_t *out;
+    float *lse;
+    float *parts;
+    struct Split *splits;
+};
+
+// A tile of queries whose keys more than one workgroup takes: the first of them
+// says so, and up to which workgroup it goes.
+struct Split {
+    uint32_t last;  // 0: none begins here
+    uint32_t head, row0, rows;
+    uint32_t first_token;
+    uint32_t pad[3];
+};
+
+struct Request {
+    int32_t length, first, count;  // keys, first query, queries
+    __device__ __forceinline__ int32_t past() const { return length - count; }
+};
+
+__device__ __forceinline__ Request load_request(const AttentionArgs &a, uint32_t r) {
+    Request q;
+    const int64_t room = static_cast<int64_t>(a.width) << a.cache.shift;
+    q.length = static_cast<int32_t>(min(static_cast<int64_t>(max(a.lengths[r], 0)), room));
+    if (a.starts == nullptr) {
+        q.first = static_cast<int32_t>(r);
+        q.count = r < a.tokens ? 1 : 0;
+    } else {
+        const int32_t tokens = static_cast<int32_t>(a.tokens);
+        q.first = min(max(a.starts[r], 0), tokens);
+        const int32_t n = min(max(a.starts[r + 1], q.first), tokens) - q.first;
+        q.count = min(n, static_cast<int32_t>(a.most));
+        // queries past `most` are the last ones: the others' keys end before theirs
+        if (a.causal) q.length = max(q.length - (n - q.count), 0);
+    }
+    return q;
+}
+
+// Where a request's keys begin, and their number in spans (at least one, which
+// writes the zeros of queries that see none).
+__device__ __forceinline__ uint32_t first_key(const AttentionArgs &a, const Request &q) {
+    return a.window == 0 ? 0u : static_cast<uint32_t>(max(q.past() + 1 - static_cast<int64_t>(a.window), static_cast<int64_t>(0))) & ~(kStep - 1);
+}
+__device__ __forceinline__ uint32_t spans_of(const AttentionArgs &a, const Request &q) {
+    const uint32_t first = first_key(a, q), length = static_cast<uint32_t>(q.length);
+    return length > first ? (length - first + kSpan - 1) / kSpan : 1u;
+}
+__device__ __forceinline__ uint64_t tiles_of(const AttentionArgs &a, const Request &q) {
+    return (static_cast<uint64_t>(q.count) * a.group + kRows - 1) / kRows;
+}
+
+template <int NB>
+struct Shape {
+    static constexpr int kLane = NB == 1 ? 2 : NB == 2 ? 4 : NB <= 4 ? 8 : 16;  // values of a lane's channels
+    static constexpr int kLanes = 32 * NB / kLane;                              // of 16 that hold channels
+    static constexpr int kWords = kLane <= 8 ? 1 : 2;
+    // words of a lane's key scales: a lane has 8 NB channels from 8 NB g on
+    static constexpr int kScales = NB % 4 == 0 ? NB / 4 : NB <= 2 ? 1 : NB;
+    static constexpr int kRow = 16 * kLane + 4;  // floats of a row of sums in LDS
+};
+
+// 32 keys and values as a lane takes them.  Lane l = 16 g + i.  Keys: the row of
+// token 16 a + 4 (i % 4) + i / 4 of the two sixteens a, channels [8 NB g, 8 NB (g
+// + 1)).  The products' lane then holds, for query i, the tokens 16 a + 4 r + g =
+// 4 j + g with j = 4 a + r: the eight that it holds of the values' rows, channels
+// [kLane i, kLane (i + 1)), so the weights stay where they are.
+template <int NB>
+struct Tile {
+    using S = Shape<NB>;
+    uint32_t k[2][NB], ks[2][S::kScales], v[8][S::kWords], vs[2];
+    uint32_t bad;  // bit a: the sixteen is on no page
+
+    __device__ __forceinline__ void load(const AttentionArgs &a, uint32_t h, uint32_t t, uint32_t id0, uint32_t id1, uint32_t lane) {
+        const uint32_t g = lane >> 4, i = lane & 15, page_mask = a.cache.page() - 1;
+        const uint32_t row = a.cache.row_bytes();
+        bad = 0;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            uint32_t id = s ? id1 : id0;
+            if (id >= a.cache.count) {
+                bad |= 1u << s;
+                id = 0;
+            }
+            const uint8_t *head = a.cache.head(id, h);
+            const uint32_t in = (t + 16 * s) & page_mask;
+            const uint8_t *kp = head + a.cache.codes_at(0, in), *vp = head + a.cache.codes_at(1, in);
+            const uint8_t *ksp = head + a.cache.scale_at(0, in, 0), *vsp = head + a.cache.scale_at(1, in, 0);
+            const uint32_t token = 4 * (i & 3) + (i >> 2);
+            __builtin_memcpy(k[s], __builtin_assume_aligned(kp + token * row + g * (4 * NB), NB % 4 == 0 ? 16 : NB % 2 == 0 ? 8 : 4), 4 * NB);
+            const uint32_t ci = S::kLanes == 16 ? i : min(i, static_cast<uint32_t>(S::kLanes - 1));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint8_t *p = vp + (4 * r + g) * row + ci * (S::kLane / 2);
+                if constexpr (S::kLane == 2) v[4 * s + r][0] = *p;
+                else if constexpr (S::kLane == 4) v[4 * s + r][0] = *reinterpret_cast<const uint16_t *>(p);
+                else __builtin_memcpy(v[4 * s + r], __builtin_assume_aligned(p, 4 * S::kWords), 4 * S::kWords);
+            }
+#pragma unroll
+            for (int u = 0; u < S::kScales; ++u) {
+                const uint32_t b = NB % 4 == 0 ? g * (NB / 4) + u : (g * NB + u) >> 2;
+                ks[s][u] = ksp[(i >> 2) * (4 * NB) + 4 * b + (i & 3)];
+            }
+            vs[s] = *reinterpret_cast<const uint32_t *>(vsp + g * (4 * NB) + 4 * ((ci * S::kLane) >> 5));
+        }
+    }
+};
+
+__device__ __forceinline__ uint32_t cvt(uint32_t codes, float scale, int byte) {
+    switch (byte) {  // an immediate of the instruction
+        case 0: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0));
+        case 1: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1));
+        case 2: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2));
+        default: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3));
+    }
+}
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// Eight FP32 values as P vectors of BF16 whose sums they are (to 8 P bits).
+template <int P>
+__device__ __forceinline__ void pieces(float x[8], u32x4 out[P]) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w = pack2<Mx4Type::BF16>(x[2 * i], x[2 * i + 1]);
+            out[p][i] = w;
+            if (p + 1 < P) {
+                x[2 * i] -= __uint_as_float(w << 16);
+                x[2 * i + 1] -= __uint_as_float(w & 0xFFFF0000u);
+            }
+        }
+    }
+}
+
+template <class F>
+__device__ __forceinline__ void by_device_type(Mx4Type t, F &&fn) {
+    if (t == Mx4Type::BF16) fn(std::integral_constant<Mx4Type, Mx4Type::BF16>{});
+    else if (t == Mx4Type::F16) fn(std::integral_constant<Mx4Type, Mx4Type::F16>{});
+    else fn(std::integral_constant<Mx4Type, Mx4Type::F32>{});
+}
+
+// One row's eight channels of the result, or its logarithm: sums over sum, and
+// the reference.
+__device__ __forceinline__ void write_row(const AttentionArgs &a, uint64_t token, uint32_t head, uint32_t at, float v[8],
+                                          float sum, float top) {
+    const bool none = top == -__builtin_inff() && sum == 0.0f;
+    const float inverse = none ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = none ? 0.0f : v[i] * inverse;
+    const uint32_t dim = a.cache.dim;
+    if (at < dim)
+        by_device_type(a.out_type, [&](auto t) {
+            store8<decltype(t)::value>(a.out, token * a.ldo + static_cast<uint64_t>(head) * dim + at, dim - at, v);
+        });
+    if (at == 0 && a.lse != nullptr)
+        a.lse[token * a.cache.heads * a.group + head] = none ? top : (top + __log2f(sum)) * 0.6931471805599453f;
+}
+
+// A wave's state for its tile of 16 queries: lane (g, i) has query i's reference,
+// its share of the sum, and of the channels' sums those of kLane (4 g + r) + c.
+template <int NB, int P>
+struct Rows {
+    using S = Shape<NB>;
+    u32x4 q[P][NB];
+    f32x4 o[S::kLane];
+    float top, base, sum;  // base: top, 0 where that is minus infinity
+
+    __device__ __forceinline__ void begin(const AttentionArgs &a, const Request &rq, uint32_t h, uint32_t row0, uint32_t rows, uint32_t lane) {
+        const uint32_t g = lane >> 4, i = lane & 15, row = row0 + i;
+        const uint64_t token = static_cast<uint32_t>(rq.first) + row / a.group;
+        const uint64_t at = token * a.ldq + static_cast<uint64_t>(h * a.group + row % a.group) * a.cache.dim;
+#pragma unroll
+        for (int s = 0; s < NB; ++s) {
+            const uint32_t c = (g * NB + s) * 8;
+            float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (i < rows && c < a.cache.dim)
+                by_device_type(a.q_type, [&](auto t) { load8<decltype(t)::value>(a.q, at + c, a.cache.dim - c, x); });
+            if (a.negate) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = -x[e];
+            }
+            u32x4 w[P];
+            pieces<P>(x, w);
+#pragma unroll
+            for (int p = 0; p < P; ++p) q[p][s] = w[p];
+        }
+#pragma unroll
+        for (int c = 0; c < S::kLane; ++c) o[c] = f32x4{0, 0, 0, 0};
+        top = -__builtin_inff();
+        base = sum = 0.0f;
+    }
+
+    // lim, low: the query sees the tokens [low, lim).  any_lim, any_low: some of
+    // the tile's queries see those.
+    template <bool MASKED>
+    __device__ __forceinline__ void step(const AttentionArgs &a, const Tile<NB> &tile, uint32_t t, uint32_t lane, int32_t lim,
+                                         int32_t low, int32_t any_lim, int32_t any_low, bool mixed) {
+        const uint32_t g = lane >> 4, i = lane & 15;
+        f32x4 x[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            x[s] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < NB; ++u) {
+                const float scale = __uint_as_float(tile.ks[s][NB % 4 == 0 ? u / 4 : NB <= 2 ? 0 : u] << 23);
+                const uint32_t w = tile.k[s][u];
+                const u32x4 k = {cvt(w, scale, 0), cvt(w, scale, 1), cvt(w, scale, 2), cvt(w, scale, 3)};
+#pragma unroll
+                for (int p = 0; p < P; ++p) x[s] = mfma(k, q[p][u], x[s]);
+            }
+        }
+        float w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            w[j] = x[j >> 2][j & 3] * a.factor;
+            if constexpr (MASKED) {
+                const int32_t at = static_cast<int32_t>(t + 4 * j + g);
+                if (at >= lim || at < low || (tile.bad >> (j >> 2) & 1)) w[j] = -__builtin_inff();
+            }
+        }
+        float high = w[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) high = fmaxf(high, w[j]);
+        if (__any(high > top + kSlack)) {
+            high = fmaxf(high, __shfl_xor(high, 16));
+            high = fmaxf(high, __shfl_xor(high, 32));
+            const float now = fmaxf(top, high), keep = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top - now);
+            sum *= keep;
+#pragma unroll
+            for (int c = 0; c < S::kLane; ++c) o[c] *= keep;
+            top = now;
+            base = now == -__builtin_inff() ? 0.0f : now;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            w[j] = __builtin_amdgcn_exp2f(w[j] - base);
+            sum += w[j];
+        }
+        u32x4 pw[P];
+        pieces<P>(w, pw);
+
+        uint32_t v[8][S::kWords];
+        float scale[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            uint32_t byte = (tile.vs[j >> 2] >> (8 * (j & 3))) & 0xFFu;
+#pragma unroll
+            for (int d = 0; d < S::kWords; ++d) v[j][d] = tile.v[j][d];
+            if constexpr (MASKED) {
+                // what no query sees may hold anything, NaN among it
+                const int32_t at = static_cast<int32_t>(t + 4 * j + g);
+                if (at >= any_lim || at < any_low || (tile.bad >> (j >> 2) & 1)) {
+                    byte = 127;
+#pragma unroll
+                    for (int d = 0; d < S::kWords; ++d) v[j][d] = 0;
+                }
+                if (mixed) poison(a, byte, v[j], t + 4 * j, lane, lim, low);
+            }
+            scale[j] = __uint_as_float(byte << 23);
+        }
+#pragma unroll
+        for (int c = 0; c < S::kLane; c += 2) {
+            u32x4 even, odd;
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const uint32_t x0 = cvt(v[j][c >> 3], scale[j], (c >> 1) & 3), x1 = cvt(v[j + 1][c >> 3], scale[j + 1], (c >> 1) & 3);
+                even[j >> 1] = __builtin_amdgcn_perm(x1, x0, 0x05040100u);
+                odd[j >> 1] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
+            }
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                o[c] = mfma(even, pw[p], o[c]);
+                o[c + 1] = mfma(odd, pw[p], o[c + 1]);
+            }
+        }
+    }
+
+    // A NaN block of values that some of the tile's queries see and others do not:
+    // the products would give 0 times NaN to those that do not.  It leaves the
+    // products and goes into the sums of those that do.
+    __device__ __forceinline__ void poison(const AttentionArgs &a, uint32_t &byte, uint32_t v[S::kWords], uint32_t t0, uint32_t lane,
+                                           int32_t lim, int32_t low) {
+        uint64_t nan = __ballot(byte == 255u);
+        if (nan == 0) return;
+        if (byte == 255u) {
+            byte = 127;
+#pragma unroll
+            for (int d = 0; d < S::kWords; ++d) v[d] = 0;
+        }
+        while (nan != 0) {
+            const uint32_t from = static_cast<uint32_t>(__builtin_ctzll(nan));
+            nan &= nan - 1;
+            const int32_t at = static_cast<int32_t>(t0 + (from >> 4));
+            const uint32_t block = ((from & 15) * S::kLane) >> 5;
+            if (at >= lim || at < low) continue;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (((4 * (lane >> 4) + r) * S::kLane) >> 5 == block) {
+#pragma unroll
+                    for (int c = 0; c < S::kLane; ++c) o[c][r] = __builtin_nanf("");
+                }
+        }
+    }
+};
+
+// Each workgroup takes an equal share of all spans of all requests' tiles: every
+// tile of every head, in order, so that contexts of any lengths keep all CUs busy
+// alike.  A tile that lies in one share is written at once; of one that does not,
+// each share leaves its sums, and the join below adds them.
+template <int NB, int P>
+__global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void kv4_attention_kernel(AttentionArgs a) {
+    using S = Shape<NB>;
+    __shared__ uint64_t sums[kWaves];
+    __shared__ uint32_t found;
+    __shared__ uint64_t found_base;
+    __shared__ float tops[kWaves][kRows], totals[kWaves][kRows];
+    __shared__ __attribute__((aligned(16))) float acc[kWaves][kRows][S::kRow];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t heads = a.cache.heads;
+
+    // this thread's run of requests, and the spans before it
+    const uint32_t per = (a.requests + kThreads - 1) / kThreads;
+    const uint32_t r_begin = min(tid * per, a.requests), r_end = min(r_begin + per, a.requests);
+    uint64_t mine = 0;
+    for (uint32_t r = r_begin; r < r_end; ++r) {
+        const Request q = load_request(a, r);
+        mine += tiles_of(a, q) * spans_of(a, q);
+    }
+    mine *= heads;
+    uint64_t before = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint64_t o = __shfl_up(before, d);
+        if (lane >= static_cast<uint32_t>(d)) before += o;
+    }
+    if (lane == 63) sums[wave] = before;
+    __syncthreads();
+    uint64_t total = 0;
+    before -= mine;
+    for (uint32_t w = 0; w < kWaves; ++w) {
+        if (w < wave) before += sums[w];
+        total += sums[w];
+    }
+    // no share is empty but those behind the last: a split tile's lie side by side
+    const uint64_t shares = min(total, static_cast<uint64_t>(gridDim.x)), share = min(static_cast<uint64_t>(blockIdx.x), shares);
+    const uint64_t begin = shares ? total * share / shares : 0, end = share < shares ? total * (share + 1) / shares : begin;
+    if (begin < end && begin >= before && begin < before + mine) {
+        uint64_t base = before;
+        for (uint32_t r = r_begin; r < r_end; ++r) {
+            const Request q = load_request(a, r);
+            const uint64_t n = tiles_of(a, q) * spans_of(a, q) * heads;
+            if (begin < base + n) {
+                found = r;
+                found_base = base;
+                break;
+            }
+            base += n;
+        }
+    }
+    __syncthreads();
+    if (begin >= end) {
+        if (tid == 0) a.splits[blockIdx.x].last = 0;
+        return;
+    }
+    uint32_t r = __builtin_amdgcn_readfirstlane(found);
+    uint64_t base = found_base;
+    Request rq = load_request(a, r);
+    bool says = false;  // this workgroup has written its split
+
+    Rows<NB, P> rows;
+    for (uint64_t x = begin; x < end;) {
+        const uint32_t spans = spans_of(a, rq);
+        const uint64_t n = tiles_of(a, rq) * spans * heads;
+        if (x >= base + n) {
+            base += n;
+            rq = load_request(a, ++r);
+            continue;
+        }
+        const uint64_t tile = (x - base) / spans;
+        const uint32_t j0 = static_cast<uint32_t>((x - base) - tile * spans);
+        const uint32_t j1 = static_cast<uint32_t>(min(static_cast<uint64_t>(spans), j0 + (end - x)));
+        const uint64_t tiles = tiles_of(a, rq);
+        const uint32_t h = static_cast<uint32_t>(tile / tiles), row0 = static_cast<uint32_t>(tile - h * tiles) * kRows;
+        const uint32_t count = min(kRows, static_cast<uint32_t>(rq.count) * a.group - row0);
+        x += j1 - j0;
+
+        // what the tile's queries see
+        const int32_t qa = static_cast<int32_t>(row0 / a.group), qb = static_cast<int32_t>((row0 + count - 1) / a.group);
+        const int32_t past = rq.past(), window = static_cast<int32_t>(min(a.window, 0x7FFFFFFFu));
+        const auto lim_of = [&](int32_t query) { return a.causal ? past + query + 1 : rq.length; };
+        const auto low_of = [&](int32_t query) { return window ? past + query + 1 - window : 0; };
+        const int32_t any_lim = lim_of(qb), any_low = low_of(qa), all_lim = lim_of(qa), all_low = low_of(qb);
+        const int32_t mine_q = static_cast<int32_t>((row0 + min(lane & 15, count - 1)) / a.group);
+        const int32_t lim = lim_of(mine_q), low = low_of(mine_q);
+        const uint32_t t0 = first_key(a, rq);
+        const int32_t from = max(static_cast<int32_t>(t0 + j0 * kSpan), any_low & ~static_cast<int32_t>(kStep - 1));
+        const int32_t to = min(static_cast<int32_t>(min(static_cast<uint64_t>(t0) + static_cast<uint64_t>(j1) * kSpan, 0x7FFFFFFFull)), any_lim);
+
+        rows.begin(a, rq, h, row0, count, lane);
+        const int32_t t_first = from + static_cast<int32_t>(wave * kStep);
+        const int32_t *entries = a.table + static_cast<uint64_t>(r) * a.width;
+        const uint32_t last_entry = static_cast<uint32_t>(max(rq.length - 1, 0)) >> a.cache.shift;
+        uint32_t ids = 0;
+        // page numbers of 32 steps, a lane each sixteen
+        const auto load = [&](Tile<NB> &tile_, int32_t t, uint32_t it) {
+            if ((it & 31) == 0) {
+                const uint32_t at = static_cast<uint32_t>(t) + (lane >> 1) * kSpan + (lane & 1) * 16;
+                ids = static_cast<uint32_t>(entries[min(at >> a.cache.shift, last_entry)]);
+            }
+            const int from_lane = static_cast<int>((it & 31) * 2);
+            tile_.load(a, h, static_cast<uint32_t>(t), static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(ids), from_lane)),
+                       static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(ids), from_lane + 1)), lane);
+        };
+        const auto compute = [&](const Tile<NB> &tile_, int32_t t) {
+            if (t + static_cast<int32_t>(kStep) <= all_lim && t >= all_low && tile_.bad == 0)
+                rows.template step<false>(a, tile_, static_cast<uint32_t>(t), lane, lim, low, any_lim, any_low, false);
+            else
+                rows.template step<true>(a, tile_, static_cast<uint32_t>(t), lane, lim, low, any_lim, any_low, qa != qb);
+        };
+        if (t_first < to) {
+            Tile<NB> one, two;
+            uint32_t it = 0;
+            load(one, t_first, it);
+            for (int32_t t = t_first; t < to; t += 2 * static_cast<int32_t>(kSpan)) {
+                const int32_t second = t + static_cast<int32_t>(kSpan), third = second + static_cast<int32_t>(kSpan);
+                if (second < to) load(two, second, it + 1);
+                compute(one, t);
+                if (second >= to) break;
+                if (third < to) load(one, third, it + 2);
+                compute(two, second);
+                it += 2;
+            }
+        }
+
+        // the waves' sums together
+        float sum = rows.sum + __shfl_xor(rows.sum, 16);
+        sum += __shfl_xor(sum, 32);
+        const uint32_t g = lane >> 4, i = lane & 15;
+        if (g == 0) {
+            tops[wave][i] = rows.top;
+            totals[wave][i] = sum;
+        }
+        if (i < count) {
+#pragma unroll
+            for (int rr = 0; rr < 4; ++rr)
+                if (32 * NB == 16 * S::kLane || (4 * g + rr) * S::kLane < 32 * NB) {
+                    float *p = &acc[wave][i][(4 * g + rr) * S::kLane];
+#pragma unroll
+                    for (int c = 0; c < S::kLane; ++c) p[c] = rows.o[c][rr];
+                }
+        }
+        __syncthreads();
+        const bool whole = j0 == 0 && j1 == spans;
+        float *part = a.parts + (static_cast<uint64_t>(blockIdx.x) * 2 + (j0 == 0 ? 1 : 0)) * (kRows * (32 * NB + 2));
+        for (uint32_t item = tid; item < count * (4 * NB); item += kThreads) {
+            const uint32_t n_row = item / (4 * NB), at = (item - n_row * (4 * NB)) * 8;
+            float top = tops[0][n_row];
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) top = fmaxf(top, tops[w][n_row]);
+            float v[8] = {0, 0, 0, 0, 0, 0, 0, 0}, all = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                // without a reference there are zeros, or NaN
+                const float keep = tops[w][n_row] == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(tops[w][n_row] - top);
+                all += keep * totals[w][n_row];
+                const float *p = &acc[w][n_row][at];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += keep * p[e];
+            }
+            if (whole) {
+                const uint32_t row = row0 + n_row;
+                write_row(a, static_cast<uint64_t>(rq.first) + row / a.group, h * a.group + row % a.group, at, v, all, top);
+            } else {
+                float *p = part + n_row * (32 * NB + 2);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) p[at + e] = v[e];
+                if (at == 0) {
+                    p[32 * NB] = top;
+                    p[32 * NB + 1] = all;
+                }
+            }
+        }
+        if (j0 == 0 && j1 < spans) {
+            says = true;
+            if (tid == 0) {
+                // the share that holds the tile's last span
+                const uint64_t last = base + (tile + 1) * spans - 1;
+                Split s{};
+                s.last = static_cast<uint32_t>(((last + 1) * shares - 1) / total);
+                s.head = h;
+                s.row0 = row0;
+                s.rows = count;
+                s.first_token = static_cast<uint32_t>(rq.first);
+                a.splits[blockIdx.x] = s;
+            }
+        }
+        __syncthreads();  // LDS is free again
+    }
+    if (!says && tid == 0) a.splits[blockIdx.x].last = 0;
+}
+
+// A wave a row of a split tile: its parts lie with the workgroups from the one
+// that says so to the last.
+template <int NB>
+__global__ __launch_bounds__(256) void kv4_join_kernel(AttentionArgs a) {
+    const Split s = a.splits[blockIdx.x];
+    const uint32_t n_row = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (s.last == 0 || n_row >= s.rows) return;
+    constexpr uint32_t kPart = kRows * (32 * NB + 2);
+    const auto part = [&](uint32_t b) {
+        return a.parts + (static_cast<uint64_t>(b) * 2 + (b == blockIdx.x ? 1 : 0)) * kPart + n_row * (32 * NB + 2);
+    };
+    float top = -__builtin_inff();
+    for (uint32_t b = blockIdx.x + lane; b <= s.last; b += 64) top = fmaxf(top, part(b)[32 * NB]);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    // lanes: parts beside one another, eight channels each
+    constexpr uint32_t kEights = 4 * NB, kBeside = NB <= 1 ? 16 : NB == 2 ? 8 : NB <= 4 ? 4 : 2;
+    const uint32_t e = lane % (64 / kBeside), beside = lane / (64 / kBeside);
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0}, all = 0.0f;
+    if (e < kEights)
+        for (uint32_t b = blockIdx.x + beside; b <= s.last; b += kBeside) {
+            const float *p = part(b);
+            const float mine = p[32 * NB];
+            const float keep = mine == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(mine - top);
+            all += keep * p[32 * NB + 1];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += keep * p[e * 8 + i];
+        }
+#pragma unroll
+    for (uint32_t d = 64 / kBeside; d < 64; d <<= 1) {
+        all += __shfl_xor(all, d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += __shfl_xor(v[i], d);
+    }
+    if (beside != 0 || e >= kEights) return;
+    const uint32_t row = s.row0 + n_row;
+    write_row(a, static_cast<uint64_t>(s.first_token) + row / a.group, s.head * a.group + row % a.group, e * 8, v, all, top);
+}
+
+struct Plan {
+    uint32_t groups;
+    bool joins;
+    uint64_t parts, bytes;  // bytes of the parts, and of all
+};
+void check_sizes(const Kv4Cache &c, uint32_t width, uint32_t requests, uint64_t tokens, uint32_t q_heads) {
+    BSQ_REQUIRE(q_heads >= 1 && q_heads % c.heads == 0, "kv4 attention: query heads are a multiple of the cache's");
+    BSQ_REQUIRE(q_heads <= 65535, "kv4 attention: up to 65535 query heads");
+    BSQ_REQUIRE(tokens <= 0x7FFFFFFFull && tokens * (q_heads / c.heads) <= 0x7FFFFFFFull, "kv4 attention: too many queries");
+    BSQ_REQUIRE(requests <= 1u << 20, "kv4 attention: up to 2^20 requests");
+    BSQ_REQUIRE(static_cast<uint64_t>(width) << c.shift <= 0x7FFFFFFFull - kSpan, "kv4 attention: rows of the table are too long");
+}
+Plan plan_of(const Kv4Cache &c, uint32_t width, uint32_t requests, uint64_t tokens, uint32_t most, uint32_t q_heads) {
+    const uint64_t group = q_heads / c.heads;
+    // no more tiles and spans than these
+    const uint64_t rows = std::min<uint64_t>(tokens, static_cast<uint64_t>(requests) * most) * group;
+    const uint64_t tiles = (rows / kRows + std::min<uint64_t>(requests, tokens)) * c.heads;
+    const uint64_t spans = ceil_div(std::max<uint64_t>(static_cast<uint64_t>(width) << c.shift, 1), kSpan) + 1;
+    Plan p;
+    p.groups = static_cast<uint32_t>(std::min<uint64_t>(2ull * cu_count(), tiles * spans));
+    p.joins = p.groups > 1;
+    p.parts = round256(static_cast<uint64_t>(p.groups) * 2 * kRows * (32 * c.blocks + 2) * 4);
+    p.bytes = p.parts + round256(p.groups * sizeof(Split));
+    return p;
+}
+
+template <class F>
+void by_blocks(uint32_t blocks, F &&fn) {
+    switch (blocks) {
+        case 1: fn(std::integral_constant<int, 1>{}); return;
+        case 2: fn(std::integral_constant<int, 2>{}); return;
+        case 3: fn(std::integral_constant<int, 3>{}); return;
+        case 4: fn(std::integral_constant<int, 4>{}); return;
+        case 5: fn(std::integral_constant<int, 5>{}); return;
+        case 6: fn(std::integral_constant<int, 6>{}); return;
+        case 7: fn(std::integral_constant<int, 7>{}); return;
+        case 8: fn(std::integral_constant<int, 8>{}); return;
+    }
+    fail("kv4: unknown head size");
+}
+
+}  // namespace
+}  // namespace bsq
+
+using namespace bsq;
+
+extern "C" {
+
+uint64_t bsq_kv4_attention_workspace(const bsq_kv4_cache_t *cache, uint32_t width, uint32_t requests, uint64_t tokens,
+                                     uint32_t most, uint32_t q_heads) {
+    return size_query([&] {
+        const Kv4Cache c = kv4_cache(cache, false);
+        check_sizes(c, width, requests, tokens, q_heads);
+        return plan_of(c, width, requests, tokens, most, q_heads).bytes;
+    });
+}
+
+int bsq_kv4_attention(const bsq_kv4_cache_t *cache, const int32_t *d_table, uint32_t width, const int32_t *d_lengths,
+                      const int32_t *d_starts, uint32_t requests, const void *d_q, int q_type, uint64_t tokens, uint32_t most,
+                      uint32_t q_heads, uint64_t ldq, float scale, int causal, uint32_t window, void *d_out, int out_type,
+                      uint64_t ldo, float *d_lse, void *d_work, uint64_t work_bytes, void *stream) {
+    return entry([&] {
+        const Mx4Type tq = type_of(q_type), to = type_of(out_type);
+        const bool some = tokens > 0 && requests > 0 && most > 0;
+        AttentionArgs a{};
+        a.cache = kv4_cache(cache, some);
+        check_sizes(a.cache, width, requests, tokens, q_heads);
+        const uint64_t row = static_cast<uint64_t>(q_heads) * a.cache.dim;
+        BSQ_REQUIRE(ldq >= row && ldo >= row, "kv4 attention: rows overlap");
+        BSQ_REQUIRE(ldq <= 1ull << 28 && ldo <= 1ull << 28, "kv4 attention: rows too far apart");
+        BSQ_REQUIRE(std::isfinite(scale), "kv4 attention: the scale is not finite");
+        BSQ_REQUIRE(causal == 0 || causal == 1, "kv4 attention: causal is 0 or 1");
+        BSQ_REQUIRE(causal == 1 || window == 0, "kv4 attention: a window is of causal attention");
+        BSQ_REQUIRE(d_starts != nullptr || tokens == requests, "kv4 attention: without starts each request has one query");
+        if (!some) return;
+        BSQ_REQUIRE(d_lengths != nullptr && (width == 0 || d_table != nullptr), "kv4 attention: null argument");
+        check_dense(d_q, tq, "kv4 attention: null queries");
+        check_dense(d_out, to, "kv4 attention: null output");
+        const Plan p = plan_of(a.cache, width, requests, tokens, most, q_heads);
+        check_work(d_work, work_bytes, p.bytes);
+        const int depth = std::max(tq == Mx4Type::F32 ? 3 : tq == Mx4Type::F16 ? 2 : 1, to == Mx4Type::F32 ? 3 : to == Mx4Type::F16 ? 2 : 1);
+        a.table = d_table;
+        a.lengths = d_lengths;
+        a.starts = d_starts;
+        a.width = width;
+        a.requests = requests;
+        a.q = static_cast<const uint8_t *>(d_q);
+        a.q_type = tq;
+        a.out_type = to;
+        a.ldq = ldq;
+        a.ldo = ldo;
+        a.tokens = static_cast<uint32_t>(tokens);
+        a.most = std::min<uint32_t>(most, 0x7FFFFFFFu);
+        a.group = q_heads / a.cache.heads;
+        a.factor = static_cast<float>(std::fabs(static_cast<double>(scale)) * 1.44269504088896340736);
+        a.negate = scale < 0.0f;
+        a.causal = causal != 0;
+        a.window = window;
+        a.out = static_cast<uint8_t *>(d_out);
+        a.lse = d_lse;
+        a.parts = static_cast<float *>(d_work);
+        a.splits = reinterpret_cast<Split *>(static_cast<uint8_t *>(d_work) + p.parts);
+        hipStream_t s = static_cast<hipStream_t>(stream);
+        by_blocks(a.cache.blocks, [&](auto nb) {
+            constexpr int NB = decltype(nb)::value;
+            if (depth == 1) kv4_attention_kernel<NB, 1><<<p.groups, kThreads, 0, s>>>(a);
+            else if (depth == 2) kv4_attention_kernel<NB, 2><<<p.groups, kThreads, 0, s>>>(a);
+            else kv4_attention_kernel<NB, 3><<<p.groups, kThreads, 0, s>>>(a);
+            BSQ_HIP(hipGetLastError());
+            const unsigned rows = static_cast<unsigned>(std::min<uint64_t>(kRows, static_cast<uint64_t>(a.most) * a.group));
+            if (p.joins) kv4_join_kernel<NB><<<dim3(p.groups, (rows + 3) / 4), 256, 0, s>>>(a);
+        });
+        BSQ_HIP(hipGetLastError());
+    });
+}
+
+}  // extern "C"

@@ -443,6 +443,119 @@ BSQ_API int bsq_moe_linear_backward(const void *d_d_out, int d_type, uint64_t to
                                     uint32_t experts, void *d_dx, uint64_t lddx, float *d_d_weights, void *d_dw,
                                     int g_type, void *d_work, uint64_t work_bytes, void *stream);
 
+/* ---------------------------------------------------------------------------
+ * 7. Attention over a paged cache of keys and values in MX4, rotary positions
+ *    and a step's bookkeeping (no reference counterpart).
+ *
+ *    The cache: `pages` pages of `page` tokens.  A page holds, head after head
+ *    of keys and values, the keys' codes, the values' codes, the keys' scales
+ *    and the values' scales; a head's row is padded with zeros to whole blocks of
+ *    32 values (B blocks).  Codes: a token's 16 B bytes, two codes a byte with the
+ *    first in the low half, tokens side by side.  Scales, bytes as in group 6: 16
+ *    tokens side by side (16 B bytes), in them that of token t and block b at
+ *    4 (B (t % 4) + b) + t / 4.  A slot is page * page size + place in the page.
+ *
+ *    Whole numbers are int32.  As in group 6 all calls are asynchronous on
+ *    `stream`, keep nothing between calls, take their workspace from the caller
+ *    and can be captured; types, leading dimensions, returns and size queries are
+ *    those of group 6 too.  What device arrays hold is not checked by the host:
+ *    page numbers and slots outside the cache, lengths outside the table and
+ *    starts outside the tokens are left out by the kernels, as said below.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+    uint8_t *d_pages; /* bsq_kv4_cache_bytes bytes, 16-byte aligned */
+    uint64_t pages;   /* pages * page < 2^31 */
+    uint32_t page;    /* tokens of a page: 16, 32, 64, 128 or 256 */
+    uint32_t heads;   /* of keys and values */
+    uint32_t dim;     /* values of a head, 1 to 256 */
+} bsq_kv4_cache_t;
+BSQ_API uint64_t bsq_kv4_cache_bytes(uint64_t pages, uint32_t page, uint32_t heads, uint32_t dim);
+
+/* A step's bookkeeping.  Request r holds d_lengths[r] tokens, in the pages of
+ * its row of d_table (`width` entries), and gets d_new[r] more; below zero it
+ * has ended.  d_free is a stack of free pages (room for all `pages`, the first
+ * *d_free_count in use).  First the ended requests' pages go onto it, in the
+ * order of requests and of their rows; then each request in turn takes the pages
+ * that its new tokens need beyond those it holds, from the top, into its row.
+ * A request is not served where the stack runs out (nor are those behind it that
+ * need a page), its row is too short, or its tokens go past `tokens`.
+ * Written: d_lengths_out[r], the length with the new tokens (as it was where not
+ * served, 0 where ended; may be d_lengths); d_left[0], the pages left on the
+ * stack (d_left may be d_free_count), and d_left[1], the requests not served;
+ * d_starts[0 .. requests], where each request's new tokens begin among the
+ * `tokens` places; and for each place its request (d_requests, may be NULL), its
+ * position and its slot: -1 behind the last token, position and slot also of
+ * requests not served.  Up to 16384 requests; requests * width < 2^31. */
+BSQ_API uint64_t bsq_kv4_plan_workspace(uint32_t requests);
+BSQ_API int bsq_kv4_plan(const int32_t *d_lengths, const int32_t *d_new, uint32_t requests, int32_t *d_table,
+                         uint32_t width, uint32_t page, int32_t *d_free, uint64_t pages, const int32_t *d_free_count,
+                         int32_t *d_lengths_out, int32_t *d_left, int32_t *d_starts, uint64_t tokens,
+                         int32_t *d_requests, int32_t *d_positions, int32_t *d_slots, void *d_work, uint64_t work_bytes,
+                         void *stream);
+
+/* Rotary positions: of a head's first `dims` values (even), pair i = (x[i],
+ * x[i + dims / 2]), or (x[2 i], x[2 i + 1]) if `interleaved`, becomes factor
+ * (a cos t - b sin t, b cos t + a sin t), t = position * d_frequencies[i]; the
+ * others stay as they are.  Angles, sine, cosine and the pair's products are
+ * FP64, rounded once through FP32 to the type. */
+typedef struct {
+    const double *d_frequencies; /* dims / 2 */
+    uint32_t dims;
+    int interleaved;
+    float factor;
+} bsq_rope_t;
+/* Fills host arrays: frequencies base^(-2 i / dims), for contexts `stretch` times
+ * `length`: scaling 0 as they are (stretch is not used); 1 all over stretch; 2
+ * those of the base times stretch^(dims / (dims - 2)); 3 by parts: pairs that
+ * turn over 32 times in `length` positions as they are, those that turn less
+ * than once over stretch, a ramp between.  *factor: 1, for 3 it is
+ * 1 + ln(stretch) / 10. */
+BSQ_API int bsq_rope_frequencies(uint32_t dims, double base, int scaling, double stretch, double length,
+                                 double *frequencies, float *factor);
+/* out = x turned (`back`: turned back, times factor: the gradient of x from that
+ * of out); tokens rows of `heads` heads side by side; out may be x, with its
+ * rows.  Rows whose position is below zero are left as they are. */
+BSQ_API int bsq_rope(const bsq_rope_t *rope, const int32_t *d_positions, const void *d_x, int type, uint64_t tokens,
+                     uint32_t heads, uint32_t dim, uint64_t ldx, int back, void *d_out, uint64_t ldo, void *stream);
+
+/* A step's tokens: queries (q_heads heads; d_q may be NULL) turned to d_q_out
+ * (may be d_q, with its rows), keys turned, rounded to their type and packed,
+ * values packed, both into the cache at d_slots.  rope NULL: nothing is turned,
+ * and d_positions may be NULL.  A token whose position is below zero is left
+ * out, one whose slot is outside the cache leaves only its queries.  Where two
+ * tokens have one slot, it holds parts of either. */
+BSQ_API int bsq_kv4_append(const bsq_kv4_cache_t *cache, const bsq_rope_t *rope, const int32_t *d_positions,
+                           const int32_t *d_slots, uint64_t tokens, int type, const void *d_q, uint32_t q_heads,
+                           uint64_t ldq, void *d_q_out, uint64_t ldqo, const void *d_k, uint64_t ldk, const void *d_v,
+                           uint64_t ldv, void *stream);
+/* The keys and values at d_slots (either may be NULL); rows of slots outside the
+ * cache are left as they are. */
+BSQ_API int bsq_kv4_read(const bsq_kv4_cache_t *cache, const int32_t *d_slots, uint64_t tokens, int type, void *d_k,
+                         uint64_t ldk, void *d_v, uint64_t ldv, void *stream);
+
+/* Attention: request r has the keys and values 0 .. d_lengths[r] - 1, in the
+ * pages of its row of d_table, and the queries d_starts[r] .. d_starts[r + 1] - 1
+ * of `tokens` (d_starts NULL: query r), `most` of them at most; its last query
+ * is at the last key's position.  Query head h reads head h / (q_heads / heads)
+ * of keys and values:
+ *   out = sum over the seen j of softmax(scale q . k[j]) v[j]
+ * `causal`: a query sees the keys up to its own position, with a `window` above
+ * zero only the last `window` of them; else all of its request's (window 0).
+ * Keys on page numbers outside the cache are not seen.  A query that sees none
+ * gives zeros.  d_lse (tokens x q_heads, may be NULL): the natural logarithm of
+ * the softmax's sum, minus infinity where no key is seen.  Sums and softmax are
+ * FP32; products with queries are exact to FP32 in every type, the softmax's
+ * weights are rounded to BF16 where both q and out are BF16, are held to 16 bits
+ * where FP16 is the finest type among them, and to FP32 where one is FP32.
+ * Queries behind the last request's, and past `most`, are left as they are. */
+BSQ_API uint64_t bsq_kv4_attention_workspace(const bsq_kv4_cache_t *cache, uint32_t width, uint32_t requests,
+                                             uint64_t tokens, uint32_t most, uint32_t q_heads);
+BSQ_API int bsq_kv4_attention(const bsq_kv4_cache_t *cache, const int32_t *d_table, uint32_t width,
+                              const int32_t *d_lengths, const int32_t *d_starts, uint32_t requests, const void *d_q,
+                              int q_type, uint64_t tokens, uint32_t most, uint32_t q_heads, uint64_t ldq, float scale,
+                              int causal, uint32_t window, void *d_out, int out_type, uint64_t ldo, float *d_lse,
+                              void *d_work, uint64_t work_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
