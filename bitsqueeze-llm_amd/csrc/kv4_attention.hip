@@ -1,16 +1,6 @@
-// Attention over the paged MX4 cache (kv4.hpp).
-//
-// out_i = sum_j p_ij v_j / sum_j p_ij, p_ij = 2^(x_ij - m_i), x_ij = scale log2(e)
-// q_i . k_j, in one pass over the keys with m_i a running reference.  m_i is
-// raised only where some x_ij lies more than 8 above it: the sums are FP32, so a
-// reference that is up to 2^8 low costs nothing, and most tiles need no rescale
-// and no exchange between lanes.
-//
-// Keys and values are converted to BF16, which holds E2M1 times a power of two
-// exactly, and multiplied on the BF16 matrix instructions; queries that BF16 does
-// not hold are split into two (FP16) or three (FP32) BF16 pieces, so that products
-// are those of FP32.  The weights p go in the same number of pieces.
-#include "kv4.hpp"
+// Attention over the paged MX4 cache: single tokens and a few queries a request
+// (kv4_attention.hpp), the entry point, and the join of split tiles.
+#include "kv4_attention.hpp"
 
 #include <algorithm>
 #include <cmath>
@@ -18,66 +8,10 @@
 namespace bsq {
 namespace {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr uint32_t kRows = 16;                   // (token, head of the group) pairs of a tile of queries
-constexpr uint32_t kStep = 32;                   // keys a wave takes at once
-constexpr uint32_t kSpan = kStep * kWaves;       // keys a workgroup takes at once
-constexpr float kSlack = 8.0f;
-
-struct AttentionArgs {
-    Kv4Cache cache;
-    const int32_t *table, *lengths, *starts;
-    uint32_t width, requests;
-    const uint8_t *q;
-    Mx4Type q_type, out_type;
-    uint64_t ldq, ldo;
-    uint32_t tokens, most, group;  // group: query heads to a head of keys
-    float factor;                  // scale log2(e), not below zero
-    bool negate;                   // the scale is below zero
-    bool causal;
-    uint32_t window;
-    uint8_t *out;
-    float *lse;
-    float *parts;
-    struct Split *splits;
-};
-
-// A tile of queries whose keys more than one workgroup takes: the first of them
-// says so, and up to which workgroup it goes.
-struct Split {
-    uint32_t last;  // 0: none begins here
-    uint32_t head, row0, rows;
-    uint32_t first_token;
-    uint32_t pad[3];
-};
-
-struct Request {
-    int32_t length, first, count;  // keys, first query, queries
-    __device__ __forceinline__ int32_t past() const { return length - count; }
-};
-
-__device__ __forceinline__ Request load_request(const AttentionArgs &a, uint32_t r) {
-    Request q;
-    const int64_t room = static_cast<int64_t>(a.width) << a.cache.shift;
-    q.length = static_cast<int32_t>(min(static_cast<int64_t>(max(a.lengths[r], 0)), room));
-    if (a.starts == nullptr) {
-        q.first = static_cast<int32_t>(r);
-        q.count = r < a.tokens ? 1 : 0;
-    } else {
-        const int32_t tokens = static_cast<int32_t>(a.tokens);
-        q.first = min(max(a.starts[r], 0), tokens);
-        const int32_t n = min(max(a.starts[r + 1], q.first), tokens) - q.first;
-        q.count = min(n, static_cast<int32_t>(a.most));
-        // queries past `most` are the last ones: the others' keys end before theirs
-        if (a.causal) q.length = max(q.length - (n - q.count), 0);
-    }
-    return q;
-}
+constexpr uint32_t kStep = 32;              // keys a wave takes at once
+constexpr uint32_t kSpan = kStep * kWaves;  // keys a workgroup takes at once
 
 // Where a request's keys begin, and their number in spans (at least one, which
 // writes the zeros of queries that see none).
@@ -89,7 +23,8 @@ __device__ __forceinline__ uint32_t spans_of(const AttentionArgs &a, const Reque
     return length > first ? (length - first + kSpan - 1) / kSpan : 1u;
 }
 __device__ __forceinline__ uint64_t tiles_of(const AttentionArgs &a, const Request &q) {
-    return (static_cast<uint64_t>(q.count) * a.group + kRows - 1) / kRows;
+    const uint64_t rows = static_cast<uint64_t>(q.count) * a.group;
+    return rows > a.few ? 0 : (rows + kTileRows - 1) / kTileRows;
 }
 
 template <int NB>
@@ -147,58 +82,6 @@ struct Tile {
         }
     }
 };
-
-__device__ __forceinline__ uint32_t cvt(uint32_t codes, float scale, int byte) {
-    switch (byte) {  // an immediate of the instruction
-        case 0: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0));
-        case 1: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1));
-        case 2: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2));
-        default: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3));
-    }
-}
-__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-// Eight FP32 values as P vectors of BF16 whose sums they are (to 8 P bits).
-template <int P>
-__device__ __forceinline__ void pieces(float x[8], u32x4 out[P]) {
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t w = pack2<Mx4Type::BF16>(x[2 * i], x[2 * i + 1]);
-            out[p][i] = w;
-            if (p + 1 < P) {
-                x[2 * i] -= __uint_as_float(w << 16);
-                x[2 * i + 1] -= __uint_as_float(w & 0xFFFF0000u);
-            }
-        }
-    }
-}
-
-template <class F>
-__device__ __forceinline__ void by_device_type(Mx4Type t, F &&fn) {
-    if (t == Mx4Type::BF16) fn(std::integral_constant<Mx4Type, Mx4Type::BF16>{});
-    else if (t == Mx4Type::F16) fn(std::integral_constant<Mx4Type, Mx4Type::F16>{});
-    else fn(std::integral_constant<Mx4Type, Mx4Type::F32>{});
-}
-
-// One row's eight channels of the result, or its logarithm: sums over sum, and
-// the reference.
-__device__ __forceinline__ void write_row(const AttentionArgs &a, uint64_t token, uint32_t head, uint32_t at, float v[8],
-                                          float sum, float top) {
-    const bool none = top == -__builtin_inff() && sum == 0.0f;
-    const float inverse = none ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = none ? 0.0f : v[i] * inverse;
-    const uint32_t dim = a.cache.dim;
-    if (at < dim)
-        by_device_type(a.out_type, [&](auto t) {
-            store8<decltype(t)::value>(a.out, token * a.ldo + static_cast<uint64_t>(head) * dim + at, dim - at, v);
-        });
-    if (at == 0 && a.lse != nullptr)
-        a.lse[token * a.cache.heads * a.group + head] = none ? top : (top + __log2f(sum)) * 0.6931471805599453f;
-}
 
 // A wave's state for its tile of 16 queries: lane (g, i) has query i's reference,
 // its share of the sum, and of the channels' sums those of kLane (4 g + r) + c.
@@ -357,8 +240,8 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void kv4_attention_kerne
     __shared__ uint64_t sums[kWaves];
     __shared__ uint32_t found;
     __shared__ uint64_t found_base;
-    __shared__ float tops[kWaves][kRows], totals[kWaves][kRows];
-    __shared__ __attribute__((aligned(16))) float acc[kWaves][kRows][S::kRow];
+    __shared__ float tops[kWaves][kTileRows], totals[kWaves][kTileRows];
+    __shared__ __attribute__((aligned(16))) float acc[kWaves][kTileRows][S::kRow];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t heads = a.cache.heads;
 
@@ -403,7 +286,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void kv4_attention_kerne
     }
     __syncthreads();
     if (begin >= end) {
-        if (tid == 0) a.splits[blockIdx.x].last = 0;
+        if (tid == 0) a.splits[blockIdx.x].parts = 0;
         return;
     }
     uint32_t r = __builtin_amdgcn_readfirstlane(found);
@@ -424,8 +307,8 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void kv4_attention_kerne
         const uint32_t j0 = static_cast<uint32_t>((x - base) - tile * spans);
         const uint32_t j1 = static_cast<uint32_t>(min(static_cast<uint64_t>(spans), j0 + (end - x)));
         const uint64_t tiles = tiles_of(a, rq);
-        const uint32_t h = static_cast<uint32_t>(tile / tiles), row0 = static_cast<uint32_t>(tile - h * tiles) * kRows;
-        const uint32_t count = min(kRows, static_cast<uint32_t>(rq.count) * a.group - row0);
+        const uint32_t h = static_cast<uint32_t>(tile / tiles), row0 = static_cast<uint32_t>(tile - h * tiles) * kTileRows;
+        const uint32_t count = min(kTileRows, static_cast<uint32_t>(rq.count) * a.group - row0);
         x += j1 - j0;
 
         // what the tile's queries see
@@ -495,7 +378,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void kv4_attention_kerne
         }
         __syncthreads();
         const bool whole = j0 == 0 && j1 == spans;
-        float *part = a.parts + (static_cast<uint64_t>(blockIdx.x) * 2 + (j0 == 0 ? 1 : 0)) * (kRows * (32 * NB + 2));
+        float *part = a.parts + (static_cast<uint64_t>(blockIdx.x) * 2 + (j0 == 0 ? 1 : 0)) * (kTileRows * part_row(NB));
         for (uint32_t item = tid; item < count * (4 * NB); item += kThreads) {
             const uint32_t n_row = item / (4 * NB), at = (item - n_row * (4 * NB)) * 8;
             float top = tops[0][n_row];
@@ -515,7 +398,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void kv4_attention_kerne
                 const uint32_t row = row0 + n_row;
                 write_row(a, static_cast<uint64_t>(rq.first) + row / a.group, h * a.group + row % a.group, at, v, all, top);
             } else {
-                float *p = part + n_row * (32 * NB + 2);
+                float *p = part + n_row * part_row(NB);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) p[at + e] = v[e];
                 if (at == 0) {
@@ -529,33 +412,27 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void kv4_attention_kerne
             if (tid == 0) {
                 // the share that holds the tile's last span
                 const uint64_t last = base + (tile + 1) * spans - 1;
-                Split s{};
-                s.last = static_cast<uint32_t>(((last + 1) * shares - 1) / total);
-                s.head = h;
-                s.row0 = row0;
-                s.rows = count;
-                s.first_token = static_cast<uint32_t>(rq.first);
-                a.splits[blockIdx.x] = s;
+                const uint32_t last_share = static_cast<uint32_t>(((last + 1) * shares - 1) / total), b = blockIdx.x;
+                a.splits[b] = {last_share - b + 1, 2 * b + 1, 2 * b + 2, 2, h, row0, count, static_cast<uint32_t>(rq.first)};
             }
         }
         __syncthreads();  // LDS is free again
     }
-    if (!says && tid == 0) a.splits[blockIdx.x].last = 0;
+    if (!says && tid == 0) a.splits[blockIdx.x].parts = 0;
 }
 
-// A wave a row of a split tile: its parts lie with the workgroups from the one
-// that says so to the last.
+// A wave a row of a split tile.
 template <int NB>
-__global__ __launch_bounds__(256) void kv4_join_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(256) void kv4_join_kernel(AttentionArgs a, uint32_t part_rows) {
     const Split s = a.splits[blockIdx.x];
     const uint32_t n_row = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (s.last == 0 || n_row >= s.rows) return;
-    constexpr uint32_t kPart = kRows * (32 * NB + 2);
+    if (s.parts == 0 || n_row >= s.rows) return;
     const auto part = [&](uint32_t b) {
-        return a.parts + (static_cast<uint64_t>(b) * 2 + (b == blockIdx.x ? 1 : 0)) * kPart + n_row * (32 * NB + 2);
+        const uint64_t number = b == 0 ? s.first : s.next + static_cast<uint64_t>(b - 1) * s.step;
+        return a.parts + (number * part_rows + n_row) * part_row(NB);
     };
     float top = -__builtin_inff();
-    for (uint32_t b = blockIdx.x + lane; b <= s.last; b += 64) top = fmaxf(top, part(b)[32 * NB]);
+    for (uint32_t b = lane; b < s.parts; b += 64) top = fmaxf(top, part(b)[32 * NB]);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
     // lanes: parts beside one another, eight channels each
@@ -563,7 +440,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttentionArgs a) {
     const uint32_t e = lane % (64 / kBeside), beside = lane / (64 / kBeside);
     float v[8] = {0, 0, 0, 0, 0, 0, 0, 0}, all = 0.0f;
     if (e < kEights)
-        for (uint32_t b = blockIdx.x + beside; b <= s.last; b += kBeside) {
+        for (uint32_t b = beside; b < s.parts; b += kBeside) {
             const float *p = part(b);
             const float mine = p[32 * NB];
             const float keep = mine == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(mine - top);
@@ -582,10 +459,16 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttentionArgs a) {
     write_row(a, static_cast<uint64_t>(s.first_token) + row / a.group, s.head * a.group + row % a.group, e * 8, v, all, top);
 }
 
+// Requests of more rows than this are a prompt's: 16 rows a tile read and convert
+// the keys once for each tile, 128 rows once for them all.
+constexpr uint32_t kFewRows = 64;
+
 struct Plan {
-    uint32_t groups;
-    bool joins;
-    uint64_t parts, bytes;  // bytes of the parts, and of all
+    uint32_t few;               // AttentionArgs' own
+    uint32_t groups = 0;        // of the kernel of few queries
+    uint64_t tiles = 0;         // of the prompts' kernel
+    uint32_t each = 1;
+    uint64_t splits = 0, parts_bytes = 0, bytes = 0;
 };
 void check_sizes(const Kv4Cache &c, uint32_t width, uint32_t requests, uint64_t tokens, uint32_t q_heads) {
     BSQ_REQUIRE(q_heads >= 1 && q_heads % c.heads == 0, "kv4 attention: query heads are a multiple of the cache's");
@@ -595,32 +478,40 @@ void check_sizes(const Kv4Cache &c, uint32_t width, uint32_t requests, uint64_t 
     BSQ_REQUIRE(static_cast<uint64_t>(width) << c.shift <= 0x7FFFFFFFull - kSpan, "kv4 attention: rows of the table are too long");
 }
 Plan plan_of(const Kv4Cache &c, uint32_t width, uint32_t requests, uint64_t tokens, uint32_t most, uint32_t q_heads) {
-    const uint64_t group = q_heads / c.heads;
-    // no more tiles and spans than these
+    const uint64_t group = q_heads / c.heads, keys = std::max<uint64_t>(static_cast<uint64_t>(width) << c.shift, 1);
     const uint64_t rows = std::min<uint64_t>(tokens, static_cast<uint64_t>(requests) * most) * group;
-    const uint64_t tiles = (rows / kRows + std::min<uint64_t>(requests, tokens)) * c.heads;
-    const uint64_t spans = ceil_div(std::max<uint64_t>(static_cast<uint64_t>(width) << c.shift, 1), kSpan) + 1;
+    const uint64_t some = std::min<uint64_t>(requests, tokens);
+    const bool prompts = static_cast<uint64_t>(most) * group > kFewRows;
     Plan p;
-    p.groups = static_cast<uint32_t>(std::min<uint64_t>(2ull * cu_count(), tiles * spans));
-    p.joins = p.groups > 1;
-    p.parts = round256(static_cast<uint64_t>(p.groups) * 2 * kRows * (32 * c.blocks + 2) * 4);
-    p.bytes = p.parts + round256(p.groups * sizeof(Split));
+    // one request is one kernel's, whatever its queries
+    p.few = prompts ? (requests == 1 ? 0 : kFewRows) : 0xFFFFFFFFu;
+    uint64_t parts = 0;
+    if (p.few > 0) {  // no more tiles and spans than these
+        const uint64_t tiles = (rows / kTileRows + some) * c.heads, spans = ceil_div(keys, kSpan) + 1;
+        p.groups = static_cast<uint32_t>(std::min<uint64_t>(2ull * cu_count(), tiles * spans));
+        p.splits = p.groups;
+        parts = static_cast<uint64_t>(p.groups) * 2 * kTileRows;
+    }
+    if (prompts) {
+        p.tiles = rows / kPromptRows + std::min<uint64_t>(some, ceil_div(rows, p.few + 1));
+        // two workgroups a CU; a share of at least 1024 keys
+        const uint64_t shares = 2ull * cu_count() / (p.tiles * c.heads);
+        p.each = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(shares, keys / 1024)));
+        if (p.each > 1) {
+            p.splits = std::max<uint64_t>(p.splits, p.tiles * c.heads);
+            parts = std::max<uint64_t>(parts, p.tiles * c.heads * p.each * kPromptRows);
+        }
+    }
+    p.parts_bytes = round256(parts * part_row(c.blocks) * 4);
+    p.bytes = p.parts_bytes + round256(p.splits * sizeof(Split));
     return p;
 }
 
-template <class F>
-void by_blocks(uint32_t blocks, F &&fn) {
-    switch (blocks) {
-        case 1: fn(std::integral_constant<int, 1>{}); return;
-        case 2: fn(std::integral_constant<int, 2>{}); return;
-        case 3: fn(std::integral_constant<int, 3>{}); return;
-        case 4: fn(std::integral_constant<int, 4>{}); return;
-        case 5: fn(std::integral_constant<int, 5>{}); return;
-        case 6: fn(std::integral_constant<int, 6>{}); return;
-        case 7: fn(std::integral_constant<int, 7>{}); return;
-        case 8: fn(std::integral_constant<int, 8>{}); return;
-    }
-    fail("kv4: unknown head size");
+template <int NB>
+void join(const AttentionArgs &a, uint64_t splits, uint32_t part_rows, uint64_t rows, hipStream_t s) {
+    rows = std::min<uint64_t>(rows, part_rows);
+    kv4_join_kernel<NB><<<dim3(static_cast<unsigned>(splits), static_cast<unsigned>((rows + 3) / 4)), 256, 0, s>>>(a, part_rows);
+    BSQ_HIP(hipGetLastError());
 }
 
 }  // namespace
@@ -683,18 +574,25 @@ int bsq_kv4_attention(const bsq_kv4_cache_t *cache, const int32_t *d_table, uint
         a.out = static_cast<uint8_t *>(d_out);
         a.lse = d_lse;
         a.parts = static_cast<float *>(d_work);
-        a.splits = reinterpret_cast<Split *>(static_cast<uint8_t *>(d_work) + p.parts);
+        a.splits = reinterpret_cast<Split *>(static_cast<uint8_t *>(d_work) + p.parts_bytes);
+        a.few = p.few;
+        a.each = p.each;
         hipStream_t s = static_cast<hipStream_t>(stream);
+        const uint64_t rows = static_cast<uint64_t>(a.most) * a.group;
         by_blocks(a.cache.blocks, [&](auto nb) {
             constexpr int NB = decltype(nb)::value;
-            if (depth == 1) kv4_attention_kernel<NB, 1><<<p.groups, kThreads, 0, s>>>(a);
-            else if (depth == 2) kv4_attention_kernel<NB, 2><<<p.groups, kThreads, 0, s>>>(a);
-            else kv4_attention_kernel<NB, 3><<<p.groups, kThreads, 0, s>>>(a);
-            BSQ_HIP(hipGetLastError());
-            const unsigned rows = static_cast<unsigned>(std::min<uint64_t>(kRows, static_cast<uint64_t>(a.most) * a.group));
-            if (p.joins) kv4_join_kernel<NB><<<dim3(p.groups, (rows + 3) / 4), 256, 0, s>>>(a);
+            if (p.groups > 0) {
+                if (depth == 1) kv4_attention_kernel<NB, 1><<<p.groups, kThreads, 0, s>>>(a);
+                else if (depth == 2) kv4_attention_kernel<NB, 2><<<p.groups, kThreads, 0, s>>>(a);
+                else kv4_attention_kernel<NB, 3><<<p.groups, kThreads, 0, s>>>(a);
+                BSQ_HIP(hipGetLastError());
+                if (p.groups > 1) join<NB>(a, p.groups, kTileRows, rows, s);
+            }
+            if (p.tiles > 0) {
+                launch_kv4_prompt(a, depth, p.tiles, s);
+                if (p.each > 1) join<NB>(a, p.tiles * a.cache.heads, kPromptRows, rows, s);
+            }
         });
-        BSQ_HIP(hipGetLastError());
     });
 }
 

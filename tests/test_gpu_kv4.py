@@ -462,6 +462,89 @@ def test_scores_that_rise_and_fall():
         check_attention(c, table, [640], [1], q, 1.0, B.TYPE_F32)
 
 
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("heads,group,dim,page,count,past", [
+    (1, 1, 64, 16, 65, 0), (2, 4, 128, 16, 50, 100), (1, 5, 96, 32, 90, 37), (1, 3, 256, 64, 60, 200), (1, 17, 33, 16, 9, 20),
+    (2, 2, 160, 16, 64, 70), (1, 1, 200, 256, 129, 5), (1, 2, 8, 16, 150, 0), (1, 1, 192, 16, 100, -30), (1, 80, 64, 16, 3, 150),
+])
+def test_prompts(type, heads, group, dim, page, count, past):
+    # alone (one kernel), beside others (two), in a window
+    rng = np.random.default_rng(dim + count)
+    c = filled(rng, max(4, 640 // page), page, heads, dim)
+    length = count + past
+    for lengths, counts in (([length], [count]), ([20, length, 0, 77], [1, count, 2, 70])):
+        table = tables(rng, c, lengths, -(-320 // page))
+        q = rng.standard_normal((sum(counts), heads * group, dim))
+        check_attention(c, table, lengths, counts, q, dim**-0.5, type, extra=5)
+        check_attention(c, table, lengths, counts, q, dim**-0.5, type, window=45)
+
+
+@pytest.mark.parametrize("type", TYPES)
+def test_prompts_not_causal(type):
+    rng = np.random.default_rng(24)
+    c = filled(rng, 20, 16, 2, 64)
+    lengths, counts = [100, 0, 250], [90, 70, 3]
+    q = rng.standard_normal((sum(counts), 4, 64))
+    check_attention(c, tables(rng, c, lengths, 17), lengths, counts, q, 0.125, type, causal=False)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 4.0])
+def test_scales_of_prompts(scale):
+    rng = np.random.default_rng(26)
+    c = filled(rng, 12, 16, 1, 64)
+    q = rng.standard_normal((80, 2, 64))
+    check_attention(c, tables(rng, c, [150], 10), [150], [80], q, scale, B.TYPE_F32)
+
+
+@pytest.mark.parametrize("window", [0, 1500])
+def test_prompts_whose_keys_are_shared(window):
+    # few tiles of queries over long contexts: workgroups share a tile's keys
+    rng = np.random.default_rng(25)
+    c = filled(rng, 320, 16, 1, 32)
+    for lengths, counts in (([4800], [40]), ([4300, 2500, 3, 70], [50, 33, 3, 70])):
+        table = np.array([rng.permutation(320) for _ in lengths])
+        q = rng.standard_normal((sum(counts), 2, 32))
+        for type in TYPES:
+            check_attention(c, table, lengths, counts, q, 0.3, type, window=window)
+
+
+def test_prompts_pages_out_of_range():
+    rng = np.random.default_rng(28)
+    c = filled(rng, 16, 16, 1, 64)
+    lengths, counts = [200, 150], [80, 100]
+    table = tables(rng, c, lengths, 14)
+    table[0, 1], table[0, 3], table[0, 11], table[1, :] = -1, 16, 2**31 - 1, 99
+    q = rng.standard_normal((sum(counts), 2, 64))
+    got, lse, _ = check_attention(c, table, lengths, counts, q, 0.1, B.TYPE_F32)
+    assert (got[80:] == 0).all() and (lse[80:] == -np.inf).all()
+
+
+def test_prompts_nan_where_nobody_looks():
+    rng = np.random.default_rng(29)
+    for group, dim in ((1, 64), (3, 128), (1, 33), (2, 256)):
+        for type in (B.TYPE_BF16, B.TYPE_F32):
+            c = filled(rng, 16, 16, 1, dim)
+            length, n = 190, 80  # queries at 110 .. 189
+            table = np.array([rng.permutation(16)[:12]])
+            slot = lambda j: int(table[0, j // 16]) * 16 + j % 16  # noqa: E731
+            for j in range(length, 192):
+                c.put(slot(j), np.full((1, dim), np.nan), np.full((1, dim), np.nan))
+            v = c.get(slot(140), 0, 1).copy()
+            v[3] = np.nan
+            c.put(slot(140), c.get(slot(140), 0, 0)[None], v[None])
+            q = rng.standard_normal((n, group, dim))
+            got, lse, _ = check_attention(c, table, [length], [n], q, 0.1, type)
+            assert np.isnan(got[30:, :, :32]).all() and np.isfinite(got[:30]).all() and np.isfinite(got[:, :, 32:]).all()
+            check_attention(c, table, [length], [n], q, 0.1, type, window=20)
+            k = c.get(slot(150), 0, 0).copy()
+            k[0] = np.nan
+            c.put(slot(150), k[None], c.get(slot(150), 0, 1)[None])
+            got, lse, _ = check_attention(c, table, [length], [n], q, 0.1, type)
+            assert np.isnan(lse[40:]).all() and np.isfinite(lse[:40]).all()
+            got, lse, _ = check_attention(c, table, [length], [n], q, 0.1, type, window=20)
+            assert np.isfinite(lse[:40]).all() and np.isnan(lse[40:60]).all() and np.isfinite(lse[60:]).all()
+
+
 def test_long_request_over_all_workgroups():
     # one request whose keys many workgroups share, beside short ones
     rng = np.random.default_rng(11)
