@@ -13,18 +13,22 @@ constexpr int kWaves = kThreads / 64;
 constexpr uint32_t kStep = 32;              // keys a wave takes at once
 constexpr uint32_t kSpan = kStep * kWaves;  // keys a workgroup takes at once
 
-// Where a request's keys begin, and their number in spans (at least one, which
-// writes the zeros of queries that see none).
+// A tile's work: units of a.span keys (at least one, which writes the zeros of
+// queries that see none), and kExtra more for what a tile costs beside its keys:
+// page numbers, queries and first keys are waited for one after another, and the
+// waves' sums are joined.
+constexpr uint32_t kExtra = 2;
+
 __device__ __forceinline__ uint32_t first_key(const AttentionArgs &a, const Request &q) {
     return a.window == 0 ? 0u : static_cast<uint32_t>(max(q.past() + 1 - static_cast<int64_t>(a.window), static_cast<int64_t>(0))) & ~(kStep - 1);
 }
 __device__ __forceinline__ uint32_t spans_of(const AttentionArgs &a, const Request &q) {
     const uint32_t first = first_key(a, q), length = static_cast<uint32_t>(q.length);
-    return length > first ? (length - first + kSpan - 1) / kSpan : 1u;
+    return length > first ? (length - first + a.span - 1) / a.span : 1u;
 }
-__device__ __forceinline__ uint64_t tiles_of(const AttentionArgs &a, const Request &q) {
+__device__ __forceinline__ uint32_t tiles_of(const AttentionArgs &a, const Request &q) {
     const uint64_t rows = static_cast<uint64_t>(q.count) * a.group;
-    return rows > a.few ? 0 : (rows + kTileRows - 1) / kTileRows;
+    return rows > a.few ? 0u : static_cast<uint32_t>((rows + kTileRows - 1) / kTileRows);
 }
 
 template <int NB>
@@ -230,86 +234,72 @@ struct Rows {
     }
 };
 
-// Each workgroup takes an equal share of all spans of all requests' tiles: every
+// Each workgroup takes an equal share of all units of all requests' tiles: every
 // tile of every head, in order, so that contexts of any lengths keep all CUs busy
-// alike.  A tile that lies in one share is written at once; of one that does not,
-// each share leaves its sums, and the join below adds them.
+// alike.  A tile whose keys lie in one share is written at once; of one whose do
+// not, each share leaves its sums, and the join below adds them.
 template <int NB, int P>
 __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void kv4_attention_kernel(AttentionArgs a) {
     using S = Shape<NB>;
-    __shared__ uint64_t sums[kWaves];
-    __shared__ uint32_t found;
-    __shared__ uint64_t found_base;
     __shared__ float tops[kWaves][kTileRows], totals[kWaves][kTileRows];
     __shared__ __attribute__((aligned(16))) float acc[kWaves][kTileRows][S::kRow];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t heads = a.cache.heads;
 
-    // this thread's run of requests, and the spans before it
-    const uint32_t per = (a.requests + kThreads - 1) / kThreads;
-    const uint32_t r_begin = min(tid * per, a.requests), r_end = min(r_begin + per, a.requests);
-    uint64_t mine = 0;
-    for (uint32_t r = r_begin; r < r_end; ++r) {
-        const Request q = load_request(a, r);
-        mine += tiles_of(a, q) * spans_of(a, q);
+    // a lane's run of requests, and the units before it: every wave for itself,
+    // without a barrier
+    const uint32_t per = (a.requests + 63) / 64;
+    const uint32_t r_begin = min(lane * per, a.requests), r_end = min(r_begin + per, a.requests);
+    Request own{0, 0, 0};  // with one request a lane
+    uint32_t mine = 0;
+    for (uint32_t i = r_begin; i < r_end; ++i) {
+        own = load_request(a, i);
+        mine += tiles_of(a, own) * (spans_of(a, own) + kExtra);
     }
     mine *= heads;
-    uint64_t before = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = __shfl_up(before, d);
-        if (lane >= static_cast<uint32_t>(d)) before += o;
-    }
-    if (lane == 63) sums[wave] = before;
-    __syncthreads();
-    uint64_t total = 0;
-    before -= mine;
-    for (uint32_t w = 0; w < kWaves; ++w) {
-        if (w < wave) before += sums[w];
-        total += sums[w];
-    }
+    const uint32_t up_to = wave_prefix(mine), total = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(up_to), 63));
     // no share is empty but those behind the last: a split tile's lie side by side
-    const uint64_t shares = min(total, static_cast<uint64_t>(gridDim.x)), share = min(static_cast<uint64_t>(blockIdx.x), shares);
-    const uint64_t begin = shares ? total * share / shares : 0, end = share < shares ? total * (share + 1) / shares : begin;
-    if (begin < end && begin >= before && begin < before + mine) {
-        uint64_t base = before;
-        for (uint32_t r = r_begin; r < r_end; ++r) {
-            const Request q = load_request(a, r);
-            const uint64_t n = tiles_of(a, q) * spans_of(a, q) * heads;
-            if (begin < base + n) {
-                found = r;
-                found_base = base;
-                break;
-            }
-            base += n;
-        }
-    }
-    __syncthreads();
-    if (begin >= end) {
-        if (tid == 0) a.splits[blockIdx.x].parts = 0;
+    const uint32_t shares = min(total, gridDim.x), share = blockIdx.x;
+    if (share >= shares) {
+        if (tid == 0) a.splits[share].parts = 0;
         return;
     }
-    uint32_t r = __builtin_amdgcn_readfirstlane(found);
-    uint64_t base = found_base;
-    Request rq = load_request(a, r);
+    // the first `more` shares have `even` + 1 units, the others `even`
+    const uint32_t even = total / shares, more = total - even * shares;
+    const uint32_t begin = share * even + min(share, more), end = begin + even + (share < more ? 1 : 0);
+    const auto share_of = [&](uint32_t x) {
+        const uint32_t longer = more * (even + 1);
+        return x < longer ? x / (even + 1) : more + (x - longer) / even;
+    };
+    const auto request = [&](uint32_t i) {
+        if (per > 1) return load_request(a, i);
+        const int at = static_cast<int>(i);
+        return Request{__builtin_amdgcn_readlane(own.length, at), __builtin_amdgcn_readlane(own.first, at),
+                       __builtin_amdgcn_readlane(own.count, at)};
+    };
+    const uint64_t behind = __ballot(begin < up_to);
+    const uint32_t in_lane = behind ? static_cast<uint32_t>(__builtin_ctzll(behind)) : 0u;
+    uint32_t r = in_lane * per, base = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(up_to - mine), static_cast<int>(in_lane)));
+    Request rq = request(r);
     bool says = false;  // this workgroup has written its split
 
     Rows<NB, P> rows;
-    for (uint64_t x = begin; x < end;) {
-        const uint32_t spans = spans_of(a, rq);
-        const uint64_t n = tiles_of(a, rq) * spans * heads;
+    for (uint32_t x = begin; x < end;) {
+        const uint32_t spans = spans_of(a, rq), units = spans + kExtra, tiles = tiles_of(a, rq);
+        const uint32_t n = tiles * units * heads;
         if (x >= base + n) {
+            if (++r >= a.requests) break;  // starts that overlap
             base += n;
-            rq = load_request(a, ++r);
+            rq = request(r);
             continue;
         }
-        const uint64_t tile = (x - base) / spans;
-        const uint32_t j0 = static_cast<uint32_t>((x - base) - tile * spans);
-        const uint32_t j1 = static_cast<uint32_t>(min(static_cast<uint64_t>(spans), j0 + (end - x)));
-        const uint64_t tiles = tiles_of(a, rq);
-        const uint32_t h = static_cast<uint32_t>(tile / tiles), row0 = static_cast<uint32_t>(tile - h * tiles) * kTileRows;
+        const uint32_t tile = (x - base) / units, u0 = (x - base) - tile * units, u1 = min(units, u0 + (end - x));
+        const uint32_t h = tile / tiles, row0 = (tile - h * tiles) * kTileRows;
         const uint32_t count = min(kTileRows, static_cast<uint32_t>(rq.count) * a.group - row0);
-        x += j1 - j0;
+        x += u1 - u0;
+        // the units ahead of the keys come first
+        const uint32_t j0 = max(u0, kExtra) - kExtra, j1 = max(u1, kExtra) - kExtra;
+        if (j1 <= j0) continue;
 
         // what the tile's queries see
         const int32_t qa = static_cast<int32_t>(row0 / a.group), qb = static_cast<int32_t>((row0 + count - 1) / a.group);
@@ -320,10 +310,9 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void kv4_attention_kerne
         const int32_t mine_q = static_cast<int32_t>((row0 + min(lane & 15, count - 1)) / a.group);
         const int32_t lim = lim_of(mine_q), low = low_of(mine_q);
         const uint32_t t0 = first_key(a, rq);
-        const int32_t from = max(static_cast<int32_t>(t0 + j0 * kSpan), any_low & ~static_cast<int32_t>(kStep - 1));
-        const int32_t to = min(static_cast<int32_t>(min(static_cast<uint64_t>(t0) + static_cast<uint64_t>(j1) * kSpan, 0x7FFFFFFFull)), any_lim);
+        const int32_t from = max(static_cast<int32_t>(t0 + j0 * a.span), any_low & ~static_cast<int32_t>(kStep - 1));
+        const int32_t to = min(static_cast<int32_t>(min(t0 + static_cast<uint64_t>(j1) * a.span, static_cast<uint64_t>(0x7FFFFFFF))), any_lim);
 
-        rows.begin(a, rq, h, row0, count, lane);
         const int32_t t_first = from + static_cast<int32_t>(wave * kStep);
         const int32_t *entries = a.table + static_cast<uint64_t>(r) * a.width;
         const uint32_t last_entry = static_cast<uint32_t>(max(rq.length - 1, 0)) >> a.cache.shift;
@@ -344,10 +333,11 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void kv4_attention_kerne
             else
                 rows.template step<true>(a, tile_, static_cast<uint32_t>(t), lane, lim, low, any_lim, any_low, qa != qb);
         };
+        Tile<NB> one, two;
+        if (t_first < to) load(one, t_first, 0);
+        rows.begin(a, rq, h, row0, count, lane);  // while the first keys are on their way
         if (t_first < to) {
-            Tile<NB> one, two;
             uint32_t it = 0;
-            load(one, t_first, it);
             for (int32_t t = t_first; t < to; t += 2 * static_cast<int32_t>(kSpan)) {
                 const int32_t second = t + static_cast<int32_t>(kSpan), third = second + static_cast<int32_t>(kSpan);
                 if (second < to) load(two, second, it + 1);
@@ -410,10 +400,9 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void kv4_attention_kerne
         if (j0 == 0 && j1 < spans) {
             says = true;
             if (tid == 0) {
-                // the share that holds the tile's last span
-                const uint64_t last = base + (tile + 1) * spans - 1;
-                const uint32_t last_share = static_cast<uint32_t>(((last + 1) * shares - 1) / total), b = blockIdx.x;
-                a.splits[b] = {last_share - b + 1, 2 * b + 1, 2 * b + 2, 2, h, row0, count, static_cast<uint32_t>(rq.first)};
+                // up to the share that holds the tile's last unit
+                const uint32_t parts = share_of(base + (tile + 1) * units - 1) - share + 1;
+                a.splits[share] = {parts, 2 * share + 1, 2 * share + 2, 2, h, row0, count, static_cast<uint32_t>(rq.first)};
             }
         }
         __syncthreads();  // LDS is free again
@@ -465,6 +454,7 @@ constexpr uint32_t kFewRows = 64;
 
 struct Plan {
     uint32_t few;               // AttentionArgs' own
+    uint32_t span = kSpan;      // AttentionArgs' own
     uint32_t groups = 0;        // of the kernel of few queries
     uint64_t tiles = 0;         // of the prompts' kernel
     uint32_t each = 1;
@@ -487,8 +477,11 @@ Plan plan_of(const Kv4Cache &c, uint32_t width, uint32_t requests, uint64_t toke
     p.few = prompts ? (requests == 1 ? 0 : kFewRows) : 0xFFFFFFFFu;
     uint64_t parts = 0;
     if (p.few > 0) {  // no more tiles and spans than these
-        const uint64_t tiles = (rows / kTileRows + some) * c.heads, spans = ceil_div(keys, kSpan) + 1;
-        p.groups = static_cast<uint32_t>(std::min<uint64_t>(2ull * cu_count(), tiles * spans));
+        const uint64_t tiles = (rows / kTileRows + some) * c.heads;
+        uint64_t units = ceil_div(keys, p.span) + 1 + kExtra;
+        for (; tiles * units >= 1ull << 31 && p.span < 1u << 30; units = ceil_div(keys, p.span) + 1 + kExtra) p.span *= 2;
+        BSQ_REQUIRE(tiles * units < 1ull << 31, "kv4 attention: too many queries");
+        p.groups = static_cast<uint32_t>(std::min<uint64_t>(2ull * cu_count(), tiles * units));
         p.splits = p.groups;
         parts = static_cast<uint64_t>(p.groups) * 2 * kTileRows;
     }
@@ -576,6 +569,7 @@ int bsq_kv4_attention(const bsq_kv4_cache_t *cache, const int32_t *d_table, uint
         a.parts = static_cast<float *>(d_work);
         a.splits = reinterpret_cast<Split *>(static_cast<uint8_t *>(d_work) + p.parts_bytes);
         a.few = p.few;
+        a.span = p.span;
         a.each = p.each;
         hipStream_t s = static_cast<hipStream_t>(stream);
         const uint64_t rows = static_cast<uint64_t>(a.most) * a.group;
