@@ -42,7 +42,7 @@ struct AttentionArgs {
     float *parts;
     struct Split *splits;
     uint32_t few;   // requests of up to so many rows are the one kernel's, others the prompts'
-    uint32_t span;  // few queries: keys of a unit of work
+    uint32_t span;  // few queries: a unit of work is 1 << span keys
     uint32_t each;  // prompts: workgroups that share a tile's keys
 };
 
