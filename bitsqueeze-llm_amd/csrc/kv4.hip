@@ -11,11 +11,13 @@ namespace {
 // ---------------------------------------------------------------------------
 // the plan of a step
 // ---------------------------------------------------------------------------
-// Everything hangs on two prefix sums over the requests: of the pages that the
-// ended ones give back, and of the tokens and pages that the others take.  One
-// workgroup forms them, 1024 requests at a time; the places of the tokens then
+// Everything hangs on prefix sums over the requests: of the pages that the ended
+// ones give back, and of the tokens and pages that the others take.  One workgroup
+// forms them all at once, a run of requests a thread; the places of the tokens then
 // need only a search in the starts.  Small steps do both in the one launch, as a
 // second costs more than the search; large ones spread the places over a grid.
+// What bounds it are waits one after another: lengths, the sums' exchange between
+// waves, the ended requests' rows, the pages of new tokens.
 constexpr uint32_t kPlanThreads = 1024;
 constexpr uint32_t kPlanMostRequests = 16384;
 constexpr uint32_t kPlanOneLaunch = 4096;  // places
@@ -34,24 +36,36 @@ struct PlanArgs {
     int32_t *first;  // requests + 1: the first page of each from the stack's top, -1 if not served; the top
 };
 
-// The sum over the threads up to this one, and of all.
-__device__ uint64_t group_prefix(uint64_t v, uint64_t *sums, uint64_t &all) {
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+// Three sums over the threads before this one, and over all.
+struct PlanSums {
+    uint64_t v[3];
+};
+__device__ __forceinline__ PlanSums plan_prefix(const PlanSums mine, PlanSums *of_waves, PlanSums &all) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    PlanSums up = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = __shfl_up(v, d);
-        if (lane >= static_cast<uint32_t>(d)) v += o;
+        PlanSums o;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) o.v[i] = __shfl_up(up.v[i], d);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) up.v[i] += lane >= static_cast<uint32_t>(d) ? o.v[i] : 0;
     }
-    __syncthreads();  // the last call's sums have been read
-    if (lane == 63) sums[wave] = v;
+    if (lane == 63) of_waves[wave] = up;
     __syncthreads();
-    uint64_t before = 0;
-    all = 0;
-    for (uint32_t w = 0; w < waves; ++w) {
-        if (w == wave) before = all;
-        all += sums[w];
+    all = {};
+#pragma unroll
+    for (uint32_t w = 0; w < kPlanThreads / 64; ++w) {
+        const PlanSums s = of_waves[w];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            up.v[i] += w < wave ? s.v[i] : 0;
+            all.v[i] += s.v[i];
+        }
     }
-    return before + v;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) up.v[i] -= mine.v[i];
+    return up;
 }
 
 struct PlanRequest {
@@ -113,68 +127,90 @@ __device__ __forceinline__ void plan_place(const PlanArgs &a, uint32_t t, const 
 // ALL: the places too.
 template <bool ALL>
 __global__ __launch_bounds__(kPlanThreads) void kv4_plan_kernel(PlanArgs a) {
-    __shared__ uint64_t sums[kPlanThreads / 64];
-    __shared__ uint32_t before[kPlanThreads + 1];
+    struct Ended {
+        uint32_t request, before, pages;
+    };
+    __shared__ PlanSums of_waves[kPlanThreads / 64];
+    __shared__ Ended ended[kPlanThreads];
     __shared__ int32_t starts[ALL ? kPlanThreads + 1 : 1];
+    __shared__ uint32_t taken[kPlanThreads / 64], unserved[kPlanThreads / 64];
     const uint32_t tid = threadIdx.x;
     const uint32_t count = min(static_cast<uint32_t>(max(*a.count, 0)), a.pages);
-    uint64_t freed = 0;
-    for (uint32_t r0 = 0; r0 < a.requests; r0 += kPlanThreads) {
-        const uint32_t r = r0 + tid;
-        uint32_t gives = 0;
-        if (r < a.requests && a.more[r] < 0) gives = plan_request(a, r).held;
-        uint64_t all;
-        const uint64_t last = group_prefix(gives, sums, all);
-        if (all == 0) continue;
-        before[tid] = static_cast<uint32_t>(last - gives);
-        __syncthreads();
-        for (uint64_t z = tid; z < all && count + freed + z < a.pages; z += kPlanThreads) {
-            uint32_t lo = 0, hi = kPlanThreads;
-            while (hi - lo > 1) {
-                const uint32_t mid = (lo + hi) >> 1;
-                if (before[mid] <= z) lo = mid;
-                else hi = mid;
-            }
-            a.free[count + freed + z] = a.table[static_cast<uint64_t>(r0 + lo) * a.width + (z - before[lo])];
-        }
-        freed += all;
-        __syncthreads();
+    const uint32_t per = (a.requests + kPlanThreads - 1) / kPlanThreads;
+    const uint32_t r_begin = min(tid * per, a.requests), r_end = min(r_begin + per, a.requests);
+    PlanSums mine{};
+    for (uint32_t r = r_begin; r < r_end; ++r) {
+        const PlanRequest q = plan_request(a, r);
+        mine.v[0] += q.ended ? (1ull << 40) + q.held : 0;  // requests above, pages below
+        mine.v[1] += static_cast<uint64_t>(q.more);
+        mine.v[2] += q.need;
     }
-    const uint32_t top = static_cast<uint32_t>(min(static_cast<uint64_t>(count) + freed, static_cast<uint64_t>(a.pages)));
-
-    uint64_t tokens = 0, pages = 0, taken = 0, unserved = 0;
-    for (uint32_t r0 = 0; r0 < a.requests; r0 += kPlanThreads) {
-        const uint32_t r = r0 + tid;
-        PlanRequest q{0, 0, 0, 0, true, false};
-        if (r < a.requests) q = plan_request(a, r);
-        uint64_t all_tokens, all_pages, all;
-        const uint64_t end = tokens + group_prefix(static_cast<uint64_t>(q.more), sums, all_tokens);
-        const uint64_t last = pages + group_prefix(q.need, sums, all_pages);
-        const bool fits = !q.wide && end <= a.tokens && (q.need == 0 || last <= top);
-        // both counts in one sum
-        group_prefix(q.ended ? 0 : fits ? q.need : 1ull << 40, sums, all);
-        if (r < a.requests) {
-            const int32_t start = static_cast<int32_t>(min(end, static_cast<uint64_t>(a.tokens)));
+    PlanSums all;
+    PlanSums before = plan_prefix(mine, of_waves, all);
+    constexpr uint64_t kLow = (1ull << 40) - 1;
+    const uint32_t top = static_cast<uint32_t>(min(count + (all.v[0] & kLow), static_cast<uint64_t>(a.pages)));
+    const uint32_t ends = static_cast<uint32_t>(all.v[0] >> 40);
+    uint32_t most = 0, left_out = 0;
+    {
+        PlanSums at = before;
+        for (uint32_t r = r_begin; r < r_end; ++r) {
+            const PlanRequest q = plan_request(a, r);
+            at.v[1] += static_cast<uint64_t>(q.more);
+            at.v[2] += q.need;
+            const bool fits = !q.wide && at.v[1] <= a.tokens && (q.need == 0 || at.v[2] <= top);
+            const int32_t start = static_cast<int32_t>(min(at.v[1], static_cast<uint64_t>(a.tokens)));
             a.starts[r + 1] = start;
             if (ALL) starts[r + 1] = start;
+            a.first[r] = q.ended || !fits ? -1 : q.need == 0 ? 0 : static_cast<int32_t>(at.v[2] - q.need);
             a.lengths_out[r] = q.ended ? 0 : static_cast<int32_t>(fits ? q.past + q.more : q.past);
-            a.first[r] = q.ended || !fits ? -1 : q.need == 0 ? 0 : static_cast<int32_t>(last - q.need);
+            // the pages that are taken end with the last request that is served
+            if (!q.ended && fits && q.need > 0) most = static_cast<uint32_t>(at.v[2]);
+            if (!q.ended && !fits) ++left_out;
+            // more of them than the list holds: a thread each below
+            if (q.ended) {
+                const uint64_t n = at.v[0] >> 40;
+                const Ended e{r, static_cast<uint32_t>(at.v[0] & kLow), q.held};
+                if (ends <= kPlanThreads) {
+                    ended[n] = e;
+                } else {
+                    for (uint32_t i = 0; i < e.pages && count + static_cast<uint64_t>(e.before) + i < a.pages; ++i)
+                        a.free[count + e.before + i] = a.table[static_cast<uint64_t>(r) * a.width + i];
+                }
+                at.v[0] += (1ull << 40) + q.held;
+            }
         }
-        tokens += all_tokens;
-        pages += all_pages;
-        taken += all & ((1ull << 40) - 1);
-        unserved += all >> 40;
     }
+    // what of the stack is taken, and how many requests are not served
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), d)));
+        left_out += static_cast<uint32_t>(__shfl_xor(static_cast<int>(left_out), d));
+    }
+    if ((tid & 63) == 0) taken[tid >> 6] = most, unserved[tid >> 6] = left_out;
+    __syncthreads();
+    // the ended requests' pages, a wave a request
+    if (ends <= kPlanThreads)
+        for (uint32_t e = tid >> 6; e < ends; e += kPlanThreads / 64) {
+            const Ended of = ended[e];
+            const int32_t *from = a.table + static_cast<uint64_t>(of.request) * a.width;
+            const uint64_t to = static_cast<uint64_t>(count) + of.before;
+#pragma unroll 8
+            for (uint32_t i = tid & 63; i < of.pages; i += 64)
+                if (to + i < a.pages) a.free[to + i] = from[i];
+        }
     if (tid == 0) {
+        uint32_t all_taken = 0, all_unserved = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kPlanThreads / 64; ++w) all_taken = max(all_taken, taken[w]), all_unserved += unserved[w];
         a.starts[0] = 0;
         if (ALL) starts[0] = 0;
         a.first[a.requests] = static_cast<int32_t>(top);
-        a.left[0] = static_cast<int32_t>(top - taken);
-        a.left[1] = static_cast<int32_t>(unserved);
+        a.left[0] = static_cast<int32_t>(top - all_taken);
+        a.left[1] = static_cast<int32_t>(all_unserved);
     }
     if constexpr (ALL) {
         __syncthreads();
-        const int32_t total = static_cast<int32_t>(min(tokens, static_cast<uint64_t>(a.tokens)));
+        const int32_t total = static_cast<int32_t>(min(all.v[1], static_cast<uint64_t>(a.tokens)));
         for (uint32_t t = tid; t < a.tokens; t += kPlanThreads) plan_place(a, t, starts, total, top);
     }
 }
@@ -195,10 +231,12 @@ __global__ __launch_bounds__(kPlaceThreads) void kv4_places_kernel(PlanArgs a) {
 // ---------------------------------------------------------------------------
 // Angles grow with the position: at 10^6 radians FP32 is off by 0.06.  They are
 // FP64 products, brought into [-pi/4, pi/4] with pi/2 in two parts, and sine and
-// cosine their Taylor sums there (remainders below 2^-60).  FP64 runs at FP32's
-// rate on this card, a token's sines serve all its heads, and the pairs' products
-// in FP64 leave one rounding: a key next to a border of its 4-bit codes falls on
-// the side that the exact value is on.
+// cosine their Taylor sums there (remainders below 2^-60); a token's serve all its
+// heads.  A pair's products are FP64 for FP32 values, and for keys on their way into
+// the cache: next to a border of its 4-bit codes a key falls on the side that the
+// exact value is on.  Of 16-bit values they are FP32, a small part of the rounding
+// that follows: 8192 tokens of 32 heads of 128, half of it turned, forward and
+// gradient, take 57 us so, and 66 in FP64, whose conversions are slow.
 __device__ __forceinline__ void sine_cosine(double t, double &s, double &c) {
     const double n = rint(t * 0.63661977236758134308);
     double r = fma(-n, 1.57079632679489655800, t);
@@ -228,6 +266,21 @@ __device__ __forceinline__ void sine_cosine(double t, double &s, double &c) {
     if (quarter == 1 || quarter == 2) c = -c;
 }
 
+// i / d and the rest for i, d < 2^24, from 1 / d in FP32: at most one off, which is
+// put right.  The compiler's division takes some 40 instructions.
+struct Divisor {
+    uint32_t d = 1;
+    float inverse = 1.0f;
+    Divisor() = default;
+    explicit Divisor(uint32_t divisor) : d(divisor), inverse(1.0f / static_cast<float>(divisor)) {}
+    __device__ __forceinline__ void operator()(uint32_t i, uint32_t &q, uint32_t &r) const {
+        q = static_cast<uint32_t>(static_cast<float>(i) * inverse);
+        r = i - q * d;
+        if (static_cast<int32_t>(r) < 0) r += d, --q;
+        else if (r >= d) r -= d, ++q;
+    }
+};
+
 struct Turn {
     const double *frequencies = nullptr;  // none: nothing turns
     uint32_t half = 0;                    // pairs
@@ -244,36 +297,76 @@ struct RowsArgs {
     uint8_t *qo;
     uint64_t ldq, ldqo, ldk, ldv;
     uint32_t q_heads;
+    uint32_t chunks, rest;  // eights of pairs in a head, and of values that do not turn
     bool in_place;
     Kv4Cache cache;
+    Divisor by_half, by_q_heads, by_chunks, by_rest, by_heads, by_key_eights, by_eights;
 };
 
 constexpr uint32_t kRowThreads = 256;
-constexpr uint32_t kRowTokens = 8;          // most of a workgroup
+constexpr uint32_t kRowTokens = 4;          // most of a workgroup
 constexpr uint32_t kRowPairs = kKv4MaxDim / 2;
 constexpr uint32_t kKeyBytes = 16384;       // turned keys held at once
 
-// Eight pairs of a row: chunk c of the turning part, and then eights of the rest.
+// Eight pairs of a row, chunk c of the turning part; or eight values of the rest.
 template <Mx4Type T>
 struct Pairs {
+    static constexpr int kWords = Eight<T>::kWords;
     float a[8], b[8];
-    __device__ __forceinline__ void load(const uint8_t *row, const Turn &t, uint32_t c) {
-        const uint32_t at = 8 * c, left = t.half - at;
+    // as stored: loaded ahead of their use
+    struct Words {
+        Eight<T> a, b;
+    };
+    __device__ __forceinline__ static void load(Words &w, const uint8_t *row, const Turn &t, uint32_t c) {
         if (t.interleaved) {
-            load8<T>(row, 2 * at, 2 * left, a);
-            load8<T>(row, 2 * at + 8, left > 4 ? 2 * left - 8 : 0, b);
+            w.a.load(row, 16 * c, 2 * t.half);
+            w.b.load(row, 16 * c + 8, 2 * t.half);
         } else {
-            load8<T>(row, at, left, a);
-            load8<T>(row, t.half + at, left, b);
+            w.a.load(row, 8 * c, t.half);
+            w.b.load(row + t.half * (T == Mx4Type::F32 ? 4 : 2), 8 * c, t.half);
         }
+    }
+    __device__ __forceinline__ static void values(const Eight<T> &e, float v[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (T == Mx4Type::F32) {
+                v[i] = __uint_as_float(e.w[i]);
+            } else {
+                const uint32_t x = (e.w[i / 2] >> (16 * (i & 1))) & 0xFFFFu;
+                v[i] = T == Mx4Type::BF16 ? bf16_value(x) : f16_value(x);
+            }
+        }
+    }
+    // values [at, at + 8) of a row of n, as they are
+    __device__ __forceinline__ static void move(const Eight<T> &e, uint8_t *row, uint32_t at, uint32_t n) {
+        if (at + 8 <= n) {
+            __builtin_memcpy(row + at * (T == Mx4Type::F32 ? 4 : 2), e.w, sizeof(e.w));
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                if (at + i >= n) continue;
+                if constexpr (T == Mx4Type::F32) reinterpret_cast<uint32_t *>(row)[at + i] = e.w[i];
+                else reinterpret_cast<uint16_t *>(row)[at + i] = static_cast<uint16_t>(e.w[i / 2] >> (16 * (i & 1)));
+            }
+        }
+    }
+    __device__ __forceinline__ explicit Pairs(const Words &w) {
+        values(w.a, a);
+        values(w.b, b);
     }
     __device__ __forceinline__ static void turn_one(float &x, float &y, const double2 u) {
         const double p = x, q = y;
-        x = static_cast<float>(p * u.x - q * u.y);
-        y = static_cast<float>(q * u.x + p * u.y);
+        x = static_cast<float>(fma(p, u.x, -(q * u.y)));
+        y = static_cast<float>(fma(q, u.x, p * u.y));
+    }
+    __device__ __forceinline__ static void turn_one(float &x, float &y, const float2 u) {
+        const float p = x, q = y;
+        x = fmaf(p, u.x, -(q * u.y));
+        y = fmaf(q, u.x, p * u.y);
     }
     // cs: cosine and sine of pair i at cs[i * step]
-    __device__ __forceinline__ void turn(const Turn &t, const double2 *cs, uint32_t step) {
+    template <class Two>
+    __device__ __forceinline__ void turn(const Turn &t, const Two *cs, uint32_t step) {
         if (t.interleaved) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) turn_one(a[2 * i], a[2 * i + 1], cs[i * step]);
@@ -297,10 +390,7 @@ struct Pairs {
 };
 
 template <Mx4Type T>
-__device__ __forceinline__ void pack_row(const RowsArgs &a, const uint8_t *row, uint32_t which, uint32_t slot, uint32_t h,
-                                         uint32_t c) {
-    Eight<T> v;
-    v.load(row, 8 * c, a.dim);
+__device__ __forceinline__ void pack(const RowsArgs &a, const Eight<T> &v, uint32_t which, uint32_t slot, uint32_t h, uint32_t c) {
     const uint32_t byte = mx4_scale_byte(f32_bits<T>(quad_max(v.top())));
     if (slot >> a.cache.shift >= a.cache.count) return;
     uint8_t *to = a.cache.head(slot >> a.cache.shift, h);
@@ -312,86 +402,149 @@ __device__ __forceinline__ void pack_row(const RowsArgs &a, const uint8_t *row, 
 
 // A workgroup takes `per` tokens and of them the queries (blockIdx.y 0) or the
 // keys and values (1).  Sines and cosines go through LDS, once a token; turned
-// keys too, in their own type, since a pair's halves belong to two blocks.
-// ROPE alone: queries only.
+// keys too, in their own type, since a pair's halves belong to two blocks.  A
+// thread's words are on their way while sines are computed, and then one item
+// ahead.  !KV: queries only.
 template <Mx4Type T, bool KV>
 __global__ __launch_bounds__(kRowThreads) void kv4_rows_kernel(RowsArgs a) {
     constexpr uint32_t size = T == Mx4Type::F32 ? 4 : 2;
+    using P = Pairs<T>;
     __shared__ double2 cs[kRowTokens * kRowPairs];
+    float2 *cs32 = reinterpret_cast<float2 *>(cs);
+    constexpr bool kWide = T == Mx4Type::F32;
     __shared__ __attribute__((aligned(16))) uint8_t turned[KV ? kKeyBytes : 16];
     const uint32_t tid = threadIdx.x;
     const uint64_t t0 = static_cast<uint64_t>(blockIdx.x) * a.per;
     const uint32_t here = static_cast<uint32_t>(min(static_cast<uint64_t>(a.per), a.tokens - t0));
     const Turn &turn = a.turn;
-    const uint32_t chunks = (turn.half + 7) >> 3;
-    if (turn.frequencies != nullptr) {
+    const uint32_t chunks = a.chunks;
+    const auto absent = [&](uint32_t t) { return a.positions != nullptr && a.positions[t0 + t] < 0; };
+    const auto sines = [&](auto wide) {
+        if (turn.frequencies == nullptr) return;
         for (uint32_t i = tid; i < here * turn.half; i += kRowThreads) {
-            const uint32_t t = i / turn.half, j = i - t * turn.half;
+            uint32_t t, j;
+            a.by_half(i, t, j);
             double s, c;
             sine_cosine(static_cast<double>(a.positions[t0 + t]) * turn.frequencies[j], s, c);
-            cs[(t * 8 + (j & 7)) * chunks + (j >> 3)] = {c * turn.cosine, s * turn.sine};
+            c *= turn.cosine, s *= turn.sine;
+            const uint32_t to = (t * 8 + (j & 7)) * chunks + (j >> 3);
+            if constexpr (decltype(wide)::value) cs[to] = {c, s};
+            else cs32[to] = {static_cast<float>(c), static_cast<float>(s)};
         }
         __syncthreads();
-    }
-    const auto absent = [&](uint64_t t) { return a.positions != nullptr && a.positions[t] < 0; };
+    };
     if (!KV || blockIdx.y == 0) {
         if (a.q == nullptr) return;
-        const uint32_t rest = a.in_place ? 0 : (a.dim - 2 * turn.half + 7) >> 3, each = chunks + rest;
-        for (uint32_t i = tid; i < here * a.q_heads * each; i += kRowThreads) {
-            const uint32_t row = i / each, c = i - row * each, t = row / a.q_heads, h = row - t * a.q_heads;
-            if (absent(t0 + t)) continue;
-            const uint8_t *from = a.q + ((t0 + t) * a.ldq + static_cast<uint64_t>(h) * a.dim) * size;
-            uint8_t *to = a.qo + ((t0 + t) * a.ldqo + static_cast<uint64_t>(h) * a.dim) * size;
-            if (c < chunks) {
-                Pairs<T> p;
-                p.load(from, turn, c);
-                p.turn(turn, cs + t * 8 * chunks + c, chunks);
-                p.store(to, turn, c);
+        // what turns comes first, what is only moved behind it: waves do the one or the
+        // other
+        const uint32_t turning = here * a.q_heads * chunks, all = turning + (a.in_place ? 0u : here * a.q_heads * a.rest);
+        struct Item {
+            uint32_t t, h, c;
+        };
+        const auto item_of = [&](uint32_t i) {
+            Item n;
+            uint32_t row;
+            if (i < turning) a.by_chunks(i, row, n.c);
+            else a.by_rest(i - turning, row, n.c);
+            a.by_q_heads(row, n.t, n.h);
+            return n;
+        };
+        const auto load = [&](typename P::Words &w, uint32_t i, const Item &n) {
+            const uint8_t *from = a.q + ((t0 + n.t) * a.ldq + static_cast<uint64_t>(n.h) * a.dim) * size;
+            if (i < turning) P::load(w, from, turn, n.c);
+            else w.a.load(from, 2 * turn.half + 8 * n.c, a.dim);
+        };
+        typename P::Words next;
+        Item then{0, 0, 0};
+        if (tid < all) load(next, tid, then = item_of(tid));
+        sines(std::bool_constant<kWide>{});
+        for (uint32_t i = tid; i < all; i += kRowThreads) {
+            const typename P::Words now = next;
+            const Item n = then;
+            if (i + kRowThreads < all) load(next, i + kRowThreads, then = item_of(i + kRowThreads));
+            if (absent(n.t)) continue;
+            uint8_t *to = a.qo + ((t0 + n.t) * a.ldqo + static_cast<uint64_t>(n.h) * a.dim) * size;
+            if (i < turning) {
+                P p(now);
+                if constexpr (kWide) p.turn(turn, cs + n.t * 8 * chunks + n.c, chunks);
+                else p.turn(turn, cs32 + n.t * 8 * chunks + n.c, chunks);
+                p.store(to, turn, n.c);
             } else {
-                const uint32_t at = 2 * turn.half + 8 * (c - chunks);
-                float v[8];
-                load8<T>(from, at, a.dim - at, v);
-                store8<T>(to, at, a.dim - at, v);
+                P::move(now.a, to, 2 * turn.half + 8 * n.c, a.dim);
             }
         }
         return;
     }
     if constexpr (KV) {
         const uint32_t eights = a.cache.blocks * 4, heads = a.cache.heads, rows = here * heads;
-        const auto slot_of = [&](uint64_t t) { return absent(t) ? 0xFFFFFFFFu : static_cast<uint32_t>(a.slots[t]); };
-        // a quad of lanes never parts: `eights` is a multiple of four
-        for (uint32_t i = tid; i < rows * eights; i += kRowThreads) {
-            const uint32_t row = i / eights, c = i - row * eights, t = row / heads, h = row - t * heads;
-            const uint32_t slot = slot_of(t0 + t);
-            pack_row<T>(a, a.v + ((t0 + t) * a.ldv + static_cast<uint64_t>(h) * a.dim) * size, 1, slot, h, c);
-            if (turn.frequencies == nullptr)
-                pack_row<T>(a, a.k + ((t0 + t) * a.ldk + static_cast<uint64_t>(h) * a.dim) * size, 0, slot, h, c);
+        const auto slot_of = [&](uint32_t t) { return absent(t) ? 0xFFFFFFFFu : static_cast<uint32_t>(a.slots[t0 + t]); };
+        const uint32_t stride = a.cache.blocks * 32 * size + 16, most = kKeyBytes / stride, each = chunks + a.rest;
+        const auto load_key = [&](typename P::Words &w, uint32_t r0, uint32_t i) {
+            uint32_t n, c, t, h;
+            a.by_key_eights(i, n, c);
+            a.by_heads(r0 + n, t, h);
+            const uint8_t *from = a.k + ((t0 + t) * a.ldk + static_cast<uint64_t>(h) * a.dim) * size;
+            if (c < chunks) P::load(w, from, turn, c);
+            else w.a.load(from, 2 * turn.half + 8 * (c - chunks), a.dim);
+        };
+        const bool turns = turn.frequencies != nullptr;
+        typename P::Words next;
+        if (turns && tid < min(most, rows) * each) load_key(next, 0, tid);
+        // values; a quad of lanes never parts: `eights` is a multiple of four
+        Eight<T> word;
+        const auto value_at = [&](uint32_t i, uint32_t &t, uint32_t &h, uint32_t &c) {
+            uint32_t row;
+            a.by_eights(i, row, c);
+            a.by_heads(row, t, h);
+        };
+        const auto load_value = [&](const uint8_t *base, uint64_t ld, uint32_t i) {
+            uint32_t t, h, c;
+            value_at(i, t, h, c);
+            word.load(base + ((t0 + t) * ld + static_cast<uint64_t>(h) * a.dim) * size, 8 * c, a.dim);
+        };
+        const auto pack_rows = [&](const uint8_t *base, uint64_t ld, uint32_t which) {
+            for (uint32_t i = tid; i < rows * eights; i += kRowThreads) {
+                const Eight<T> now = word;
+                if (i + kRowThreads < rows * eights) load_value(base, ld, i + kRowThreads);
+                uint32_t t, h, c;
+                value_at(i, t, h, c);
+                pack<T>(a, now, which, slot_of(t), h, c);
+            }
+        };
+        if (tid < rows * eights) load_value(a.v, a.ldv, tid);
+        sines(std::true_type{});
+        pack_rows(a.v, a.ldv, 1);
+        if (!turns) {
+            if (tid < rows * eights) load_value(a.k, a.ldk, tid);
+            pack_rows(a.k, a.ldk, 0);
+            return;
         }
-        if (turn.frequencies == nullptr) return;
-        const uint32_t stride = a.cache.blocks * 32 * size + 16, most = kKeyBytes / stride;
-        const uint32_t each = chunks + ((a.dim - 2 * turn.half + 7) >> 3);
         for (uint32_t r0 = 0; r0 < rows; r0 += most) {
             const uint32_t count = min(most, rows - r0);
+            if (r0 > 0 && tid < count * each) load_key(next, r0, tid);
             for (uint32_t i = tid; i < count * each; i += kRowThreads) {
-                const uint32_t n = i / each, c = i - n * each, row = r0 + n, t = row / heads, h = row - t * heads;
-                const uint8_t *from = a.k + ((t0 + t) * a.ldk + static_cast<uint64_t>(h) * a.dim) * size;
+                const typename P::Words now = next;
+                if (i + kRowThreads < count * each) load_key(next, r0, i + kRowThreads);
+                uint32_t n, c, t, h;
+                a.by_key_eights(i, n, c);
+                a.by_heads(r0 + n, t, h);
                 uint8_t *to = turned + n * stride;
                 if (c < chunks) {
-                    Pairs<T> p;
-                    p.load(from, turn, c);
+                    P p(now);
                     p.turn(turn, cs + t * 8 * chunks + c, chunks);
                     p.store(to, turn, c);
                 } else {
-                    const uint32_t at = 2 * turn.half + 8 * (c - chunks);
-                    float v[8];
-                    load8<T>(from, at, a.dim - at, v);
-                    store8<T>(to, at, a.dim - at, v);
+                    P::move(now.a, to, 2 * turn.half + 8 * (c - chunks), a.dim);
                 }
             }
             __syncthreads();
             for (uint32_t i = tid; i < count * eights; i += kRowThreads) {
-                const uint32_t n = i / eights, c = i - n * eights, row = r0 + n, t = row / heads, h = row - t * heads;
-                pack_row<T>(a, turned + n * stride, 0, slot_of(t0 + t), h, c);
+                uint32_t n, c, t, h;
+                a.by_eights(i, n, c);
+                a.by_heads(r0 + n, t, h);
+                Eight<T> v;
+                v.load(turned + n * stride, 8 * c, a.dim);
+                pack<T>(a, v, 0, slot_of(t), h, c);
             }
             __syncthreads();
         }
@@ -400,11 +553,21 @@ __global__ __launch_bounds__(kRowThreads) void kv4_rows_kernel(RowsArgs a) {
 
 void launch_rows(const RowsArgs &rows, Mx4Type type, bool kv, hipStream_t stream) {
     RowsArgs a = rows;
-    // a token's rows keep a workgroup busy from some 2048 values on; of smaller
-    // ones it takes several, where enough workgroups remain
-    const uint64_t values = static_cast<uint64_t>(std::max(a.q_heads, kv ? a.cache.heads : 0u)) * a.dim;
+    a.chunks = (a.turn.half + 7) / 8;
+    a.rest = (a.dim - 2 * a.turn.half + 7) / 8;
+    a.by_half = Divisor(std::max(a.turn.half, 1u));
+    a.by_q_heads = Divisor(std::max(a.q_heads, 1u));
+    a.by_chunks = Divisor(std::max(a.chunks, 1u));
+    a.by_rest = Divisor(std::max(a.rest, 1u));
+    a.by_key_eights = Divisor(std::max(a.chunks + a.rest, 1u));
+    a.by_heads = Divisor(std::max(kv ? a.cache.heads : 1u, 1u));
+    a.by_eights = Divisor(std::max(kv ? a.cache.blocks * 4 : 1u, 1u));
+    // several tokens a workgroup share the wait for their sines, as long as eight
+    // workgroups a CU remain
     a.per = 1;
-    while (a.per < kRowTokens && a.per * values < 2048 && a.tokens / a.per > 8ull * cu_count()) a.per *= 2;
+    while (a.per < kRowTokens && a.tokens / (2 * a.per) >= 8ull * cu_count()) a.per *= 2;
+    // items are counted in 24 bits
+    while (a.per > 1 && static_cast<uint64_t>(a.per) * std::max(a.q_heads, kv ? a.cache.heads : 0u) * kKv4MaxDim / 8 >= 1u << 24) a.per /= 2;
     const uint64_t groups = ceil_div(a.tokens, a.per);
     BSQ_REQUIRE(groups <= 0xFFFFFFFFull / (2 * kRowThreads), "kv4: too many tokens");
     by_type(type, [&](auto ty) {
@@ -415,23 +578,25 @@ void launch_rows(const RowsArgs &rows, Mx4Type type, bool kv, hipStream_t stream
     BSQ_HIP(hipGetLastError());
 }
 
-// Eight values a lane.
+// Eight values a lane; a workgroup takes `per` tokens.
 template <Mx4Type T>
-__global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Cache cache, const int32_t *slots, uint64_t tokens, uint8_t *k,
-                                                       uint64_t ldk, uint8_t *v, uint64_t ldv) {
+__global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Cache cache, const int32_t *slots, uint64_t tokens, uint32_t per,
+                                                       Divisor by_heads, Divisor by_eights, uint8_t *k, uint64_t ldk, uint8_t *v,
+                                                       uint64_t ldv) {
     constexpr uint32_t size = T == Mx4Type::F32 ? 4 : 2;
-    const uint32_t eights = (cache.dim + 7) >> 3, each = cache.heads * eights;
     const uint32_t which = k == nullptr ? 1 : blockIdx.y;
     uint8_t *out = which ? v : k;
-    const uint64_t ld = which ? ldv : ldk, all = tokens * each;
-    for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<uint64_t>(gridDim.x) * 256) {
-        const uint64_t token = i / each;
-        const uint32_t in = static_cast<uint32_t>(i - token * each), h = in / eights, c = in - h * eights;
-        const uint32_t slot = static_cast<uint32_t>(slots[token]), t = slot & (cache.page() - 1);
+    const uint64_t ld = which ? ldv : ldk, t0 = static_cast<uint64_t>(blockIdx.x) * per;
+    const uint32_t here = static_cast<uint32_t>(min(static_cast<uint64_t>(per), tokens - t0));
+    for (uint32_t i = threadIdx.x; i < here * by_heads.d * by_eights.d; i += 256) {
+        uint32_t row, c, t, h;
+        by_eights(i, row, c);
+        by_heads(row, t, h);
+        const uint32_t slot = static_cast<uint32_t>(slots[t0 + t]), in = slot & (cache.page() - 1);
         if (slot >> cache.shift >= cache.count) continue;
         const uint8_t *from = cache.head(slot >> cache.shift, h);
-        const uint32_t codes = *reinterpret_cast<const uint32_t *>(from + cache.codes_at(which, t) + 4 * c);
-        const uint32_t byte = from[cache.scale_at(which, t, c >> 2)];
+        const uint32_t codes = *reinterpret_cast<const uint32_t *>(from + cache.codes_at(which, in) + 4 * c);
+        const uint32_t byte = from[cache.scale_at(which, in, c >> 2)];
         const float scale = byte == 255u ? __builtin_nanf("") : byte == 0u ? 0x1p-127f : mx4_power(byte);
         float x[8];
 #pragma unroll
@@ -442,7 +607,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Cache cache, const int
             const float level = __uint_as_float((n & 7u) << 22) * 0x1p126f;
             x[j] = (n & 8u ? -level : level) * scale;
         }
-        store8<T>(out + (token * ld + static_cast<uint64_t>(h) * cache.dim) * size, 8 * c, cache.dim - 8 * c, x);
+        store8<T>(out + ((t0 + t) * ld + static_cast<uint64_t>(h) * cache.dim) * size, 8 * c, cache.dim - 8 * c, x);
     }
 }
 
@@ -640,11 +805,14 @@ int bsq_kv4_read(const bsq_kv4_cache_t *cache, const int32_t *d_slots, uint64_t 
         BSQ_REQUIRE(d_slots != nullptr, "kv4 read: null slots");
         if (d_k != nullptr) check_dense(d_k, t, "");
         if (d_v != nullptr) check_dense(d_v, t, "");
-        const uint64_t items = tokens * c.heads * ((c.dim + 7) / 8);
+        const uint32_t eights = (c.dim + 7) / 8, per = std::max(1u, 1024u / (c.heads * eights));
+        const uint64_t groups = ceil_div(tokens, per);
+        BSQ_REQUIRE(groups <= 0xFFFFFFFFull / 512, "kv4: too many tokens");
         by_type(t, [&](auto ty) {
-            const dim3 grid(static_cast<unsigned>(std::min<uint64_t>(ceil_div(items, 256), 1u << 20)), d_k && d_v ? 2 : 1);
+            const dim3 grid(static_cast<unsigned>(groups), d_k && d_v ? 2 : 1);
             kv4_read_kernel<decltype(ty)::value><<<grid, 256, 0, static_cast<hipStream_t>(stream)>>>(
-                c, d_slots, tokens, static_cast<uint8_t *>(d_k), ldk, static_cast<uint8_t *>(d_v), ldv);
+                c, d_slots, tokens, per, Divisor(c.heads), Divisor(eights), static_cast<uint8_t *>(d_k), ldk,
+                static_cast<uint8_t *>(d_v), ldv);
         });
         BSQ_HIP(hipGetLastError());
     });

@@ -496,8 +496,9 @@ BSQ_API int bsq_kv4_plan(const int32_t *d_lengths, const int32_t *d_new, uint32_
 /* Rotary positions: of a head's first `dims` values (even), pair i = (x[i],
  * x[i + dims / 2]), or (x[2 i], x[2 i + 1]) if `interleaved`, becomes factor
  * (a cos t - b sin t, b cos t + a sin t), t = position * d_frequencies[i]; the
- * others stay as they are.  Angles, sine, cosine and the pair's products are
- * FP64, rounded once through FP32 to the type. */
+ * others stay as they are.  Angles, sine and cosine are FP64; the pair's products
+ * are FP64 for FP32 values and for keys that go into the cache, FP32 for other
+ * 16-bit values; rounded through FP32 to the type. */
 typedef struct {
     const double *d_frequencies; /* dims / 2 */
     uint32_t dims;

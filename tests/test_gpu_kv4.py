@@ -3,9 +3,11 @@ rotary positions, append, read and attention against their definitions in 64 bit
 (_kv4ref.py).
 
 The plan's whole numbers and the cache's bytes are defined bit by bit.  Turned
-values are FP64 products rounded once through FP32: half a unit in the last place
-of each (2^-24 and the type's), and 2^-40 of the pair for angles (2^21 positions
-times FP64's 2^-53, and sine and cosine).  Attention is held to attention_bound,
+values are rounded through FP32: half a unit in the last place of each (2^-24 and
+the type's), and 2^-40 of the pair for angles (2^21 positions times FP64's 2^-53,
+and sine and cosine).  Products of FP32 values are FP64; of 16-bit ones FP32: sine
+and cosine rounded, one product rounded and a fused sum, 3 2^-24 of the pair's
+largest (sine plus cosine up to sqrt 2): 2^-22.  Attention is held to attention_bound,
 plus the output type's rounding."""
 import numpy as np
 import pytest
@@ -128,7 +130,8 @@ def test_plan_lengths_and_counts_out_of_range():
 # ---------------------------------------------------------------------------
 def turned_bound(want, x, type):
     """What turned values may be off by, from their pairs' magnitudes."""
-    return (ROUNDING[type] + 2.0**-24) * np.abs(want) + 2.0**-40 * np.abs(x).max() + LOWEST[type]
+    products = 2.0**-40 if type == B.TYPE_F32 else 2.0**-22
+    return (ROUNDING[type] + 2.0**-24) * np.abs(want) + products * np.abs(x).max() + LOWEST[type]
 
 
 @pytest.mark.parametrize("type", TYPES)
