@@ -400,8 +400,9 @@ __device__ __forceinline__ void pack(const RowsArgs &a, const Eight<T> &v, uint3
     if ((c & 3) == 0) to[a.cache.scale_at(which, t, c >> 2)] = static_cast<uint8_t>(byte);
 }
 
-// A workgroup takes `per` tokens and of them the queries (blockIdx.y 0) or the
-// keys and values (1).  Sines and cosines go through LDS, once a token; turned
+// A workgroup takes `per` tokens and of them the queries or the keys and values:
+// eight of the one, eight of the other in turn, so that every XCD has both at once,
+// queries that wait for memory and keys that compute.  Sines and cosines go through LDS, once a token; turned
 // keys too, in their own type, since a pair's halves belong to two blocks.  A
 // thread's words are on their way while sines are computed, and then one item
 // ahead.  !KV: queries only.
@@ -414,7 +415,9 @@ __global__ __launch_bounds__(kRowThreads) void kv4_rows_kernel(RowsArgs a) {
     constexpr bool kWide = T == Mx4Type::F32;
     __shared__ __attribute__((aligned(16))) uint8_t turned[KV ? kKeyBytes : 16];
     const uint32_t tid = threadIdx.x;
-    const uint64_t t0 = static_cast<uint64_t>(blockIdx.x) * a.per;
+    const uint32_t group = KV ? blockIdx.x / 16 * 8 + blockIdx.x % 8 : blockIdx.x;
+    const uint64_t t0 = static_cast<uint64_t>(group) * a.per;
+    if (KV && t0 >= a.tokens) return;
     const uint32_t here = static_cast<uint32_t>(min(static_cast<uint64_t>(a.per), a.tokens - t0));
     const Turn &turn = a.turn;
     const uint32_t chunks = a.chunks;
@@ -433,7 +436,7 @@ __global__ __launch_bounds__(kRowThreads) void kv4_rows_kernel(RowsArgs a) {
         }
         __syncthreads();
     };
-    if (!KV || blockIdx.y == 0) {
+    if (!KV || blockIdx.x / 8 % 2 == 0) {
         if (a.q == nullptr) return;
         // what turns comes first, what is only moved behind it: waves do the one or the
         // other
@@ -565,13 +568,13 @@ void launch_rows(const RowsArgs &rows, Mx4Type type, bool kv, hipStream_t stream
     // several tokens a workgroup share the wait for their sines, as long as eight
     // workgroups a CU remain
     a.per = 1;
-    while (a.per < kRowTokens && a.tokens / (2 * a.per) >= 8ull * cu_count()) a.per *= 2;
+    while (a.per < kRowTokens && a.tokens / (2 * a.per) >= 3ull * cu_count()) a.per *= 2;
     // items are counted in 24 bits
     while (a.per > 1 && static_cast<uint64_t>(a.per) * std::max(a.q_heads, kv ? a.cache.heads : 0u) * kKv4MaxDim / 8 >= 1u << 24) a.per /= 2;
     const uint64_t groups = ceil_div(a.tokens, a.per);
-    BSQ_REQUIRE(groups <= 0xFFFFFFFFull / (2 * kRowThreads), "kv4: too many tokens");
+    BSQ_REQUIRE(groups <= 0xFFFFFFFFull / (2 * kRowThreads) - 16, "kv4: too many tokens");
     by_type(type, [&](auto ty) {
-        const dim3 grid(static_cast<unsigned>(groups), kv ? 2 : 1);
+        const unsigned grid = static_cast<unsigned>(kv ? ceil_div(groups, 8) * 16 : groups);
         if (kv) kv4_rows_kernel<decltype(ty)::value, true><<<grid, kRowThreads, 0, stream>>>(a);
         else kv4_rows_kernel<decltype(ty)::value, false><<<grid, kRowThreads, 0, stream>>>(a);
     });
@@ -643,7 +646,7 @@ uint64_t bsq_kv4_cache_bytes(uint64_t pages, uint32_t page, uint32_t heads, uint
     return size_query([&] {
         const bsq_kv4_cache_t c{nullptr, pages, page, heads, dim};
         const Kv4Cache k = kv4_cache(&c, false);
-        return pages * heads * k.head_bytes;
+        return pages * heads * static_cast<uint64_t>(k.head_bytes);
     });
 }
 
@@ -805,7 +808,9 @@ int bsq_kv4_read(const bsq_kv4_cache_t *cache, const int32_t *d_slots, uint64_t 
         BSQ_REQUIRE(d_slots != nullptr, "kv4 read: null slots");
         if (d_k != nullptr) check_dense(d_k, t, "");
         if (d_v != nullptr) check_dense(d_v, t, "");
-        const uint32_t eights = (c.dim + 7) / 8, per = std::max(1u, 1024u / (c.heads * eights));
+        const uint32_t eights = (c.dim + 7) / 8;
+        uint32_t per = std::max(1u, 1024u / (c.heads * eights));
+        while (per > 1 && tokens / per < 2ull * cu_count()) per /= 2;
         const uint64_t groups = ceil_div(tokens, per);
         BSQ_REQUIRE(groups <= 0xFFFFFFFFull / 512, "kv4: too many tokens");
         by_type(t, [&](auto ty) {

@@ -19,13 +19,13 @@ constexpr uint32_t kKv4MaxDim = 256;
 
 struct Kv4Cache {
     uint8_t *pages;
-    uint64_t head_bytes;
+    uint32_t head_bytes;  // of a page fewer than 2^31
     uint32_t count, shift, heads, dim, blocks;  // a page has 1 << shift tokens
 
     __host__ __device__ uint32_t page() const { return 1u << shift; }
     __host__ __device__ uint32_t row_bytes() const { return blocks * 16; }
     __device__ __forceinline__ uint8_t *head(uint32_t page_number, uint32_t h) const {
-        return pages + (static_cast<uint64_t>(page_number) * heads + h) * head_bytes;
+        return pages + static_cast<uint64_t>(page_number) * (heads * head_bytes) + h * head_bytes;
     }
     // from a head's bytes: the codes and the scale byte of block b of token t
     // (in the page) of the keys (0) or values (1)
@@ -51,7 +51,9 @@ inline Kv4Cache kv4_cache(const bsq_kv4_cache_t *c, bool followed = true) {
         BSQ_REQUIRE((reinterpret_cast<uintptr_t>(c->d_pages) & 15) == 0, "kv4: pages are 16-byte aligned");
     }
     const uint32_t blocks = static_cast<uint32_t>(ceil_div(c->dim, kMx4Block));
-    return {c->d_pages, static_cast<uint64_t>(34 * blocks) << shift, static_cast<uint32_t>(c->pages), shift, c->heads,
+    const uint64_t head_bytes = static_cast<uint64_t>(34 * blocks) << shift;
+    BSQ_REQUIRE(head_bytes * c->heads <= 0x7FFFFFFFull, "kv4: a page has 2^31 bytes or more");
+    return {c->d_pages, static_cast<uint32_t>(head_bytes), static_cast<uint32_t>(c->pages), shift, c->heads,
             c->dim, blocks};
 }
 

@@ -70,7 +70,7 @@ struct Tile {
     };
 
     // head: of head h on page 0; the addresses up to a lane's places are scalar
-    __device__ __forceinline__ void load(const Kv4Cache &cache, const uint8_t *head, uint64_t page_bytes, uint32_t t, uint32_t id0,
+    __device__ __forceinline__ void load(const Kv4Cache &cache, const uint8_t *head, uint32_t page_bytes, uint32_t t, uint32_t id0,
                                          uint32_t id1, const Places &at) {
         const uint32_t bad0 = id0 >= cache.count ? 1u : 0u, bad1 = id1 >= cache.count ? 2u : 0u;
         bad = bad0 | bad1;
@@ -78,7 +78,7 @@ struct Tile {
         for (int s = 0; s < 2; ++s) {
             const uint32_t id = (s ? bad1 : bad0) ? 0u : (s ? id1 : id0);
             const uint32_t in = (t + 16 * s) & (cache.page() - 1);
-            const uint8_t *p = head + id * page_bytes;
+            const uint8_t *p = head + static_cast<uint64_t>(id) * page_bytes;
             const uint8_t *kp = p + in * kRow, *vp = kp + (kRow << cache.shift);
             const uint8_t *ksp = p + (2 * kRow << cache.shift) + in * NB, *vsp = ksp + (NB << cache.shift);
             __builtin_memcpy(k[s], __builtin_assume_aligned(kp + at.k, NB % 4 == 0 ? 16 : NB % 2 == 0 ? 8 : 4), 4 * NB);
@@ -398,13 +398,9 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void kv4_attention_kerne
 
     // Page numbers through the scalar cache, a step ahead of the keys on them: a
     // vector load would have to be waited for together with the keys before it.
-    typedef const __attribute__((address_space(4))) int32_t *Entries;
-    const auto entry_of = [&](const Work &w, int32_t t) {
-        const uint32_t last_entry = static_cast<uint32_t>(max(w.rq.length - 1, 0)) >> a.cache.shift;
-        return static_cast<uint32_t>(((Entries)(a.table + static_cast<uint64_t>(w.r) * a.width))[min(static_cast<uint32_t>(t) >> a.cache.shift, last_entry)]);
-    };
+    const auto entry_of = [&](const Work &w, int32_t t) { return page_of(a, w.r, w.rq, static_cast<uint32_t>(t)); };
     const typename Tile<NB>::Places places(lane);
-    const uint64_t page_bytes = a.cache.head_bytes * heads;
+    const uint32_t page_bytes = a.cache.head_bytes * heads;
     const auto load = [&](Tile<NB> &to, const Work &w, int32_t t, uint32_t id0, uint32_t id1) {
         to.load(a.cache, a.cache.pages + w.h * a.cache.head_bytes, page_bytes, static_cast<uint32_t>(t), id0, id1, places);
     };

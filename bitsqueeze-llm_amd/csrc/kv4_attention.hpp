@@ -79,6 +79,15 @@ __device__ __forceinline__ Request load_request(const AttentionArgs &a, uint32_t
     return q;
 }
 
+// The number of the page of token t, or of the last one's: by a scalar load, which
+// is waited for apart from the keys' vector loads.  The table is read only here and
+// written by no kernel that runs beside this one.
+__device__ __forceinline__ uint32_t page_of(const AttentionArgs &a, uint32_t r, const Request &q, uint32_t t) {
+    typedef const __attribute__((address_space(4))) int32_t *Entries;
+    const uint32_t last = static_cast<uint32_t>(max(q.length - 1, 0)) >> a.cache.shift;
+    return static_cast<uint32_t>(((Entries)(a.table + static_cast<uint64_t>(r) * a.width))[min(t >> a.cache.shift, last)]);
+}
+
 __device__ __forceinline__ uint32_t cvt(uint32_t codes, float scale, int byte) {
     switch (byte) {  // an immediate of the instruction
         case 0: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0));

@@ -4,8 +4,9 @@
 // 128 rows of queries (tokens times the heads of a group) share the keys: a
 // workgroup of four waves converts 64 keys and values at a time to BF16 in LDS, once
 // for all rows, and every wave multiplies them with 32 rows.  The next 64 are
-// converted into a second buffer while these are multiplied, from words that were
-// loaded a step earlier, at pages looked up two steps earlier.
+// converted into a second buffer while these are multiplied, 16 by each wave, from
+// words that were loaded a step earlier, at a page that was looked up two steps
+// earlier and is the wave's alone, so that addresses are scalar.
 //
 // Products are S^T = K Q^T and O^T = V^T P^T on 32 x 32 tiles, so a lane holds one
 // row of queries: its reference, sum and weights never leave it but to its partner
@@ -25,21 +26,21 @@ __device__ __forceinline__ uint32_t tiles_of(const AttentionArgs &a, const Reque
     return rows <= a.few ? 0u : static_cast<uint32_t>((rows + kPromptRows - 1) / kPromptRows);
 }
 
-// 64 keys and values as a thread converts them: of one token a block of keys, and
-// of the eight tokens whose weights a lane holds together four channels of values.
+// What a lane converts of 16 keys and values: of one token a block of keys, and of
+// the eight tokens whose weights a lane holds together four channels of values.
 struct Raw {
     uint32_t k[4], ks, nan;
     uint32_t v[8], vs[4];
-    uint32_t bad;  // 1: the key's sixteen is on no page, 2: the values'
 };
 
 template <int NB, int P>
-__global__ __launch_bounds__(kThreads, NB <= 4 && P == 1 ? 2 : 1) void kv4_prompt_kernel(AttentionArgs a, uint32_t tiles) {
-    constexpr int kUnits = 64 * NB, kRounds = (kUnits + kThreads - 1) / kThreads;
+__global__ __launch_bounds__(kThreads, NB <= 4 && P <= 2 ? 2 : 1) void kv4_prompt_kernel(AttentionArgs a, uint32_t tiles) {
+    constexpr int kUnits = 16 * NB, kRounds = (kUnits + 63) / 64;  // a wave's
+    constexpr uint32_t kRow = 16 * NB;                             // bytes of a token's codes
     constexpr uint32_t kKeyRow = 32 * NB + 8, kValueRow = kKeys + 8;  // elements; 16 bytes on: other banks
     __shared__ __attribute__((aligned(16))) uint16_t keys[2][kKeys][kKeyRow];
     __shared__ __attribute__((aligned(16))) uint16_t vals[2][32 * NB][kValueRow];
-    __shared__ uint8_t nans[2][kUnits];
+    __shared__ uint8_t nans[2][kKeys * NB];
     __shared__ uint32_t bads[2][4];
     __shared__ uint32_t sums[kThreads / 64];
     __shared__ uint32_t found[2];
@@ -130,77 +131,75 @@ __global__ __launch_bounds__(kThreads, NB <= 4 && P == 1 ? 2 : 1) void kv4_promp
         for (int e = 0; e < 16; ++e) o[c][e] = 0.0f;
     float top = -__builtin_inff(), base = 0.0f, sum = 0.0f;
 
-    const int32_t *entries = a.table + static_cast<uint64_t>(r) * a.width;
-    const uint32_t last_entry = static_cast<uint32_t>(max(rq.length - 1, 0)) >> a.cache.shift;
-    const uint32_t page_mask = a.cache.page() - 1, row_bytes = a.cache.row_bytes();
-    struct Ids {
-        uint32_t k, v;
+    // this wave's sixteen of a step, lane by lane: unit u of `kUnits`
+    struct Unit {
+        uint32_t token, block;    // of keys
+        uint32_t half, quarter;   // of the tokens, of the channels (four) of values
+        bool real;
     };
-    const auto load_ids = [&](Ids id[kRounds], int32_t t) {
+    const auto unit_of = [&](int n) {
+        const uint32_t u = lane + 64 * n;
+        return Unit{u / NB, u % NB, u & 1, u >> 1, kUnits % 64 == 0 || u < static_cast<uint32_t>(kUnits)};
+    };
+    // above zero, so that what is not seen stays at minus infinity
+    const float factor = fmaxf(a.factor, 0x1p-126f);
+    const uint32_t page_bytes = a.cache.head_bytes * heads;
+    const uint8_t *const head0 = a.cache.pages + h * a.cache.head_bytes;
+    const auto id_of = [&](int32_t t) { return page_of(a, r, rq, static_cast<uint32_t>(t) + 16 * wave); };
+    const auto load_raw = [&](Raw raw[kRounds], uint32_t id, int32_t t) {
+        const uint32_t in = (static_cast<uint32_t>(t) + 16 * wave) & (a.cache.page() - 1);
+        const uint8_t *p = head0 + static_cast<uint64_t>(id >= a.cache.count ? 0u : id) * page_bytes;
+        const uint8_t *keys_at = p + in * kRow, *values_at = keys_at + (kRow << a.cache.shift);
+        const uint8_t *ks_at = p + (2 * kRow << a.cache.shift) + in * NB, *vs_at = ks_at + (NB << a.cache.shift);
 #pragma unroll
         for (int n = 0; n < kRounds; ++n) {
-            const uint32_t u = tid + n * kThreads;
-            const uint32_t kt = static_cast<uint32_t>(t) + (u / NB & 48), vt = static_cast<uint32_t>(t) + ((u & 6) << 3);
-            id[n].k = static_cast<uint32_t>(entries[min(kt >> a.cache.shift, last_entry)]);
-            id[n].v = static_cast<uint32_t>(entries[min(vt >> a.cache.shift, last_entry)]);
-        }
-    };
-    const auto load_raw = [&](Raw raw[kRounds], const Ids id[kRounds], int32_t t) {
-#pragma unroll
-        for (int n = 0; n < kRounds; ++n) {
-            const uint32_t u = tid + n * kThreads;
-            if (kUnits % kThreads != 0 && u >= static_cast<uint32_t>(kUnits)) continue;
+            const Unit u = unit_of(n);
+            if (!u.real) continue;
             Raw &w = raw[n];
-            w.bad = (id[n].k >= a.cache.count ? 1u : 0u) | (id[n].v >= a.cache.count ? 2u : 0u);
-            const uint32_t kt = u / NB, kb = u % NB;
-            {
-                const uint32_t in_page = (static_cast<uint32_t>(t) + kt) & page_mask;
-                const uint8_t *p = a.cache.head(w.bad & 1 ? 0 : id[n].k, h);
-                __builtin_memcpy(w.k, __builtin_assume_aligned(p + a.cache.codes_at(0, in_page) + 16 * kb, 16), 16);
-                w.ks = p[a.cache.scale_at(0, in_page, kb)];
-                w.nan = mixed && edge(t) ? p[a.cache.scale_at(1, in_page, kb)] : 0u;
-            }
-            const uint32_t g = (u & 6) << 3, hh = u & 1, cq = u >> 3;
-            const uint32_t in_page = (static_cast<uint32_t>(t) + g) & page_mask;
-            const uint8_t *p = a.cache.head(w.bad & 2 ? 0 : id[n].v, h);
-            const uint8_t *codes = p + a.cache.codes_at(1, in_page + 4 * hh) + 2 * cq;
+            __builtin_memcpy(w.k, __builtin_assume_aligned(keys_at + (u.token * kRow + 16 * u.block), 16), 16);
+            // words of four tokens' scales, the byte picked as it is used
+            const uint32_t scale_at = 4 * ((u.token & 3) * NB + u.block);
+            w.ks = *reinterpret_cast<const uint32_t *>(ks_at + scale_at);
+            w.nan = mixed && edge(t) ? *reinterpret_cast<const uint32_t *>(vs_at + scale_at) : 0u;
+            const uint32_t codes_at = 4 * u.half * kRow + 2 * u.quarter;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                w.v[j] = *reinterpret_cast<const uint16_t *>(codes + ((j & 3) + 8 * (j >> 2)) * row_bytes);
-            const uint8_t *scales = p + a.cache.scale_at(1, in_page, cq >> 3);
+                w.v[j] = *reinterpret_cast<const uint16_t *>(values_at + codes_at + ((j & 3) + 8 * (j >> 2)) * kRow);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w.vs[j] = *reinterpret_cast<const uint32_t *>(scales + j * 4 * NB);
+            for (int j = 0; j < 4; ++j) w.vs[j] = *reinterpret_cast<const uint32_t *>(vs_at + 4 * (u.quarter >> 3) + j * 4 * NB);
         }
     };
-    const auto convert = [&](Raw raw[kRounds], int32_t t, uint32_t buffer) {
+    const auto convert = [&](Raw raw[kRounds], uint32_t id, int32_t t, uint32_t buffer) {
+        const bool bad = id >= a.cache.count;
+        if (lane == 0) bads[buffer][wave] = bad;
 #pragma unroll
         for (int n = 0; n < kRounds; ++n) {
-            const uint32_t u = tid + n * kThreads;
-            if (kUnits % kThreads != 0 && u >= static_cast<uint32_t>(kUnits)) continue;
+            const Unit u = unit_of(n);
+            if (!u.real) continue;
             Raw &w = raw[n];
-            const uint32_t kt = u / NB, kb = u % NB, g = (u & 6) << 3, hh = u & 1, cq = u >> 3;
-            if (kb == 0 && (kt & 15) == 0) bads[buffer][kt >> 4] = w.bad & 1;
+            const uint32_t token = 16 * wave + u.token;
+            const uint32_t ks_shift = 8 * ((u.token >> 2) & 3);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w.vs[j] >>= 8 * hh;  // the token's byte lowest, that of the one eight on third
-            if (edge(t) || (w.bad & 2)) {
-                if (mixed) nans[buffer][u] = w.nan == 255u;
+            for (int j = 0; j < 4; ++j) w.vs[j] >>= 8 * u.half;  // the token's byte lowest, that of the one eight on third
+            if (edge(t) || bad) {
+                if (mixed) nans[buffer][token * NB + u.block] = (w.nan >> ks_shift & 0xFFu) == 255u;
                 // what no query sees may hold anything, NaN among it; a NaN block that
                 // some see and others do not goes past the products
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const int32_t at = t + static_cast<int32_t>(g + 4 * hh + (j & 3) + 8 * (j >> 2));
+                    const int32_t at = t + static_cast<int32_t>(16 * wave + 4 * u.half + (j & 3) + 8 * (j >> 2));
                     const uint32_t shift = 16 * (j >> 2), byte = w.vs[j & 3] >> shift & 0xFFu;
-                    if (at >= any_lim || at < any_low || (w.bad & 2) || (mixed && byte == 255u)) {
+                    if (at >= any_lim || at < any_low || bad || (mixed && byte == 255u)) {
                         w.v[j] = 0;
                         w.vs[j & 3] = (w.vs[j & 3] & ~(0xFFu << shift)) | 127u << shift;
                     }
                 }
             }
-            const float ks = __uint_as_float(w.ks << 23);
+            const float ks = __uint_as_float((w.ks >> ks_shift & 0xFFu) << 23);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const u32x4 x = {cvt(w.k[c], ks, 0), cvt(w.k[c], ks, 1), cvt(w.k[c], ks, 2), cvt(w.k[c], ks, 3)};
-                *reinterpret_cast<u32x4 *>(&keys[buffer][kt][32 * kb + 8 * c]) = x;
+                *reinterpret_cast<u32x4 *>(&keys[buffer][token][32 * u.block + 8 * c]) = x;
             }
             float scale[8];
 #pragma unroll
@@ -214,22 +213,21 @@ __global__ __launch_bounds__(kThreads, NB <= 4 && P == 1 ? 2 : 1) void kv4_promp
                     even[j >> 1] = __builtin_amdgcn_perm(x1, x0, 0x05040100u);
                     odd[j >> 1] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
                 }
-                *reinterpret_cast<u32x4 *>(&vals[buffer][4 * cq + 2 * c][8 * (u & 7)]) = even;
-                *reinterpret_cast<u32x4 *>(&vals[buffer][4 * cq + 2 * c + 1][8 * (u & 7)]) = odd;
+                *reinterpret_cast<u32x4 *>(&vals[buffer][4 * u.quarter + 2 * c][16 * wave + 8 * u.half]) = even;
+                *reinterpret_cast<u32x4 *>(&vals[buffer][4 * u.quarter + 2 * c + 1][16 * wave + 8 * u.half]) = odd;
             }
         }
     };
 
     if (s0 < s1) {
         const auto at = [&](uint32_t s) { return begin + static_cast<int32_t>(min(s, s1 - 1) * kKeys); };
-        Ids id[kRounds];
         Raw raw[kRounds];
-        load_ids(id, at(s0));
+        uint32_t id = id_of(at(s0)), then = id_of(at(s0 + 1));  // of `raw`, and of the step behind it
         load_raw(raw, id, at(s0));
-        load_ids(id, at(s0 + 1));
-        convert(raw, at(s0), 0);
+        convert(raw, id, at(s0), 0);
+        id = then;
         load_raw(raw, id, at(s0 + 1));
-        load_ids(id, at(s0 + 2));
+        then = id_of(at(s0 + 2));
         __syncthreads();
         for (uint32_t s = s0; s < s1; ++s) {
             const uint32_t buffer = (s - s0) & 1;
@@ -247,9 +245,10 @@ __global__ __launch_bounds__(kThreads, NB <= 4 && P == 1 ? 2 : 1) void kv4_promp
                 }
             }
             if (s + 1 < s1) {
-                convert(raw, at(s + 1), buffer ^ 1);
+                convert(raw, id, at(s + 1), buffer ^ 1);
+                id = then;
                 load_raw(raw, id, at(s + 2));
-                load_ids(id, at(s + 3));
+                then = id_of(at(s + 3));
             }
             const uint32_t bad = bads[buffer][0] | bads[buffer][1] << 1 | bads[buffer][2] << 2 | bads[buffer][3] << 3;
             const bool masked = edge(t) || __builtin_amdgcn_readfirstlane(bad) != 0;
@@ -263,7 +262,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 && P == 1 ? 2 : 1) void kv4_promp
                     }
                 if (mixed && edge(t)) {
                     uint32_t any = 0;
-                    for (uint32_t u = lane; u < static_cast<uint32_t>(kUnits); u += 64) any |= nans[buffer][u];
+                    for (uint32_t u = lane; u < kKeys * NB; u += 64) any |= nans[buffer][u];
                     if (__any(any != 0))
                         for (uint32_t key = 0; key < kKeys; ++key) {
                             const int32_t where = t + static_cast<int32_t>(key);
@@ -282,7 +281,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 && P == 1 ? 2 : 1) void kv4_promp
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) high = fmaxf(high, x[n][e]);
-            high = masked && high == -__builtin_inff() ? high : high * a.factor;
+            high *= factor;
             if (__any(high > top + kSlack)) {
                 high = fmaxf(high, __shfl_xor(high, 32));
                 const float now = fmaxf(top, high), keep = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top - now);
@@ -299,8 +298,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 && P == 1 ? 2 : 1) void kv4_promp
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float score = x[m >> 1][8 * (m & 1) + e];
-                    w[e] = __builtin_amdgcn_exp2f(fmaf(score, a.factor, -base));
-                    if (masked && score == -__builtin_inff()) w[e] = 0.0f;
+                    w[e] = __builtin_amdgcn_exp2f(fmaf(score, factor, -base));
                     sum += w[e];
                 }
                 pieces<P>(w, pw[m]);
