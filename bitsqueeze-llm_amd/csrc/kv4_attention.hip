@@ -580,8 +580,12 @@ Plan plan_of(const Kv4Cache &c, uint32_t width, uint32_t requests, uint64_t toke
     }
     if (prompts) {
         p.tiles = rows / kPromptRows + std::min<uint64_t>(some, ceil_div(rows, p.few + 1));
-        // two workgroups a CU; a share of at least 1024 keys
-        const uint64_t shares = 2ull * cu_count() / (p.tiles * c.heads);
+        // Two workgroups of a CU run at once; up to four are made, as tiles have keys
+        // of their own numbers (5 chunks of 500 tokens over 500 to 8000 keys in 400
+        // tiles: 197 us with each tile whole, 171 in halves, 174 in quarters; 2048
+        // tiles of a prompt 639 whole and 758 in halves).  A share has at least 1024
+        // keys.
+        const uint64_t shares = 4ull * cu_count() / (p.tiles * c.heads);
         p.each = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(shares, keys / 1024)));
         if (p.each > 1) {
             p.splits = std::max<uint64_t>(p.splits, p.tiles * c.heads);
