@@ -145,7 +145,8 @@ def abi_leg(src, ddst, n, wl, reps=5):
 # Sources of operators that no workload here runs: layers on 4-bit matrices, and
 # attention over a 4-bit cache.
 MX4_SOURCES = {"mx4.hip", "mx4.hpp", "mx4_gemm.hip", "moe.hip"}
-KV4_SOURCES = {"kv4.hip", "kv4.hpp", "kv4_attention.hip", "kv4_attention.hpp", "kv4_prompt.hip"}
+KV4_SOURCES = {"kv4.hip", "kv4.hpp", "kv4_attention.hip", "kv4_attention.hpp", "kv4_few.hpp", "kv4_few_bf16.hip",
+               "kv4_few_f16.hip", "kv4_few_f32.hip", "kv4_prompt.hip"}
 OTHER_SOURCES = MX4_SOURCES | KV4_SOURCES
 
 

@@ -176,6 +176,25 @@ void by_blocks(uint32_t blocks, F &&fn) {
     fail("kv4: unknown head size");
 }
 
+// Few queries: a wave takes kStep keys at once.
+constexpr int kFewThreads = 256, kFewWaves = kFewThreads / 64;
+constexpr uint32_t kStep = 32;
+// A tile's work: units of 1 << a.span keys (at least one, which writes the zeros of
+// queries that see none), and kExtra more for what a tile costs beside its keys:
+// its queries, reference and first keys wait for one another, and its sums are
+// written.  0, 1, 2, 3, 4, 6, 8 of them: 145, 108, 92, 81, 77, 77, 78 us for 128
+// requests of 16 to 16384 keys, 8 heads of 128; 110.5 to 109 us for 8 of 40 to 90
+// thousand, where they hardly count.
+constexpr uint32_t kExtra = 4;
+// Units that a share has at least: more shares are more parts to join, fewer leave
+// waves idle (2, 4, 6, 8, 12: 17.1, 15.8, 17.4, 19.1, 22.3 us for 16 requests of 400
+// to 1200 keys, 18.9, 19.5, 18.5, 20.1, 24.5 for 9 of 100 to 5000 in FP32).
+constexpr uint32_t kLeast = 4;
+
+// Requests of up to a.few rows, P BF16 pieces, in shares of `waves` waves.
+template <int P>
+void launch_kv4_few(const AttentionArgs &a, uint32_t waves, hipStream_t stream);
+
 // Requests of more than a.few rows; depth: BF16 pieces.  grid: `tiles` tiles of
 // kPromptRows rows (no fewer than there are) times the heads times a.each.  With
 // a.each > 1 the parts and splits are tile-major, of each tile and head.
