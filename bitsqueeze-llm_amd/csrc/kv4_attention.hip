@@ -87,6 +87,7 @@ Plan plan_of(const Kv4Cache &c, uint32_t width, uint32_t requests, uint64_t toke
     }
     if (prompts) {
         p.tiles = rows / kPromptRows + std::min<uint64_t>(some, ceil_div(rows, p.few + 1));
+        grid_of(p.tiles * c.heads, kPromptThreads, "kv4 attention: too many queries");
         // Two workgroups of a CU run at once; up to four are made, as tiles have keys
         // of their own numbers (5 chunks of 500 tokens over 500 to 8000 keys in 400
         // tiles: 197 us with each tile whole, 171 in halves, 174 in quarters; 2048
@@ -167,7 +168,7 @@ int bsq_kv4_attention(const bsq_kv4_cache_t *cache, const int32_t *d_table, uint
         a.factor = static_cast<float>(std::fabs(static_cast<double>(scale)) * 1.44269504088896340736);
         a.negate = scale < 0.0f;
         a.causal = causal != 0;
-        a.window = window;
+        a.window = window >= static_cast<uint64_t>(width) << a.cache.shift ? 0u : window;  // all of a request's
         a.out = static_cast<uint8_t *>(d_out);
         a.lse = d_lse;
         a.parts = static_cast<float *>(d_work);

@@ -23,6 +23,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr uint32_t kTileRows = 16;       // rows of a tile of few queries; a row is a (token, head of the group)
 constexpr uint32_t kPromptRows = 128;    // and of a prompt's
+constexpr int kPromptThreads = 256;
 constexpr float kSlack = 8.0f;           // of the reference under the largest score
 
 struct AttentionArgs {

@@ -292,12 +292,21 @@ __global__ __launch_bounds__(kFewThreads, NB <= 4 ? 2 : 1) void kv4_attention_ke
     const uint32_t per = (a.requests + 63) / 64;
     const uint32_t r_begin = min(lane * per, a.requests), r_end = min(r_begin + per, a.requests);
     Request own{0, 0, 0};  // with one request a lane
-    uint32_t mine = 0;
+    uint64_t units_here = 0;
     for (uint32_t i = r_begin; i < r_end; ++i) {
         own = load_request(a, i);
-        mine += tiles_of(a, own) * (spans_of(a, own) + kExtra);
+        units_here += static_cast<uint64_t>(tiles_of(a, own)) * (spans_of(a, own) + kExtra);
     }
-    mine *= heads;
+    units_here *= heads;
+    // The host has seen to it that all fit 31 bits, unless starts overlap: those that
+    // then do not are no work.
+    const bool too_many = __any(units_here >= 1u << 25) && [&] {
+        uint64_t sum = units_here;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+        return sum >= 1ull << 31;
+    }();
+    const uint32_t mine = too_many ? 0u : static_cast<uint32_t>(units_here);
     const uint32_t up_to = wave_prefix(mine), total = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(up_to), 63));
     // no share is empty but those behind the last: a split tile's lie side by side
     const uint32_t shares = min(max(total / kLeast, min(total, 1u)), waves);
@@ -351,10 +360,10 @@ __global__ __launch_bounds__(kFewThreads, NB <= 4 ? 2 : 1) void kv4_attention_ke
     const int32_t window = static_cast<int32_t>(min(a.window, 0x7FFFFFFFu));
     const auto query_of = [&](const Request &q, uint32_t row) { return q.count == 1 ? 0 : static_cast<int32_t>(row / a.group); };
     const auto lim_of = [&](const Request &q, int32_t query) { return a.causal ? q.past() + query + 1 : q.length; };
-    const auto low_of = [&](const Request &q, int32_t query) { return window ? q.past() + query + 1 - window : 0; };
+    const auto low_of = [&](const Request &q, int32_t query) { return window ? max(q.past() + query + 1, 0) - window : 0; };
     const auto next = [&](Work &w) __attribute__((always_inline)) {
         while (x < end) {
-            if (h == heads || tiles == 0) {
+            if (h >= heads || tiles == 0) {
                 if (++r >= a.requests) return false;  // starts that overlap
                 rq = request(r);
                 units = spans_of(a, rq) + kExtra, tiles = tiles_of(a, rq);

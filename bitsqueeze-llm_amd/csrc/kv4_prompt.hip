@@ -18,7 +18,7 @@
 namespace bsq {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = kPromptThreads;
 constexpr uint32_t kKeys = 64;
 
 __device__ __forceinline__ uint32_t tiles_of(const AttentionArgs &a, const Request &q) {
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 && P <= 2 ? 2 : 1) void kv4_promp
     const int32_t qa = static_cast<int32_t>(row0 / a.group), qb = static_cast<int32_t>((row0 + count - 1) / a.group);
     const int32_t past = rq.past(), window = static_cast<int32_t>(min(a.window, 0x7FFFFFFFu));
     const auto lim_of = [&](int32_t query) { return a.causal ? past + query + 1 : rq.length; };
-    const auto low_of = [&](int32_t query) { return window ? past + query + 1 - window : 0; };
+    const auto low_of = [&](int32_t query) { return window ? max(past + query + 1, 0) - window : 0; };
     const int32_t any_lim = lim_of(qb), any_low = low_of(qa), all_lim = lim_of(qa), all_low = low_of(qb);
     const uint32_t i = lane & 31, half = lane >> 5, row = wave * 32 + i, mine = row0 + min(row, count - 1);
     const int32_t lim = lim_of(static_cast<int32_t>(mine / a.group)), low = low_of(static_cast<int32_t>(mine / a.group));
@@ -355,7 +355,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 && P <= 2 ? 2 : 1) void kv4_promp
 }  // namespace
 
 void launch_kv4_prompt(const AttentionArgs &a, int depth, uint64_t tiles, hipStream_t stream) {
-    const unsigned groups = grid_of(tiles * a.cache.heads * a.each, kThreads, "kv4 attention: too many queries");
+    const unsigned groups = static_cast<unsigned>(tiles * a.cache.heads * a.each);  // checked with the sizes
     const uint32_t n = static_cast<uint32_t>(tiles);
     by_blocks(a.cache.blocks, [&](auto nb) {
         constexpr int NB = decltype(nb)::value;

@@ -571,6 +571,17 @@ def test_many_requests():
         check_attention(c, table, lengths, list(counts), q, 0.2, B.TYPE_BF16)
 
 
+@pytest.mark.parametrize("window", [1, 319, 320, 2**31 - 1, 2**31, 2**32 - 1])
+def test_windows_of_any_size(window):
+    # as long as the table, longer than 31 bits; queries ahead of the first key
+    rng = np.random.default_rng(30)
+    c = filled(rng, 20, 16, 1, 64)
+    lengths, counts = [320, 10, 300], [3, 40, 90]
+    table = np.array([rng.permutation(20) for _ in lengths])
+    q = rng.standard_normal((sum(counts), 2, 64))
+    check_attention(c, table, lengths, counts, q, 0.1, B.TYPE_F32, window=window)
+
+
 def test_rows_behind_and_past_most_are_left():
     rng = np.random.default_rng(13)
     c = filled(rng, 12, 16, 1, 64)
