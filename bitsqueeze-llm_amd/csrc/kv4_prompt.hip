@@ -234,16 +234,17 @@ __global__ __launch_bounds__(kThreads, NB <= 4 && P <= 2 ? 2 : 1) void kv4_promp
             const int32_t t = at(s);
             f32x16 x[2];
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
+            for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) x[n][e] = 0.0f;
 #pragma unroll
-                for (int c = 0; c < 2 * NB; ++c) {
+            for (int c = 0; c < 2 * NB; ++c)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
                     const u32x4 k = *reinterpret_cast<const u32x4 *>(&keys[buffer][32 * n + i][16 * c + 8 * half]);
 #pragma unroll
                     for (int p = 0; p < P; ++p) x[n] = mfma(k, q[p][c], x[n]);
                 }
-            }
             if (s + 1 < s1) {
                 convert(raw, id, at(s + 1), buffer ^ 1);
                 id = then;
@@ -304,9 +305,9 @@ __global__ __launch_bounds__(kThreads, NB <= 4 && P <= 2 ? 2 : 1) void kv4_promp
                 pieces<P>(w, pw[m]);
             }
 #pragma unroll
-            for (int c = 0; c < NB; ++c)
+            for (int m = 0; m < 4; ++m)
 #pragma unroll
-                for (int m = 0; m < 4; ++m) {
+                for (int c = 0; c < NB; ++c) {
                     const u32x4 v = *reinterpret_cast<const u32x4 *>(&vals[buffer][32 * c + i][16 * m + 8 * half]);
 #pragma unroll
                     for (int p = 0; p < P; ++p) o[c] = mfma(v, pw[m][p], o[c]);
