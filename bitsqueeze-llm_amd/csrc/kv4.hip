@@ -17,7 +17,8 @@ namespace {
 // need only a search in the starts.  Small steps do both in the one launch, as a
 // second costs more than the search; large ones spread the places over a grid.
 // What bounds it are waits one after another: lengths, the sums' exchange between
-// waves, the ended requests' rows, the pages of new tokens.
+// waves, the ended requests' rows, the pages of new tokens (64 requests 7.7 us, the
+// host's launch; 2000 with 40 that end 20 us).
 constexpr uint32_t kPlanThreads = 1024;
 constexpr uint32_t kPlanMostRequests = 16384;
 constexpr uint32_t kPlanOneLaunch = 4096;  // places
@@ -405,7 +406,9 @@ __device__ __forceinline__ void pack(const RowsArgs &a, const Eight<T> &v, uint3
 // queries that wait for memory and keys that compute.  Sines and cosines go through LDS, once a token; turned
 // keys too, in their own type, since a pair's halves belong to two blocks.  A
 // thread's words are on their way while sines are computed, and then one item
-// ahead.  !KV: queries only.
+// ahead.  !KV: queries only, 29 us for 8192 tokens of 32 heads of 128 in BF16, 4.6
+// TB/s.  With 8 heads of keys and values 48 us, 3.7 TB/s: packing them takes vector
+// instructions and two barriers.
 template <Mx4Type T, bool KV>
 __global__ __launch_bounds__(kRowThreads) void kv4_rows_kernel(RowsArgs a) {
     constexpr uint32_t size = T == Mx4Type::F32 ? 4 : 2;

@@ -1,6 +1,14 @@
 // Attention over the paged MX4 cache: single tokens and a few queries a request
 // (kv4_attention.hpp).  A source for each number of pieces instantiates it, as the
 // compiler takes its time over the kernels.
+//
+// Long contexts are bound by HBM: 8 requests of 40 to 90 thousand keys, 32 query
+// heads on 8 of 128, take 107 us with the join, 5.0 TB/s of the 5.07 that a large
+// copy reaches.  Of ragged ones (128 requests of 16 to 16384 keys, 76 us, 4.4 TB/s)
+// and short ones (16 of 400 to 1200, 15.4 us) what a tile costs beside its keys is
+// the rest; a step of 32 keys takes a wave alone on its SIMD 0.85 us, mostly waits
+// for its keys, which are asked for one step ahead.  A form with a workgroup's waves
+// on one tile, joined in LDS, took 89 us for the ragged and 15.5 for the short ones.
 #pragma once
 
 #include "kv4_attention.hpp"

@@ -13,6 +13,13 @@
 // 32 lanes on.  Lane l = 32 h + i holds of S^T's 32 keys those at 8 b + 4 h + r; the
 // values' rows of 16 lie in LDS in the order 0-3, 8-11, 4-7, 12-15, so that the
 // eight weights that a lane has are the eight that the next product wants of it.
+//
+// Bound by the matrix instructions and the vector ones between them, which two waves
+// a SIMD overlap only in part: a prompt of 8192, 32 heads on 8 of 128, takes 623 to
+// 655 us, 840 to 880 TFLOP/s (1173 in a large BF16 product of the library); a wave's
+// 64 keys are 32 matrix instructions and some 240 others, 32 of them exponentials.
+// Waves of raised priority during the products: 695 us against 669.  Tiles of 16 rows
+// (kv4_few.hpp) take 2790.
 #include "kv4_attention.hpp"
 
 namespace bsq {
