@@ -18,28 +18,34 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttentionArgs a, uint32_t
         const uint64_t number = b == 0 ? s.first : s.next + static_cast<uint64_t>(b - 1) * s.step;
         return a.parts + (number * part_rows + n_row) * part_row(NB);
     };
-    float top = -__builtin_inff();
-    for (uint32_t b = lane; b < s.parts; b += 64) top = fmaxf(top, part(b)[32 * NB]);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    // lanes: parts beside one another, eight channels each
+    // lanes: parts beside one another, eight channels each; in one pass, so that a
+    // part's reference and its sums are waited for together
     constexpr uint32_t kEights = 4 * NB, kBeside = NB <= 1 ? 16 : NB == 2 ? 8 : NB <= 4 ? 4 : 2;
     const uint32_t e = lane % (64 / kBeside), beside = lane / (64 / kBeside);
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0}, all = 0.0f;
+    float top = -__builtin_inff(), all = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    const auto add = [&](float their_top, float their_all, const float their[8]) {
+        // without a reference there are zeros, or NaN
+        const float now = fmaxf(top, their_top);
+        const float keep = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(top - now);
+        const float take = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(their_top - now);
+        all = all * keep + their_all * take;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = v[i] * keep + their[i] * take;
+        top = now;
+    };
     if (e < kEights)
         for (uint32_t b = beside; b < s.parts; b += kBeside) {
             const float *p = part(b);
-            const float mine = p[32 * NB];
-            const float keep = mine == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(mine - top);
-            all += keep * p[32 * NB + 1];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] += keep * p[e * 8 + i];
+            float x[8];
+            __builtin_memcpy(x, __builtin_assume_aligned(p + e * 8, 16), 32);
+            add(p[32 * NB], p[32 * NB + 1], x);
         }
 #pragma unroll
     for (uint32_t d = 64 / kBeside; d < 64; d <<= 1) {
-        all += __shfl_xor(all, d);
+        float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += __shfl_xor(v[i], d);
+        for (int i = 0; i < 8; ++i) x[i] = __shfl_xor(v[i], d);
+        add(__shfl_xor(top, d), __shfl_xor(all, d), x);
     }
     if (beside != 0 || e >= kEights) return;
     const uint32_t row = s.row0 + n_row;

@@ -48,14 +48,14 @@ struct AttentionArgs {
 };
 
 // A tile of queries whose keys more than one workgroup takes: its parts, `rows`
-// rows of sums, reference and sum each (part_floats), are number first, next, next
-// + step ...
+// rows of sums, the reference and their sum (part_row floats, whole 16 bytes), are
+// number first, next, next + step ...
 struct Split {
     uint32_t parts;  // 0: none
     uint32_t first, next, step;
     uint32_t head, row0, rows, first_token;
 };
-constexpr uint32_t part_row(uint32_t blocks) { return 32 * blocks + 2; }
+constexpr uint32_t part_row(uint32_t blocks) { return 32 * blocks + 4; }
 
 struct Request {
     int32_t length, first, count;  // keys, first query, queries

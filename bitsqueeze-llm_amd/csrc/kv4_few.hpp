@@ -473,8 +473,7 @@ __global__ __launch_bounds__(kFewThreads, NB <= 4 ? 2 : 1) void kv4_attention_ke
                 if (w.whole) {
                     write_row(a, token, head, at, v, sum, rows.top);
                 } else if (32 * NB == 16 * S::kLane || at < 32 * NB) {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) part[at + k] = v[k];
+                    __builtin_memcpy(__builtin_assume_aligned(part + at, 16), v, 32);
                 }
             }
             if (!w.whole && g == 0) {

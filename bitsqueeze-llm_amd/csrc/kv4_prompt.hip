@@ -334,7 +334,10 @@ __global__ __launch_bounds__(kThreads, NB <= 4 && P <= 2 ? 2 : 1) void kv4_promp
 #pragma unroll
         for (int c = 0; c < NB; ++c)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) p[32 * c + 8 * (e >> 2) + 4 * half + (e & 3)] = o[c][e];
+            for (int e = 0; e < 16; e += 4) {
+                const f32x4 v = {o[c][e], o[c][e + 1], o[c][e + 2], o[c][e + 3]};
+                *reinterpret_cast<f32x4 *>(p + 32 * c + 2 * e + 4 * half) = v;
+            }
         if (half == 0) {
             p[32 * NB] = top;
             p[32 * NB + 1] = sum;
