@@ -8,8 +8,8 @@
 namespace bsq {
 namespace {
 
-// A wave a row of a split tile.
-template <int NB>
+// A wave a row of a split tile; kAtOnce parts are asked for together.
+template <int NB, uint32_t kAtOnce>
 __global__ __launch_bounds__(256) void kv4_join_kernel(AttentionArgs a, uint32_t part_rows) {
     const Split s = a.splits[blockIdx.x];
     const uint32_t n_row = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -19,7 +19,9 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttentionArgs a, uint32_t
         return a.parts + (number * part_rows + n_row) * part_row(NB);
     };
     // lanes: parts beside one another, eight channels each; in one pass, so that a
-    // part's reference and its sums are waited for together
+    // part's reference and its sums are waited for together.  Four parts at once where
+    // tiles have many (32 of 8 requests of 40 to 90 thousand keys: 6.5 us, one by one
+    // 9.3), one where they have few (two of a chunk's tile: 19 us, with four 24).
     constexpr uint32_t kEights = 4 * NB, kBeside = NB <= 1 ? 16 : NB == 2 ? 8 : NB <= 4 ? 4 : 2;
     const uint32_t e = lane % (64 / kBeside), beside = lane / (64 / kBeside);
     float top = -__builtin_inff(), all = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -34,11 +36,17 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttentionArgs a, uint32_t
         top = now;
     };
     if (e < kEights)
-        for (uint32_t b = beside; b < s.parts; b += kBeside) {
-            const float *p = part(b);
-            float x[8];
-            __builtin_memcpy(x, __builtin_assume_aligned(p + e * 8, 16), 32);
-            add(p[32 * NB], p[32 * NB + 1], x);
+        for (uint32_t b0 = beside; b0 < s.parts; b0 += kAtOnce * kBeside) {
+            float x[kAtOnce][8], tops[kAtOnce], sums[kAtOnce];
+#pragma unroll
+            for (uint32_t n = 0; n < kAtOnce; ++n) {
+                const float *p = part(min(b0 + n * kBeside, s.parts - 1));
+                __builtin_memcpy(x[n], __builtin_assume_aligned(p + e * 8, 16), 32);
+                tops[n] = p[32 * NB], sums[n] = p[32 * NB + 1];
+            }
+#pragma unroll
+            for (uint32_t n = 0; n < kAtOnce; ++n)
+                if (b0 + n * kBeside < s.parts) add(tops[n], sums[n], x[n]);
         }
 #pragma unroll
     for (uint32_t d = 64 / kBeside; d < 64; d <<= 1) {
@@ -111,10 +119,10 @@ Plan plan_of(const Kv4Cache &c, uint32_t width, uint32_t requests, uint64_t toke
     return p;
 }
 
-template <int NB>
+template <int NB, uint32_t kAtOnce>
 void join(const AttentionArgs &a, uint64_t splits, uint32_t part_rows, uint64_t rows, hipStream_t s) {
     rows = std::min<uint64_t>(rows, part_rows);
-    kv4_join_kernel<NB><<<dim3(static_cast<unsigned>(splits), static_cast<unsigned>((rows + 3) / 4)), 256, 0, s>>>(a, part_rows);
+    kv4_join_kernel<NB, kAtOnce><<<dim3(static_cast<unsigned>(splits), static_cast<unsigned>((rows + 3) / 4)), 256, 0, s>>>(a, part_rows);
     BSQ_HIP(hipGetLastError());
 }
 
@@ -190,11 +198,11 @@ int bsq_kv4_attention(const bsq_kv4_cache_t *cache, const int32_t *d_table, uint
                 if (depth == 1) launch_kv4_few<1>(a, p.waves, s);
                 else if (depth == 2) launch_kv4_few<2>(a, p.waves, s);
                 else launch_kv4_few<3>(a, p.waves, s);
-                if (p.waves > 1) join<NB>(a, p.waves, kTileRows, rows, s);
+                if (p.waves > 1) join<NB, 4>(a, p.waves, kTileRows, rows, s);
             }
             if (p.tiles > 0) {
                 launch_kv4_prompt(a, depth, p.tiles, s);
-                if (p.each > 1) join<NB>(a, p.tiles * a.cache.heads, kPromptRows, rows, s);
+                if (p.each > 1) join<NB, 1>(a, p.tiles * a.cache.heads, kPromptRows, rows, s);
             }
         });
     });
