@@ -627,12 +627,6 @@ Turn turn_of(const bsq_rope_t *rope, uint32_t dim, int back) {
             back ? -static_cast<double>(rope->factor) : rope->factor};
 }
 
-bool overlap(const void *a, uint64_t a_bytes, const void *b, uint64_t b_bytes) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return x < y + b_bytes && y < x + a_bytes;
-}
-uint64_t span(uint64_t tokens, uint64_t ld, uint64_t width, Mx4Type t) { return ((tokens - 1) * ld + width) * type_bytes(t); }
-
 void check_tokens(uint64_t tokens, uint64_t ld) {
     BSQ_REQUIRE(tokens <= 0x7FFFFFFFull, "kv4: too many tokens");
     BSQ_REQUIRE(ld <= 1ull << 28, "kv4: rows too far apart");

@@ -57,4 +57,11 @@ inline Kv4Cache kv4_cache(const bsq_kv4_cache_t *c, bool followed = true) {
             c->dim, blocks};
 }
 
+// Rows of `width` values, `ld` apart, from the first byte to the last.
+inline uint64_t span(uint64_t tokens, uint64_t ld, uint64_t width, Mx4Type t) { return ((tokens - 1) * ld + width) * type_bytes(t); }
+inline bool overlap(const void *a, uint64_t a_bytes, const void *b, uint64_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + b_bytes && y < x + a_bytes;
+}
+
 }  // namespace bsq

@@ -548,7 +548,8 @@ BSQ_API int bsq_kv4_read(const bsq_kv4_cache_t *cache, const int32_t *d_slots, u
  * FP32; products with queries are exact to FP32 in every type, the softmax's
  * weights are rounded to BF16 where both q and out are BF16, are held to 16 bits
  * where FP16 is the finest type among them, and to FP32 where one is FP32.
- * Queries behind the last request's, and past `most`, are left as they are. */
+ * Queries behind the last request's, and past `most`, are left as they are.  out
+ * may not overlap the queries' rows. */
 BSQ_API uint64_t bsq_kv4_attention_workspace(const bsq_kv4_cache_t *cache, uint32_t width, uint32_t requests,
                                              uint64_t tokens, uint32_t most, uint32_t q_heads);
 BSQ_API int bsq_kv4_attention(const bsq_kv4_cache_t *cache, const int32_t *d_table, uint32_t width,

@@ -136,7 +136,7 @@ def test_read(change, word):
 
 def attention_args(**change):
     a = dict(cache=cache(), table=D, width=8, lengths=D, starts=D, requests=3, q=D, q_type=1, tokens=6, most=4, q_heads=4, ldq=256,
-             scale=0.125, causal=1, window=0, out=D, out_type=1, ldo=256, lse=None, work=D, work_bytes=1 << 30, stream=None)
+             scale=0.125, causal=1, window=0, out=1 << 20, out_type=1, ldo=256, lse=None, work=D, work_bytes=1 << 30, stream=None)
     a.update(change)
     return a.values()
 
@@ -149,6 +149,7 @@ def attention_args(**change):
     (dict(starts=None), "starts"), (dict(lengths=None), "null"), (dict(table=None), "null"), (dict(q=None), "queries"),
     (dict(out=None), "output"), (dict(q=D + 1), "unaligned"), (dict(out=D + 1), "unaligned"), (dict(work_bytes=64), "workspace"), (dict(work=None), "null"),
     (dict(q_type=3), "type"), (dict(out_type=-1), "type"), (dict(work=D + 8), "aligned"),
+    (dict(out=D), "overlaps"), (dict(out=D, ldq=768), "overlaps"), (dict(out=D + 6 * 512 - 16), "overlaps"), (dict(q=(1 << 20) + 16, out_type=0), "overlaps"),
 ])
 def test_attention(change, word):
     if B.device_count() < 1 and ("work" in change or "work_bytes" in change):
