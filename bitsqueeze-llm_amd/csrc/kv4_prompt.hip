@@ -107,7 +107,9 @@ __global__ __launch_bounds__(kThreads, NB <= 4 && P <= 2 ? 2 : 1) void kv4_promp
     const uint32_t steps = any_lim > begin ? static_cast<uint32_t>(any_lim - begin + kKeys - 1) / kKeys : 0u;
     const uint32_t s0 = static_cast<uint32_t>(static_cast<uint64_t>(steps) * share / a.each);
     const uint32_t s1 = static_cast<uint32_t>(static_cast<uint64_t>(steps) * (share + 1) / a.each);
-    const auto edge = [&](int32_t t) { return t + static_cast<int32_t>(kKeys) > all_lim || t < all_low; };
+    // tables may end within the last kKeys of 31 bits, so nothing is added to t; a tile
+    // with keys has all_lim above -kPromptRows
+    const auto edge = [&](int32_t t) { return t > all_lim - static_cast<int32_t>(kKeys) || t < all_low; };
 
     // queries: lane (h, i) has row i's channels 16 s + 8 h .. + 8
     const uint64_t token = static_cast<uint32_t>(rq.first) + mine / a.group;
