@@ -158,7 +158,7 @@ struct Rows {
                 for (int e = 0; e < 8; ++e) x[e] = -x[e];
             }
             u32x4 w[P];
-            pieces<P>(x, w);
+            pieces<P, true>(x, w);
 #pragma unroll
             for (int p = 0; p < P; ++p) q[p][s] = w[p];
         }

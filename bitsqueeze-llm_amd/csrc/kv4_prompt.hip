@@ -128,7 +128,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 && P <= 2 ? 2 : 1) void kv4_promp
                 for (int e = 0; e < 8; ++e) x[e] = -x[e];
             }
             u32x4 w[P];
-            pieces<P>(x, w);
+            pieces<P, true>(x, w);
 #pragma unroll
             for (int p = 0; p < P; ++p) q[p][s] = w[p];
         }
