@@ -103,22 +103,24 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
 __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
-// Eight FP32 values as P vectors of BF16 whose sums they are (to 8 P bits).  LARGE:
-// values that BF16 would round to infinity are taken too (above 2^128 - 2^119): BF16's
-// largest, 2^128 - 2^120, and a rest that the other pieces hold; infinities are NaN,
-// as their pieces' products add up to.
-template <int P, bool LARGE = false>
+// Eight FP32 values as P vectors of BF16 whose sums they are (to 8 P bits).  QUERIES:
+// of any size, infinities among them.  Those that BF16 would round to infinity (above
+// 2^128 - 2^119) are BF16's largest, 2^128 - 2^120, and a rest that the other pieces
+// hold.  Infinities are NaN: so is a softmax over their products with any keys, but the
+// kernels take scores that are all minus infinity for keys that nobody sees.
+template <int P, bool QUERIES = false>
 __device__ __forceinline__ void pieces(float x[8], u32x4 out[P]) {
     constexpr float kMost = 0x1.FEp127f;
-    constexpr bool kLarge = LARGE && P > 1;
+    if constexpr (QUERIES) {
 #pragma unroll
-    for (int i = 0; i < 8 && kLarge; ++i) x[i] += x[i] - x[i];
+        for (int i = 0; i < 8; ++i) x[i] += x[i] - x[i];
+    }
 #pragma unroll
     for (int p = 0; p < P; ++p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             uint32_t w;
-            if (kLarge && p == 0)  // a NaN is one in the rest
+            if (QUERIES && P > 1 && p == 0)  // a NaN is one in the rest
                 w = pack2<Mx4Type::BF16>(__builtin_amdgcn_fmed3f(x[2 * i], -kMost, kMost), __builtin_amdgcn_fmed3f(x[2 * i + 1], -kMost, kMost));
             else
                 w = pack2<Mx4Type::BF16>(x[2 * i], x[2 * i + 1]);

@@ -57,3 +57,23 @@ def test_the_smallest_queries(count, exponent):
     off = 2.0**-134 * np.abs(c.values(0)).sum(2).max()
     assert (np.abs(got - want) <= bound + 2 * off * of[0] + 2.0**-24 * np.abs(want)).all()
     assert (np.abs(lse - want_lse) <= lse_bound + off).all()
+
+
+@pytest.mark.parametrize("type,out_type", TYPES)
+@pytest.mark.parametrize("count", [6, 90])
+def test_infinite_queries(type, out_type, count):
+    # infinity times a key is infinite or NaN, so the softmax over any keys is NaN,
+    # also where all scores are minus infinity; a query that sees no key stays zero
+    rng = np.random.default_rng(count)
+    c = small_keys(rng, 8, 64, positive=(3, 40))
+    q = rng.standard_normal((count, 2, 64)) * 100
+    q[0, 0, 3], q[count - 1, 1, 3] = -np.inf, -np.inf
+    q[count - 2, 0, 40], q[count - 3, 1, 40] = np.inf, np.nan
+    q[count - 4, 0, 5], q[count - 4, 1, 5] = -np.inf, np.inf
+    for length in (100, 3):  # of three keys the first queries see none
+        for scale in (0.1, -0.1):
+            got, lse, _ = check_attention(c, tables(rng, c, [length], 7), [length], [count], q, scale, type, out_type)
+            bad = np.isnan(lse)
+            assert bad.sum() == (6 if length == 100 else 3)
+            assert (np.isnan(got).all(2) == bad).all()
+    assert (got[: count - 3] == 0).all()
