@@ -132,15 +132,16 @@ struct Rows {
     }
     __device__ __forceinline__ void begin(const AttentionArgs &a, const Ahead &ahead, const Request &rq, uint32_t h, uint32_t row0,
                                           uint32_t rows, uint32_t lane) {
-        uint32_t special = 0;  // its halves' top bits: some exponent is the largest
 #pragma unroll
         for (int s = 0; s < NB; ++s) {
             float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if constexpr (P == 1) {  // BF16 as it is
+            if constexpr (P == 1) {  // BF16 as it is, but infinities NaN as in pieces(): 0x7F80 | 1
+                constexpr mx4_u16x2 kFinite = {0x7F7F, 0x7F7F};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    q[0][s][e] = a.negate ? ahead.w[s][e] ^ 0x80008000u : ahead.w[s][e];
-                    special |= (ahead.w[s][e] & 0x7F807F80u) + 0x00800080u;
+                    const uint32_t w = ahead.w[s][e];
+                    const mx4_u16x2 above = __builtin_elementwise_sub_sat(__builtin_bit_cast(mx4_u16x2, w & 0x7FFF7FFFu), kFinite);
+                    q[0][s][e] = (a.negate ? w ^ 0x80008000u : w) | __builtin_bit_cast(uint32_t, above);
                 }
                 continue;
             }
@@ -165,14 +166,6 @@ struct Rows {
             pieces<P, true>(x, w);
 #pragma unroll
             for (int p = 0; p < P; ++p) q[p][s] = w[p];
-        }
-        if constexpr (P == 1) {
-            if (__any((special & 0x80008000u) != 0)) {  // infinities are NaN, as in pieces()
-#pragma unroll
-                for (int s = 0; s < NB; ++s)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) q[0][s][e] |= (((q[0][s][e] & 0x7F807F80u) + 0x00800080u) & 0x80008000u) >> 9;
-            }
         }
 #pragma unroll
         for (int c = 0; c < S::kLane; ++c) o[c] = f32x4{0, 0, 0, 0};
