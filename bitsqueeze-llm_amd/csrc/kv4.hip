@@ -735,7 +735,7 @@ int bsq_rope(const bsq_rope_t *rope, const int32_t *d_positions, const void *d_x
         check_dense(d_x, t, "rope: null input");
         check_dense(d_out, t, "rope: null output");
         a.in_place = d_x == d_out && ldx == ldo;
-        BSQ_REQUIRE(a.in_place || !overlap(d_x, span(tokens, ldx, width, t), d_out, span(tokens, ldo, width, t)),
+        BSQ_REQUIRE(a.in_place || !overlap(tokens, CallRows(d_x, ldx, width, t), CallRows(d_out, ldo, width, t)),
                     "rope: out overlaps x");
         a.positions = d_positions;
         a.tokens = tokens;
@@ -771,8 +771,8 @@ int bsq_kv4_append(const bsq_kv4_cache_t *cache, const bsq_rope_t *rope, const i
             check_dense(d_q, t, "");
             check_dense(d_q_out, t, "kv4 append: null output");
             a.in_place = d_q == d_q_out && ldq == ldqo;
-            const uint64_t out = span(tokens, ldqo, q_width, t);
-            BSQ_REQUIRE(a.in_place || !overlap(d_q, span(tokens, ldq, q_width, t), d_q_out, out), "kv4 append: queries' output overlaps them");
+            BSQ_REQUIRE(a.in_place || !overlap(tokens, CallRows(d_q, ldq, q_width, t), CallRows(d_q_out, ldqo, q_width, t)),
+                        "kv4 append: queries' output overlaps them");
             if (!(a.in_place && rope == nullptr)) {  // else nothing changes
                 a.q = static_cast<const uint8_t *>(d_q);
                 a.qo = static_cast<uint8_t *>(d_q_out);

@@ -57,11 +57,22 @@ inline Kv4Cache kv4_cache(const bsq_kv4_cache_t *c, bool followed = true) {
             c->dim, blocks};
 }
 
-// Rows of `width` values, `ld` apart, from the first byte to the last.
-inline uint64_t span(uint64_t tokens, uint64_t ld, uint64_t width, Mx4Type t) { return ((tokens - 1) * ld + width) * type_bytes(t); }
-inline bool overlap(const void *a, uint64_t a_bytes, const void *b, uint64_t b_bytes) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return x < y + b_bytes && y < x + a_bytes;
+// A call's rows: `bytes` each, `pitch` bytes apart.
+struct CallRows {
+    uintptr_t at;
+    uint64_t pitch, bytes;
+    CallRows(const void *p, uint64_t ld, uint64_t width, Mx4Type t)
+        : at(reinterpret_cast<uintptr_t>(p)), pitch(ld * type_bytes(t)), bytes(width * type_bytes(t)) {}
+};
+// Whether rows of two kinds, `tokens` of either, share a byte.  Of one pitch they may
+// lie side by side; of two they count as sharing one wherever their spans cross.
+inline bool overlap(uint64_t tokens, const CallRows &a, const CallRows &b) {
+    const uint64_t a_span = (tokens - 1) * a.pitch + a.bytes, b_span = (tokens - 1) * b.pitch + b.bytes;
+    if (a.at >= b.at + b_span || b.at >= a.at + a_span) return false;
+    if (a.pitch != b.pitch) return true;
+    const CallRows &low = a.at <= b.at ? a : b, &high = a.at <= b.at ? b : a;
+    const uint64_t on = (high.at - low.at) % low.pitch;  // bytes from a row of `low` to one of `high`
+    return on < low.bytes || on + high.bytes > low.pitch;
 }
 
 }  // namespace bsq

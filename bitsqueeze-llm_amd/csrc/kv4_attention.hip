@@ -164,7 +164,7 @@ int bsq_kv4_attention(const bsq_kv4_cache_t *cache, const int32_t *d_table, uint
         check_dense(d_q, tq, "kv4 attention: null queries");
         check_dense(d_out, to, "kv4 attention: null output");
         // others may still read queries where a tile's results are written
-        BSQ_REQUIRE(!overlap(d_q, span(tokens, ldq, row, tq), d_out, span(tokens, ldo, row, to)), "kv4 attention: out overlaps the queries");
+        BSQ_REQUIRE(!overlap(tokens, CallRows(d_q, ldq, row, tq), CallRows(d_out, ldo, row, to)), "kv4 attention: out overlaps the queries");
         const Plan p = plan_of(a.cache, width, requests, tokens, most, q_heads);
         check_work(d_work, work_bytes, p.bytes);
         const int depth = std::max(tq == Mx4Type::F32 ? 3 : tq == Mx4Type::F16 ? 2 : 1, to == Mx4Type::F32 ? 3 : to == Mx4Type::F16 ? 2 : 1);

@@ -458,8 +458,9 @@ BSQ_API int bsq_moe_linear_backward(const void *d_d_out, int d_type, uint64_t to
  *    Whole numbers are int32.  As in group 6 all calls are asynchronous on
  *    `stream`, keep nothing between calls, take their workspace from the caller
  *    and can be captured; types, leading dimensions, returns and size queries are
- *    those of group 6 too.  What device arrays hold is not checked by the host:
- *    page numbers and slots outside the cache, lengths outside the table and
+ *    those of group 6 too.  Results may lie beside what a call reads, in other
+ *    columns of rows of one distance; results on it are refused where the calls
+ *    say so.  What device arrays hold is not checked by the host: page numbers and slots outside the cache, lengths outside the table and
  *    starts outside the tokens are left out by the kernels, as said below.
  * ------------------------------------------------------------------------- */
 typedef struct {
@@ -515,7 +516,8 @@ BSQ_API int bsq_rope_frequencies(uint32_t dims, double base, int scaling, double
                                  double *frequencies, float *factor);
 /* out = x turned (`back`: turned back, times factor: the gradient of x from that
  * of out); tokens rows of `heads` heads side by side; out may be x, with its
- * rows.  Rows whose position is below zero are left as they are. */
+ * rows, else it may not lie on them.  Rows whose position is below zero are left as
+ * they are. */
 BSQ_API int bsq_rope(const bsq_rope_t *rope, const int32_t *d_positions, const void *d_x, int type, uint64_t tokens,
                      uint32_t heads, uint32_t dim, uint64_t ldx, int back, void *d_out, uint64_t ldo, void *stream);
 
@@ -550,7 +552,7 @@ BSQ_API int bsq_kv4_read(const bsq_kv4_cache_t *cache, const int32_t *d_slots, u
  * every type (FP32 queries in steps of 2^-133), the softmax's weights are rounded
  * to BF16 where both q and out are BF16, are held to 16 bits where FP16 is the
  * finest type among them, and to FP32 where one is FP32.  Queries behind the last
- * request's, and past `most`, are left as they are.  out may not overlap the
+ * request's, and past `most`, are left as they are.  out may not lie on the
  * queries' rows. */
 BSQ_API uint64_t bsq_kv4_attention_workspace(const bsq_kv4_cache_t *cache, uint32_t width, uint32_t requests,
                                              uint64_t tokens, uint32_t most, uint32_t q_heads);
