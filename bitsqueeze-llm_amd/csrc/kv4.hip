@@ -774,6 +774,10 @@ int bsq_kv4_append(const bsq_kv4_cache_t *cache, const bsq_rope_t *rope, const i
             BSQ_REQUIRE(a.in_place || !overlap(tokens, CallRows(d_q, ldq, q_width, t), CallRows(d_q_out, ldqo, q_width, t)),
                         "kv4 append: queries' output overlaps them");
             if (!(a.in_place && rope == nullptr)) {  // else nothing changes
+                // other workgroups read those at the same time
+                const CallRows out(d_q_out, ldqo, q_width, t);
+                BSQ_REQUIRE(!overlap(tokens, out, CallRows(d_k, ldk, width, t)) && !overlap(tokens, out, CallRows(d_v, ldv, width, t)),
+                            "kv4 append: queries' output overlaps keys or values");
                 a.q = static_cast<const uint8_t *>(d_q);
                 a.qo = static_cast<uint8_t *>(d_q_out);
                 a.q_heads = q_heads;

@@ -460,8 +460,9 @@ BSQ_API int bsq_moe_linear_backward(const void *d_d_out, int d_type, uint64_t to
  *    and can be captured; types, leading dimensions, returns and size queries are
  *    those of group 6 too.  Results may lie beside what a call reads, in other
  *    columns of rows of one distance; results on it are refused where the calls
- *    say so.  What device arrays hold is not checked by the host: page numbers and slots outside the cache, lengths outside the table and
- *    starts outside the tokens are left out by the kernels, as said below.
+ *    say so.  What device arrays hold is not checked by the host: page numbers and
+ *    slots outside the cache, lengths outside the table and starts outside the
+ *    tokens are left out by the kernels, as said below.
  * ------------------------------------------------------------------------- */
 typedef struct {
     uint8_t *d_pages; /* bsq_kv4_cache_bytes bytes, 16-byte aligned */
@@ -522,11 +523,12 @@ BSQ_API int bsq_rope(const bsq_rope_t *rope, const int32_t *d_positions, const v
                      uint32_t heads, uint32_t dim, uint64_t ldx, int back, void *d_out, uint64_t ldo, void *stream);
 
 /* A step's tokens: queries (q_heads heads; d_q may be NULL) turned to d_q_out
- * (may be d_q, with its rows), keys turned, rounded to their type and packed,
- * values packed, both into the cache at d_slots.  rope NULL: nothing is turned,
- * and d_positions may be NULL.  A token whose position is below zero is left
- * out, one whose slot is outside the cache leaves only its queries.  Where two
- * tokens have one slot, it holds parts of either. */
+ * (may be d_q, with its rows, else it may not lie on them; never on keys or
+ * values), keys turned, rounded to their type and packed, values packed, both into
+ * the cache at d_slots.  rope NULL: nothing is turned, and d_positions may be
+ * NULL.  A token whose position is below zero is left out, one whose slot is
+ * outside the cache leaves only its queries.  Where two tokens have one slot, it
+ * holds parts of either. */
 BSQ_API int bsq_kv4_append(const bsq_kv4_cache_t *cache, const bsq_rope_t *rope, const int32_t *d_positions,
                            const int32_t *d_slots, uint64_t tokens, int type, const void *d_q, uint32_t q_heads,
                            uint64_t ldq, void *d_q_out, uint64_t ldqo, const void *d_k, uint64_t ldk, const void *d_v,

@@ -4,7 +4,38 @@ work, and pointers are never reached."""
 import pytest
 
 import bitsqz_amd as B
-from test_kv4_refusals import D, attention_args, refused, rope
+from test_kv4_refusals import D, attention_args, cache, refused, rope
+
+Q, K, V = 256, 128, 128  # columns of one product's rows, BF16
+ROW = Q + K + V
+
+
+def append(**change):
+    a = dict(cache=cache(), rope=rope(), positions=D, slots=D, tokens=4, type=1, q=D, q_heads=4, ldq=ROW, q_out=D, ldqo=ROW,
+             k=D + 2 * Q, ldk=ROW, v=D + 2 * (Q + K), ldv=ROW, stream=None)
+    a.update(change)
+    return B.lib().bsq_kv4_append(*a.values())
+
+
+@pytest.mark.parametrize("change", [
+    # on the keys, on the values, on the end of either, in rows of the same distance
+    dict(q_out=D + 2 * Q), dict(q_out=D + 2 * (Q + K) - 2), dict(q_out=D + 2 * (ROW - 1)),
+    # in place, and keys or values among the queries, or in rows of another distance
+    dict(k=D), dict(v=D + 2 * Q - 16), dict(ldk=ROW - 8),
+    # beside the product's rows
+    dict(q_out=1 << 20, ldqo=Q, k=1 << 20, ldk=K), dict(q_out=1 << 20, ldqo=Q, v=(1 << 20) + 2 * 4 * Q - 2, ldv=V),
+    dict(q_out=1 << 20, ldqo=Q, k=(1 << 20) - 2, ldk=K),
+])
+def test_append(change):
+    refused(append(**change), "overlaps")
+
+
+def test_append_of_nothing_to_turn():
+    # in place and without positions no query is written
+    a = dict(rope=None, k=D, v=D, positions=None)
+    if B.device_count() < 1:
+        assert append(**a) == 1 and "overlap" not in B.lib().bsq_last_error().decode()
+
 
 @pytest.mark.parametrize("change", [
     dict(out=D + 2 * 255, ldq=512, ldo=512), dict(q=D + 2 * 255, out=D, ldq=512, ldo=512),  # a column in common
