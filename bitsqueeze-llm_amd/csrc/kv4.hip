@@ -809,6 +809,8 @@ int bsq_kv4_read(const bsq_kv4_cache_t *cache, const int32_t *d_slots, uint64_t 
         BSQ_REQUIRE(d_slots != nullptr, "kv4 read: null slots");
         if (d_k != nullptr) check_dense(d_k, t, "");
         if (d_v != nullptr) check_dense(d_v, t, "");
+        BSQ_REQUIRE(d_k == nullptr || d_v == nullptr || !overlap(tokens, CallRows(d_k, ldk, width, t), CallRows(d_v, ldv, width, t)),
+                    "kv4 read: keys and values overlap");
         const uint32_t eights = (c.dim + 7) / 8;
         uint32_t per = std::max(1u, 1024u / (c.heads * eights));
         while (per > 1 && tokens / per < 2ull * cu_count()) per /= 2;

@@ -533,8 +533,8 @@ BSQ_API int bsq_kv4_append(const bsq_kv4_cache_t *cache, const bsq_rope_t *rope,
                            const int32_t *d_slots, uint64_t tokens, int type, const void *d_q, uint32_t q_heads,
                            uint64_t ldq, void *d_q_out, uint64_t ldqo, const void *d_k, uint64_t ldk, const void *d_v,
                            uint64_t ldv, void *stream);
-/* The keys and values at d_slots (either may be NULL); rows of slots outside the
- * cache are left as they are. */
+/* The keys and values at d_slots (either may be NULL; they may not lie on one
+ * another); rows of slots outside the cache are left as they are. */
 BSQ_API int bsq_kv4_read(const bsq_kv4_cache_t *cache, const int32_t *d_slots, uint64_t tokens, int type, void *d_k,
                          uint64_t ldk, void *d_v, uint64_t ldv, void *stream);
 

@@ -53,3 +53,12 @@ def test_rope(change):
     a = dict(rope=rope(), positions=D, x=D, type=1, tokens=4, heads=2, dim=64, ldx=128, back=0, out=1 << 20, ldo=128, stream=None)
     a.update(change)
     refused(B.lib().bsq_rope(*a.values()), "overlaps")
+
+
+@pytest.mark.parametrize("change", [
+    dict(), dict(v=D + 2 * 127), dict(k=D + 2 * 3 * 128, v=D), dict(v=D + 256, ldk=256, ldv=255), dict(v=D + 254, ldk=256, ldv=256),
+])
+def test_read(change):
+    a = dict(cache=cache(), slots=D, tokens=4, type=1, k=D, ldk=128, v=D, ldv=128, stream=None)
+    a.update(change)
+    refused(B.lib().bsq_kv4_read(*a.values()), "overlap")
