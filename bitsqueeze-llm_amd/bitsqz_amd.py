@@ -941,7 +941,8 @@ class Kv4Cache:
 
     def step(self, new: np.ndarray, tokens: int | None = None) -> dict:
         """The places of the requests' new tokens (below zero: the request has
-        ended), `tokens` of them where given; as host arrays."""
+        ended), `tokens` of them where given; as host arrays.  "unserved" counts the
+        requests that were not served: their tokens have no slot and are given again."""
         new = np.ascontiguousarray(new, np.int32)
         _agree(new.shape == (self.requests,), f"Kv4Cache: new tokens of {self.requests} requests")
         tokens = int(np.maximum(new, 0).sum()) if tokens is None else tokens
@@ -954,9 +955,10 @@ class Kv4Cache:
                                  self.work.nbytes, None), "kv4_plan")
         check(lib().bsq_stream_synchronize(None), "sync")
         self.tokens, self.most = tokens, int(max(new.max(), 1))
-        left = self.left.download(np.int32, 2)
+        left, positions = self.left.download(np.int32, 2), self.positions.download(np.int32, tokens)
+        self.absent = positions < 0  # no token's, or of a request that was not served
         return {"starts": self.starts.download(np.int32, self.requests + 1), "requests": of.download(np.int32, tokens),
-                "positions": self.positions.download(np.int32, tokens), "slots": self.slots.download(np.int32, tokens),
+                "positions": positions, "slots": self.slots.download(np.int32, tokens),
                 "lengths": self.lengths.download(np.int32, self.requests), "left": int(left[0]), "unserved": int(left[1])}
 
     def _step_of(self, x: np.ndarray, heads: int | None, what: str):
@@ -999,7 +1001,8 @@ class Kv4Cache:
     def attend(self, q: np.ndarray, scale: float | None = None, type: int = TYPE_F32, out_type: int = TYPE_F32,
                causal: bool = True, window: int = 0):
         """(out, lse) of the step's queries over their requests' keys and values;
-        zeros and minus infinity for places that are no token."""
+        zeros and minus infinity for places that are no token, and for the tokens of
+        requests that were not served."""
         q = _typed(q, type)
         self._step_of(q, None, "queries")
         _agree(q.shape[1] % self.heads == 0, f"Kv4Cache: queries of a multiple of {self.heads} heads")
@@ -1013,4 +1016,6 @@ class Kv4Cache:
                                       self.dim**-0.5 if scale is None else scale, int(causal), window, out.ptr, out_type,
                                       heads * self.dim, lse.ptr, work.ptr, work.nbytes, None), "kv4_attention")
         check(lib().bsq_stream_synchronize(None), "sync")
-        return out.download(t, q.size).reshape(q.shape), lse.download(np.float32, n * heads).reshape(n, heads)
+        out, lse = out.download(t, q.size).reshape(q.shape), lse.download(np.float32, n * heads).reshape(n, heads)
+        out[self.absent], lse[self.absent] = 0, -np.inf
+        return out, lse

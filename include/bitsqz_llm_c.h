@@ -480,7 +480,8 @@ BSQ_API uint64_t bsq_kv4_cache_bytes(uint64_t pages, uint32_t page, uint32_t hea
  * order of requests and of their rows; then each request in turn takes the pages
  * that its new tokens need beyond those it holds, from the top, into its row.
  * A request is not served where the stack runs out (nor are those behind it that
- * need a page), its row is too short, or its tokens go past `tokens`.
+ * need a page), its row is too short, or the tokens up to its last, those of the
+ * requests before it among them, are more than `tokens`.
  * Written: d_lengths_out[r], the length with the new tokens (as it was where not
  * served, 0 where ended; may be d_lengths); d_left[0], the pages left on the
  * stack (d_left may be d_free_count), and d_left[1], the requests not served;
@@ -554,8 +555,11 @@ BSQ_API int bsq_kv4_read(const bsq_kv4_cache_t *cache, const int32_t *d_slots, u
  * every type (FP32 queries in steps of 2^-133), the softmax's weights are rounded
  * to BF16 where both q and out are BF16, are held to 16 bits where FP16 is the
  * finest type among them, and to FP32 where one is FP32.  Queries behind the last
- * request's, and past `most`, are left as they are.  out may not lie on the
- * queries' rows. */
+ * request's, and past `most`, are left as they are.  Starts do not fall: of queries
+ * that two requests have, the results are either's or left as they are.  The tokens
+ * of a request that the plan did not serve lie between its starts like others, and
+ * get what they would as the last of the keys that it holds: their results mean
+ * nothing.  out may not lie on the queries' rows. */
 BSQ_API uint64_t bsq_kv4_attention_workspace(const bsq_kv4_cache_t *cache, uint32_t width, uint32_t requests,
                                              uint64_t tokens, uint32_t most, uint32_t q_heads);
 BSQ_API int bsq_kv4_attention(const bsq_kv4_cache_t *cache, const int32_t *d_table, uint32_t width,
