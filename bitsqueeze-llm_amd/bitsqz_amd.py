@@ -921,7 +921,8 @@ def rope(x: np.ndarray, positions: np.ndarray, turn: Turn, type: int = TYPE_F32,
 class Kv4Cache:
     """A paged cache of one layer with its bookkeeping: step(), then append() and
     attend() of that step's tokens.  All pages are free at first, all requests
-    empty."""
+    empty.  Several layers' caches have each their own plan of a step; layers that
+    share one call the library's functions."""
 
     def __init__(self, pages: int, page: int, heads: int, dim: int, requests: int, width: int):
         """width: the most pages of a request."""

@@ -568,12 +568,12 @@ void launch_rows(const RowsArgs &rows, Mx4Type type, bool kv, hipStream_t stream
     a.by_key_eights = Divisor(std::max(a.chunks + a.rest, 1u));
     a.by_heads = Divisor(std::max(kv ? a.cache.heads : 1u, 1u));
     a.by_eights = Divisor(std::max(kv ? a.cache.blocks * 4 : 1u, 1u));
-    // several tokens a workgroup share the wait for their sines, as long as eight
-    // workgroups a CU remain
+    // several tokens a workgroup share the wait for their sines, as long as three times
+    // as many groups of tokens as CUs remain (with keys and values a group is two
+    // workgroups)
     a.per = 1;
     while (a.per < kRowTokens && a.tokens / (2 * a.per) >= 3ull * cu_count()) a.per *= 2;
-    // items are counted in 24 bits
-    while (a.per > 1 && static_cast<uint64_t>(a.per) * std::max(a.q_heads, kv ? a.cache.heads : 0u) * kKv4MaxDim / 8 >= 1u << 24) a.per /= 2;
+    static_assert(kRowTokens * 65535 * (kKv4MaxDim / 8 + 1) < 1u << 24, "items are divided in 24 bits");
     const uint64_t groups = ceil_div(a.tokens, a.per);
     BSQ_REQUIRE(groups <= 0xFFFFFFFFull / (2 * kRowThreads) - 16, "kv4: too many tokens");
     by_type(type, [&](auto ty) {

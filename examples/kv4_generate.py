@@ -7,9 +7,12 @@ own lengths, then a token at a time for each; one request ends on the way.
 
     x = embedding[token]
     q, k, v = x W^T                          bsq_mx4_linear
-    q, k turned, k and v into the cache      bsq_kv4_plan (once a step), bsq_kv4_append
+    q, k turned, k and v into the cache      bsq_kv4_plan, bsq_kv4_append
     a = attention of q over the cache        bsq_kv4_attention
     x = x + a O^T, x = x + relu(x U^T) D^T   bsq_mx4_linear
+
+Each layer's cache plans its own pages here; a program that calls the library
+itself plans once a step, and its layers share the table and the places.
 
 The weights are random.  At the end the tokens of the requests that go on are
 computed once more, each as one prompt; prints the largest difference of the
