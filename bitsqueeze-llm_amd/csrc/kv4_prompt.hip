@@ -150,8 +150,9 @@ __global__ __launch_bounds__(kThreads, NB <= 4 && P <= 2 ? 2 : 1) void kv4_promp
         const uint32_t u = lane + 64 * n;
         return Unit{u / NB, u % NB, u & 1, u >> 1, kUnits % 64 == 0 || u < static_cast<uint32_t>(kUnits)};
     };
-    // above zero, so that what is not seen stays at minus infinity
-    const float factor = fmaxf(a.factor, 0x1p-126f);
+    // above zero, so that what is not seen stays at minus infinity; with the smallest
+    // value scores of any size count as zero, to 2^-21
+    const float factor = fmaxf(a.factor, 0x1p-149f);
     const uint32_t page_bytes = a.cache.head_bytes * heads;
     const uint8_t *const head0 = a.cache.pages + h * a.cache.head_bytes;
     const auto id_of = [&](int32_t t) { return page_of(a, r, rq, static_cast<uint32_t>(t) + 16 * wave); };
