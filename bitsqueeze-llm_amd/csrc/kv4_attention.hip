@@ -161,6 +161,8 @@ int bsq_kv4_attention(const bsq_kv4_cache_t *cache, const int32_t *d_table, uint
         BSQ_REQUIRE(ldq >= row && ldo >= row, "kv4 attention: rows overlap");
         BSQ_REQUIRE(ldq <= 1ull << 28 && ldo <= 1ull << 28, "kv4 attention: rows too far apart");
         BSQ_REQUIRE(std::isfinite(scale), "kv4 attention: the scale is not finite");
+        const float factor = static_cast<float>(std::fabs(static_cast<double>(scale)) * 1.44269504088896340736);
+        BSQ_REQUIRE(std::isfinite(factor), "kv4 attention: the scale is too large");
         BSQ_REQUIRE(causal == 0 || causal == 1, "kv4 attention: causal is 0 or 1");
         BSQ_REQUIRE(causal == 1 || window == 0, "kv4 attention: a window is of causal attention");
         BSQ_REQUIRE(d_starts != nullptr || tokens == requests, "kv4 attention: without starts each request has one query");
@@ -186,7 +188,7 @@ int bsq_kv4_attention(const bsq_kv4_cache_t *cache, const int32_t *d_table, uint
         a.tokens = static_cast<uint32_t>(tokens);
         a.most = std::min<uint32_t>(most, 0x7FFFFFFFu);
         a.group = q_heads / a.cache.heads;
-        a.factor = static_cast<float>(std::fabs(static_cast<double>(scale)) * 1.44269504088896340736);
+        a.factor = factor;
         a.negate = scale < 0.0f;
         a.causal = causal != 0;
         a.window = window >= static_cast<uint64_t>(width) << a.cache.shift ? 0u : window;  // all of a request's

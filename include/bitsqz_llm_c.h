@@ -545,6 +545,7 @@ BSQ_API int bsq_kv4_read(const bsq_kv4_cache_t *cache, const int32_t *d_slots, u
  * is at the last key's position.  Query head h reads head h / (q_heads / heads)
  * of keys and values:
  *   out = sum over the seen j of softmax(scale q . k[j]) v[j]
+ * (|scale| up to 2.35e38).
  * `causal`: a query sees the keys up to its own position, with a `window` above
  * zero only the last `window` of them; else all of its request's (window 0).
  * Keys on page numbers outside the cache are not seen.  A query that sees none
