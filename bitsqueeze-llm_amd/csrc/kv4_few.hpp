@@ -5,10 +5,12 @@
 // Long contexts are bound by HBM: 8 requests of 40 to 90 thousand keys, 32 query
 // heads on 8 of 128, take 107 us with the join, 5.0 TB/s of the 5.07 that a large
 // copy reaches.  Of ragged ones (128 requests of 16 to 16384 keys, 76 us, 4.4 TB/s)
-// and short ones (16 of 400 to 1200, 14.9 us) what a tile costs beside its keys is
+// and short ones (16 of 400 to 1200, 15.0 us) what a tile costs beside its keys is
 // the rest; each further step of 32 keys adds a wave alone on its SIMD some 0.8 us
-// (least shares of 4 to 12 steps, 15.8 to 22.3 us); keys are asked for one step ahead.  A form with a workgroup's waves
-// on one tile, joined in LDS, took 89 us for the ragged and 15.5 for the short ones.
+// (least shares of 4 to 12 steps, 15.8 to 22.3 us); keys are asked for one step ahead.
+// A form with a workgroup's waves on one tile, joined in LDS, took 89 us for the ragged
+// and 15.5 for the short ones; 9 requests of 5 queries over 100 to 5000 keys, 12 heads
+// of 64 in FP32, took 15.4 with it and take 18.4 with waves as shares.
 #pragma once
 
 #include "kv4_attention.hpp"

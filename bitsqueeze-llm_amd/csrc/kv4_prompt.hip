@@ -15,8 +15,8 @@
 // eight weights that a lane has are the eight that the next product wants of it.
 //
 // Bound by the matrix instructions and the vector ones between them, which two waves
-// a SIMD overlap only in part: a prompt of 8192, 32 heads on 8 of 128, takes 623 to
-// 655 us, 840 to 880 TFLOP/s (1173 in a large BF16 product of the library); a wave's
+// a SIMD overlap only in part: a prompt of 8192, 32 heads on 8 of 128, takes 613 to
+// 655 us, 840 to 897 TFLOP/s (1173 in a large BF16 product of the library); a wave's
 // 64 keys are 32 matrix instructions and some 240 others, 32 of them exponentials.
 // Waves of raised priority during the products: 695 us against 669.  Tiles of 16 rows
 // (kv4_few.hpp) take 2790.

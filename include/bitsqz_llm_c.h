@@ -552,15 +552,16 @@ BSQ_API int bsq_kv4_read(const bsq_kv4_cache_t *cache, const int32_t *d_slots, u
  * gives zeros.  d_lse (tokens x q_heads, may be NULL): the natural logarithm of
  * the softmax's sum, minus infinity where no key is seen.  Sums and softmax are
  * FP32, and so are the scores before their scale: a query whose scores are all
- * below FP32's range gives zeros too.  Products with queries are exact to FP32 in
- * every type (FP32 queries in steps of 2^-133), the softmax's weights are rounded
- * to BF16 where both q and out are BF16, are held to 16 bits where FP16 is the
- * finest type among them, and to FP32 where one is FP32.  Queries behind the last
- * request's, and past `most`, are left as they are.  Starts do not fall: of queries
- * that two requests have, the results are either's or left as they are.  The tokens
- * of a request that the plan did not serve lie between its starts like others, and
- * get what they would as the last of the keys that it holds: their results mean
- * nothing.  out may not lie on the queries' rows. */
+ * below FP32's range gives zeros too.  One that holds an infinity or a NaN gives
+ * NaN if it sees a key.  Products with queries are exact to FP32 in every type
+ * (FP32 queries in steps of 2^-133), the softmax's weights are rounded to BF16 where
+ * both q and out are BF16, are held to 16 bits where FP16 is the finest type among
+ * them, and to FP32 where one is FP32.  Queries behind the last request's, and past
+ * `most`, are left as they are.  Starts do not fall: of queries that two requests
+ * have, the results are either's or left as they are.  The tokens of a request that
+ * the plan did not serve lie between its starts like others, and get what they
+ * would as the last of the keys that it holds: their results mean nothing.  out
+ * may not lie on the queries' rows. */
 BSQ_API uint64_t bsq_kv4_attention_workspace(const bsq_kv4_cache_t *cache, uint32_t width, uint32_t requests,
                                              uint64_t tokens, uint32_t most, uint32_t q_heads);
 BSQ_API int bsq_kv4_attention(const bsq_kv4_cache_t *cache, const int32_t *d_table, uint32_t width,
